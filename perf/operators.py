@@ -104,10 +104,10 @@ def draw(rng):
         sequences, chunk, history = max(1, sequences // 2), max(1, chunk * 2 // 3), max(1, history * 2 // 3)
     while sequences * (chunk + history) * kv * head * BYTES[cache] > 200000 * 8 * 128 * 2:
         sequences, history = max(1, sequences // 2), max(1, history * 2 // 3)
+    while sequences * chunk * heads * head * BYTES[rows] > 1 << 28:
+        chunk //= 2
     if op == "append":
         history = min(history, 4096)
-        while sequences * chunk * heads * head * BYTES[rows] > 1 << 28:
-            chunk //= 2
         return {"op": op, "kind": kind, "rows": rows, "cache": cache, "heads": heads, "kv": kv, "head": head,
                 "page": page, "sequences": sequences, "chunk": chunk, "history": history, "norm": rng.random() < 0.5,
                 "cache_layout": layout, **rope}
