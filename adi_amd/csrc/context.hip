@@ -74,6 +74,11 @@ adi_hip_codebook *upload(adi_hip_context *ctx, adi_hip_codebook::Kind kind,
 
 }  // namespace
 
+void record_error(std::string message) {
+    std::lock_guard<std::mutex> lock(g_create_error_mutex);
+    g_create_error = std::move(message);
+}
+
 KernelStat &stat_for(adi_hip_context *ctx, const char *name) {
     for (auto &stat : ctx->stats) {
         if (stat.name == name) {
@@ -91,10 +96,7 @@ using namespace adi_hip;
 extern "C" {
 
 int adi_hip_context_create(int device, adi_hip_context **out) {
-    auto record = [](const std::string &message) {
-        std::lock_guard<std::mutex> lock(g_create_error_mutex);
-        g_create_error = message;
-    };
+    const auto record = [](std::string message) { record_error(std::move(message)); };
     if (out == nullptr) {
         record("adi_hip_context_create: null output pointer");
         return ADI_HIP_INVALID_ARGUMENT;

@@ -210,6 +210,27 @@ int guarded(adi_hip_context *ctx, F &&function) {
     }
 }
 
+// Leaves a message for adi_hip_last_error(NULL).
+void record_error(std::string message);
+
+// guarded() for calls that take no context and touch no device.
+template <typename F>
+int guarded_host(F &&function) {
+    try {
+        function();
+        return ADI_HIP_OK;
+    } catch (const Failure &failure) {
+        record_error(failure.message);
+        return failure.status;
+    } catch (const std::bad_alloc &) {
+        record_error("host allocation failed");
+        return ADI_HIP_OUT_OF_MEMORY;
+    } catch (const std::exception &error) {
+        record_error(error.what());
+        return ADI_HIP_DEVICE_ERROR;
+    }
+}
+
 KernelStat &stat_for(adi_hip_context *ctx, const char *name);
 
 // Launches `kernel` on the context stream. With profiling on, the launch

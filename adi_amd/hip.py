@@ -118,6 +118,38 @@ class RequestStatus(C.Structure):
                 ("prefill_seconds", C.c_double), ("decode_seconds", C.c_double)]
 
 
+class RopeOptions(C.Structure):
+    _fields_ = [("rotary", u32), ("layout", u32), ("scaling", u32), ("theta", C.c_double),
+                ("factor", C.c_double), ("original", C.c_double), ("fast", C.c_double),
+                ("slow", C.c_double), ("magnitude", C.c_double)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("type", u32), ("data", vp), ("token_stride", u64), ("head_stride", u64)]
+
+
+class PagedCacheStruct(C.Structure):
+    _fields_ = [("type", u32), ("heads", u32), ("head_size", u32), ("page_size", u32), ("pages", u32),
+                ("keys", vp), ("values", vp), ("page_stride", u64), ("entry_stride", u64),
+                ("head_stride", u64)]
+
+
+class PagedBatchStruct(C.Structure):
+    _fields_ = [("sequences", u32), ("tokens", u32), ("max_tokens", u32), ("max_length", u32),
+                ("offsets", vp), ("lengths", vp), ("table", vp), ("table_stride", u32)]
+
+
+class PagedAppendArguments(C.Structure):
+    _fields_ = [("rope", vp), ("keys", Rows), ("values", Rows), ("key_norm", vp), ("query_heads", u32),
+                ("queries", Rows), ("queries_out", Rows), ("query_norm", vp), ("weight_offset", f32),
+                ("epsilon", f32)]
+
+
+class PagedAttentionArguments(C.Structure):
+    _fields_ = [("query_heads", u32), ("queries", Rows), ("outputs", Rows), ("gate", Rows),
+                ("scale", f32), ("window", u32)]
+
+
 class KernelProfile(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("launches", C.c_uint64), ("total_ms", C.c_double)]
 
@@ -205,6 +237,18 @@ SIGNATURES = [
     ("adi_hip_batcher_request_error", C.c_char_p, [vp, u64]),
     ("adi_hip_batcher_release", C.c_int, [vp, u64]),
     ("adi_hip_batcher_force_failure", C.c_int, [vp, C.c_int]),
+    ("adi_hip_rope_frequencies", C.c_int,
+     [C.POINTER(RopeOptions), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    ("adi_hip_rope_create", C.c_int, [vp, C.POINTER(RopeOptions), C.POINTER(vp)]),
+    ("adi_hip_rope_destroy", None, [vp]),
+    ("adi_hip_rope_rows", C.c_int, [vp, vp, C.POINTER(Rows), u32, u32, u32, vp, C.POINTER(Rows)]),
+    ("adi_hip_paged_check", C.c_int, [C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct)]),
+    ("adi_hip_paged_append", C.c_int,
+     [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), C.POINTER(PagedAppendArguments)]),
+    ("adi_hip_paged_workspace_create", C.c_int, [vp, C.c_size_t, C.POINTER(vp)]),
+    ("adi_hip_paged_workspace_destroy", None, [vp]),
+    ("adi_hip_paged_attention", C.c_int,
+     [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), C.POINTER(PagedAttentionArguments), vp]),
     ("adi_hip_profiling_enable", C.c_int, [vp, C.c_int]),
     ("adi_hip_profiling_read", C.c_int, [vp, C.POINTER(KernelProfile), u32, C.POINTER(u32)]),
     # include/adi_hip_gguf.h
@@ -1084,3 +1128,235 @@ def prefill(ctx: Context, model: Model, tokens, sequence: Sequence, logits=None,
     toks = (u32 * max(len(tokens), 1))(*[int(t) for t in tokens])
     ctx.check(ctx.lib.adi_hip_prefill(ctx.handle, C.byref(model.struct), toks, len(tokens), ubatch,
                                       C.byref(sequence.struct), _addr(logits)))
+
+
+# ---- rotary positions, and a paged cache of many sequences -------------------
+
+F32, F16, BF16 = 0, 1, 2
+ROPE_LAYOUTS = {"halves": 0, "pairs": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+def _refuse(message: str):
+    raise HipError(INVALID_ARGUMENT, message)
+
+
+_type_codes: dict = {}
+
+
+def _type_of(t) -> int:
+    if not _type_codes:
+        import torch
+        _type_codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    code = _type_codes.get(t.dtype)
+    if code is None:
+        _refuse(f"rows of type {t.dtype} are not supported")
+    return code
+
+
+def _rows(ctx: Context, t, tokens: int, heads: Optional[int], head_size: int) -> Rows:
+    """A tensor [tokens, heads, head size] (any strides of the first two) as
+    adi_hip_rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_size or (heads is not None and shape[1] != heads):
+        _refuse(f"rows of shape {tuple(shape)}, expected [{tokens}, {heads or 'heads'}, {head_size}]")
+    if stride[2] != 1 and shape[2] > 1:
+        _refuse("a head's elements must be contiguous")
+    if not t.is_cuda or t.device.index != ctx.device:
+        _refuse(f"rows on {t.device}, the context is on cuda:{ctx.device}")
+    if stride[0] == 0 and shape[0] > 1 or stride[1] == 0 and shape[1] > 1:
+        _refuse("broadcast rows are not supported")
+    return Rows(_type_of(t), t.data_ptr(), stride[0], stride[1])
+
+
+def _device_words(ctx: Context, t, name: str, *shape):
+    """A contiguous int32 (or uint32) tensor of the context's device."""
+    if tuple(t.shape) != shape or not t.is_contiguous() or t.element_size() != 4 or t.is_floating_point():
+        _refuse(f"{name} must be a contiguous int32 tensor of shape {shape}")
+    if not t.is_cuda or t.device.index != ctx.device:
+        _refuse(f"{name} on {t.device}, the context is on cuda:{ctx.device}")
+    return t
+
+
+def _bf16_weight(ctx: Context, t, size: int) -> Optional[int]:
+    if t is None:
+        return None
+    if tuple(t.shape) != (size,) or not t.is_contiguous() or t.element_size() != 2 or _dtype_name(t) not in (
+            "bfloat16", "int16"):
+        _refuse(f"a norm weight must be {size} contiguous bf16 values")
+    if not t.is_cuda or t.device.index != ctx.device:
+        _refuse(f"a norm weight on {t.device}, the context is on cuda:{ctx.device}")
+    return t.data_ptr()
+
+
+def _dtype_name(t) -> str:
+    return str(t.dtype).replace("torch.", "")
+
+
+def _rope_options(rotary, layout, theta, scaling, factor, original, fast, slow, magnitude) -> RopeOptions:
+    if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
+        _refuse(f"rope: unknown layout {layout!r} or scaling {scaling!r}")
+    return RopeOptions(rotary, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], theta, factor, original, fast, slow,
+                       magnitude)
+
+
+def rope_frequencies(rotary: int, layout: str = "halves", theta: float = 1e4, scaling: str = "none",
+                     factor: float = 1.0, original: float = 0.0, fast: float = 0.0, slow: float = 0.0,
+                     magnitude: float = 0.0):
+    """(frequencies, magnitude) of a rotation, float64 on the host; needs no
+    GPU. The options are adi_hip_rope_options' (include/adi_hip.h)."""
+    o = _rope_options(rotary, layout, theta, scaling, factor, original, fast, slow, magnitude)
+    lib = load()
+    out = np.empty(max(int(rotary) // 2, 1), np.float64)
+    m = C.c_double()
+    status = lib.adi_hip_rope_frequencies(C.byref(o), out.ctypes.data_as(C.POINTER(C.c_double)), C.byref(m))
+    if status != OK:
+        raise HipError(status, lib.adi_hip_last_error(None).decode())
+    return out, m.value
+
+
+class Rope:
+    """A rotation's frequencies on the device (adi_hip_rope): `rotary`
+    dimensions of a head, in "halves" or "pairs", scaled for a context `factor`
+    times the `original` one by "linear", "ntk", "yarn" or "bands"."""
+
+    def __init__(self, ctx: Context, rotary: int, layout: str = "halves", theta: float = 1e4,
+                 scaling: str = "none", factor: float = 1.0, original: float = 0.0, fast: float = 0.0,
+                 slow: float = 0.0, magnitude: float = 0.0):
+        self.handle = None
+        o = _rope_options(rotary, layout, theta, scaling, factor, original, fast, slow, magnitude)
+        handle = vp()
+        ctx.check(ctx.lib.adi_hip_rope_create(ctx.handle, C.byref(o), C.byref(handle)))
+        self.lib, self.handle, self.rotary = ctx.lib, handle, rotary
+
+    def close(self) -> None:
+        if self.handle:
+            self.lib.adi_hip_rope_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rope_rows(ctx: Context, rope: Rope, x, positions, out) -> None:
+    """Rotates rows x [tokens, heads, head size] to positions [tokens] (device
+    int32) into out (of x's shape and type; may be x)."""
+    tokens, heads, size = x.shape
+    a, b = _rows(ctx, x, tokens, heads, size), _rows(ctx, out, tokens, heads, size)
+    _device_words(ctx, positions, "positions", tokens)
+    status = ctx.lib.adi_hip_rope_rows(ctx.handle, rope.handle, a, tokens, heads, size, positions.data_ptr(), b)
+    if status:
+        ctx.check(status)
+
+
+class PagedCache:
+    """adi_hip_paged_cache over two tensors [pages, page size, KV heads, head
+    size] of one type and one layout (any strides of the first three
+    dimensions: a head-major pool is such a view)."""
+
+    def __init__(self, ctx: Context, keys, values):
+        if keys.dim() != 4 or keys.shape != values.shape or keys.stride() != values.stride() or \
+                keys.dtype != values.dtype or keys.stride(3) != 1:
+            _refuse("a paged cache needs keys and values [pages, page size, heads, head size] of one type and layout")
+        if not keys.is_cuda or keys.device.index != ctx.device or values.device != keys.device:
+            _refuse(f"a paged cache on {keys.device}, the context is on cuda:{ctx.device}")
+        pages, page_size, heads, size = keys.shape
+        self.keys, self.values = keys, values
+        self.heads, self.head_size, self.page_size, self.pages = heads, size, page_size, pages
+        self.struct = PagedCacheStruct(_type_of(keys), heads, size, page_size, pages, keys.data_ptr(),
+                                       values.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2))
+
+
+class PagedBatch:
+    """adi_hip_paged_batch: device int32 tensors offsets [sequences + 1],
+    lengths [sequences] and table [sequences, pages of a sequence], which
+    the calls read when they run, and the host's bounds on them: `tokens`
+    rows, at most max_tokens new ones and max_length entries a sequence."""
+
+    def __init__(self, ctx: Context, offsets, lengths, table, tokens: int, max_tokens: int, max_length: int):
+        n = int(lengths.shape[0])
+        _device_words(ctx, lengths, "lengths", n)
+        _device_words(ctx, offsets, "offsets", n + 1)
+        _device_words(ctx, table, "table", n, int(table.shape[-1]))
+        self.offsets, self.lengths, self.table = offsets, lengths, table
+        self.tokens = tokens
+        self.struct = PagedBatchStruct(n, tokens, max_tokens, max_length, offsets.data_ptr(), lengths.data_ptr(),
+                                       table.data_ptr(), int(table.shape[1]))
+
+
+def paged_check(cache: PagedCacheStruct, offsets, lengths, table, tokens: int, max_tokens: int,
+                max_length: int) -> None:
+    """adi_hip_paged_check of a batch's host arrays (numpy) against a cache's
+    descriptor; needs no GPU."""
+    held = [np.ascontiguousarray(a).astype(np.uint32, casting="unsafe") for a in (offsets, lengths, table)]
+    n = held[1].size
+    if held[0].shape != (n + 1,) or held[2].ndim != 2 or held[2].shape[0] != n:
+        _refuse("paged batch: offsets, lengths and table do not fit each other")
+    batch = PagedBatchStruct(n, tokens, max_tokens, max_length, *(a.ctypes.data for a in held), held[2].shape[1])
+    lib = load()
+    status = lib.adi_hip_paged_check(C.byref(cache), C.byref(batch))
+    if status != OK:
+        raise HipError(status, lib.adi_hip_last_error(None).decode())
+
+
+class PagedWorkspace:
+    """Device memory in which attention calls join the parts of long
+    histories (adi_hip_paged_workspace); one for calls that may run at once
+    each."""
+
+    def __init__(self, ctx: Context, size: int = 0):
+        self.handle = None
+        handle = vp()
+        ctx.check(ctx.lib.adi_hip_paged_workspace_create(ctx.handle, size, C.byref(handle)))
+        self.lib, self.handle = ctx.lib, handle
+
+    def close(self) -> None:
+        if self.handle:
+            self.lib.adi_hip_paged_workspace_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+_no_rows = Rows()
+
+
+def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, keys, values, rope: Optional[Rope] = None,
+                 key_norm=None, queries=None, query_norm=None, queries_out=None, weight_offset: float = 1.0,
+                 epsilon: float = 1e-6) -> None:
+    """Appends keys and values [tokens, KV heads, head size] to their
+    sequences' pages, normalized by key_norm (bf16 [head size]) and rotated
+    where given, and normalizes and rotates queries [tokens, heads, head size]
+    alike into queries_out (default: in place)."""
+    n, size = batch.tokens, cache.head_size
+    q, o, heads = _no_rows, _no_rows, 0
+    if queries is not None:
+        heads = queries.shape[1]
+        q = _rows(ctx, queries, n, heads, size)
+        o = q if queries_out is None else _rows(ctx, queries_out, n, heads, size)
+    a = PagedAppendArguments(rope.handle if rope is not None else None, _rows(ctx, keys, n, cache.heads, size),
+                             _rows(ctx, values, n, cache.heads, size), _bf16_weight(ctx, key_norm, size), heads, q, o,
+                             _bf16_weight(ctx, query_norm, size), weight_offset, epsilon)
+    status = ctx.lib.adi_hip_paged_append(ctx.handle, cache.struct, batch.struct, a)
+    if status:
+        ctx.check(status)
+
+
+def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, queries, out, workspace: PagedWorkspace,
+                    scale: float = 0.0, window: int = 0, gate=None) -> None:
+    """Causal attention of queries [tokens, heads, head size] over their
+    sequences' pages into out, times sigmoid(gate) where given; scale 0 is
+    1 / sqrt(head size), window 0 none."""
+    n, size, heads = batch.tokens, cache.head_size, queries.shape[1]
+    a = PagedAttentionArguments(heads, _rows(ctx, queries, n, heads, size), _rows(ctx, out, n, heads, size),
+                                _no_rows if gate is None else _rows(ctx, gate, n, heads, size), scale, window)
+    status = ctx.lib.adi_hip_paged_attention(ctx.handle, cache.struct, batch.struct, a, workspace.handle)
+    if status:
+        ctx.check(status)

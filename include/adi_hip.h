@@ -49,7 +49,9 @@ int adi_hip_context_create(int device, adi_hip_context **out);
 void adi_hip_context_destroy(adi_hip_context *ctx);
 
 /* Message of the last failed call on this context ("" if none). A NULL
- * context gives the message of the last failed adi_hip_context_create. */
+ * context gives the message of the last failed adi_hip_context_create, or
+ * of the last failed call that takes no context (adi_hip_rope_frequencies,
+ * adi_hip_paged_check) where that came later. */
 const char *adi_hip_last_error(const adi_hip_context *ctx);
 
 /* Stream the context launches on (a hipStream_t; NULL = the null stream). */
@@ -667,6 +669,198 @@ int adi_hip_batcher_release(adi_hip_batcher *batcher, uint64_t request);
 #define ADI_HIP_BATCHER_FAIL_ADMISSION 1
 #define ADI_HIP_BATCHER_FAIL_STEP 2
 int adi_hip_batcher_force_failure(adi_hip_batcher *batcher, int where);
+
+/* ---- rotary positions, and a paged cache of many sequences ----------------- */
+
+/* Element types of the rows and caches below. */
+#define ADI_HIP_F32 0
+#define ADI_HIP_F16 1
+#define ADI_HIP_BF16 2
+
+/* Which two dimensions of a head's first `rotary` turn together: i and
+ * i + rotary / 2, as apply_rope (src/executor.cpp:60-72) turns them, or 2 i
+ * and 2 i + 1. */
+#define ADI_HIP_ROPE_HALVES 0
+#define ADI_HIP_ROPE_PAIRS 1
+
+/* How the frequencies f_i = theta^(-2 i / rotary) are stretched for contexts
+ * `factor` times the `original` one:
+ *   plain    f_i (the checkpoint's, src/model.cpp:606-615)
+ *   linear   f_i / factor
+ *   NTK      theta' = theta factor^(rotary / (rotary - 2)): the last pair is
+ *            stretched by factor, the first not at all (rotary above 2)
+ *   YaRN     between the pairs that turn `fast` and `slow` times over the
+ *            original context, i_t = rotary ln(original / (2 pi t)) /
+ *            (2 ln theta) rounded outwards and kept within 0 .. rotary - 1, a
+ *            linear ramp from f_i to f_i / factor; rows are multiplied by
+ *            0.1 ln(factor) + 1
+ *   bands    by the turns t_i = original f_i / (2 pi): f_i where
+ *            t_i >= fast, f_i / factor where t_i <= slow, between them
+ *            linear in t_i. */
+#define ADI_HIP_ROPE_PLAIN 0
+#define ADI_HIP_ROPE_LINEAR 1
+#define ADI_HIP_ROPE_NTK 2
+#define ADI_HIP_ROPE_YARN 3
+#define ADI_HIP_ROPE_BANDS 4
+
+typedef struct {
+    uint32_t rotary;   /* turned dimensions of a head: even, 2 to 1024 */
+    uint32_t layout;   /* ADI_HIP_ROPE_HALVES or ADI_HIP_ROPE_PAIRS */
+    uint32_t scaling;  /* ADI_HIP_ROPE_PLAIN .. ADI_HIP_ROPE_BANDS */
+    double theta;      /* above 1 */
+    double factor;     /* at least 1 (not read for plain) */
+    double original;   /* YaRN, bands: at least 1 */
+    double fast, slow; /* YaRN, bands: turns, fast > slow > 0; both 0: 32 and 1, 4 and 1 */
+    double magnitude;  /* what turned dimensions are multiplied by; 0: the scaling's own */
+} adi_hip_rope_options;
+
+/* On the host, no GPU needed: the rotary / 2 frequencies (radians a position)
+ * and the magnitude (either may be NULL). ADI_HIP_INVALID_ARGUMENT for
+ * options outside the ranges above (the message: adi_hip_last_error(NULL)). */
+int adi_hip_rope_frequencies(const adi_hip_rope_options *options, double *frequencies,
+                             double *magnitude);
+
+/* The frequencies on the context's device. Used by calls of any context of
+ * that device; destroying it waits for the device. */
+typedef struct adi_hip_rope adi_hip_rope;
+int adi_hip_rope_create(adi_hip_context *ctx, const adi_hip_rope_options *options,
+                        adi_hip_rope **out);
+void adi_hip_rope_destroy(adi_hip_rope *rope);
+
+/* Rows [tokens][heads][head size] in device memory; the strides of a token
+ * and of a head are in elements, those of a head one element apart. */
+typedef struct {
+    uint32_t type; /* ADI_HIP_F32, ADI_HIP_F16, ADI_HIP_BF16 */
+    void *data;
+    uint64_t token_stride;
+    uint64_t head_stride;
+} adi_hip_rows;
+
+/* Turns the first `rotary` of head_size dimensions (rotary <= head_size <=
+ * 65536, any size and strides) of every head of `tokens` rows to positions[token]
+ * (DEVICE), and copies the others: angles and their reduction in 64 bits, sines
+ * and products in 32, rounded once to the rows' type (the input's and output's
+ * are one). apply_rope (src/executor.cpp:60-72) for rows of any layout. The
+ * output may be the input (same data and strides); other overlaps are not
+ * allowed. tokens 0 is no call. */
+int adi_hip_rope_rows(adi_hip_context *ctx, const adi_hip_rope *rope, const adi_hip_rows *input,
+                      uint32_t tokens, uint32_t heads, uint32_t head_size,
+                      const uint32_t *positions, const adi_hip_rows *output);
+
+/* A pool of pages of `page_size` cache entries each, an entry `heads` keys
+ * and values of head_size elements: entry e of page p, head h is at p
+ * page_stride + e entry_stride + h head_stride (elements) of keys and of
+ * values. So [page][entry][head][size], [page][head][entry][size] and pools
+ * inside larger arrays are all one descriptor; a contiguous cache of
+ * full_attention_forward (src/executor.cpp:332-418) is a pool whose pages lie
+ * end to end. */
+typedef struct {
+    uint32_t type;      /* ADI_HIP_F32, ADI_HIP_F16, ADI_HIP_BF16 */
+    uint32_t heads;     /* KV heads, at least 1 */
+    uint32_t head_size; /* 64, 128 or 256 */
+    uint32_t page_size; /* a power of two, 8 to 4096 */
+    uint32_t pages;     /* at least 1 */
+    void *keys;         /* 16-byte aligned, the strides multiples of 16 bytes */
+    void *values;
+    uint64_t page_stride, entry_stride, head_stride;
+} adi_hip_paged_cache;
+
+/* The sequences of one step: sequence s has the new rows offsets[s] ..
+ * offsets[s + 1] - 1 of the row arrays and lengths[s] entries, its new ones
+ * included, entry p in page table[s][p / page_size] at p % page_size. Its
+ * i-th of n new tokens is at position lengths[s] - n + i; one before position
+ * 0 (a length below n: padding in front) has no entry, sees nothing, and its
+ * query is turned to position 0. Rows behind the last sequence's belong to none.
+ *
+ * The arrays are read on the device, so a captured call replays with what
+ * they hold then. The host values bound them: a sequence with more than
+ * max_tokens rows or max_length entries is appended nowhere and its
+ * attention is NaN; an entry whose page number is not below `pages` is not
+ * written, and rows that see it are NaN. */
+typedef struct {
+    uint32_t sequences;
+    uint32_t tokens;         /* rows of the row arrays, below 2^30 */
+    uint32_t max_tokens;     /* new rows of a sequence at most */
+    uint32_t max_length;     /* entries of a sequence at most, below 2^28 */
+    const uint32_t *offsets; /* DEVICE [sequences + 1], ascending, at most tokens */
+    const uint32_t *lengths; /* DEVICE [sequences] */
+    const uint32_t *table;   /* DEVICE [sequences][table_stride] */
+    uint32_t table_stride;   /* at least max_length / page_size, rounded up */
+} adi_hip_paged_batch;
+
+/* On the host, no GPU needed: checks a cache's and a batch's fields as the
+ * calls below do, and the contents of offsets, lengths and table, HOST arrays
+ * here, against them: ascending offsets, max_tokens and max_length, and the
+ * page numbers of the entries below each length. ADI_HIP_INVALID_ARGUMENT
+ * with the message in adi_hip_last_error(NULL). The pointers keys and values are
+ * checked for alignment only. */
+int adi_hip_paged_check(const adi_hip_paged_cache *cache, const adi_hip_paged_batch *batch);
+
+/* Appends the batch's new keys and values to their sequences' pages, the key
+ * (and query) half of full_attention_forward before its attention
+ * (src/executor.cpp:376-400) for rows of many sequences: per head an RMS norm
+ * with a weight (where key_norm is given), x / sqrt(mean x^2 + epsilon)
+ * (weight_offset + w), then the rotation to the token's position (where rope
+ * is given), in 32 bits, rounded once to the cache's type; values are only
+ * rounded. With query_heads above 0 the queries are normalized and turned
+ * alike into queries_out (which may be `queries`: same data and strides).
+ * Other entries of the pool stay as they are, and so do query rows of no
+ * sequence. Query rows of a sequence over the batch's bounds are NaN.
+ *
+ * Rows and cache types: f32 rows into an f32 or bf16 cache, else one type for
+ * both. Rows are 16-byte aligned, their strides multiples of 16 bytes; rotary is
+ * at most head_size. Two sequences of a step must not append to one entry. */
+typedef struct {
+    const adi_hip_rope *rope;   /* may be NULL */
+    adi_hip_rows keys, values;  /* [tokens][heads][head_size] */
+    const uint16_t *key_norm;   /* bf16 [head_size], DEVICE; may be NULL */
+    uint32_t query_heads;       /* 0: no queries */
+    adi_hip_rows queries, queries_out;
+    const uint16_t *query_norm; /* may be NULL */
+    float weight_offset, epsilon;
+} adi_hip_paged_append_arguments;
+int adi_hip_paged_append(adi_hip_context *ctx, const adi_hip_paged_cache *cache,
+                         const adi_hip_paged_batch *batch,
+                         const adi_hip_paged_append_arguments *arguments);
+
+/* Device memory in which attention calls join the parts of a long history:
+ * `bytes` (0: 64 MiB; at least 1 MiB), allocated here, so that a call never
+ * allocates and may be captured. Calls with one workspace run one after another
+ * (one stream, or ordered by the caller): two captured graphs that may run at
+ * once need one each. Destroying it waits for the device. */
+typedef struct adi_hip_paged_workspace adi_hip_paged_workspace;
+int adi_hip_paged_workspace_create(adi_hip_context *ctx, size_t bytes,
+                                   adi_hip_paged_workspace **out);
+void adi_hip_paged_workspace_destroy(adi_hip_paged_workspace *workspace);
+
+/* Attention of the batch's rows over their sequences' pages (which hold the
+ * rows' own entries already: adi_hip_paged_append first), grouped_query_online_
+ * attention (src/attention.cpp:40) for many sequences at once, single tokens and
+ * chunks together: query head h of the token at position p reads KV head h /
+ * (query_heads / heads), entries max(0, p - window + 1) .. p (window 0: from 0),
+ *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale (q . k_j - max_j q . k_j)),
+ * times sigmoid(gate) where a gate is given. A row that sees no entry is 0.
+ * Values that are not finite in entries a row does not see have no effect on it;
+ * in entries it sees they make its outputs infinite or NaN.
+ *
+ * Rows and cache types: f32 rows over an f32 or bf16 cache, else f16 or
+ * bf16 for both (queries, gate and outputs have one type). f32 rows get
+ * products of 32-bit accuracy; f16 and bf16 rows round the weights w_j to the
+ * type (sums in 32 bits). Scores must stay within a float. query_heads is a multiple
+ * of heads, at most 256 times it. The outputs overlap neither queries nor gate. Rows of no sequence
+ * stay as they are. */
+typedef struct {
+    uint32_t query_heads;
+    adi_hip_rows queries;  /* [tokens][query_heads][head_size] */
+    adi_hip_rows outputs;
+    adi_hip_rows gate;     /* data NULL: none */
+    float scale;           /* positive; 0: 1 / sqrt(head_size) */
+    uint32_t window;       /* 0: none */
+} adi_hip_paged_attention_arguments;
+int adi_hip_paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache,
+                            const adi_hip_paged_batch *batch,
+                            const adi_hip_paged_attention_arguments *arguments,
+                            adi_hip_paged_workspace *workspace);
 
 /* ---- kernel profiling ----------------------------------------------------- */
 
