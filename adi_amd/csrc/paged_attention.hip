@@ -39,8 +39,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kStepRows = 16;    // of a KV head, k_paged_step
 constexpr uint32_t kStepKeys = 32;    // a wave's tile
-constexpr uint32_t kChunkRows = 128;  // of a block, k_paged_chunk
-constexpr uint32_t kChunkKeys = 32;   // a block's tile
 constexpr uint32_t kSpanUnit = 128;   // parts of a history are multiples of this
 constexpr float kNegative = -__builtin_huge_valf();
 
@@ -48,10 +46,10 @@ struct AttendArgs {
     PagedView c;
     RowsView queries, outputs, gate;
     float log2_scale;     // scale log2 e
+    float slack;          // kSlack / log2_scale
     uint32_t window;
     uint32_t group;       // query heads of a KV head
     uint32_t span, parts; // entries of a part of a history, parts at most
-    uint32_t tiles;       // k_paged_chunk: row tiles of a sequence at most
     float *partial;       // [part][token][head][D + 4]: sums, maximum, denominator (parts > 1)
 };
 
@@ -69,7 +67,13 @@ __device__ __forceinline__ int32_t base_of(const AttendArgs &a, int32_t first_po
     return a.window == 0u || first <= 0 ? 0 : first & ~static_cast<int32_t>(kSpanUnit - 1u);
 }
 
-// exp2(log2_scale (s - m)), s not above m: for f32 rows the difference is taken
+// How far (in powers of two of a weight) a row's scores may pass the level its
+// sums are held at before they are rescaled to a new one: random scores pass
+// their running maximum every few tiles, so the rescaling would be a third of the
+// vector work; a weight of 2^8 is as exact as one of 1.
+constexpr float kSlack = 8.0f;
+
+// exp2(log2_scale (s - m)), s at most kSlack above m: for f32 rows the difference is taken
 // first, so that its rounding is relative to it; for 16-bit rows in one
 // multiply-add.
 template <bool EXACT>
@@ -91,22 +95,36 @@ __device__ __forceinline__ uint32_t pack(float x, float y) {
     }
 }
 
-// Two floats as pairs of 16-bit pieces: one, rounded to nearest, or three whose
-// sum they are, exactly (an infinity or NaN is its first piece).
+// Two floats as pairs of 16-bit pieces: one, rounded to nearest; three bf16
+// pieces whose sum they are, exactly (an infinity gives NaN); or two f16 pieces,
+// 22 bits, of values scaled to f16's range.
 template <typename T, uint32_t N>
 __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[N]) {
     if constexpr (N == 1) {
         out[0] = pack<T>(x, y);
+    } else if constexpr (N == 2) {
+        const f32x2 v = {x, y};
+        const f16x2 hi = __builtin_convertvector(v, f16x2);
+        out[0] = __builtin_bit_cast(uint32_t, hi);
+        out[1] = pack<T>(x - static_cast<float>(hi.x), y - static_cast<float>(hi.y));
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) {
             const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
             out[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-            const float ra = x - __uint_as_float(a & 0xFFFF0000u), rb = y - __uint_as_float(b & 0xFFFF0000u);
-            x = (a & 0x7F800000u) == 0x7F800000u ? 0.0f : ra;
-            y = (b & 0x7F800000u) == 0x7F800000u ? 0.0f : rb;
+            x -= __uint_as_float(a & 0xFFFF0000u);
+            y -= __uint_as_float(b & 0xFFFF0000u);
         }
     }
+}
+
+// The power of two that brings values of a largest magnitude of these float bits
+// to 2^14 .. 2^15, as an exponent (2^126 at most), and what takes it back.
+__device__ __forceinline__ uint32_t scale_exponent(uint32_t largest) { return min(268u - (largest >> 23), 253u); }
+__device__ __forceinline__ float scale_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
+__device__ __forceinline__ float unscale_of(uint32_t exponent) { return __uint_as_float((254u - exponent) << 23); }
+__device__ __forceinline__ uint32_t magnitude(uint32_t largest, float v) {
+    return max(largest, __float_as_uint(v) & 0x7FFFFFFFu);
 }
 
 template <typename T>
@@ -130,11 +148,12 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     }
 }
 
-// The piece products of a K step, smallest first.
+// The piece products of a K step, smallest first: all down to 2^-16 of a product
+// of three pieces (of 8 bits), or 2^-11 of two (of 11).
 template <typename T, uint32_t A, uint32_t B, typename C>
 __device__ __forceinline__ C product(const u32x4 (&a)[A], const u32x4 (&b)[B], C c) {
 #pragma unroll
-    for (int32_t order = 2; order >= 0; --order) {
+    for (int32_t order = A == 2u ? 1 : 2; order >= 0; --order) {
 #pragma unroll
         for (int32_t i = 0; i < static_cast<int32_t>(A); ++i) {
             const int32_t j = order - i;
@@ -172,6 +191,19 @@ __device__ __forceinline__ Page page_of(const PagedView &c, const uint32_t *tabl
     return {(bad ? 0u : page) * c.page_stride + (entry & ((1u << c.page_shift) - 1u)) * c.entry_stride, bad};
 }
 
+// The weight of an entry for a row at its maximum so far, outside the tiles' way:
+// for the few entries that hold values that are not finite.
+template <typename T, typename R, uint32_t D, bool EXACT>
+__device__ __forceinline__ float odd_weight(const AttendArgs &a, const uint32_t *table, const T *keys, const R *query,
+                                         uint32_t entry, float maximum) {
+    const T *const key = keys + page_of(a.c, table, entry).at;
+    float score = 0.0f;
+    for (uint32_t d = 0; d < D; ++d) {
+        score = fmaf(static_cast<float>(query[d]), static_cast<float>(key[d]), score);
+    }
+    return weight_of<EXACT>(score, maximum == kNegative ? 0.0f : maximum, a.log2_scale);
+}
+
 // N consecutive outputs of a row, gated.
 template <typename R, uint32_t N>
 __device__ __forceinline__ void store_output(const AttendArgs &a, uint32_t token, uint32_t head, uint32_t at,
@@ -202,7 +234,7 @@ __device__ __forceinline__ void store_output(const AttendArgs &a, uint32_t token
 template <typename R, uint32_t D>
 __device__ __forceinline__ void fill_rows(const AttendArgs &a, const SequenceRows &s, uint32_t kv) {
     const uint64_t items = static_cast<uint64_t>(s.count) * a.group * (D / 4u);
-    for (uint64_t i = threadIdx.x; i < items; i += kThreads) {
+    for (uint64_t i = threadIdx.x; i < items; i += blockDim.x) {
         const uint32_t row = static_cast<uint32_t>(i / (D / 4u)), at = static_cast<uint32_t>(i % (D / 4u)) * 4u;
         const float v = s.over ? __builtin_nanf("") : 0.0f;
         float out[4] = {v, v, v, v};
@@ -303,7 +335,14 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
             sums[i][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
-    float maximum = kNegative, denominator = 0.0f;
+    // the level of the row's weights (kNegative before its first score), and the
+    // score from which it is raised
+    float maximum = kNegative, limit = kNegative, denominator = 0.0f;
+    // a tile that some row does not see whole
+    const auto edge_tile = [&](int32_t first) {
+        return first + static_cast<int32_t>(kKeys) > first_position + 1 || first < all_from;
+    };
+    bool odd_tile = false;
 
     for (int32_t first = begin + static_cast<int32_t>(wave * kKeys); first < end; first += 4 * kKeys) {
         // Key operands: row i of A is key first + kHeld (i / 4) + i % 4 (+ 4
@@ -377,9 +416,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
             }
         }
         const int32_t own_first = first + static_cast<int32_t>(kHeld * g);  // the lane's keys
-        // a tile that some row does not see whole (uniform but for bad pages)
-        const bool edge = first + static_cast<int32_t>(kKeys) > first_position + 1 || first < all_from;
-        bool careful = false;
+        const bool edge = edge_tile(first);
         if (__any(edge || value_page.bad)) {
             bool odd = false;
 #pragma unroll
@@ -395,16 +432,20 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
 #pragma unroll
                     for (uint32_t w = 0; w < kWords; ++w) {
                         held[i][k][w] = any ? held[i][k][w] : 0;
-                        if constexpr (kFloat) {
-                            odd |= odd_float(held[i][k][w]);
-                        } else {
-                            odd |= odd_pair<T>(held[i][k][w]);
+                        // (with one token every row sees the same entries)
+                        if (s.count > 1u) {
+                            if constexpr (kFloat) {
+                                odd |= odd_float(held[i][k][w]);
+                                held[i][k][w] = odd_float(held[i][k][w]) ? 0.0f : held[i][k][w];
+                            } else {
+                                odd |= odd_pair<T>(held[i][k][w]);
+                                held[i][k][w] = clean_pair<T>(held[i][k][w]);
+                            }
                         }
                     }
                 }
             }
-            // with one token every row sees the same entries
-            careful = s.count > 1u && __any(odd);
+            odd_tile |= __any(odd) != 0;
         }
         float top = score[0];
 #pragma unroll
@@ -413,10 +454,12 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
         }
         top = fmaxf(top, lane_xor<16>(top));
         top = fmaxf(top, lane_xor<32>(top));
-        if (__any(top > maximum)) {
-            const float next = fmaxf(maximum, top);
-            const float factor = next == kNegative ? 1.0f : weight_of<P == 3>(maximum, next, args.log2_scale);
-            maximum = next;
+        if (__any(top > limit)) {
+            // (a row's level does not depend on the wave's other rows)
+            const bool raised = top > limit;
+            const float factor = raised ? weight_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
+            maximum = raised ? top : maximum;
+            limit = raised ? top + args.slack : limit;
             denominator *= factor;
 #pragma unroll
             for (uint32_t i = 0; i < kGroups; ++i) {
@@ -431,54 +474,6 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
         for (uint32_t k = 0; k < kHeld; ++k) {
             score[k] = weight_of<P == 3>(score[k], level, args.log2_scale);
             denominator += score[k];
-        }
-        if (careful) {
-            // Entries with infinities or NaN of which some rows see only a
-            // part: their values are taken out of the products and added for the
-            // rows that see them.
-            for (uint32_t from = 0; from < 4u; ++from) {
-#pragma unroll
-                for (uint32_t k = 0; k < kHeld; ++k) {
-                    const int32_t entry = first + static_cast<int32_t>(kHeld * from + k);
-                    const float weight = __shfl(score[k], static_cast<int>(from * 16u + c));
-                    const bool visible = entry <= position && entry >= oldest;
-#pragma unroll
-                    for (uint32_t i = 0; i < kGroups; ++i) {
-#pragma unroll
-                        for (uint32_t n = 0; n < kSide; ++n) {
-#pragma unroll
-                            for (uint32_t r = 0; r < 4u; ++r) {
-                                // row r of the lane's results is the chunk of lane 4 g + r
-                                const int source = static_cast<int>(from * 16u + 4u * g + r);
-                                float v;
-                                if constexpr (kFloat) {
-                                    v = __shfl(held[i][k][n], source);
-                                } else {
-                                    const uint32_t pair = __shfl(held[i][k][n / 2u], source);
-                                    const uint16_t bits = static_cast<uint16_t>(n & 1u ? pair >> 16 : pair);
-                                    v = static_cast<float>(__builtin_bit_cast(T, bits));
-                                }
-                                sums[i][n][r] += visible && odd_float(v) ? v * weight : 0.0f;
-                            }
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < kGroups; ++i) {
-#pragma unroll
-                for (uint32_t k = 0; k < kHeld; ++k) {
-                    constexpr uint32_t kWords = sizeof(Chunk) / 4u;
-#pragma unroll
-                    for (uint32_t w = 0; w < kWords; ++w) {
-                        if constexpr (kFloat) {
-                            held[i][k][w] = odd_float(held[i][k][w]) ? 0.0f : held[i][k][w];
-                        } else {
-                            held[i][k][w] = clean_pair<T>(held[i][k][w]);
-                        }
-                    }
-                }
-            }
         }
         if constexpr (kFloat) {
 #pragma unroll
@@ -519,6 +514,31 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
         }
     }
 
+    if (odd_tile) {
+        // Values that are not finite, in tiles of which some rows see only a
+        // part: the products left them out, the rows that see them get them.
+        for (int32_t first = begin + static_cast<int32_t>(wave * kKeys); first < end; first += 4 * kKeys) {
+            for (int32_t entry = first; edge_tile(first) && entry < min(first + static_cast<int32_t>(kKeys), end);
+                 ++entry) {
+                const float weight = odd_weight<T, R, D, P == 3>(args, table, keys, query, entry, maximum);
+                const bool visible = entry <= position && entry >= oldest;
+                const Page page = page_of(cache, table, entry);
+                const T *const value = values + page.at;
+#pragma unroll
+                for (uint32_t i = 0; i < kGroups; ++i) {
+#pragma unroll
+                    for (uint32_t n = 0; n < kSide; ++n) {
+#pragma unroll
+                        for (uint32_t r = 0; r < 4u; ++r) {
+                            const float v = static_cast<float>(value[16u * kSide * i + kSide * (4u * g + r) + n]);
+                            sums[i][n][r] += visible && !page.bad && odd_float(v) ? v * weight : 0.0f;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
     // the row's lanes' parts of the denominator, then the waves
     denominator += lane_xor<16>(denominator);
     denominator += lane_xor<32>(denominator);
@@ -550,7 +570,6 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
         }
     }
     __syncthreads();
-    const bool whole = args.parts == 1u;
     for (uint32_t i = t; i < rows * (D / 4u); i += kThreads) {
         const uint32_t r = i / (D / 4u), at = i % (D / 4u) * 4u;
         float top = kNegative;
@@ -568,8 +587,15 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
             sum += *reinterpret_cast<const f32x4 *>(&lds.sums[w][r][at]);
         }
         const uint32_t row_token = s.first + r / args.group, row_head = kv * args.group + r % args.group;
-        if (whole) {
-            const bool none = first_position + static_cast<int32_t>(r / args.group) < 0;
+        // a row whose entries are all in this part is done
+        const int32_t place = first_position + static_cast<int32_t>(r / args.group);
+        const int32_t from = window == 0 ? 0 : max(0, place - window + 1);
+        const int32_t part_end = begin + static_cast<int32_t>(args.span);
+        const bool none = place < 0;
+        if (none ? part != 0u : place < begin || from >= part_end) {
+            continue;  // the part holds nothing the row sees
+        }
+        if (none || (from >= begin && place < part_end)) {
             float out[4];
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k) {
@@ -589,17 +615,18 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
 
 // ---- joining the parts of a history -------------------------------------------
 
-// Block (token, query head), a thread a dimension.
+// A wave a row (token, query head) of more than one part: lane l takes the
+// factors of parts l, l + 64, ... and dimensions D / 64 l .. of every part.
 template <typename R, uint32_t D, bool EXACT>
-__global__ __launch_bounds__(D) void k_paged_join(AttendArgs args) {
+__global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
+    constexpr uint32_t kSide = D / 64u;
     const PagedView &cache = args.c;
-    const uint32_t heads = cache.heads * args.group;
+    const uint32_t heads = cache.heads * args.group, lane = threadIdx.x & 63u;
     const uint64_t rows = static_cast<uint64_t>(cache.tokens) * heads;
-    for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    for (uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4ull) {
         const uint32_t token = static_cast<uint32_t>(row / heads), head = static_cast<uint32_t>(row % heads);
         uint32_t sequence = 0;
         for (uint32_t s = 0; s < cache.sequences; s += 64u) {
-            const uint32_t lane = threadIdx.x & 63u;
             const bool before = s + lane < cache.sequences && cache.offsets[s + lane + 1u] <= token;
             const uint32_t ended = static_cast<uint32_t>(__popcll(__ballot(before)));
             sequence += ended;
@@ -619,77 +646,191 @@ __global__ __launch_bounds__(D) void k_paged_join(AttendArgs args) {
         const int32_t base = base_of(args, first_position);
         const int32_t window = static_cast<int32_t>(args.window);
         const int32_t oldest = window == 0 ? 0 : max(0, position - window + 1);
-        float sum = 0.0f, total = 0.0f, top = kNegative;
-        if (position >= 0) {
-            const uint32_t from = static_cast<uint32_t>(oldest - base) / args.span;
-            const uint32_t to = static_cast<uint32_t>(position - base) / args.span;
-            for (uint32_t p = from; p <= to; ++p) {
-                top = fmaxf(top, partial_row<D>(args, p, token, head)[D]);
-            }
-            for (uint32_t p = from; p <= to; ++p) {
-                const float *part = partial_row<D>(args, p, token, head);
-                const float factor =
-                    part[D] == kNegative && top == kNegative ? 1.0f : weight_of<EXACT>(part[D], top, args.log2_scale);
-                total += part[D + 1u] * factor;
-                sum += part[threadIdx.x] * factor;
+        const uint32_t from = static_cast<uint32_t>(oldest - base) / args.span;
+        const uint32_t to = position < 0 ? from : static_cast<uint32_t>(position - base) / args.span;
+        if (from == to) {
+            continue;  // (written by its one part)
+        }
+        float top = kNegative;
+        for (uint32_t p = from + lane; p <= to; p += 64u) {
+            top = fmaxf(top, partial_row<D>(args, p, token, head)[D]);
+        }
+        top = fmaxf(top, lane_xor<1>(top));
+        top = fmaxf(top, lane_xor<2>(top));
+        top = fmaxf(top, lane_xor<4>(top));
+        top = fmaxf(top, lane_xor<8>(top));
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
+        float total = 0.0f, sum[kSide];
+#pragma unroll
+        for (uint32_t k = 0; k < kSide; ++k) {
+            sum[k] = 0.0f;
+        }
+        struct alignas(4u * kSide) Side {
+            float v[kSide];
+        };
+#pragma unroll 8
+        for (uint32_t p = from; p <= to; ++p) {
+            const float *part = partial_row<D>(args, p, token, head);
+            const float m = part[D], d = part[D + 1u];
+            const Side v = *reinterpret_cast<const Side *>(part + kSide * lane);
+            const float factor = m == kNegative && top == kNegative ? 1.0f : weight_of<EXACT>(m, top, args.log2_scale);
+            total += d * factor;
+#pragma unroll
+            for (uint32_t k = 0; k < kSide; ++k) {
+                sum[k] += v.v[k] * factor;
             }
         }
-        float out[1] = {position < 0 ? 0.0f : sum / total};
-        store_output<R, 1>(args, token, head, threadIdx.x, out);
+        const float scale = 1.0f / total;
+#pragma unroll
+        for (uint32_t k = 0; k < kSide; ++k) {
+            sum[k] *= scale;
+        }
+        store_output<R, kSide>(args, token, head, kSide * lane, sum);
     }
 }
 
 // ---- more rows ----------------------------------------------------------------
 
-// LDS places: 16-byte pieces of a row of D 16-bit values are permuted so that
-// the reads of a phase fall on different banks: keys, where 16 rows are read at
-// one piece, by the row; values, where four rows are read at 64 bytes, by four
-// pieces. A row of 64 values is half the banks, so two rows share a turn.
-template <uint32_t D>
+// The shapes of k_paged_chunk: rows of a wave (the columns of its matrix
+// products, 32 or 16), waves, keys of a tile, tiles in LDS at once, blocks a CU.
+template <uint32_t ROWS, uint32_t WAVES, uint32_t KEYS, uint32_t BUFFERS, uint32_t BLOCKS>
+struct ChunkShape {
+    static constexpr uint32_t kRows = ROWS, kWaves = WAVES, kKeys = KEYS, kBuffers = BUFFERS, kBlocks = BLOCKS;
+};
+template <typename T, typename R, uint32_t D>
+struct ChunkOf {
+    // 16-bit rows: 32 rows a wave, so that an operand read from LDS feeds as
+    // many products as the LDS can keep up with
+    using Shape = ChunkShape<32, 4, D == 64 ? 64 : 32, 2, D == 256 ? 1 : 2>;
+};
+template <typename T, uint32_t D>
+struct ChunkOf<T, float, D> {
+    // f32 rows: three pieces of a query, of which 16 rows a wave leave room for
+    // two waves a SIMD
+    using Shape = ChunkShape<16, 8, 32, std::is_same_v<T, float> ? 1 : 2, 1>;
+};
+template <typename T, typename R, uint32_t D>
+constexpr uint32_t chunk_rows() {
+    using Shape = typename ChunkOf<T, R, D>::Shape;
+    return Shape::kRows * Shape::kWaves;
+}
+
+// LDS places: the 16-byte pieces of an entry's D 16-bit values are permuted so
+// that the reads of a phase fall on different banks. Keys: the 16 entries that a
+// phase's lanes read at one piece get different turns. Values: the entries that
+// a transposing read's half wave reads side by side, four at 64 bytes (32
+// rows a wave) or eight at 32 bytes (16). A row of 64 values is half the banks,
+// so two rows share a turn.
+template <uint32_t D, uint32_t ROWS>
 __device__ __forceinline__ uint32_t key_place(uint32_t row, uint32_t piece) {
-    const uint32_t turn = D == 64u ? (row >> 1) & 7u : row & 15u;
+    uint32_t turn;
+    if constexpr (ROWS == 32) {
+        turn = D == 64u ? (row >> 1) & 7u : row & 15u;
+    } else {
+        turn = D == 64u ? (row >> 1 & 1u) | (row >> 3 & 3u) << 1 : (row & 3u) | (row >> 3 & 3u) << 2;
+    }
     return row * (D * 2u) + ((piece ^ turn) << 4);
 }
-template <uint32_t D>
+template <uint32_t D, uint32_t ROWS>
 __device__ __forceinline__ uint32_t value_place(uint32_t row, uint32_t piece) {
-    const uint32_t turn = D == 64u ? (row & 2u) << 1 : (row & 3u) << 2;
+    uint32_t turn;
+    if constexpr (ROWS == 32) {
+        turn = D == 64u ? (row & 2u) << 1 : (row & 3u) << 2;
+    } else {
+        turn = D == 64u ? (row & 2u) | (row >> 3 & 1u) << 2 : (row & 3u) << 1 | (row >> 3 & 1u) << 3;
+    }
     return row * (D * 2u) + ((piece ^ turn) << 4);
 }
 
-// Block (row tile, KV head, part, sequence): 128 rows, 32 a wave, lane l row
-// l % 32 and half h = l / 32.
 template <typename T, typename R, uint32_t D>
-__global__ __launch_bounds__(kThreads, 1) void k_paged_chunk(AttendArgs args) {
+constexpr size_t chunk_lds() {
+    using Shape = typename ChunkOf<T, R, D>::Shape;
+    constexpr size_t pieces = std::is_same_v<T, float> ? 5 : 2;
+    return pieces * Shape::kBuffers * Shape::kKeys * D * 2 + 16 + 2 * Shape::kBuffers * Shape::kKeys * 4 +
+           Shape::kWaves * 64 * 4;
+}
+
+// Block (row tile, KV head, part, sequence). Lane l of a wave is row l % ROWS
+// of the wave's and piece l / ROWS of its keys.
+template <typename T, typename R, uint32_t D>
+__global__ __launch_bounds__((ChunkOf<T, R, D>::Shape::kWaves * 64u), (ChunkOf<T, R, D>::Shape::kBlocks *
+                                                                     ChunkOf<T, R, D>::Shape::kWaves / 4u))
+void k_paged_chunk(AttendArgs args) {
+    using Shape = typename ChunkOf<T, R, D>::Shape;
     constexpr bool kFloat = std::is_same_v<T, float>;
     using M = std::conditional_t<kFloat, __bf16, T>;  // the matrix cores' type
     constexpr uint32_t P = std::is_same_v<R, float> ? 3u : 1u;
     constexpr uint32_t Q = kFloat ? 3u : 1u;
-    constexpr uint32_t kPlane = kChunkKeys * D * 2u;
-    constexpr uint32_t kPieces = D / 8u;                                // of a row
-    constexpr uint32_t kLoads = kChunkKeys * kPieces / kThreads;        // a thread's pieces of a tile
-    static_assert(kChunkKeys * kPieces % kThreads == 0 || D == 32u);
+    // f32 keys: two f16 pieces of each, scaled by a power of two a row and a key
+    // (three products instead of six, and a query in two thirds of the registers)
+    using N = std::conditional_t<kFloat, _Float16, M>;
+    constexpr uint32_t QP = kFloat ? 2u : P, KP = kFloat ? 2u : 1u;
+    constexpr uint32_t W = Shape::kRows, kKeys = Shape::kKeys, kBlock = Shape::kWaves * 64u, kBuffers = Shape::kBuffers;
+    constexpr uint32_t kBlockRows = W * Shape::kWaves;
+    constexpr uint32_t kSub = kKeys / 32u;             // 32 keys at a time through the products
+    constexpr uint32_t kHeld = W == 32u ? 16u : 8u;    // a lane's keys of 32
+    constexpr uint32_t kStepDims = W == 32u ? 16u : 32u;
+    using Acc = std::conditional_t<W == 32u, f32x16, f32x4>;
+    constexpr uint32_t kRegisters = W == 32u ? 16u : 4u;
+    constexpr uint32_t kPlane = kKeys * D * 2u, kBuffer = (KP + Q) * kPlane;
+    constexpr uint32_t kPieces = D / 8u;                              // of an entry's key or value
+    constexpr uint32_t kLoads = 2u * kKeys * kPieces / kBlock;        // a thread's pieces of a tile
+    static_assert(2u * kKeys * kPieces % kBlock == 0 && kLoads >= 1u);
     extern __shared__ __align__(16) unsigned char lds[];
-    unsigned char *const key_lds = lds;
-    unsigned char *const value_lds = lds + Q * kPlane;
-    // the last tile with a value that is not finite, and with a bad page
-    volatile uint32_t *const odd = reinterpret_cast<volatile uint32_t *>(lds + 2u * Q * kPlane);
-    volatile uint32_t *const bad_key = odd + 4u;  // [kChunkKeys]
+    // whether a tile had a value that is not finite; each buffer's last tile with
+    // a bad page, and its entries
+    volatile uint32_t *const marks = reinterpret_cast<volatile uint32_t *>(lds + kBuffers * kBuffer);
+    volatile uint32_t *const bad_key = marks + 4u;                    // [kBuffers][kKeys]
+    // what takes the scores of a key back from its scale
+    float *const key_unscale = reinterpret_cast<float *>(lds + kBuffers * kBuffer) + 4u + kBuffers * kKeys;  // as bad_key
+    uint32_t *const page_ids = reinterpret_cast<uint32_t *>(key_unscale + kBuffers * kKeys);
     const PagedView &cache = args.c;
-    // the blocks of one (KV head, part, sequence) read the same entries: their
-    // number is a multiple of 8 or the group's, so they share an XCD (block b
-    // runs on XCD b % 8); the tiles with the longest histories come first
-    const uint32_t groups = cache.heads * args.parts * cache.sequences;
-    const uint32_t padded = groups < 8u ? groups : (groups + 7u) & ~7u;
-    const uint32_t which = blockIdx.x % padded, tile = args.tiles - 1u - blockIdx.x / padded;
-    if (which >= groups) {
+    // the blocks of one (KV head, part) of a sequence read the same entries: where
+    // there are 8 or more such pairs their number is rounded up to a multiple
+    // of 8, so that each stays on one XCD (block b runs on XCD b % 8)
+    const uint32_t pairs = cache.heads * args.parts;
+    const uint32_t padded = pairs < 8u ? pairs : (pairs + 7u) & ~7u;
+    const uint32_t which = blockIdx.x % padded;
+    if (which >= pairs) {
         return;
     }
-    const uint32_t kv = which % cache.heads, part = which / cache.heads % args.parts;
-    const uint32_t sequence = which / (cache.heads * args.parts);
+    const uint32_t kv = which % cache.heads, part = which / cache.heads;
+    // the row tiles of all sequences in order, those of a sequence from its last
+    // (the longest histories) on: this block's is found by a running sum over
+    // 64 sequences at a time (a block for each tile that max_tokens allows
+    // instead: 6144 of them for one chunk of 512 tokens beside 31 single ones,
+    // of which 5766 only wait for a CU)
+    uint32_t sequence = ~0u, tile = blockIdx.x / padded;
+    for (uint32_t first = 0; first < cache.sequences; first += 64u) {
+        const uint32_t own = first + (threadIdx.x & 63u);
+        uint32_t tiles = 0;
+        if (own < cache.sequences) {
+            const uint32_t a = min(cache.offsets[own], cache.tokens), b = min(cache.offsets[own + 1u], cache.tokens);
+            const uint32_t count = min(b > a ? b - a : 0u, cache.max_tokens);
+            tiles = (count * args.group + kBlockRows - 1u) / kBlockRows;
+        }
+        uint32_t sum = tiles;
+#pragma unroll
+        for (uint32_t d = 1; d < 64u; d *= 2u) {
+            const uint32_t below = __shfl_up(sum, d);
+            sum += (threadIdx.x & 63u) >= d ? below : 0u;
+        }
+        const uint64_t past = __ballot(sum > tile);
+        if (past != 0u) {
+            const int lane = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            sequence = first + static_cast<uint32_t>(lane);
+            tile = __shfl(sum, lane) - 1u - tile;
+            break;
+        }
+        tile -= __shfl(sum, 63);
+    }
+    if (sequence == ~0u) {
+        return;
+    }
+    sequence = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(sequence)));
+    tile = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tile)));
     const SequenceRows s = sequence_rows(cache, sequence);
-    if (s.count == 0u) {
-        return;
-    }
     if (s.over || s.length == 0u) {
         if (part == 0u && tile == 0u) {
             fill_rows<R, D>(args, s, kv);
@@ -697,311 +838,456 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_chunk(AttendArgs args) {
         return;
     }
     const uint32_t rows = s.count * args.group;
-    if (tile * kChunkRows >= rows) {
+    if (tile * kBlockRows >= rows) {
         return;
     }
     const uint32_t t = threadIdx.x, lane = t & 63u;
     const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(t >> 6)));
-    const uint32_t column = lane & 31u, half = lane >> 5;
+    const uint32_t column = lane % W, side = lane / W;
     const int32_t first_position = static_cast<int32_t>(s.length) - static_cast<int32_t>(s.count);
     const int32_t window = static_cast<int32_t>(args.window);
     const auto place = [&](uint32_t row) { return first_position + static_cast<int32_t>(row / args.group); };
     const auto from = [&](int32_t position) { return window == 0 ? 0 : max(0, position - window + 1); };
-    const uint32_t block_last = min((tile + 1u) * kChunkRows, rows) - 1u;
-    const int32_t block_low = place(tile * kChunkRows), block_high = place(block_last);
-    const uint32_t wave_row = tile * kChunkRows + wave * 32u;
+    const uint32_t block_last = min((tile + 1u) * kBlockRows, rows) - 1u;
+    const int32_t block_low = place(tile * kBlockRows), block_high = place(block_last);
+    const int32_t block_from = from(block_low), block_all = from(block_high);
+    const uint32_t wave_row = tile * kBlockRows + wave * W;
     const bool wave_live = wave_row < rows;
-    const int32_t wave_low = place(min(wave_row, rows - 1u)), wave_high = place(min(wave_row + 31u, rows - 1u));
+    const int32_t wave_low = place(min(wave_row, rows - 1u)), wave_high = place(min(wave_row + W - 1u, rows - 1u));
     const uint32_t row = min(wave_row + column, rows - 1u);
     const uint32_t token = s.first + row / args.group, head = kv * args.group + row % args.group;
     const int32_t position = place(row), oldest = from(position);
     // entries of the part that some row of the block sees
-    int32_t begin = base_of(args, first_position) + static_cast<int32_t>(part * args.span);
+    const int32_t base = base_of(args, first_position);
+    int32_t begin = base + static_cast<int32_t>(part * args.span);
     const int32_t end = min(begin + static_cast<int32_t>(args.span), block_high + 1);
-    begin = max(begin, from(block_low) & ~static_cast<int32_t>(kChunkKeys - 1u));
-    const bool whole = args.parts == 1u;
-    if (begin >= end && !whole) {
+    begin = max(begin, block_from & ~static_cast<int32_t>(kKeys - 1u));
+    if (begin >= end && (part != 0u || block_high >= 0)) {
         return;
     }
     const uint32_t *const table = cache.table + static_cast<uint64_t>(sequence) * cache.table_stride;
     const T *const keys = reinterpret_cast<const T *>(cache.keys) + kv * cache.head_stride;
     const T *const values = reinterpret_cast<const T *>(cache.values) + kv * cache.head_stride;
-    if (t < 2u) {
-        odd[t] = ~0u;
+    const R *const query = reinterpret_cast<const R *>(args.queries.data) + token * args.queries.token_stride +
+                           head * args.queries.head_stride;
+    if (t < 4u) {
+        marks[t] = ~0u;
     }
 
-    // the row's query: step j holds dimensions 16 j + 8 half + 0 .. 7
-    u32x4 query_pieces[D / 16u][P];
-    {
-        const R *const query = reinterpret_cast<const R *>(args.queries.data) + token * args.queries.token_stride +
-                               head * args.queries.head_stride + 8u * half;
-#pragma unroll
-        for (uint32_t j = 0; j < D / 16u; ++j) {
-            if constexpr (P == 1) {
-                query_pieces[j][0] = *reinterpret_cast<const u32x4 *>(query + 16u * j);
-            } else {
-                const f32x4 lo = *reinterpret_cast<const f32x4 *>(query + 16u * j);
-                const f32x4 hi = *reinterpret_cast<const f32x4 *>(query + 16u * j + 4u);
-#pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k) {
-                    uint32_t pieces[P];
-                    k < 2u ? split<M>(lo[2u * k], lo[2u * k + 1u], pieces)
-                           : split<M>(hi[2u * k - 4u], hi[2u * k - 3u], pieces);
-#pragma unroll
-                    for (uint32_t p = 0; p < P; ++p) {
-                        query_pieces[j][p][k] = pieces[p];
-                    }
-                }
-            }
+    // the numbers of kBlock pages at a time
+    uint32_t first_page = 0;
+    const auto fill_pages = [&](int32_t entry) {
+        first_page = static_cast<uint32_t>(entry) >> cache.page_shift;
+        const uint32_t id = first_page + t;
+        uint32_t page = ~0u;
+        if (id <= static_cast<uint32_t>(end - 1) >> cache.page_shift) {
+            page = table[id];
         }
-    }
+        page_ids[t] = page < cache.pages ? page : ~0u;
+    };
 
-    // A tile passes through registers: piece t + 256 i of it, of row piece /
-    // kPieces.
+    // A tile passes through registers: pieces t + kBlock i of its keys, then
+    // values, piece p of entry p / kPieces.
     using Piece = std::conditional_t<kFloat, f32x4, u32x4>;
     constexpr uint32_t kWide = kFloat ? 2u : 1u;
-    Piece key_in[kLoads][kWide], value_in[kLoads][kWide];
+    Piece in[kLoads][kWide];
     uint32_t bad_in = 0;
+    const auto entry_of = [&](uint32_t i) { return (t + kBlock * i) % (kKeys * kPieces) / kPieces; };
+    const auto is_value = [&](uint32_t i) { return t + kBlock * i >= kKeys * kPieces; };
+    const uint32_t page_mask = (1u << cache.page_shift) - 1u;
     const auto load = [&](int32_t first) {
         bad_in = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t piece = t + kThreads * i, at = piece % kPieces * 8u;
-            const int32_t entry = first + static_cast<int32_t>(piece / kPieces);
-            Page page{0, false};
+            const int32_t entry = first + static_cast<int32_t>(entry_of(i));
+            uint64_t at = t % kPieces * 8u;
             if (entry < end) {
-                page = page_of(cache, table, entry);
+                const uint32_t page = page_ids[(static_cast<uint32_t>(entry) >> cache.page_shift) - first_page];
+                bad_in |= page == ~0u ? 1u << i : 0u;
+                at += (page == ~0u ? 0u : page) * cache.page_stride + (entry & page_mask) * cache.entry_stride;
             }
-            bad_in |= page.bad ? 1u << i : 0u;
+            const Piece *const piece = reinterpret_cast<const Piece *>((is_value(i) ? values : keys) + at);
 #pragma unroll
             for (uint32_t w = 0; w < kWide; ++w) {
-                key_in[i][w] = reinterpret_cast<const Piece *>(keys + page.at + at)[w];
-                value_in[i][w] = reinterpret_cast<const Piece *>(values + page.at + at)[w];
+                in[i][w] = piece[w];
             }
         }
     };
-    const auto stage = [&](int32_t first, bool edge) {
-        if (edge || bad_in != 0u) {
+    const auto edge_tile = [&](int32_t first) {
+        return first + static_cast<int32_t>(kKeys) > block_low + 1 || first < block_all;
+    };
+    const auto stage = [&](int32_t first, uint32_t buffer) {
+        unsigned char *const to = lds + buffer * kBuffer;
+        if (edge_tile(first) || bad_in != 0u) {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const uint32_t piece = t + kThreads * i;
-                const int32_t entry = first + static_cast<int32_t>(piece / kPieces);
+                const int32_t entry = first + static_cast<int32_t>(entry_of(i));
                 const bool bad = (bad_in >> i & 1u) != 0u;
-                const bool any = entry < end && entry >= from(block_low) && !bad;
-                bool seen = false;
+                if (bad) {
+                    marks[1u + buffer] = static_cast<uint32_t>(first);
+                }
+                if (is_value(i)) {
+                    const bool any = entry < end && entry >= block_from && !bad;
+                    bool seen = false;
 #pragma unroll
-                for (uint32_t w = 0; w < kWide; ++w) {
+                    for (uint32_t w = 0; w < kWide; ++w) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 4u; ++k) {
-                        value_in[i][w][k] = any ? value_in[i][w][k] : 0;
-                        if constexpr (kFloat) {
-                            seen |= odd_float(value_in[i][w][k]);
-                            value_in[i][w][k] = odd_float(value_in[i][w][k]) ? 0.0f : value_in[i][w][k];
-                        } else {
-                            seen |= odd_pair<T>(value_in[i][w][k]);
-                            value_in[i][w][k] = clean_pair<T>(value_in[i][w][k]);
+                        for (uint32_t k = 0; k < 4u; ++k) {
+                            in[i][w][k] = any ? in[i][w][k] : 0;
+                            if constexpr (kFloat) {
+                                seen |= odd_float(in[i][w][k]);
+                                in[i][w][k] = odd_float(in[i][w][k]) ? 0.0f : in[i][w][k];
+                            } else {
+                                seen |= odd_pair<T>(in[i][w][k]);
+                                in[i][w][k] = clean_pair<T>(in[i][w][k]);
+                            }
                         }
                     }
+                    if (seen) {
+                        marks[0] = 1u;
+                    }
                 }
-                if (seen) {
-                    odd[0] = static_cast<uint32_t>(first);
-                }
-                if (bad) {
-                    odd[1] = static_cast<uint32_t>(first);
-                }
-                if (piece % kPieces == 0u) {
-                    bad_key[piece / kPieces] = bad ? static_cast<uint32_t>(first) : ~0u;
+                if (t % kPieces == 0u && !is_value(i)) {
+                    bad_key[buffer * kKeys + entry_of(i)] = bad ? static_cast<uint32_t>(first) : ~0u;
                 }
             }
         }
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t piece = t + kThreads * i, entry = piece / kPieces, at = piece % kPieces;
+            const uint32_t entry = entry_of(i), piece = t % kPieces;
+            const uint32_t at = is_value(i) ? KP * kPlane + value_place<D, W>(entry, piece) : key_place<D, W>(entry, piece);
             if constexpr (kFloat) {
-                u32x4 k[Q], v[Q];
+                const auto store = [&](auto count, float scale) {
+                    constexpr uint32_t kCount = decltype(count)::value;
+                    using Kind = std::conditional_t<kCount == 2u, N, M>;
+                    u32x4 out[kCount];
 #pragma unroll
-                for (uint32_t n = 0; n < 4u; ++n) {
-                    uint32_t pieces[Q];
-                    split<M>(key_in[i][n / 2u][2u * n % 4u], key_in[i][n / 2u][2u * n % 4u + 1u], pieces);
+                    for (uint32_t n = 0; n < 4u; ++n) {
+                        uint32_t pieces[kCount];
+                        split<Kind>(in[i][n / 2u][2u * n % 4u] * scale, in[i][n / 2u][2u * n % 4u + 1u] * scale, pieces);
 #pragma unroll
-                    for (uint32_t p = 0; p < Q; ++p) {
-                        k[p][n] = pieces[p];
+                        for (uint32_t p = 0; p < kCount; ++p) {
+                            out[p][n] = pieces[p];
+                        }
                     }
-                    split<M>(value_in[i][n / 2u][2u * n % 4u], value_in[i][n / 2u][2u * n % 4u + 1u], pieces);
 #pragma unroll
-                    for (uint32_t p = 0; p < Q; ++p) {
-                        v[p][n] = pieces[p];
+                    for (uint32_t p = 0; p < kCount; ++p) {
+                        *reinterpret_cast<u32x4 *>(to + p * kPlane + at) = out[p];
                     }
-                }
+                };
+                if (is_value(i)) {
+                    store(std::integral_constant<uint32_t, Q>{}, 1.0f);
+                } else {
+                    uint32_t largest = 0;
 #pragma unroll
-                for (uint32_t p = 0; p < Q; ++p) {
-                    *reinterpret_cast<u32x4 *>(key_lds + p * kPlane + key_place<D>(entry, at)) = k[p];
-                    *reinterpret_cast<u32x4 *>(value_lds + p * kPlane + value_place<D>(entry, at)) = v[p];
+                    for (uint32_t w = 0; w < kWide; ++w) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 4u; ++k) {
+                            largest = magnitude(largest, in[i][w][k]);
+                        }
+                    }
+                    largest = max(largest, lane_xor_bits<1>(largest));
+                    largest = max(largest, lane_xor_bits<2>(largest));
+                    largest = max(largest, lane_xor_bits<4>(largest));
+                    if constexpr (kPieces > 8u) {
+                        largest = max(largest, lane_xor_bits<8>(largest));
+                    }
+                    if constexpr (kPieces > 16u) {
+                        largest = max(largest, lane_xor_bits<16>(largest));
+                    }
+                    const uint32_t exponent = scale_exponent(largest);
+                    if (piece == 0u) {
+                        key_unscale[buffer * kKeys + entry] = unscale_of(exponent);
+                    }
+                    store(std::integral_constant<uint32_t, KP>{}, scale_of(exponent));
                 }
             } else {
-                *reinterpret_cast<u32x4 *>(key_lds + key_place<D>(entry, at)) = key_in[i][0];
-                *reinterpret_cast<u32x4 *>(value_lds + value_place<D>(entry, at)) = value_in[i][0];
+                *reinterpret_cast<u32x4 *>(to + at) = in[i][0];
             }
         }
     };
 
-    f32x16 sums[D / 32u];
+    // the row's query: step j holds dimensions kStepDims j + 8 side + 0 .. 7
+    u32x4 query_pieces[D / kStepDims][QP];
+    float query_scale = 1.0f, query_unscale = 1.0f;
+    if constexpr (kFloat) {
+        uint32_t largest = 0;
 #pragma unroll
-    for (uint32_t m = 0; m < D / 32u; ++m) {
+        for (uint32_t j = 0; j < D / kStepDims; ++j) {
 #pragma unroll
-        for (uint32_t r = 0; r < 16u; ++r) {
+            for (uint32_t k = 0; k < 8u; ++k) {
+                largest = magnitude(largest, query[kStepDims * j + 8u * side + k]);
+            }
+        }
+        static_assert(!kFloat || W == 16u);
+        largest = max(largest, lane_xor_bits<16>(largest));
+        largest = max(largest, lane_xor_bits<32>(largest));
+        query_scale = scale_of(scale_exponent(largest));
+        query_unscale = unscale_of(scale_exponent(largest));
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < D / kStepDims; ++j) {
+        const R *const at = query + kStepDims * j + 8u * side;
+        if constexpr (P == 1) {
+            query_pieces[j][0] = *reinterpret_cast<const u32x4 *>(at);
+        } else {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(at) * query_scale;
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(at + 4u) * query_scale;
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                uint32_t pieces[QP];
+                k < 2u ? split<N>(lo[2u * k], lo[2u * k + 1u], pieces)
+                       : split<N>(hi[2u * k - 4u], hi[2u * k - 3u], pieces);
+#pragma unroll
+                for (uint32_t p = 0; p < QP; ++p) {
+                    query_pieces[j][p][k] = pieces[p];
+                }
+            }
+        }
+    }
+
+    Acc sums[D / W];
+#pragma unroll
+    for (uint32_t m = 0; m < D / W; ++m) {
+#pragma unroll
+        for (uint32_t r = 0; r < kRegisters; ++r) {
             sums[m][r] = 0.0f;
         }
     }
-    float maximum = kNegative, denominator = 0.0f;
-    // register r of a score tile is key 8 (r / 4) + 4 half + r % 4
-    const auto key_of = [&](uint32_t r) { return static_cast<int32_t>(8u * (r / 4u) + 4u * half + r % 4u); };
+    // the level of the row's weights (kNegative before its first score), and the
+    // score from which it is raised
+    float maximum = kNegative, limit = kNegative, denominator = 0.0f;
+    // a lane's keys of 32, and register r of sums[m]
+    const auto key_of = [&](uint32_t r) {
+        return W == 32u ? 8u * (r / 4u) + 4u * side + r % 4u : 8u * side + r;
+    };
+    const auto dimension_of = [&](uint32_t m, uint32_t r) {
+        return W == 32u ? 32u * m + 8u * (r / 4u) + 4u * side + r % 4u : 16u * m + 4u * side + r;
+    };
 
-    if (begin < end) {
-        load(begin);
-    }
-    for (int32_t first = begin; first < end; first += static_cast<int32_t>(kChunkKeys)) {
-        const bool edge = first + static_cast<int32_t>(kChunkKeys) > block_low + 1 || first < from(block_high);
-        __syncthreads();  // the last tile's reads (and the first's marks) are done
-        stage(first, edge);
-        __syncthreads();
-        if (first + static_cast<int32_t>(kChunkKeys) < end) {
-            load(first + static_cast<int32_t>(kChunkKeys));
+    const auto compute = [&](int32_t first, uint32_t buffer) {
+        if (!wave_live || first > wave_high || first + static_cast<int32_t>(kKeys) <= from(wave_low)) {
+            return;  // nothing of the tile is seen by the wave's rows
         }
-        if (!wave_live || first > wave_high || first + static_cast<int32_t>(kChunkKeys) <= from(wave_low)) {
-            continue;  // nothing of the tile is seen by the wave's rows
-        }
-        f32x16 score;
+        const unsigned char *const key_lds = lds + buffer * kBuffer;
+        const unsigned char *const value_lds = key_lds + KP * kPlane;
+        float score[kSub][kHeld];
 #pragma unroll
-        for (uint32_t r = 0; r < 16u; ++r) {
-            score[r] = 0.0f;
-        }
+        for (uint32_t b = 0; b < kSub; ++b) {
+            // with 16 rows a wave two products of 16 keys, interleaved so that
+            // a lane's eight results are eight keys in a row
+            constexpr uint32_t kProducts = W == 32u ? 1u : 2u;
 #pragma unroll
-        for (uint32_t j = 0; j < D / 16u; ++j) {
-            u32x4 k[Q];
+            for (uint32_t h = 0; h < kProducts; ++h) {
+                Acc acc;
 #pragma unroll
-            for (uint32_t p = 0; p < Q; ++p) {
-                k[p] = *reinterpret_cast<const u32x4 *>(key_lds + p * kPlane + key_place<D>(column, 2u * j + half));
+                for (uint32_t r = 0; r < kRegisters; ++r) {
+                    acc[r] = 0.0f;
+                }
+                const uint32_t entry = 32u * b + (W == 32u ? column : 8u * (column / 4u) + 4u * h + column % 4u);
+                u32x4 k[2][KP];
+                const auto read = [&](uint32_t j) {
+#pragma unroll
+                    for (uint32_t p = 0; p < KP; ++p) {
+                        k[j & 1u][p] = *reinterpret_cast<const u32x4 *>(
+                            key_lds + p * kPlane + key_place<D, W>(entry, kStepDims / 8u * j + side));
+                    }
+                };
+                read(0u);
+#pragma unroll
+                for (uint32_t j = 0; j < D / kStepDims; ++j) {
+                    if (j + 1u < D / kStepDims) {
+                        read(j + 1u);
+                    }
+                    acc = product<N>(k[j & 1u], query_pieces[j], acc);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (uint32_t r = 0; r < kRegisters; ++r) {
+                    score[b][h * kRegisters + r] = acc[r];
+                    if constexpr (kFloat) {
+                        score[b][h * kRegisters + r] =
+                            acc[r] * query_unscale * key_unscale[buffer * kKeys + 32u * b + key_of(h * kRegisters + r)];
+                    }
+                }
             }
-            score = product<M>(k, query_pieces[j], score);
         }
-        const bool bad_tile = odd[1] == static_cast<uint32_t>(first);
-        if (bad_tile || first + static_cast<int32_t>(kChunkKeys) > wave_low + 1 || first < from(wave_high)) {
+        const bool bad_tile = marks[1u + buffer] == static_cast<uint32_t>(first);
+        if (bad_tile || first + static_cast<int32_t>(kKeys) > wave_low + 1 || first < from(wave_high)) {
 #pragma unroll
-            for (uint32_t r = 0; r < 16u; ++r) {
-                const int32_t entry = first + key_of(r);
-                const bool visible = entry <= position && entry >= oldest;
-                const bool bad = bad_tile && bad_key[key_of(r)] == static_cast<uint32_t>(first);
-                score[r] = !visible ? kNegative : bad ? __builtin_nanf("") : score[r];
+            for (uint32_t b = 0; b < kSub; ++b) {
+#pragma unroll
+                for (uint32_t r = 0; r < kHeld; ++r) {
+                    const uint32_t key = 32u * b + key_of(r);
+                    const int32_t entry = first + static_cast<int32_t>(key);
+                    const bool visible = entry <= position && entry >= oldest;
+                    const bool bad = bad_tile && bad_key[buffer * kKeys + key] == static_cast<uint32_t>(first);
+                    score[b][r] = !visible ? kNegative : bad ? __builtin_nanf("") : score[b][r];
+                }
             }
         }
-        float top = score[0];
+        float top = score[0][0];
 #pragma unroll
-        for (uint32_t r = 1; r < 16u; ++r) {
-            top = fmaxf(top, score[r]);
+        for (uint32_t b = 0; b < kSub; ++b) {
+#pragma unroll
+            for (uint32_t r = 0; r < kHeld; ++r) {
+                top = fmaxf(top, score[b][r]);
+            }
+        }
+        if constexpr (W == 16u) {
+            top = fmaxf(top, lane_xor<16>(top));
         }
         top = fmaxf(top, lane_xor<32>(top));
-        if (__any(top > maximum)) {
-            const float next = fmaxf(maximum, top);
-            const float factor = next == kNegative ? 1.0f : weight_of<P == 3>(maximum, next, args.log2_scale);
-            maximum = next;
+        if (__any(top > limit)) {
+            // (a row's level does not depend on the wave's other rows)
+            const bool raised = top > limit;
+            const float factor = raised ? weight_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
+            maximum = raised ? top : maximum;
+            limit = raised ? top + args.slack : limit;
             denominator *= factor;
 #pragma unroll
-            for (uint32_t m = 0; m < D / 32u; ++m) {
+            for (uint32_t m = 0; m < D / W; ++m) {
                 sums[m] *= factor;
             }
         }
         const float level = maximum == kNegative ? 0.0f : maximum;
 #pragma unroll
-        for (uint32_t r = 0; r < 16u; ++r) {
-            score[r] = weight_of<P == 3>(score[r], level, args.log2_scale);
-            denominator += score[r];
-        }
+        for (uint32_t b = 0; b < kSub; ++b) {
 #pragma unroll
-        for (uint32_t u = 0; u < 2u; ++u) {
-            u32x4 weights[P];
+            for (uint32_t r = 0; r < kHeld; ++r) {
+                score[b][r] = weight_of<P == 3>(score[b][r], level, args.log2_scale);
+                denominator += score[b][r];
+            }
+            // steps of 16 keys (32 rows a wave) or 32
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                uint32_t pieces[P];
-                split<M>(score[8u * u + 2u * k], score[8u * u + 2u * k + 1u], pieces);
+            for (uint32_t u = 0; u < kHeld / 8u; ++u) {
+                u32x4 weights[P];
 #pragma unroll
-                for (uint32_t p = 0; p < P; ++p) {
-                    weights[p][k] = pieces[p];
+                for (uint32_t k = 0; k < 4u; ++k) {
+                    uint32_t pieces[P];
+                    split<M>(score[b][8u * u + 2u * k], score[b][8u * u + 2u * k + 1u], pieces);
+#pragma unroll
+                    for (uint32_t p = 0; p < P; ++p) {
+                        weights[p][k] = pieces[p];
+                    }
+                }
+                // the values transposed: lane i of 16 takes row i / 4 of four
+                // entries at dimension 4 (i % 4), and gets dimension i of the four
+                const uint32_t entry = 32u * b + (lane & 15u) / 4u + (W == 32u ? 16u * u + 4u * side : 8u * side);
+                const uint32_t next = entry + (W == 32u ? 8u : 4u);
+                const uint32_t dimension = (W == 32u ? (lane >> 4 & 1u) * 16u : 0u) + (lane & 3u) * 4u;
+                u32x4 v[2][Q];
+                const auto read = [&](uint32_t m) {
+#pragma unroll
+                    for (uint32_t p = 0; p < Q; ++p) {
+                        const uint32_t d = W * m + dimension;
+                        const auto four = [&](uint32_t e) {
+                            auto *at = (__attribute__((address_space(3))) s16x4 *)(
+                                value_lds + p * kPlane + value_place<D, W>(e, d / 8u) + d % 8u * 2u);
+                            return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at));
+                        };
+                        const u32x2 lo = four(entry), hi = four(next);
+                        v[m & 1u][p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                    }
+                };
+                read(0u);
+#pragma unroll
+                for (uint32_t m = 0; m < D / W; ++m) {
+                    if (m + 1u < D / W) {
+                        read(m + 1u);
+                    }
+                    sums[m] = product<M>(v[m & 1u], weights, sums[m]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            // lane i of 16 takes row i / 4 of four entries at 4 (i % 4), and
-            // gets dimension i of the four
-            const uint32_t entry = 16u * u + 4u * half + (lane & 15u) / 4u;
-            const uint32_t side = (lane >> 4 & 1u) * 16u + (lane & 3u) * 4u;
-#pragma unroll
-            for (uint32_t m = 0; m < D / 32u; ++m) {
-                u32x4 v[Q];
-#pragma unroll
-                for (uint32_t p = 0; p < Q; ++p) {
-                    const uint32_t d = 32u * m + side;
-                    const auto read = [&](uint32_t e) {
-                        auto *at = (__attribute__((address_space(3))) s16x4 *)(value_lds + p * kPlane +
-                                                                              value_place<D>(e, d / 8u) + d % 8u * 2u);
-                        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at));
-                    };
-                    const u32x2 lo = read(entry), hi = read(entry + 8u);
-                    v[p] = u32x4{lo.x, lo.y, hi.x, hi.y};
-                }
-                sums[m] = product<M>(v, weights, sums[m]);
+        }
+    };
+
+    const int32_t step = static_cast<int32_t>(kKeys);
+    if (begin < end) {
+        fill_pages(begin);
+        __syncthreads();
+        load(begin);
+        if constexpr (kBuffers == 2u) {
+            stage(begin, 0u);
+            if (begin + step < end) {
+                load(begin + step);
             }
         }
-        if (odd[0] == static_cast<uint32_t>(first)) {
-            // Values that are not finite, which the products left out, for the
-            // rows that see them.
-            for (int32_t k = 0; k < static_cast<int32_t>(kChunkKeys); ++k) {
-                const int32_t entry = first + k;
-                if (entry >= end) {
-                    break;
-                }
-                const Page page = page_of(cache, table, entry);
-                if (page.bad) {
-                    continue;  // (its score is NaN already)
-                }
-                float weight = 0.0f;
-#pragma unroll
-                for (uint32_t r = 0; r < 16u; ++r) {
-                    weight = key_of(r) == k ? score[r] : weight;
-                }
-                const float other = lane_xor<32>(weight);
-                weight = static_cast<uint32_t>(k >> 2 & 1) == half ? weight : other;
+    }
+    uint32_t buffer = 0;
+    for (int32_t first = begin; first < end; first += step) {
+        // the tile that this turn loads
+        const int32_t ahead = first + (kBuffers == 2u ? 2 : 1) * step;
+        const bool more = ahead < end;
+        __syncthreads();  // the other buffer's (or the buffer's) readers are done
+        if (more && (static_cast<uint32_t>(ahead + step - 1) >> cache.page_shift) - first_page >= kBlock) {
+            fill_pages(ahead);
+            __syncthreads();
+        }
+        if constexpr (kBuffers == 2u) {
+            if (first + step < end) {
+                stage(first + step, buffer ^ 1u);
+            }
+        } else {
+            stage(first, 0u);
+            __syncthreads();
+        }
+        if (more) {
+            load(ahead);
+        }
+        compute(first, buffer);
+        buffer ^= kBuffers - 1u;
+    }
+
+    if (marks[0] != ~0u) {
+        // Values that are not finite, in tiles of which some rows see only a part:
+        // the products left them out, the rows that see them get them.
+        for (int32_t first = begin; first < end; first += step) {
+            for (int32_t entry = first; edge_tile(first) && entry < min(first + step, end); ++entry) {
+                const float weight = odd_weight<T, R, D, P == 3>(args, table, keys, query, entry, maximum);
                 const bool visible = entry <= position && entry >= oldest;
-                const T *const value = values + page.at + 4u * half;
+                const Page page = page_of(cache, table, entry);
+                const T *const value = values + page.at;
 #pragma unroll
-                for (uint32_t m = 0; m < D / 32u; ++m) {
+                for (uint32_t m = 0; m < D / W; ++m) {
 #pragma unroll
-                    for (uint32_t r = 0; r < 16u; ++r) {
-                        const float v = static_cast<float>(value[32u * m + 8u * (r / 4u) + r % 4u]);
-                        sums[m][r] += visible && odd_float(v) ? v * weight : 0.0f;
+                    for (uint32_t r = 0; r < kRegisters; ++r) {
+                        const float v = static_cast<float>(value[dimension_of(m, r)]);
+                        sums[m][r] += visible && !page.bad && odd_float(v) ? v * weight : 0.0f;
                     }
                 }
             }
         }
     }
 
+    if constexpr (W == 16u) {
+        denominator += lane_xor<16>(denominator);
+    }
     denominator += lane_xor<32>(denominator);
     if (!wave_live || wave_row + column >= rows) {
         return;
     }
-    if (!whole && (position < begin || oldest >= end)) {
+    // a row whose entries are all in this part is done
+    const bool none = position < 0;
+    const bool whole = none || (oldest >= base + static_cast<int32_t>(part * args.span) &&
+                                position < base + static_cast<int32_t>((part + 1u) * args.span));
+    if (none ? part != 0u : position < begin || oldest >= end) {
         return;  // the part holds nothing the row sees
     }
     float *const to = whole ? nullptr : partial_row<D>(args, part, token, head);
+    const float scale = none ? 0.0f : 1.0f / denominator;
 #pragma unroll
-    for (uint32_t m = 0; m < D / 32u; ++m) {
+    for (uint32_t m = 0; m < D / W; ++m) {
 #pragma unroll
-        for (uint32_t q = 0; q < 4u; ++q) {
-            const uint32_t at = 32u * m + 8u * q + 4u * half;
-            f32x4 v = {sums[m][4u * q], sums[m][4u * q + 1u], sums[m][4u * q + 2u], sums[m][4u * q + 3u]};
+        for (uint32_t q = 0; q < kRegisters / 4u; ++q) {
+            const uint32_t at = dimension_of(m, 4u * q);
+            const f32x4 v = {sums[m][4u * q], sums[m][4u * q + 1u], sums[m][4u * q + 2u], sums[m][4u * q + 3u]};
             if (whole) {
                 float out[4];
 #pragma unroll
                 for (uint32_t k = 0; k < 4u; ++k) {
-                    out[k] = position < 0 ? 0.0f : v[k] / denominator;
+                    out[k] = none ? 0.0f : v[k] * scale;
                 }
                 store_output<R, 4>(args, token, head, at, out);
             } else {
@@ -1009,7 +1295,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_chunk(AttendArgs args) {
             }
         }
     }
-    if (!whole && half == 0u) {
+    if (!whole && side == 0u) {
         to[D] = maximum;
         to[D + 1u] = denominator;
     }
@@ -1021,6 +1307,7 @@ template <typename T, typename R, uint32_t D>
 void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged_workspace *workspace) {
     const PagedView &c = args.c;
     const uint32_t heads = c.heads * args.group;
+    constexpr uint32_t kBlockRows = chunk_rows<T, R, D>();
     const bool step = uint64_t(c.max_tokens) * args.group <= kStepRows;
     // entries a row tile may see, its base rounded down with a window
     uint64_t extent = c.max_length;
@@ -1029,8 +1316,8 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
     }
     const uint64_t row_tiles =
         step ? c.sequences
-             : std::min<uint64_t>(ceil_div(uint64_t(c.max_tokens) * args.group, kChunkRows) * uint64_t(c.sequences),
-                                  uint64_t(c.tokens) * args.group / kChunkRows + c.sequences);
+             : std::min<uint64_t>(ceil_div(uint64_t(c.max_tokens) * args.group, kBlockRows) * uint64_t(c.sequences),
+                                  uint64_t(c.tokens) * args.group / kBlockRows + c.sequences);
     // parts: as many as give two blocks a CU, within the workspace
     const uint64_t blocks = row_tiles * c.heads;
     const uint64_t part_bytes = uint64_t(c.tokens) * heads * (D + 4u) * sizeof(float);
@@ -1047,21 +1334,20 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
         launch(ctx, "paged_step", k_paged_step<T, R, D>, dim3(args.parts * c.heads, c.sequences), dim3(kThreads), 0,
                args);
     } else {
-        constexpr uint32_t Q = std::is_same_v<T, float> ? 3u : 1u;
-        constexpr size_t lds = 2u * Q * kChunkKeys * D * 2u + 16u + kChunkKeys * 4u;
+        using Shape = typename ChunkOf<T, R, D>::Shape;
+        constexpr size_t lds = chunk_lds<T, R, D>();
         static const bool raised = set_lds_limit(reinterpret_cast<const void *>(k_paged_chunk<T, R, D>), lds);
         (void)raised;
-        args.tiles = ceil_div(uint64_t(c.max_tokens) * args.group, kChunkRows);
-        const uint64_t groups = uint64_t(c.heads) * args.parts * c.sequences;
-        const uint64_t grid = (groups < 8u ? groups : (groups + 7u) / 8u * 8u) * args.tiles;
-        require(grid < (1u << 24), "paged attention: too many rows");
-        launch(ctx, "paged_chunk", k_paged_chunk<T, R, D>, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), lds,
-               args);
+        const uint64_t pairs = uint64_t(c.heads) * args.parts;
+        const uint64_t grid = (pairs < 8u ? pairs : (pairs + 7u) / 8u * 8u) * row_tiles;
+        require(grid < (1u << 23), "paged attention: too many rows");
+        launch(ctx, "paged_chunk", k_paged_chunk<T, R, D>, dim3(static_cast<uint32_t>(grid)),
+               dim3(Shape::kWaves * 64u), lds, args);
     }
     if (args.parts > 1) {
         const uint64_t rows = uint64_t(c.tokens) * heads;
         launch(ctx, "paged_join", k_paged_join<R, D, std::is_same_v<R, float>>,
-               dim3(static_cast<uint32_t>(std::min<uint64_t>(rows, 1u << 20))), dim3(D), 0, args);
+               dim3(static_cast<uint32_t>(std::min<uint64_t>((rows + 3) / 4, 1u << 20))), dim3(kThreads), 0, args);
     }
 }
 
@@ -1103,8 +1389,9 @@ void paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache, con
     const double scale = a->scale == 0.0f ? 1.0 / std::sqrt(double(cache->head_size)) : double(a->scale);
     const uint32_t window = std::min(a->window, 1u << 30);
     const AttendArgs args{paged_view(*cache, *batch), rows_view(a->queries), rows_view(a->outputs), rows_view(a->gate),
-                          static_cast<float>(scale * 1.4426950408889634), window, a->query_heads / cache->heads, 0, 0,
-                          0, nullptr};
+                          static_cast<float>(scale * 1.4426950408889634),
+                          static_cast<float>(kSlack / (scale * 1.4426950408889634)), window, a->query_heads / cache->heads, 0, 0,
+                          nullptr};
     if (type == ADI_HIP_F32 && cache->type == ADI_HIP_F32) {
         launch_attention<float, float>(ctx, args, workspace, cache->head_size);
     } else if (type == ADI_HIP_F32) {
