@@ -165,6 +165,25 @@ __device__ __forceinline__ C product(const u32x4 (&a)[A], const u32x4 (&b)[B], C
     return c;
 }
 
+// The same for X sums at once, turn by turn: a product that adds to the one
+// before it waits twice its own time.
+template <typename T, uint32_t X, uint32_t A, uint32_t B, typename C>
+__device__ __forceinline__ void products(const u32x4 (&a)[X][A], const u32x4 (&b)[B], C *(&c)[X]) {
+#pragma unroll
+    for (int32_t order = A == 2u ? 1 : 2; order >= 0; --order) {
+#pragma unroll
+        for (int32_t i = 0; i < static_cast<int32_t>(A); ++i) {
+            const int32_t j = order - i;
+            if (j >= 0 && j < static_cast<int32_t>(B)) {
+#pragma unroll
+                for (uint32_t x = 0; x < X; ++x) {
+                    *c[x] = mfma<T>(a[x][i], b[j], *c[x]);
+                }
+            }
+        }
+    }
+}
+
 // Whether either 16-bit value of a pair is an infinity or NaN.
 template <typename T>
 __device__ __forceinline__ bool odd_pair(uint32_t v) {
@@ -702,13 +721,25 @@ template <typename T, typename R, uint32_t D>
 struct ChunkOf {
     // 16-bit rows: 32 rows a wave, so that an operand read from LDS feeds as
     // many products as the LDS can keep up with
-    using Shape = ChunkShape<32, 4, D == 64 ? 64 : 32, 2, D == 256 ? 1 : 2>;
+#ifndef S64
+#define S64 ChunkShape<32, 4, 64, 1, 3>
+#endif
+#ifndef S128
+#define S128 ChunkShape<32, 8, 64, 2, 1>
+#endif
+    using Shape = std::conditional_t<D == 64, S64, std::conditional_t<D == 128, S128, ChunkShape<32, 4, 32, 2, 1>>>;
 };
 template <typename T, uint32_t D>
 struct ChunkOf<T, float, D> {
     // f32 rows: three pieces of a query, of which 16 rows a wave leave room for
     // two waves a SIMD
-    using Shape = ChunkShape<16, 8, 32, std::is_same_v<T, float> ? 1 : 2, 1>;
+#ifndef VAHEAD
+#define VAHEAD 2u
+#endif
+#ifndef SB
+#define SB ChunkShape<16, 8, 32, 1, 1>
+#endif
+    using Shape = std::conditional_t<std::is_same_v<T, float>, ChunkShape<16, 8, 32, 1, 1>, SB>;
 };
 template <typename T, typename R, uint32_t D>
 constexpr uint32_t chunk_rows() {
@@ -747,7 +778,7 @@ template <typename T, typename R, uint32_t D>
 constexpr size_t chunk_lds() {
     using Shape = typename ChunkOf<T, R, D>::Shape;
     constexpr size_t pieces = std::is_same_v<T, float> ? 5 : 2;
-    return pieces * Shape::kBuffers * Shape::kKeys * D * 2 + 16 + 2 * Shape::kBuffers * Shape::kKeys * 4 +
+    return pieces * Shape::kBuffers * Shape::kKeys * D * 2 + 16 + 4 * Shape::kKeys * 4 +
            Shape::kWaves * 64 * 4;
 }
 
@@ -775,16 +806,17 @@ void k_paged_chunk(AttendArgs args) {
     constexpr uint32_t kRegisters = W == 32u ? 16u : 4u;
     constexpr uint32_t kPlane = kKeys * D * 2u, kBuffer = (KP + Q) * kPlane;
     constexpr uint32_t kPieces = D / 8u;                              // of an entry's key or value
-    constexpr uint32_t kLoads = 2u * kKeys * kPieces / kBlock;        // a thread's pieces of a tile
-    static_assert(2u * kKeys * kPieces % kBlock == 0 && kLoads >= 1u);
+    constexpr uint32_t kLoads = (kKeys * kPieces + kBlock - 1u) / kBlock;  // a thread's pieces of a tile's keys
     extern __shared__ __align__(16) unsigned char lds[];
     // whether a tile had a value that is not finite; each buffer's last tile with
     // a bad page, and its entries
-    volatile uint32_t *const marks = reinterpret_cast<volatile uint32_t *>(lds + kBuffers * kBuffer);
-    volatile uint32_t *const bad_key = marks + 4u;                    // [kBuffers][kKeys]
+    // (plain LDS accesses, ordered by the barriers: volatile ones through a generic
+    // pointer waited for every load in flight)
+    uint32_t *const marks = reinterpret_cast<uint32_t *>(lds + kBuffers * kBuffer);
+    uint32_t *const bad_key = marks + 4u;                             // [2][kKeys]
     // what takes the scores of a key back from its scale
-    float *const key_unscale = reinterpret_cast<float *>(lds + kBuffers * kBuffer) + 4u + kBuffers * kKeys;  // as bad_key
-    uint32_t *const page_ids = reinterpret_cast<uint32_t *>(key_unscale + kBuffers * kKeys);
+    float *const key_unscale = reinterpret_cast<float *>(lds + kBuffers * kBuffer) + 4u + 2u * kKeys;  // [2][kKeys]
+    uint32_t *const page_ids = reinterpret_cast<uint32_t *>(key_unscale + 2u * kKeys);
     const PagedView &cache = args.c;
     // the blocks of one (KV head, part) of a sequence read the same entries: where
     // there are 8 or more such pairs their number is rounded up to a multiple
@@ -886,123 +918,176 @@ void k_paged_chunk(AttendArgs args) {
         page_ids[t] = page < cache.pages ? page : ~0u;
     };
 
-    // A tile passes through registers: pieces t + kBlock i of its keys, then
-    // values, piece p of entry p / kPieces.
+    // A tile's keys and its values pass through registers: pieces t + kBlock i of
+    // either, piece p of entry p / kPieces.
     using Piece = std::conditional_t<kFloat, f32x4, u32x4>;
     constexpr uint32_t kWide = kFloat ? 2u : 1u;
-    Piece in[kLoads][kWide];
-    uint32_t bad_in = 0;
-    const auto entry_of = [&](uint32_t i) { return (t + kBlock * i) % (kKeys * kPieces) / kPieces; };
-    const auto is_value = [&](uint32_t i) { return t + kBlock * i >= kKeys * kPieces; };
+    struct Held {
+        Piece piece[kLoads][kWide];
+        uint32_t bad;
+    };
+    const auto entry_of = [&](uint32_t i) { return (t + kBlock * i) / kPieces; };
+    // (with few pieces some threads have none)
+    const bool loads = kKeys * kPieces >= kBlock || t < kKeys * kPieces;
     const uint32_t page_mask = (1u << cache.page_shift) - 1u;
-    const auto load = [&](int32_t first) {
-        bad_in = 0;
+    // Where a page holds whole tiles (its size and the tiles' are powers of
+    // two), a tile's page is one number and a thread's places in it are fixed.
+    const bool paged_tiles = page_mask >= kKeys - 1u;
+    uint64_t fixed[kLoads];
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+        fixed[i] = loads ? t % kPieces * 8u + entry_of(i) * cache.entry_stride : 0u;
+    }
+    const auto load = [&](Held &held, const T *from_pool, int32_t first) {
+        held.bad = 0;
+        const auto take = [&](uint32_t i, uint64_t at) {
+            const Piece *const piece = reinterpret_cast<const Piece *>(from_pool + at);
+#pragma unroll
+            for (uint32_t w = 0; w < kWide; ++w) {
+                held.piece[i][w] = piece[w];
+            }
+        };
+        if (paged_tiles) {
+            const uint32_t id = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
+                static_cast<int>(page_ids[(static_cast<uint32_t>(first) >> cache.page_shift) - first_page])));
+            held.bad = id == ~0u ? (1u << kLoads) - 1u : 0u;
+            const uint64_t tile_at = (id == ~0u ? 0u : id) * cache.page_stride + (first & page_mask) * cache.entry_stride;
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                take(i, tile_at + fixed[i]);
+            }
+            return;
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
             const int32_t entry = first + static_cast<int32_t>(entry_of(i));
             uint64_t at = t % kPieces * 8u;
-            if (entry < end) {
+            if (entry < end && loads) {
                 const uint32_t page = page_ids[(static_cast<uint32_t>(entry) >> cache.page_shift) - first_page];
-                bad_in |= page == ~0u ? 1u << i : 0u;
+                held.bad |= page == ~0u ? 1u << i : 0u;
                 at += (page == ~0u ? 0u : page) * cache.page_stride + (entry & page_mask) * cache.entry_stride;
             }
-            const Piece *const piece = reinterpret_cast<const Piece *>((is_value(i) ? values : keys) + at);
-#pragma unroll
-            for (uint32_t w = 0; w < kWide; ++w) {
-                in[i][w] = piece[w];
-            }
+            take(i, at);
         }
     };
     const auto edge_tile = [&](int32_t first) {
         return first + static_cast<int32_t>(kKeys) > block_low + 1 || first < block_all;
     };
-    const auto stage = [&](int32_t first, uint32_t buffer) {
+    // `turn` is the tile's of two that marks of bad pages are kept for
+    const auto stage_keys = [&](Held &held, int32_t first, uint32_t buffer, uint32_t turn) {
         unsigned char *const to = lds + buffer * kBuffer;
-        if (edge_tile(first) || bad_in != 0u) {
+        if ((edge_tile(first) || held.bad != 0u) && loads) {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const int32_t entry = first + static_cast<int32_t>(entry_of(i));
-                const bool bad = (bad_in >> i & 1u) != 0u;
+                const bool bad = (held.bad >> i & 1u) != 0u;
                 if (bad) {
-                    marks[1u + buffer] = static_cast<uint32_t>(first);
+                    marks[1u + turn] = static_cast<uint32_t>(first);
                 }
-                if (is_value(i)) {
-                    const bool any = entry < end && entry >= block_from && !bad;
-                    bool seen = false;
-#pragma unroll
-                    for (uint32_t w = 0; w < kWide; ++w) {
-#pragma unroll
-                        for (uint32_t k = 0; k < 4u; ++k) {
-                            in[i][w][k] = any ? in[i][w][k] : 0;
-                            if constexpr (kFloat) {
-                                seen |= odd_float(in[i][w][k]);
-                                in[i][w][k] = odd_float(in[i][w][k]) ? 0.0f : in[i][w][k];
-                            } else {
-                                seen |= odd_pair<T>(in[i][w][k]);
-                                in[i][w][k] = clean_pair<T>(in[i][w][k]);
-                            }
-                        }
-                    }
-                    if (seen) {
-                        marks[0] = 1u;
-                    }
-                }
-                if (t % kPieces == 0u && !is_value(i)) {
-                    bad_key[buffer * kKeys + entry_of(i)] = bad ? static_cast<uint32_t>(first) : ~0u;
+                if (t % kPieces == 0u) {
+                    bad_key[turn * kKeys + entry_of(i)] = bad ? static_cast<uint32_t>(first) : ~0u;
                 }
             }
         }
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
             const uint32_t entry = entry_of(i), piece = t % kPieces;
-            const uint32_t at = is_value(i) ? KP * kPlane + value_place<D, W>(entry, piece) : key_place<D, W>(entry, piece);
+            const uint32_t at = key_place<D, W>(entry, piece);
             if constexpr (kFloat) {
-                const auto store = [&](auto count, float scale) {
-                    constexpr uint32_t kCount = decltype(count)::value;
-                    using Kind = std::conditional_t<kCount == 2u, N, M>;
-                    u32x4 out[kCount];
+                uint32_t largest = 0;
 #pragma unroll
-                    for (uint32_t n = 0; n < 4u; ++n) {
-                        uint32_t pieces[kCount];
-                        split<Kind>(in[i][n / 2u][2u * n % 4u] * scale, in[i][n / 2u][2u * n % 4u + 1u] * scale, pieces);
+                for (uint32_t w = 0; w < kWide; ++w) {
 #pragma unroll
-                        for (uint32_t p = 0; p < kCount; ++p) {
-                            out[p][n] = pieces[p];
-                        }
+                    for (uint32_t k = 0; k < 4u; ++k) {
+                        largest = magnitude(largest, held.piece[i][w][k]);
                     }
+                }
+                largest = max(largest, lane_xor_bits<1>(largest));
+                largest = max(largest, lane_xor_bits<2>(largest));
+                largest = max(largest, lane_xor_bits<4>(largest));
+                if constexpr (kPieces > 8u) {
+                    largest = max(largest, lane_xor_bits<8>(largest));
+                }
+                if constexpr (kPieces > 16u) {
+                    largest = max(largest, lane_xor_bits<16>(largest));
+                }
+                const uint32_t exponent = scale_exponent(largest);
+                const float scale = scale_of(exponent);
+                if (piece == 0u && loads) {
+                    key_unscale[buffer * kKeys + entry] = unscale_of(exponent);
+                }
+                u32x4 out[KP];
 #pragma unroll
-                    for (uint32_t p = 0; p < kCount; ++p) {
+                for (uint32_t n = 0; n < 4u; ++n) {
+                    uint32_t pieces[KP];
+                    split<N>(held.piece[i][n / 2u][2u * n % 4u] * scale, held.piece[i][n / 2u][2u * n % 4u + 1u] * scale,
+                             pieces);
+#pragma unroll
+                    for (uint32_t p = 0; p < KP; ++p) {
+                        out[p][n] = pieces[p];
+                    }
+                }
+                if (loads) {
+#pragma unroll
+                    for (uint32_t p = 0; p < KP; ++p) {
                         *reinterpret_cast<u32x4 *>(to + p * kPlane + at) = out[p];
                     }
-                };
-                if (is_value(i)) {
-                    store(std::integral_constant<uint32_t, Q>{}, 1.0f);
-                } else {
-                    uint32_t largest = 0;
+                }
+            } else if (loads) {
+                *reinterpret_cast<u32x4 *>(to + at) = held.piece[i][0];
+            }
+        }
+    };
+    const auto stage_values = [&](Held &held, int32_t first, uint32_t buffer) {
+        unsigned char *const to = lds + buffer * kBuffer + KP * kPlane;
+        if (edge_tile(first) || held.bad != 0u) {
 #pragma unroll
-                    for (uint32_t w = 0; w < kWide; ++w) {
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const int32_t entry = first + static_cast<int32_t>(entry_of(i));
+                // (what no row sees is whatever the page held before)
+                const bool any = entry < end && entry >= block_from && (held.bad >> i & 1u) == 0u;
+                bool seen = false;
 #pragma unroll
-                        for (uint32_t k = 0; k < 4u; ++k) {
-                            largest = magnitude(largest, in[i][w][k]);
+                for (uint32_t w = 0; w < kWide; ++w) {
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k) {
+                        held.piece[i][w][k] = any ? held.piece[i][w][k] : 0;
+                        if constexpr (kFloat) {
+                            seen |= odd_float(held.piece[i][w][k]);
+                            held.piece[i][w][k] = odd_float(held.piece[i][w][k]) ? 0.0f : held.piece[i][w][k];
+                        } else {
+                            seen |= odd_pair<T>(held.piece[i][w][k]);
+                            held.piece[i][w][k] = clean_pair<T>(held.piece[i][w][k]);
                         }
                     }
-                    largest = max(largest, lane_xor_bits<1>(largest));
-                    largest = max(largest, lane_xor_bits<2>(largest));
-                    largest = max(largest, lane_xor_bits<4>(largest));
-                    if constexpr (kPieces > 8u) {
-                        largest = max(largest, lane_xor_bits<8>(largest));
+                }
+                if (seen && loads) {
+                    marks[0] = 1u;
+                }
+            }
+        }
+        if (!loads) {
+            return;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t at = value_place<D, W>(entry_of(i), t % kPieces);
+            if constexpr (kFloat) {
+                u32x4 out[Q];
+#pragma unroll
+                for (uint32_t n = 0; n < 4u; ++n) {
+                    uint32_t pieces[Q];
+                    split<M>(held.piece[i][n / 2u][2u * n % 4u], held.piece[i][n / 2u][2u * n % 4u + 1u], pieces);
+#pragma unroll
+                    for (uint32_t p = 0; p < Q; ++p) {
+                        out[p][n] = pieces[p];
                     }
-                    if constexpr (kPieces > 16u) {
-                        largest = max(largest, lane_xor_bits<16>(largest));
-                    }
-                    const uint32_t exponent = scale_exponent(largest);
-                    if (piece == 0u) {
-                        key_unscale[buffer * kKeys + entry] = unscale_of(exponent);
-                    }
-                    store(std::integral_constant<uint32_t, KP>{}, scale_of(exponent));
+                }
+#pragma unroll
+                for (uint32_t p = 0; p < Q; ++p) {
+                    *reinterpret_cast<u32x4 *>(to + p * kPlane + at) = out[p];
                 }
             } else {
-                *reinterpret_cast<u32x4 *>(to + at) = in[i][0];
+                *reinterpret_cast<u32x4 *>(to + at) = held.piece[i][0];
             }
         }
     };
@@ -1065,54 +1150,74 @@ void k_paged_chunk(AttendArgs args) {
         return W == 32u ? 32u * m + 8u * (r / 4u) + 4u * side + r % 4u : 16u * m + 4u * side + r;
     };
 
-    const auto compute = [&](int32_t first, uint32_t buffer) {
-        if (!wave_live || first > wave_high || first + static_cast<int32_t>(kKeys) <= from(wave_low)) {
-            return;  // nothing of the tile is seen by the wave's rows
-        }
+    // 16-bit rows add their rounded weights up on the matrix cores too, as a row of
+    // ones among the values (the vector units are the busier ones there)
+    Acc ones_sum;
+#pragma unroll
+    for (uint32_t r = 0; r < kRegisters; ++r) {
+        ones_sum[r] = 0.0f;
+    }
+    const uint32_t one = std::is_same_v<M, _Float16> ? 0x3C003C00u : 0x3F803F80u;
+
+    // (a wave whose rows see nothing of a tile passes it by)
+    const auto sees = [&](int32_t first) {
+        return wave_live && first <= wave_high && first + static_cast<int32_t>(kKeys) > from(wave_low);
+    };
+    const auto scores = [&](uint32_t buffer, float (&score)[kSub][kHeld]) {
         const unsigned char *const key_lds = lds + buffer * kBuffer;
-        const unsigned char *const value_lds = key_lds + KP * kPlane;
-        float score[kSub][kHeld];
 #pragma unroll
         for (uint32_t b = 0; b < kSub; ++b) {
             // with 16 rows a wave two products of 16 keys, interleaved so that
             // a lane's eight results are eight keys in a row
             constexpr uint32_t kProducts = W == 32u ? 1u : 2u;
+            Acc acc[kProducts], *to[kProducts];
 #pragma unroll
             for (uint32_t h = 0; h < kProducts; ++h) {
-                Acc acc;
 #pragma unroll
                 for (uint32_t r = 0; r < kRegisters; ++r) {
-                    acc[r] = 0.0f;
+                    acc[h][r] = 0.0f;
                 }
-                const uint32_t entry = 32u * b + (W == 32u ? column : 8u * (column / 4u) + 4u * h + column % 4u);
-                u32x4 k[2][KP];
-                const auto read = [&](uint32_t j) {
+                to[h] = &acc[h];
+            }
+            u32x4 k[2][kProducts][KP];
+            const auto read = [&](uint32_t j) {
+#pragma unroll
+                for (uint32_t h = 0; h < kProducts; ++h) {
+                    const uint32_t entry = 32u * b + (W == 32u ? column : 8u * (column / 4u) + 4u * h + column % 4u);
 #pragma unroll
                     for (uint32_t p = 0; p < KP; ++p) {
-                        k[j & 1u][p] = *reinterpret_cast<const u32x4 *>(
+                        k[j & 1u][h][p] = *reinterpret_cast<const u32x4 *>(
                             key_lds + p * kPlane + key_place<D, W>(entry, kStepDims / 8u * j + side));
                     }
-                };
-                read(0u);
+                }
+            };
+            read(0u);
 #pragma unroll
-                for (uint32_t j = 0; j < D / kStepDims; ++j) {
-                    if (j + 1u < D / kStepDims) {
-                        read(j + 1u);
-                    }
-                    acc = product<N>(k[j & 1u], query_pieces[j], acc);
+            for (uint32_t j = 0; j < D / kStepDims; ++j) {
+                if (j + 1u < D / kStepDims) {
+                    read(j + 1u);
+                }
+                products<N>(k[j & 1u], query_pieces[j], to);
+                if constexpr (P == 3u) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
+            }
+#pragma unroll
+            for (uint32_t h = 0; h < kProducts; ++h) {
 #pragma unroll
                 for (uint32_t r = 0; r < kRegisters; ++r) {
-                    score[b][h * kRegisters + r] = acc[r];
+                    score[b][h * kRegisters + r] = acc[h][r];
                     if constexpr (kFloat) {
                         score[b][h * kRegisters + r] =
-                            acc[r] * query_unscale * key_unscale[buffer * kKeys + 32u * b + key_of(h * kRegisters + r)];
+                            acc[h][r] * query_unscale * key_unscale[buffer * kKeys + 32u * b + key_of(h * kRegisters + r)];
                     }
                 }
             }
         }
-        const bool bad_tile = marks[1u + buffer] == static_cast<uint32_t>(first);
+    };
+    const auto attend = [&](int32_t first, uint32_t buffer, uint32_t turn, float (&score)[kSub][kHeld]) {
+        const unsigned char *const value_lds = lds + buffer * kBuffer + KP * kPlane;
+        const bool bad_tile = marks[1u + turn] == static_cast<uint32_t>(first);
         if (bad_tile || first + static_cast<int32_t>(kKeys) > wave_low + 1 || first < from(wave_high)) {
 #pragma unroll
             for (uint32_t b = 0; b < kSub; ++b) {
@@ -1121,7 +1226,7 @@ void k_paged_chunk(AttendArgs args) {
                     const uint32_t key = 32u * b + key_of(r);
                     const int32_t entry = first + static_cast<int32_t>(key);
                     const bool visible = entry <= position && entry >= oldest;
-                    const bool bad = bad_tile && bad_key[buffer * kKeys + key] == static_cast<uint32_t>(first);
+                    const bool bad = bad_tile && bad_key[turn * kKeys + key] == static_cast<uint32_t>(first);
                     score[b][r] = !visible ? kNegative : bad ? __builtin_nanf("") : score[b][r];
                 }
             }
@@ -1149,6 +1254,9 @@ void k_paged_chunk(AttendArgs args) {
             for (uint32_t m = 0; m < D / W; ++m) {
                 sums[m] *= factor;
             }
+            if constexpr (P == 1u) {
+                ones_sum *= factor;
+            }
         }
         const float level = maximum == kNegative ? 0.0f : maximum;
 #pragma unroll
@@ -1156,7 +1264,9 @@ void k_paged_chunk(AttendArgs args) {
 #pragma unroll
             for (uint32_t r = 0; r < kHeld; ++r) {
                 score[b][r] = weight_of<P == 3>(score[b][r], level, args.log2_scale);
-                denominator += score[b][r];
+                if constexpr (P == 3u) {
+                    denominator += score[b][r];
+                }
             }
             // steps of 16 keys (32 rows a wave) or 32
 #pragma unroll
@@ -1171,73 +1281,156 @@ void k_paged_chunk(AttendArgs args) {
                         weights[p][k] = pieces[p];
                     }
                 }
+                if constexpr (P == 1u) {
+                    ones_sum = mfma<M>(u32x4{one, one, one, one}, weights[0], ones_sum);
+                }
                 // the values transposed: lane i of 16 takes row i / 4 of four
                 // entries at dimension 4 (i % 4), and gets dimension i of the four
                 const uint32_t entry = 32u * b + (lane & 15u) / 4u + (W == 32u ? 16u * u + 4u * side : 8u * side);
                 const uint32_t next = entry + (W == 32u ? 8u : 4u);
                 const uint32_t dimension = (W == 32u ? (lane >> 4 & 1u) * 16u : 0u) + (lane & 3u) * 4u;
-                u32x4 v[2][Q];
-                const auto read = [&](uint32_t m) {
+                // (two at a time, the next two on their way)
+                u32x4 v[VAHEAD][2][Q];
+                const auto read = [&](uint32_t i) {
 #pragma unroll
-                    for (uint32_t p = 0; p < Q; ++p) {
-                        const uint32_t d = W * m + dimension;
-                        const auto four = [&](uint32_t e) {
-                            auto *at = (__attribute__((address_space(3))) s16x4 *)(
-                                value_lds + p * kPlane + value_place<D, W>(e, d / 8u) + d % 8u * 2u);
-                            return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at));
-                        };
-                        const u32x2 lo = four(entry), hi = four(next);
-                        v[m & 1u][p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                    for (uint32_t x = 0; x < 2u; ++x) {
+#pragma unroll
+                        for (uint32_t p = 0; p < Q; ++p) {
+                            const uint32_t d = W * (2u * i + x) + dimension;
+                            const auto four = [&](uint32_t e) {
+                                auto *at = (__attribute__((address_space(3))) s16x4 *)(
+                                    value_lds + p * kPlane + value_place<D, W>(e, d / 8u) + d % 8u * 2u);
+                                return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at));
+                            };
+                            const u32x2 lo = four(entry), hi = four(next);
+                            v[i % VAHEAD][x][p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                        }
                     }
                 };
-                read(0u);
+                if (VAHEAD > 1u) read(0u);
 #pragma unroll
-                for (uint32_t m = 0; m < D / W; ++m) {
-                    if (m + 1u < D / W) {
-                        read(m + 1u);
+                for (uint32_t i = 0; i < D / W / 2u; ++i) {
+                    if (VAHEAD == 1u) read(i); else
+                    if (i + 1u < D / W / 2u) {
+                        read(i + 1u);
                     }
-                    sums[m] = product<M>(v[m & 1u], weights, sums[m]);
-                    __builtin_amdgcn_sched_barrier(0);
+                    Acc *to[2] = {&sums[2u * i], &sums[2u * i + 1u]};
+                    products<M>(v[i % VAHEAD], weights, to);
+                    if constexpr (P == 3u) {
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
         }
     };
 
     const int32_t step = static_cast<int32_t>(kKeys);
+    // pages up to a tile's end in LDS (called by all, between barriers)
+    const auto reach_pages = [&](int32_t first) {
+        if ((static_cast<uint32_t>(first + step - 1) >> cache.page_shift) - first_page >= kBlock) {
+            fill_pages(first);
+            __syncthreads();
+        }
+    };
     if (begin < end) {
         fill_pages(begin);
         __syncthreads();
-        load(begin);
+        int32_t first = begin;
+        uint32_t turn = 0;
+        float score[kSub][kHeld];
         if constexpr (kBuffers == 2u) {
-            stage(begin, 0u);
+            // two tiles in LDS: while one is computed the next is staged, from
+            // registers whose loads went out a tile before
+            Held key_in, value_in;
+            load(key_in, keys, begin);
+            load(value_in, values, begin);
+            stage_keys(key_in, begin, 0u, 0u);
+            stage_values(value_in, begin, 0u);
+            // (the queries are here before the loop: a wait for them within it
+            // would be one for the tiles on their way)
+            __builtin_amdgcn_s_waitcnt(0);
             if (begin + step < end) {
-                load(begin + step);
+                load(key_in, keys, begin + step);
+                load(value_in, values, begin + step);
             }
-        }
-    }
-    uint32_t buffer = 0;
-    for (int32_t first = begin; first < end; first += step) {
-        // the tile that this turn loads
-        const int32_t ahead = first + (kBuffers == 2u ? 2 : 1) * step;
-        const bool more = ahead < end;
-        __syncthreads();  // the other buffer's (or the buffer's) readers are done
-        if (more && (static_cast<uint32_t>(ahead + step - 1) >> cache.page_shift) - first_page >= kBlock) {
-            fill_pages(ahead);
-            __syncthreads();
-        }
-        if constexpr (kBuffers == 2u) {
-            if (first + step < end) {
-                stage(first + step, buffer ^ 1u);
-            }
+            do {
+                const int32_t ahead = first + 2 * step;
+                __syncthreads();  // the other buffer's readers are done
+                if (ahead < end) {
+                    reach_pages(ahead);
+                }
+                if (first + step < end) {
+                    stage_keys(key_in, first + step, turn ^ 1u, turn ^ 1u);
+                    stage_values(value_in, first + step, turn ^ 1u);
+                }
+                if (ahead < end) {
+                    load(key_in, keys, ahead);
+                    load(value_in, values, ahead);
+                }
+                if (sees(first)) {
+                    scores(turn, score);
+                    attend(first, turn, turn, score);
+                }
+                turn ^= 1u;
+                first += step;
+            } while (first < end);
         } else {
-            stage(first, 0u);
-            __syncthreads();
+            // one: while its keys are multiplied its values are staged, and the
+            // next one's keys while its values are; one set of registers holds what
+            // is on its way. The waves' second half stages first and the first
+            // half last: a SIMD has a wave of either, of which one then uses the
+            // vector units while the other's products run.
+            const bool early = wave >= Shape::kWaves / 2u;
+            Held in;
+            load(in, keys, begin);
+            stage_keys(in, begin, 0u, 0u);
+            __builtin_amdgcn_s_waitcnt(0);
+            load(in, values, begin);
+            do {
+                const bool live = sees(first), more = first + step < end;
+                const auto pass_values = [&] {
+                    stage_values(in, first, 0u);
+                    if (more) {
+                        load(in, keys, first + step);
+                    }
+                };
+                const auto pass_keys = [&] {
+                    if (more) {
+                        stage_keys(in, first + step, 0u, turn ^ 1u);
+                        load(in, values, first + step);
+                    }
+                };
+                __syncthreads();
+                if (early) {
+                    pass_values();
+                }
+                if (live) {
+                    scores(0u, score);
+                }
+                if (!early) {
+                    pass_values();
+                }
+                __syncthreads();
+                if (early) {
+                    pass_keys();
+                }
+                if (live) {
+                    attend(first, 0u, turn, score);
+                }
+                if (!early) {
+                    pass_keys();
+                }
+                turn ^= 1u;
+                if (more) {
+                    if (first + 2 * step < end &&
+                        (static_cast<uint32_t>(first + 3 * step - 1) >> cache.page_shift) - first_page >= kBlock) {
+                        __syncthreads();  // every wave has read its pages
+                        fill_pages(first + 2 * step);
+                    }
+                }
+                first += step;
+            } while (first < end);
         }
-        if (more) {
-            load(ahead);
-        }
-        compute(first, buffer);
-        buffer ^= kBuffers - 1u;
     }
 
     if (marks[0] != ~0u) {
@@ -1261,10 +1454,14 @@ void k_paged_chunk(AttendArgs args) {
         }
     }
 
-    if constexpr (W == 16u) {
-        denominator += lane_xor<16>(denominator);
+    if constexpr (P == 1u) {
+        denominator = ones_sum[0];
+    } else {
+        if constexpr (W == 16u) {
+            denominator += lane_xor<16>(denominator);
+        }
+        denominator += lane_xor<32>(denominator);
     }
-    denominator += lane_xor<32>(denominator);
     if (!wave_live || wave_row + column >= rows) {
         return;
     }
@@ -1318,14 +1515,36 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
         step ? c.sequences
              : std::min<uint64_t>(ceil_div(uint64_t(c.max_tokens) * args.group, kBlockRows) * uint64_t(c.sequences),
                                   uint64_t(c.tokens) * args.group / kBlockRows + c.sequences);
-    // parts: as many as give two blocks a CU, within the workspace
     const uint64_t blocks = row_tiles * c.heads;
     const uint64_t part_bytes = uint64_t(c.tokens) * heads * (D + 4u) * sizeof(float);
-    uint64_t parts = std::max<uint64_t>(2u * ctx->cu_count / blocks, 1u);
-    parts = std::min<uint64_t>({parts, workspace->bytes / part_bytes, (extent + kSpanUnit - 1) / kSpanUnit, 1024u});
-    parts = std::max<uint64_t>(parts, 1u);
-    const uint64_t span = (ceil_div(extent, parts) + kSpanUnit - 1) / kSpanUnit * kSpanUnit;
-    args.span = static_cast<uint32_t>(std::max<uint64_t>(span, kSpanUnit));
+    const uint64_t most = std::max<uint64_t>(
+        std::min<uint64_t>({workspace->bytes / part_bytes, (extent + kSpanUnit - 1) / kSpanUnit, 1024u}), 1u);
+    const auto span_of = [&](uint64_t parts) {
+        return std::max<uint64_t>((ceil_div(extent, parts) + kSpanUnit - 1) / kSpanUnit, 1u) * kSpanUnit;
+    };
+    if (step) {
+        // as many parts as give two blocks a CU
+        args.span = static_cast<uint32_t>(
+            span_of(std::clamp<uint64_t>(2u * ctx->cu_count / blocks, 1u, most)));
+    } else {
+        // the parts that end first, in units of 32 keys of a row tile (some 3 us):
+        // rounds of the blocks the chip holds (half a round more where there are
+        // several, for their uneven ends), a block's own start and end worth 6,
+        // and the parts' way through memory at 5 TB/s
+        const double resident = double(ctx->cu_count) * ChunkOf<T, R, D>::Shape::kBlocks;
+        double least = 0.0;
+        for (uint64_t parts = 1; parts <= std::min<uint64_t>(most, 64u); ++parts) {
+            const uint64_t span = span_of(parts);
+            const double count = double(blocks) * ceil_div(extent, span);
+            const double rounds = count <= resident ? 1.0 : count / resident + 0.5;
+            const double joined = span < extent ? 2.0 + 2.0 * part_bytes * ceil_div(extent, span) / 15.0e6 : 0.0;
+            const double cost = rounds * (span / 32.0 + 6.0) + joined;
+            if (parts == 1 || cost < least) {
+                least = cost;
+                args.span = static_cast<uint32_t>(span);
+            }
+        }
+    }
     args.parts = std::max(ceil_div(extent, args.span), 1u);
     args.partial = static_cast<float *>(workspace->base);
     if (step) {
