@@ -329,6 +329,14 @@ int adi_hip_paged_workspace_create(adi_hip_context *ctx, size_t bytes, adi_hip_p
         require(bytes >= size_t(1) << 20, "paged workspace: at least 1 MiB");
         void *base = nullptr;
         check_hip(hipMalloc(&base, bytes), "paged workspace allocation");
+        hipError_t error = hipMemset(base, 0, kTickets * sizeof(uint32_t));
+        if (error == hipSuccess) {
+            error = hipDeviceSynchronize();
+        }
+        if (error != hipSuccess) {
+            (void)hipFree(base);
+            check_hip(error, "paged workspace tickets");
+        }
         auto *workspace = new (std::nothrow) adi_hip_paged_workspace{ctx->device, base, bytes};
         if (workspace == nullptr) {
             (void)hipFree(base);

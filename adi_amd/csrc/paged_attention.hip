@@ -50,6 +50,8 @@ struct AttendArgs {
     uint32_t window;
     uint32_t group;       // query heads of a KV head
     uint32_t span, parts; // entries of a part of a history, parts at most
+    uint32_t mixed;       // nonzero: k_paged_step takes the sequences of few rows, k_paged_chunk the others
+    uint32_t *tickets;    // [sequence][KV head], zero between calls (k_paged_step)
     float *partial;       // [part][token][head][D + 4]: sums, maximum, denominator (parts > 1)
 };
 
@@ -261,31 +263,100 @@ __device__ __forceinline__ void fill_rows(const AttendArgs &a, const SequenceRow
     }
 }
 
+// LDS places: the 16-byte pieces of an entry's D 16-bit values are permuted so
+// that the reads of a phase fall on different banks. Keys: the 16 entries that a
+// phase's lanes read at one piece get different turns. Values: the entries that
+// a transposing read's half wave reads side by side, four at 64 bytes (32
+// rows a wave) or eight at 32 bytes (16). A row of 64 values is half the banks,
+// so two rows share a turn.
+template <uint32_t D, uint32_t ROWS>
+__device__ __forceinline__ uint32_t key_place(uint32_t row, uint32_t piece) {
+    uint32_t turn;
+    if constexpr (ROWS == 32) {
+        turn = D == 64u ? (row >> 1) & 7u : row & 15u;
+    } else {
+        turn = D == 64u ? (row >> 1 & 1u) | (row >> 3 & 3u) << 1 : (row & 3u) | (row >> 3 & 3u) << 2;
+    }
+    return row * (D * 2u) + ((piece ^ turn) << 4);
+}
+template <uint32_t D, uint32_t ROWS>
+__device__ __forceinline__ uint32_t value_place(uint32_t row, uint32_t piece) {
+    uint32_t turn;
+    if constexpr (ROWS == 32) {
+        turn = D == 64u ? (row & 2u) << 1 : (row & 3u) << 2;
+    } else {
+        turn = D == 64u ? (row & 2u) | (row >> 3 & 1u) << 2 : (row & 3u) << 1 | (row >> 3 & 1u) << 3;
+    }
+    return row * (D * 2u) + ((piece ^ turn) << 4);
+}
+
 // ---- up to 16 rows a KV head --------------------------------------------------
 
+constexpr uint32_t kStepParts = 128;  // parts of a history at most
+
+// Used one after another: the rows' queries, the waves' sums, the parts to join.
 template <uint32_t D>
 struct StepLds {
-    __align__(16) float sums[4][kStepRows][D + 4u];
+    union {
+        __align__(16) unsigned char query[kStepRows * D * 6u];
+        __align__(16) float sums[4][kStepRows][D + 4u];
+        struct {
+            // (a row's parts lie in as many banks)
+            float factor[kStepParts][kStepRows + 1u], total[kStepParts][kStepRows + 1u];
+            __align__(16) f32x4 group[kThreads];
+        } parts;
+    };
     float maximum[4][kStepRows], denominator[4][kStepRows];
+    uint32_t last;
 };
 
-// Block (KV head, part, sequence): its four waves take the part's tiles in turn.
-// Lane l is column c = l % 16 (a row), quarter g = l / 16.
+// 16 bytes written through to memory, and read past the caches that another
+// XCD's writes do not reach.
+__device__ __forceinline__ void store_through(float *base, uint32_t at, f32x4 v) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, at * 4u, 0, 16 /* sc1 */);
+}
+__device__ __forceinline__ f32x4 load_through(const float *base, uint32_t at) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(base), 0, 0x7FFFFFFF, 0x00020000);
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at * 4u, 0, 16 /* sc1 */));
+}
+
+// Whether a tile's values are on their way beside its keys, or take the keys'
+// registers when its scores are done; and the blocks a CU holds, by registers.
 template <typename T, typename R, uint32_t D>
-__global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
+constexpr bool step_eager() {
+    return D < 256u || sizeof(R) > sizeof(T);
+}
+template <typename T, typename R, uint32_t D>
+constexpr uint32_t step_blocks() {
+    return D == 256u ? (step_eager<T, R, D>() ? 1u : 2u) : 2u;
+}
+
+// Block (KV head, part, sequence): its four waves take the part's tiles in turn,
+// each straight from the cache into operands, the next tile's keys on their way
+// from the end of this one's scores and its values from the end of their
+// products. Lane l is column c = l % 16 (a row), quarter g = l / 16. The blocks
+// of a history of several parts leave theirs in the workspace, a region of
+// kStepRows rows of D + 4 each (whole cache lines, so that no two blocks write
+// one), and the last through the ticket joins them.
+template <typename T, typename R, uint32_t D>
+__global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_step(AttendArgs args) {
     constexpr bool kFloat = std::is_same_v<T, float>;  // the cache's type
     constexpr uint32_t P = std::is_same_v<R, float> ? 3u : 1u;
     // a wave's tile, and the keys of a tile that a lane holds: kKeys / 4 in a row
     constexpr uint32_t kKeys = kFloat ? 16u : 32u, kHeld = kKeys / 4u;
     // dimensions of a value row that a lane holds side by side, and groups of 16 lanes' worth
     constexpr uint32_t kSide = kFloat ? 4u : D == 64u ? 4u : 8u, kGroups = D / (16u * kSide);
+    constexpr uint32_t kRegion = kStepRows * (D + 4u);
+    constexpr bool kEager = step_eager<T, R, D>();
+    static_assert(kRegion * sizeof(float) % 128u == 0u);
     __shared__ StepLds<D> lds;
     const PagedView &cache = args.c;
     const uint32_t kv = blockIdx.x % cache.heads, part = blockIdx.x / cache.heads, sequence = blockIdx.y;
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const uint32_t c = lane & 15u, g = lane >> 4;
     const SequenceRows s = sequence_rows(cache, sequence);
-    if (s.count == 0u) {
+    if (s.count == 0u || (args.mixed != 0u && s.count * args.group > kStepRows)) {
         return;
     }
     if (s.over || s.length == 0u) {
@@ -301,11 +372,13 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
     const int32_t position = first_position + static_cast<int32_t>(row / args.group);
     const int32_t window = static_cast<int32_t>(args.window);
     const int32_t oldest = window == 0 ? 0 : max(0, position - window + 1);  // the row's first entry
-    const int32_t begin = base_of(args, first_position) + static_cast<int32_t>(part * args.span);
+    const int32_t base = base_of(args, first_position);
+    const int32_t begin = base + static_cast<int32_t>(part * args.span);
     const int32_t end = min(begin + static_cast<int32_t>(args.span), static_cast<int32_t>(s.length));
     if (begin >= end) {
         return;
     }
+    const uint32_t live = (s.length - static_cast<uint32_t>(base) + args.span - 1u) / args.span;
     // entries that some row sees, and those that every row sees
     const int32_t seen_from = window == 0 ? 0 : max(0, first_position - window + 1);
     const int32_t all_from = window == 0 ? 0 : max(0, static_cast<int32_t>(s.length) - window);
@@ -313,37 +386,122 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
     const T *const keys = reinterpret_cast<const T *>(cache.keys) + kv * cache.head_stride;
     const T *const values = reinterpret_cast<const T *>(cache.values) + kv * cache.head_stride;
 
+    // Key operands: row i of A is key first + kHeld (i / 4) + i % 4 (+ 4 in the
+    // second of two products with 32 keys), so that register r of the results
+    // is key first + kHeld g + r. Groups of 8 entries from a multiple of 8 share a
+    // page: this lane's for the keys it reads and for the values.
+    const uint32_t key_group = (kHeld * (c >> 2)) & ~7u, value_group = (kHeld * g) & ~7u;
+    const uint64_t key_at = ((kHeld * (c >> 2) & 7u) + (c & 3u)) * cache.entry_stride;
+    const uint64_t value_at = ((kHeld * g) & 7u) * cache.entry_stride;
+    constexpr int32_t kTurn = 4 * kKeys;  // entries of the four waves' tiles
+    struct Numbers {
+        uint32_t key, value;
+    };
+    const auto numbers_of = [&](int32_t first) {
+        const uint32_t last = static_cast<uint32_t>(end - 1);
+        return Numbers{table[min(first + key_group, last) >> cache.page_shift],
+                       table[min(first + value_group, last) >> cache.page_shift]};
+    };
+    const uint32_t page_mask = (1u << cache.page_shift) - 1u;
+    // (a page that there is not: page 0 stands in, which is always there to be read)
+    const auto place_of = [&](uint32_t number, uint32_t entry) {
+        return (number >= cache.pages ? 0u : number) * cache.page_stride + (entry & page_mask) * cache.entry_stride;
+    };
+
+    f32x4 key_float[kFloat ? D / 16u : 1u];
+    u32x4 key_half[kFloat ? 1u : 2u][kFloat ? 1u : D / 32u][1];
+    using Chunk = std::conditional_t<kFloat, f32x4, std::conditional_t<kSide == 8u, u32x4, u32x2>>;
+    Chunk held[kGroups][kHeld];
+    const auto load_keys = [&](const Numbers &n, int32_t first) {
+        const T *const key = keys + place_of(n.key, first + key_group) + key_at;
+        if constexpr (kFloat) {
+#pragma unroll
+            for (uint32_t j = 0; j < D / 16u; ++j) {
+                key_float[j] = *reinterpret_cast<const f32x4 *>(key + 16u * j + 4u * g);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h) {
+#pragma unroll
+                for (uint32_t j = 0; j < D / 32u; ++j) {
+                    key_half[h][j][0] =
+                        *reinterpret_cast<const u32x4 *>(key + 4u * h * cache.entry_stride + 32u * j + 8u * g);
+                }
+            }
+        }
+    };
+    const auto load_values = [&](const Numbers &n, int32_t first) {
+        const T *const value = values + place_of(n.value, first + value_group) + value_at;
+#pragma unroll
+        for (uint32_t i = 0; i < kGroups; ++i) {
+#pragma unroll
+            for (uint32_t k = 0; k < kHeld; ++k) {
+                held[i][k] = *reinterpret_cast<const Chunk *>(value + k * cache.entry_stride + 16u * kSide * i +
+                                                              kSide * c);
+            }
+        }
+    };
+
+    int32_t first = begin + static_cast<int32_t>(wave * kKeys);
+    Numbers now{0, 0}, next{0, 0};
+    if (first < end) {
+        now = numbers_of(first);
+        load_keys(now, first);
+        if constexpr (kEager) {
+            load_values(now, first);
+        }
+        next = numbers_of(first + kTurn);
+    }
+
     // the row's query as the products take it
     const R *const query = reinterpret_cast<const R *>(args.queries.data) + token * args.queries.token_stride +
                            head * args.queries.head_stride;
-    f32x4 query_float[kFloat ? D / 16u : 1u];
-    u32x4 query_pieces[kFloat ? 1u : D / 32u][P];
-    if constexpr (kFloat) {
-#pragma unroll
-        for (uint32_t j = 0; j < D / 16u; ++j) {
-            query_float[j] = *reinterpret_cast<const f32x4 *>(query + 16u * j + 4u * g);
+    // (f32 rows through LDS: as floats or in three pieces they are a quarter of the
+    // registers, which then hold two blocks a CU)
+    constexpr uint32_t kPlane = kStepRows * D * 2u;
+    const auto query_place = [&](uint32_t piece) {
+        if constexpr (kFloat) {
+            return c * (D * 4u) + ((piece ^ c) << 4);
+        } else {
+            return key_place<D, 32>(c, piece);
         }
-    } else if constexpr (P == 1) {
+    };
+    u32x4 query_pieces[P == 1u ? D / 32u : 1u][1];
+    if constexpr (P == 1) {
 #pragma unroll
         for (uint32_t j = 0; j < D / 32u; ++j) {
             query_pieces[j][0] = *reinterpret_cast<const u32x4 *>(query + 32u * j + 8u * g);
         }
     } else {
+        if constexpr (kFloat) {
 #pragma unroll
-        for (uint32_t j = 0; j < D / 32u; ++j) {
-            const f32x4 lo = *reinterpret_cast<const f32x4 *>(query + 32u * j + 8u * g);
-            const f32x4 hi = *reinterpret_cast<const f32x4 *>(query + 32u * j + 8u * g + 4u);
+            for (uint32_t j = 0; j < D / 64u; ++j) {
+                const uint32_t piece = 4u * (4u * j + wave) + g;
+                *reinterpret_cast<f32x4 *>(lds.query + query_place(piece)) =
+                    *reinterpret_cast<const f32x4 *>(query + 4u * piece);
+            }
+        } else {
+            for (uint32_t j = wave; j < D / 32u; j += 4u) {
+                const f32x4 lo = *reinterpret_cast<const f32x4 *>(query + 32u * j + 8u * g);
+                const f32x4 hi = *reinterpret_cast<const f32x4 *>(query + 32u * j + 8u * g + 4u);
+                u32x4 out[P];
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                uint32_t pieces[P];
-                k < 2u ? split<T>(lo[2u * k], lo[2u * k + 1u], pieces)
-                       : split<T>(hi[2u * k - 4u], hi[2u * k - 3u], pieces);
+                for (uint32_t k = 0; k < 4u; ++k) {
+                    uint32_t pieces[P];
+                    k < 2u ? split<T>(lo[2u * k], lo[2u * k + 1u], pieces)
+                           : split<T>(hi[2u * k - 4u], hi[2u * k - 3u], pieces);
+#pragma unroll
+                    for (uint32_t p = 0; p < P; ++p) {
+                        out[p][k] = pieces[p];
+                    }
+                }
 #pragma unroll
                 for (uint32_t p = 0; p < P; ++p) {
-                    query_pieces[j][p][k] = pieces[p];
+                    *reinterpret_cast<u32x4 *>(lds.query + p * kPlane + query_place(4u * j + g)) = out[p];
                 }
             }
         }
+        __syncthreads();
     }
 
     f32x4 sums[kGroups][kSide];
@@ -358,42 +516,22 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
     // score from which it is raised
     float maximum = kNegative, limit = kNegative, denominator = 0.0f;
     // a tile that some row does not see whole
-    const auto edge_tile = [&](int32_t first) {
-        return first + static_cast<int32_t>(kKeys) > first_position + 1 || first < all_from;
+    const auto edge_tile = [&](int32_t at) {
+        return at + static_cast<int32_t>(kKeys) > first_position + 1 || at < all_from;
     };
     bool odd_tile = false;
 
-    for (int32_t first = begin + static_cast<int32_t>(wave * kKeys); first < end; first += 4 * kKeys) {
-        // Key operands: row i of A is key first + kHeld (i / 4) + i % 4 (+ 4
-        // in the second of two products with 32 keys), so that register r of
-        // the results is key first + kHeld g + r. Groups of 8 entries from a
-        // multiple of 8 share a page.
-        const int32_t key_group = first + static_cast<int32_t>((kHeld * (c >> 2)) & ~7u);
-        const int32_t value_group = first + static_cast<int32_t>((kHeld * g) & ~7u);
-        Page key_page{0, false}, value_page{0, false};
-        if (key_group < end) {
-            key_page = page_of(cache, table, key_group);
-        }
-        if (value_group < end) {
-            value_page = page_of(cache, table, value_group);
-        }
-        const uint32_t key_at = (kHeld * (c >> 2) & 7u) + (c & 3u);
-        const T *const key = keys + key_page.at + key_at * cache.entry_stride;
-        const T *const value = values + value_page.at + ((kHeld * g) & 7u) * cache.entry_stride;
+    for (; first < end; first += kTurn) {
         float score[kHeld];
         if constexpr (kFloat) {
-            f32x4 k[D / 16u];
-#pragma unroll
-            for (uint32_t j = 0; j < D / 16u; ++j) {
-                k[j] = *reinterpret_cast<const f32x4 *>(key + 16u * j + 4u * g);
-            }
             f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (uint32_t j = 0; j < D / 16u; ++j) {
+                const f32x4 q = *reinterpret_cast<const f32x4 *>(lds.query + query_place(4u * j + g));
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i) {
                     acc[j & 1u] =
-                        __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][i], query_float[j][i], acc[j & 1u], 0, 0, 0);
+                        __builtin_amdgcn_mfma_f32_16x16x4f32(key_float[j][i], q[i], acc[j & 1u], 0, 0, 0);
                 }
             }
 #pragma unroll
@@ -401,50 +539,51 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
                 score[r] = acc[0][r] + acc[1][r];
             }
         } else {
-            u32x4 k[2][D / 32u][1];
+            f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-            for (uint32_t h = 0; h < 2u; ++h) {
+            for (uint32_t j = 0; j < D / 32u; ++j) {
+                u32x4 q[P];
 #pragma unroll
-                for (uint32_t j = 0; j < D / 32u; ++j) {
-                    k[h][j][0] =
-                        *reinterpret_cast<const u32x4 *>(key + 4u * h * cache.entry_stride + 32u * j + 8u * g);
+                for (uint32_t p = 0; p < P; ++p) {
+                    if constexpr (P == 1u) {
+                        q[p] = query_pieces[j][p];
+                    } else {
+                        q[p] = *reinterpret_cast<const u32x4 *>(lds.query + p * kPlane + query_place(4u * j + g));
+                    }
                 }
+                u32x4 k[2][1] = {{key_half[0][j][0]}, {key_half[1][j][0]}};
+                f32x4 *to[2] = {&acc[0], &acc[1]};
+                products<T>(k, q, to);
             }
 #pragma unroll
             for (uint32_t h = 0; h < 2u; ++h) {
-                f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (uint32_t j = 0; j < D / 32u; ++j) {
-                    acc = product<T>(k[h][j], query_pieces[j], acc);
-                }
 #pragma unroll
                 for (uint32_t r = 0; r < 4u; ++r) {
-                    score[4u * h + r] = acc[r];
+                    score[4u * h + r] = acc[h][r];
                 }
             }
         }
-        // values: kHeld entries of the lane's quarter, kSide dimensions of each group
-        using Chunk = std::conditional_t<kFloat, f32x4, std::conditional_t<kSide == 8u, u32x4, u32x2>>;
-        Chunk held[kGroups][kHeld];
-#pragma unroll
-        for (uint32_t i = 0; i < kGroups; ++i) {
-#pragma unroll
-            for (uint32_t k = 0; k < kHeld; ++k) {
-                held[i][k] = *reinterpret_cast<const Chunk *>(value + k * cache.entry_stride + 16u * kSide * i +
-                                                              kSide * c);
-            }
+        const bool bad = now.value >= cache.pages;
+        if constexpr (!kEager) {
+            load_values(now, first);
+        }
+        now = next;
+        if (kEager && first + kTurn < end) {
+            load_keys(now, first + kTurn);
+        }
+        if (first + 2 * kTurn < end) {
+            next = numbers_of(first + 2 * kTurn);
         }
         const int32_t own_first = first + static_cast<int32_t>(kHeld * g);  // the lane's keys
-        const bool edge = edge_tile(first);
-        if (__any(edge || value_page.bad)) {
+        if (__any(edge_tile(first) || bad)) {
             bool odd = false;
 #pragma unroll
             for (uint32_t k = 0; k < kHeld; ++k) {
                 const int32_t entry = own_first + static_cast<int32_t>(k);
                 const bool visible = entry <= position && entry >= oldest;
-                score[k] = !visible ? kNegative : value_page.bad ? __builtin_nanf("") : score[k];
+                score[k] = !visible ? kNegative : bad ? __builtin_nanf("") : score[k];
                 // (what no row sees is whatever the page held before)
-                const bool any = entry < static_cast<int32_t>(s.length) && entry >= seen_from && !value_page.bad;
+                const bool any = entry < end && entry >= seen_from && !bad;
 #pragma unroll
                 for (uint32_t i = 0; i < kGroups; ++i) {
                     constexpr uint32_t kWords = sizeof(Chunk) / 4u;
@@ -531,14 +670,20 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
                 }
             }
         }
+        if (first + kTurn < end) {
+            if constexpr (kEager) {
+                load_values(now, first + kTurn);
+            } else {
+                load_keys(now, first + kTurn);
+            }
+        }
     }
 
     if (odd_tile) {
         // Values that are not finite, in tiles of which some rows see only a
         // part: the products left them out, the rows that see them get them.
-        for (int32_t first = begin + static_cast<int32_t>(wave * kKeys); first < end; first += 4 * kKeys) {
-            for (int32_t entry = first; edge_tile(first) && entry < min(first + static_cast<int32_t>(kKeys), end);
-                 ++entry) {
+        for (int32_t at = begin + static_cast<int32_t>(wave * kKeys); at < end; at += kTurn) {
+            for (int32_t entry = at; edge_tile(at) && entry < min(at + static_cast<int32_t>(kKeys), end); ++entry) {
                 const float weight = odd_weight<T, R, D, P == 3>(args, table, keys, query, entry, maximum);
                 const bool visible = entry <= position && entry >= oldest;
                 const Page page = page_of(cache, table, entry);
@@ -566,69 +711,156 @@ __global__ __launch_bounds__(kThreads, 1) void k_paged_step(AttendArgs args) {
         lds.denominator[wave][c] = denominator;
     }
     __syncthreads();
-    {
-        float top = lds.maximum[0][c];
+    const auto factor_of = [&](float m, float top) {
+        return m == kNegative && top == kNegative ? 1.0f : weight_of<P == 3>(m, top, args.log2_scale);
+    };
+    const auto top_of = [&](uint32_t r) {
+        return fmaxf(fmaxf(lds.maximum[0][r], lds.maximum[1][r]), fmaxf(lds.maximum[2][r], lds.maximum[3][r]));
+    };
+    if (c < rows) {
+        const float factor = factor_of(maximum, top_of(c));
 #pragma unroll
-        for (uint32_t w = 1; w < 4u; ++w) {
-            top = fmaxf(top, lds.maximum[w][c]);
-        }
-        const float factor = maximum == kNegative && top == kNegative ? 1.0f
-                                                                        : weight_of<P == 3>(maximum, top, args.log2_scale);
-        if (c < rows) {
+        for (uint32_t i = 0; i < kGroups; ++i) {
 #pragma unroll
-            for (uint32_t i = 0; i < kGroups; ++i) {
+            for (uint32_t r = 0; r < 4u; ++r) {
 #pragma unroll
-                for (uint32_t r = 0; r < 4u; ++r) {
-#pragma unroll
-                    for (uint32_t n = 0; n < kSide; n += 4u) {
-                        *reinterpret_cast<f32x4 *>(&lds.sums[wave][c][16u * kSide * i + kSide * (4u * g + r) + n]) =
-                            f32x4{sums[i][n][r], sums[i][n + 1u][r], sums[i][n + 2u][r], sums[i][n + 3u][r]} * factor;
-                    }
+                for (uint32_t n = 0; n < kSide; n += 4u) {
+                    *reinterpret_cast<f32x4 *>(&lds.sums[wave][c][16u * kSide * i + kSide * (4u * g + r) + n]) =
+                        f32x4{sums[i][n][r], sums[i][n + 1u][r], sums[i][n + 2u][r], sums[i][n + 3u][r]} * factor;
                 }
             }
         }
     }
     __syncthreads();
+    const auto store_row = [&](uint32_t r, uint32_t at, f32x4 sum, float total) {
+        const bool none = first_position + static_cast<int32_t>(r / args.group) < 0;
+        float out[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+            out[k] = none ? 0.0f : sum[k] / total;
+        }
+        store_output<R, 4>(args, s.first + r / args.group, kv * args.group + r % args.group, at, out);
+    };
+    // this part's region of the workspace
+    float *const joint = args.partial + (static_cast<uint64_t>(sequence) * cache.heads + kv) * args.parts * kRegion;
     for (uint32_t i = t; i < rows * (D / 4u); i += kThreads) {
         const uint32_t r = i / (D / 4u), at = i % (D / 4u) * 4u;
-        float top = kNegative;
-#pragma unroll
-        for (uint32_t w = 0; w < 4u; ++w) {
-            top = fmaxf(top, lds.maximum[w][r]);
-        }
+        const float top = top_of(r);
         float total = 0.0f;
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t w = 0; w < 4u; ++w) {
-            const float m = lds.maximum[w][r];
-            total += lds.denominator[w][r] *
-                     (m == kNegative && top == kNegative ? 1.0f : weight_of<P == 3>(m, top, args.log2_scale));
+            total += lds.denominator[w][r] * factor_of(lds.maximum[w][r], top);
             sum += *reinterpret_cast<const f32x4 *>(&lds.sums[w][r][at]);
         }
-        const uint32_t row_token = s.first + r / args.group, row_head = kv * args.group + r % args.group;
-        // a row whose entries are all in this part is done
-        const int32_t place = first_position + static_cast<int32_t>(r / args.group);
-        const int32_t from = window == 0 ? 0 : max(0, place - window + 1);
-        const int32_t part_end = begin + static_cast<int32_t>(args.span);
-        const bool none = place < 0;
-        if (none ? part != 0u : place < begin || from >= part_end) {
-            continue;  // the part holds nothing the row sees
+        if (live == 1u) {
+            store_row(r, at, sum, total);
+            continue;
         }
-        if (none || (from >= begin && place < part_end)) {
-            float out[4];
+        float *const region = joint + static_cast<uint64_t>(part) * kRegion;
+        store_through(region, r * (D + 4u) + at, sum);
+        if (at == 0u) {
+            store_through(region, r * (D + 4u) + D, f32x4{top, total, 0.0f, 0.0f});
+        }
+    }
+    if (live == 1u) {
+        return;
+    }
+    wait_stores();
+    __syncthreads();
+    uint32_t *const ticket = args.tickets + static_cast<uint64_t>(sequence) * cache.heads + kv;
+    if (t == 0u) {
+        lds.last = coherent_add(ticket, 1u) + 1u == live ? 1u : 0u;
+    }
+    __syncthreads();
+    if (lds.last == 0u) {
+        return;
+    }
+    if (t == 0u) {
+        coherent_store(ticket, 0u);
+    }
+    // the parts' levels and denominators, all on their way at once, then a row's
+    // top, factors and total by a wave
+    for (uint32_t i = t; i < live * rows; i += kThreads) {
+        const uint32_t p = i / rows, r = i % rows;
+        const f32x4 v = load_through(joint, p * kRegion + r * (D + 4u) + D);
+        lds.parts.factor[p][r] = v[0];
+        lds.parts.total[p][r] = v[1];
+    }
+    __syncthreads();
+    for (uint32_t r = wave; r < rows; r += 4u) {
+        float m[kStepParts / 64u], top = kNegative, total = 0.0f;
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                out[k] = none ? 0.0f : sum[k] / total;
-            }
-            store_output<R, 4>(args, row_token, row_head, at, out);
-        } else {
-            float *to = partial_row<D>(args, part, row_token, row_head);
-            *reinterpret_cast<f32x4 *>(to + at) = sum;
-            if (at == 0u) {
-                to[D] = top;
-                to[D + 1u] = total;
+        for (uint32_t i = 0; i < kStepParts / 64u; ++i) {
+            m[i] = 64u * i + lane < live ? lds.parts.factor[64u * i + lane][r] : kNegative;
+            top = fmaxf(top, m[i]);
+        }
+        top = fmaxf(top, lane_xor<1>(top));
+        top = fmaxf(top, lane_xor<2>(top));
+        top = fmaxf(top, lane_xor<4>(top));
+        top = fmaxf(top, lane_xor<8>(top));
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
+#pragma unroll
+        for (uint32_t i = 0; i < kStepParts / 64u; ++i) {
+            if (64u * i + lane < live) {
+                const float factor = factor_of(m[i], top);
+                total += lds.parts.total[64u * i + lane][r] * factor;
+                lds.parts.factor[64u * i + lane][r] = factor;
             }
         }
+        total += lane_xor<1>(total);
+        total += lane_xor<2>(total);
+        total += lane_xor<4>(total);
+        total += lane_xor<8>(total);
+        total += lane_xor<16>(total);
+        total += lane_xor<32>(total);
+        if (lane == 0u) {
+            lds.denominator[0][r] = total;
+        }
+    }
+    __syncthreads();
+    // then their sums, four dimensions of a row a thread; where that leaves
+    // threads over, groups of them take the parts in turn
+    const uint32_t items = rows * (D / 4u), groups = max(kThreads / items, 1u);
+    const auto sum_of = [&](uint32_t i, uint32_t from, uint32_t step) {
+        const uint32_t r = i / (D / 4u), at = r * (D + 4u) + i % (D / 4u) * 4u;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr uint32_t kAhead = 16;  // loads on their way at once
+        for (uint32_t p = from; p < live; p += kAhead * step) {
+            f32x4 v[kAhead];
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u) {
+                v[u] = load_through(joint, min(p + u * step, live - 1u) * kRegion + at);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u) {
+                if (p + u * step < live) {
+                    sum += v[u] * lds.parts.factor[p + u * step][r];
+                }
+            }
+        }
+        return sum;
+    };
+    if (groups == 1u) {
+        for (uint32_t i = t; i < items; i += kThreads) {
+            const uint32_t r = i / (D / 4u);
+            store_row(r, i % (D / 4u) * 4u, sum_of(i, 0u, 1u), lds.denominator[0][r]);
+        }
+        return;
+    }
+    f32x4 *const parts = lds.parts.group;
+    if (t < groups * items) {
+        parts[t] = sum_of(t % items, t / items, groups);
+    }
+    __syncthreads();
+    if (t < items) {
+        f32x4 sum = parts[t];
+        for (uint32_t q = 1; q < groups; ++q) {
+            sum += parts[q * items + t];
+        }
+        const uint32_t r = t / (D / 4u);
+        store_row(r, t % (D / 4u) * 4u, sum, lds.denominator[0][r]);
     }
 }
 
@@ -657,8 +889,9 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
             continue;
         }
         const SequenceRows s = sequence_rows(cache, sequence);
-        if (token < s.first || token - s.first >= s.count || s.over || s.length == 0u) {
-            continue;  // (filled by the attention itself)
+        if (token < s.first || token - s.first >= s.count || s.over || s.length == 0u ||
+            (args.mixed != 0u && s.count * args.group <= kStepRows)) {
+            continue;  // (filled by the attention itself, or joined there)
         }
         const int32_t first_position = static_cast<int32_t>(s.length) - static_cast<int32_t>(s.count);
         const int32_t position = first_position + static_cast<int32_t>(token - s.first);
@@ -747,33 +980,6 @@ constexpr uint32_t chunk_rows() {
     return Shape::kRows * Shape::kWaves;
 }
 
-// LDS places: the 16-byte pieces of an entry's D 16-bit values are permuted so
-// that the reads of a phase fall on different banks. Keys: the 16 entries that a
-// phase's lanes read at one piece get different turns. Values: the entries that
-// a transposing read's half wave reads side by side, four at 64 bytes (32
-// rows a wave) or eight at 32 bytes (16). A row of 64 values is half the banks,
-// so two rows share a turn.
-template <uint32_t D, uint32_t ROWS>
-__device__ __forceinline__ uint32_t key_place(uint32_t row, uint32_t piece) {
-    uint32_t turn;
-    if constexpr (ROWS == 32) {
-        turn = D == 64u ? (row >> 1) & 7u : row & 15u;
-    } else {
-        turn = D == 64u ? (row >> 1 & 1u) | (row >> 3 & 3u) << 1 : (row & 3u) | (row >> 3 & 3u) << 2;
-    }
-    return row * (D * 2u) + ((piece ^ turn) << 4);
-}
-template <uint32_t D, uint32_t ROWS>
-__device__ __forceinline__ uint32_t value_place(uint32_t row, uint32_t piece) {
-    uint32_t turn;
-    if constexpr (ROWS == 32) {
-        turn = D == 64u ? (row & 2u) << 1 : (row & 3u) << 2;
-    } else {
-        turn = D == 64u ? (row & 2u) | (row >> 3 & 1u) << 2 : (row & 3u) << 1 | (row >> 3 & 1u) << 3;
-    }
-    return row * (D * 2u) + ((piece ^ turn) << 4);
-}
-
 template <typename T, typename R, uint32_t D>
 constexpr size_t chunk_lds() {
     using Shape = typename ChunkOf<T, R, D>::Shape;
@@ -840,7 +1046,9 @@ void k_paged_chunk(AttendArgs args) {
         if (own < cache.sequences) {
             const uint32_t a = min(cache.offsets[own], cache.tokens), b = min(cache.offsets[own + 1u], cache.tokens);
             const uint32_t count = min(b > a ? b - a : 0u, cache.max_tokens);
-            tiles = (count * args.group + kBlockRows - 1u) / kBlockRows;
+            tiles = args.mixed != 0u && count * args.group <= kStepRows
+                        ? 0u
+                        : (count * args.group + kBlockRows - 1u) / kBlockRows;
         }
         uint32_t sum = tiles;
 #pragma unroll
@@ -1503,66 +1711,81 @@ void k_paged_chunk(AttendArgs args) {
 template <typename T, typename R, uint32_t D>
 void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged_workspace *workspace) {
     const PagedView &c = args.c;
-    const uint32_t heads = c.heads * args.group;
-    constexpr uint32_t kBlockRows = chunk_rows<T, R, D>();
-    const bool step = uint64_t(c.max_tokens) * args.group <= kStepRows;
-    // entries a row tile may see, its base rounded down with a window
-    uint64_t extent = c.max_length;
+    const uint64_t heads = uint64_t(c.heads) * args.group;
+    // entries a sequence's parts may cover, their base rounded down with a window
+    uint64_t extent = std::max(c.max_length, 1u);
     if (args.window != 0) {
         extent = std::min<uint64_t>(extent, uint64_t(args.window) + c.max_tokens + kSpanUnit);
     }
-    const uint64_t row_tiles =
-        step ? c.sequences
-             : std::min<uint64_t>(ceil_div(uint64_t(c.max_tokens) * args.group, kBlockRows) * uint64_t(c.sequences),
-                                  uint64_t(c.tokens) * args.group / kBlockRows + c.sequences);
-    const uint64_t blocks = row_tiles * c.heads;
-    const uint64_t part_bytes = uint64_t(c.tokens) * heads * (D + 4u) * sizeof(float);
-    const uint64_t most = std::max<uint64_t>(
-        std::min<uint64_t>({workspace->bytes / part_bytes, (extent + kSpanUnit - 1) / kSpanUnit, 1024u}), 1u);
-    const auto span_of = [&](uint64_t parts) {
-        return std::max<uint64_t>((ceil_div(extent, parts) + kSpanUnit - 1) / kSpanUnit, 1u) * kSpanUnit;
+    const auto span_of = [&](uint64_t parts, uint64_t unit) {
+        return static_cast<uint32_t>((ceil_div(extent, parts) + unit - 1) / unit * unit);
     };
-    if (step) {
-        // as many parts as give two blocks a CU
-        args.span = static_cast<uint32_t>(
-            span_of(std::clamp<uint64_t>(2u * ctx->cu_count / blocks, 1u, most)));
-    } else {
-        // the parts that end first, in units of 32 keys of a row tile (some 3 us):
-        // rounds of the blocks the chip holds (half a round more where there are
-        // several, for their uneven ends), a block's own start and end worth 6,
-        // and the parts' way through memory at 5 TB/s
-        const double resident = double(ctx->cu_count) * ChunkOf<T, R, D>::Shape::kBlocks;
-        double least = 0.0;
-        for (uint64_t parts = 1; parts <= std::min<uint64_t>(most, 64u); ++parts) {
-            const uint64_t span = span_of(parts);
-            const double count = double(blocks) * ceil_div(extent, span);
-            const double rounds = count <= resident ? 1.0 : count / resident + 0.5;
-            const double joined = span < extent ? 2.0 + 2.0 * part_bytes * ceil_div(extent, span) / 15.0e6 : 0.0;
-            const double cost = rounds * (span / 32.0 + 6.0) + joined;
-            if (parts == 1 || cost < least) {
-                least = cost;
-                args.span = static_cast<uint32_t>(span);
-            }
+    const size_t room = workspace->bytes - kTickets * sizeof(uint32_t);
+    float *const partial = reinterpret_cast<float *>(static_cast<char *>(workspace->base) + kTickets * sizeof(uint32_t));
+    // Few rows of every sequence: k_paged_step. Many of every one (as many as
+    // there may be): k_paged_chunk. Else both, each for its sequences: in the
+    // chunk kernel a single token costs its block a tile's whole staging (31 of
+    // them beside 512 tokens: 62 us of 175).
+    const bool few = uint64_t(c.max_tokens) * args.group <= kStepRows;
+    const bool many = uint64_t(c.sequences) * c.max_tokens == c.tokens || c.sequences == 1;
+    args.mixed = !few && !many ? 1u : 0u;
+    if (few || args.mixed != 0) {
+        require(c.heads < (1u << 16) && c.sequences < (1u << 16), "paged attention: too many heads or sequences");
+        AttendArgs a = args;
+        a.partial = partial;
+        a.tickets = static_cast<uint32_t *>(workspace->base);
+        const uint64_t blocks = uint64_t(c.sequences) * c.heads;
+        const uint64_t region = uint64_t(kStepRows) * (D + 4u) * sizeof(float);
+        uint64_t parts = 1;
+        if (blocks <= kTickets) {
+            // as many as the chip holds blocks
+            parts = std::min<uint64_t>({uint64_t(step_blocks<T, R, D>()) * ctx->cu_count / blocks, room / (blocks * region), kStepParts});
+        }
+        // (one tile a wave at least)
+        constexpr uint64_t kUnit = std::is_same_v<T, float> ? 64 : 128;
+        a.span = span_of(std::max<uint64_t>(parts, 1u), kUnit);
+        a.parts = ceil_div(extent, a.span);
+        launch(ctx, "paged_step", k_paged_step<T, R, D>, dim3(a.parts * c.heads, c.sequences), dim3(kThreads), 0, a);
+        if (few) {
+            return;
         }
     }
-    args.parts = std::max(ceil_div(extent, args.span), 1u);
-    args.partial = static_cast<float *>(workspace->base);
-    if (step) {
-        require(uint64_t(args.parts) * c.heads < (1u << 24) && c.sequences < 65536u,
-                "paged attention: too many heads or sequences");
-        launch(ctx, "paged_step", k_paged_step<T, R, D>, dim3(args.parts * c.heads, c.sequences), dim3(kThreads), 0,
-               args);
-    } else {
-        using Shape = typename ChunkOf<T, R, D>::Shape;
-        constexpr size_t lds = chunk_lds<T, R, D>();
-        static const bool raised = set_lds_limit(reinterpret_cast<const void *>(k_paged_chunk<T, R, D>), lds);
-        (void)raised;
-        const uint64_t pairs = uint64_t(c.heads) * args.parts;
-        const uint64_t grid = (pairs < 8u ? pairs : (pairs + 7u) / 8u * 8u) * row_tiles;
-        require(grid < (1u << 23), "paged attention: too many rows");
-        launch(ctx, "paged_chunk", k_paged_chunk<T, R, D>, dim3(static_cast<uint32_t>(grid)),
-               dim3(Shape::kWaves * 64u), lds, args);
+    using Shape = typename ChunkOf<T, R, D>::Shape;
+    constexpr uint32_t kBlockRows = chunk_rows<T, R, D>();
+    // row tiles at most, and about how many
+    const uint64_t row_tiles =
+        std::min<uint64_t>(ceil_div(uint64_t(c.max_tokens) * args.group, kBlockRows) * uint64_t(c.sequences),
+                           uint64_t(c.tokens) * args.group / kBlockRows + c.sequences);
+    const uint64_t likely = std::min<uint64_t>(row_tiles, ceil_div(uint64_t(c.tokens) * args.group, kBlockRows) +
+                                                              (args.mixed != 0 ? 0u : c.sequences / 2u));
+    // The parts that end first, in units of 32 keys of a row tile (some 3 us):
+    // rounds of the blocks the chip holds (half a round more where there are
+    // several, for their uneven ends), a block's own start and end worth 6, and
+    // the parts' way through memory at 5 TB/s.
+    const uint64_t part_bytes = uint64_t(c.tokens) * heads * (D + 4u) * sizeof(float);
+    const uint64_t most = std::clamp<uint64_t>(room / part_bytes, 1u, 64u);
+    const double resident = double(ctx->cu_count) * Shape::kBlocks;
+    double least = 0.0;
+    for (uint64_t parts = 1; parts <= most; ++parts) {
+        const uint64_t span = span_of(parts, kSpanUnit), real = ceil_div(extent, span);
+        const double count = double(likely * c.heads * real);
+        const double rounds = count <= resident ? 1.0 : count / resident + 0.5;
+        const double cost = rounds * (span / 32.0 + 6.0) + (real > 1 ? 2.0 + 2.0 * part_bytes * real / 15.0e6 : 0.0);
+        if (parts == 1 || cost < least) {
+            least = cost;
+            args.span = static_cast<uint32_t>(span);
+        }
     }
+    args.parts = ceil_div(extent, args.span);
+    args.partial = partial;
+    constexpr size_t lds = chunk_lds<T, R, D>();
+    static const bool raised = set_lds_limit(reinterpret_cast<const void *>(k_paged_chunk<T, R, D>), lds);
+    (void)raised;
+    const uint64_t pairs = uint64_t(c.heads) * args.parts;
+    const uint64_t grid = (pairs < 8u ? pairs : (pairs + 7u) / 8u * 8u) * row_tiles;
+    require(grid < (1u << 23), "paged attention: too many rows");
+    launch(ctx, "paged_chunk", k_paged_chunk<T, R, D>, dim3(static_cast<uint32_t>(grid)), dim3(Shape::kWaves * 64u),
+           lds, args);
     if (args.parts > 1) {
         const uint64_t rows = uint64_t(c.tokens) * heads;
         launch(ctx, "paged_join", k_paged_join<R, D, std::is_same_v<R, float>>,
@@ -1609,8 +1832,8 @@ void paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache, con
     const uint32_t window = std::min(a->window, 1u << 30);
     const AttendArgs args{paged_view(*cache, *batch), rows_view(a->queries), rows_view(a->outputs), rows_view(a->gate),
                           static_cast<float>(scale * 1.4426950408889634),
-                          static_cast<float>(kSlack / (scale * 1.4426950408889634)), window, a->query_heads / cache->heads, 0, 0,
-                          nullptr};
+                          static_cast<float>(kSlack / (scale * 1.4426950408889634)), window, a->query_heads / cache->heads, 0, 0, 0,
+                          nullptr, nullptr};
     if (type == ADI_HIP_F32 && cache->type == ADI_HIP_F32) {
         launch_attention<float, float>(ctx, args, workspace, cache->head_size);
     } else if (type == ADI_HIP_F32) {

@@ -4,6 +4,7 @@
 
 #include "paged.hpp"
 
+// Tickets first, then the parts of histories.
 struct adi_hip_paged_workspace {
     int device;
     void *base;
@@ -11,6 +12,8 @@ struct adi_hip_paged_workspace {
 };
 
 namespace adi_hip {
+
+constexpr uint32_t kTickets = 1u << 16;  // words, zero between calls
 
 // adi_hip_paged_append; with `sines` the rotation of halves is taken from a
 // table [position][sines_half cosines, sines_half sines] instead of a->rope.
