@@ -57,6 +57,7 @@ struct AppendArgs {
     uint32_t half, pairs;      // rotary / 2; whether 2 i and 2 i + 1 turn together
     float magnitude;
     uint32_t query_heads, parts;
+    uint32_t run;              // tokens of a block, one after another
     float weight_offset, epsilon;
 };
 
@@ -79,120 +80,203 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 template <typename T, uint32_t N>
-struct alignas(sizeof(T) * N) Vector {
+struct alignas(sizeof(T) * N < 16u ? sizeof(T) * N : 16u) Vector {
     T v[N];
 };
 
-// A part of a token's heads (queries, then keys, then values), D / N lanes a
-// head of N = 16 bytes of input each, so a head stays within a wave. The token's
-// sequence is the number of sequences that end at or before it, counted 64
-// at a time; its sines go through LDS once a block, a head's partner dimensions
-// through the wave's own piece of LDS.
+constexpr uint32_t kAhead = 2;  // tokens whose rows are on their way
+
+// A part of the heads (queries, then keys, then values) of a run of tokens, D / N
+// lanes a head of N = 16 bytes of input each, so a head stays within a wave.
+// The token's sequence is the number of sequences that end at or before it,
+// counted 64 at a time with what is needed of them; its sines go through LDS once
+// a block, a head's partner dimensions through the wave's own piece of LDS.
+//
+// Bound by a block's chain of loads (offsets and lengths, page, store) where the
+// tokens are few (4.1 us for one, 4.3 for 32), by the rows' bytes where they are
+// many: 2,919 tokens of 32 + 8 + 8 heads of 128 in bf16, 72 MB, take 17.6 us, 4.1
+// TB/s. A block a token and part waited out that chain and its sines for every
+// one, and read its partners from LDS by the element: 28.9.
 template <typename R, typename C, uint32_t D>
 __global__ __launch_bounds__(kThreads) void k_paged_append(AppendArgs args) {
     constexpr uint32_t N = 16u / sizeof(R), L = D / N, kRows = kThreads / L;
-    __shared__ float2 wave_of[D / 2u];
+    __shared__ __align__(16) float cosine[D / 2u], sine[D / 2u];
     __shared__ __align__(16) float turned[kThreads * N];
     const PagedView &c = args.c;
-    const uint32_t t = threadIdx.x, lane = t & 63u;
-    const uint64_t jobs = static_cast<uint64_t>(c.tokens) * args.parts;
-    for (uint64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const uint32_t token = static_cast<uint32_t>(job / args.parts);
-        const uint32_t row = static_cast<uint32_t>(job % args.parts) * kRows + t / L;
-        const uint32_t at = (t % L) * N;
-        const uint32_t rows = args.query_heads + 2u * c.heads;
-        // 0 queries, 1 keys, 2 values
-        const uint32_t kind = row < args.query_heads ? 0u : row < args.query_heads + c.heads ? 1u : 2u;
-        const uint32_t head = kind == 0u ? row : (row - args.query_heads) - (kind - 1u) * c.heads;
-        const bool live = row < rows;
-        using V = Vector<R, N>;
-        V in{};
-        if (live) {
-            const RowsView &from = kind == 0u ? args.queries : kind == 1u ? args.keys : args.values;
-            in = *reinterpret_cast<const V *>(reinterpret_cast<const R *>(from.data) + token * from.token_stride +
-                                              head * from.head_stride + at);
+    const uint32_t t = threadIdx.x, lane = t & 63u, at = (t % L) * N;
+    const uint32_t rows = args.query_heads + 2u * c.heads;
+    const bool whole = args.half % (args.pairs != 0u ? N / 2u : N) == 0u;
+    // (at most D / 2 of them, so one a thread)
+    const double turns = args.turns != nullptr && t < args.half ? args.turns[t] : 0.0;
+    const uint32_t row = blockIdx.x % args.parts * kRows + t / L;
+    const bool live = row < rows;
+    // 0 queries, 1 keys, 2 values
+    const uint32_t kind = row < args.query_heads ? 0u : row < args.query_heads + c.heads ? 1u : 2u;
+    const uint32_t head = kind == 0u ? row : (row - args.query_heads) - (kind - 1u) * c.heads;
+    const RowsView &source = kind == 0u ? args.queries : kind == 1u ? args.keys : args.values;
+    const R *const in = reinterpret_cast<const R *>(source.data) + head * source.head_stride + at;
+    const uint64_t in_stride = source.token_stride;
+    R *const out = reinterpret_cast<R *>(args.queries_out.data) + head * args.queries_out.head_stride + at;
+    C *const pool = reinterpret_cast<C *>(kind == 1u ? c.keys : c.values) + head * c.head_stride + at;
+    const uint16_t *const norm = kind == 0u ? args.query_norm : kind == 1u ? args.key_norm : nullptr;
+    const bool norms = args.query_norm != nullptr || args.key_norm != nullptr;
+    float weight[N];
+    if (norms) {
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) {
+            weight[k] = norm != nullptr ? args.weight_offset + bf16_of(norm[at + k]) : 1.0f;
         }
-        uint32_t sequence = 0;
-        for (uint32_t s = 0; s < c.sequences; s += 64u) {
-            const bool before = s + lane < c.sequences && c.offsets[s + lane + 1u] <= token;
-            const uint32_t ended = static_cast<uint32_t>(__popcll(__ballot(before)));
-            sequence += ended;
-            if (ended < 64u) {
-                break;
+    }
+    const uint32_t from = blockIdx.x / args.parts * args.run, to = min(from + args.run, c.tokens);
+    using V = Vector<R, N>;
+    V next[kAhead] = {};
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) {
+        if (live && from + u < to) {
+            next[u] = *reinterpret_cast<const V *>(in + (from + u) * in_stride);
+        }
+    }
+    uint32_t sequence = ~0u, page = ~0u, page_index = ~0u;
+    SequenceRows rows_of{};
+    for (uint32_t token = from; token < to; ++token) {
+        float x[N];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) {
+            x[k] = static_cast<float>(next[0].v[k]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u + 1u < kAhead; ++u) {
+            next[u] = next[u + 1u];
+        }
+        if (live && token + kAhead < to) {
+            next[kAhead - 1u] = *reinterpret_cast<const V *>(in + (token + kAhead) * in_stride);
+        }
+        if (sequence == ~0u || token - rows_of.first >= rows_of.count) {
+            sequence = ~0u;
+            page_index = ~0u;
+            for (uint32_t s = 0; s < c.sequences; s += 64u) {
+                const uint32_t own = min(s + lane, c.sequences - 1u);
+                const uint32_t a = min(c.offsets[own], c.tokens), b = min(c.offsets[own + 1u], c.tokens);
+                const uint32_t length = c.lengths[own];
+                const uint32_t ended =
+                    static_cast<uint32_t>(__popcll(__ballot(s + lane < c.sequences && b <= token)));
+                if (ended < 64u) {
+                    if (s + ended < c.sequences) {
+                        const auto of = [&](uint32_t v) {
+                            return static_cast<uint32_t>(
+                                __builtin_amdgcn_readlane(static_cast<int>(v), static_cast<int>(ended)));
+                        };
+                        const uint32_t first = of(a), end = of(b);
+                        sequence = s + ended;
+                        rows_of.first = first;
+                        rows_of.count = end > first ? end - first : 0u;
+                        rows_of.length = of(length);
+                        rows_of.over = rows_of.count > c.max_tokens || rows_of.length > c.max_length;
+                    }
+                    break;
+                }
             }
         }
-        if (sequence >= c.sequences) {  // uniform over the block
-            continue;
-        }
-        const SequenceRows rows_of = sequence_rows(c, sequence);
-        if (token < rows_of.first || token - rows_of.first >= rows_of.count) {
+        // (uniform over the block)
+        if (sequence == ~0u || token < rows_of.first || token - rows_of.first >= rows_of.count) {
             continue;
         }
         const int64_t place = static_cast<int64_t>(rows_of.length) - rows_of.count + (token - rows_of.first);
         const bool held = !rows_of.over && place >= 0;
         const uint32_t position = held ? static_cast<uint32_t>(place) : 0u;
-        const uint32_t page =
-            held ? c.table[static_cast<uint64_t>(sequence) * c.table_stride + (position >> c.page_shift)] : ~0u;
-        if (args.half != 0u) {
-            for (uint32_t i = t; i < args.half; i += kThreads) {
-                if (args.sines != nullptr) {
-                    const float *from = args.sines + static_cast<uint64_t>(position) * 2u * args.half;
-                    wave_of[i] = make_float2(from[i], from[args.half + i]);
-                } else {
-                    const Turn turn = turn_of(position, args.turns[i]);
-                    wave_of[i] = make_float2(turn.cosine * args.magnitude, turn.sine * args.magnitude);
-                }
-            }
-            __syncthreads();
+        if (!held) {
+            page = ~0u;
+            page_index = ~0u;
+        } else if (position >> c.page_shift != page_index) {
+            page_index = position >> c.page_shift;
+            page = c.table[static_cast<uint64_t>(sequence) * c.table_stride + page_index];
         }
-        float x[N];
-#pragma unroll
-        for (uint32_t k = 0; k < N; ++k) {
-            x[k] = static_cast<float>(in.v[k]);
-        }
-        const uint16_t *norm = kind == 0u ? args.query_norm : kind == 1u ? args.key_norm : nullptr;
-        if (args.query_norm != nullptr || args.key_norm != nullptr) {
+        if (norms) {
             float squares = 0.0f;
 #pragma unroll
             for (uint32_t k = 0; k < N; ++k) {
                 squares += x[k] * x[k];
             }
             squares = row_sum<L>(squares);
-            if (norm != nullptr) {
-                const float scale = 1.0f / sqrtf(squares / static_cast<float>(D) + args.epsilon);
+            const float scale = norm != nullptr ? 1.0f / sqrtf(squares / static_cast<float>(D) + args.epsilon) : 1.0f;
 #pragma unroll
-                for (uint32_t k = 0; k < N; ++k) {
-                    x[k] *= scale * (args.weight_offset + bf16_of(norm[at + k]));
-                }
+            for (uint32_t k = 0; k < N; ++k) {
+                x[k] *= scale * weight[k];
             }
         }
         if (args.half != 0u) {
+            if (token != from) {
+                __syncthreads();  // the last token's sines are used
+            }
+            if (t < args.half) {
+                if (args.sines != nullptr) {
+                    const float *values = args.sines + static_cast<uint64_t>(position) * 2u * args.half;
+                    cosine[t] = values[t];
+                    sine[t] = values[args.half + t];
+                } else {
+                    const Turn turn = turn_of(position, turns);
+                    cosine[t] = turn.cosine * args.magnitude;
+                    sine[t] = turn.sine * args.magnitude;
+                }
+            }
             float *const own = turned + t / L * D;
             if (args.pairs == 0u) {
-#pragma unroll
-                for (uint32_t k = 0; k < N; ++k) {
-                    own[at + k] = x[k];
-                }
-                // (a head's lanes are one wave's: its LDS accesses stay in order)
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                // (read back behind the barrier)
+                store_values<float, N>(own + at, x);
             }
-            if (kind != 2u) {
-                float y[N];
+            __syncthreads();
+            if (kind != 2u && at < 2u * args.half) {
+                float y[N] = {};
+                if (whole) {
+                    // the lane's dimensions are all first or all second ones of
+                    // their pairs, or whole pairs: LDS in 16 bytes (by the
+                    // element, lanes 32 bytes apart meet on eight banks)
+                    using F = Vector<float, N>;
+                    using H = Vector<float, N / 2u>;
+                    if (args.pairs != 0u) {
+                        const H w = *reinterpret_cast<const H *>(cosine + at / 2u);
+                        const H z = *reinterpret_cast<const H *>(sine + at / 2u);
 #pragma unroll
-                for (uint32_t k = 0; k < N; ++k) {
-                    const uint32_t d = at + k;
-                    if (d >= 2u * args.half) {
-                        y[k] = x[k];
-                    } else if (args.pairs != 0u) {
-                        const float2 w = wave_of[d >> 1];
-                        y[k] = k & 1u ? x[k] * w.x + x[k ^ 1u] * w.y : x[k] * w.x - x[k ^ 1u] * w.y;
+                        for (uint32_t k = 0; k < N; ++k) {
+                            y[k] = k & 1u ? x[k] * w.v[k / 2u] + x[k ^ 1u] * z.v[k / 2u]
+                                          : x[k] * w.v[k / 2u] - x[k ^ 1u] * z.v[k / 2u];
+                        }
                     } else {
-                        const bool second = d >= args.half;
-                        const float2 w = wave_of[second ? d - args.half : d];
-                        const float other = own[second ? d - args.half : d + args.half];
-                        y[k] = second ? x[k] * w.x + other * w.y : x[k] * w.x - other * w.y;
+                        const bool second = at >= args.half;
+                        const uint32_t pair = second ? at - args.half : at;
+                        const F w = *reinterpret_cast<const F *>(cosine + pair);
+                        const F z = *reinterpret_cast<const F *>(sine + pair);
+                        const F other = *reinterpret_cast<const F *>(own + (second ? pair : pair + args.half));
+                        const float sign = second ? 1.0f : -1.0f;
+#pragma unroll
+                        for (uint32_t k = 0; k < N; ++k) {
+                            y[k] = x[k] * w.v[k] + other.v[k] * (sign * z.v[k]);
+                        }
+                    }
+                } else {
+#pragma unroll 1
+                    for (uint32_t k = 0; k < N; ++k) {
+                        const uint32_t d = at + k;
+                        float value = x[0];
+#pragma unroll
+                        for (uint32_t i = 1; i < N; ++i) {
+                            value = i == k ? x[i] : value;
+                        }
+                        if (d < 2u * args.half) {
+                            float beside = 0.0f;
+#pragma unroll
+                            for (uint32_t i = 0; i < N; ++i) {
+                                beside = (i ^ 1u) == k ? x[i] : beside;
+                            }
+                            const bool second = args.pairs != 0u ? (k & 1u) != 0u : d >= args.half;
+                            const uint32_t pair = args.pairs != 0u ? d >> 1 : second ? d - args.half : d;
+                            const float other = args.pairs != 0u ? beside : own[second ? pair : d + args.half];
+                            value = value * cosine[pair] + (second ? other : -other) * sine[pair];
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < N; ++i) {
+                            y[i] = i == k ? value : y[i];
+                        }
                     }
                 }
 #pragma unroll
@@ -202,41 +286,42 @@ __global__ __launch_bounds__(kThreads) void k_paged_append(AppendArgs args) {
             }
         }
         if (live && kind == 0u) {
-            V out;
+            if (rows_of.over) {
 #pragma unroll
-            for (uint32_t k = 0; k < N; ++k) {
-                out.v[k] = static_cast<R>(rows_of.over ? __builtin_nanf("") : x[k]);
+                for (uint32_t k = 0; k < N; ++k) {
+                    x[k] = __builtin_nanf("");
+                }
             }
-            *reinterpret_cast<V *>(reinterpret_cast<R *>(args.queries_out.data) +
-                                   token * args.queries_out.token_stride + head * args.queries_out.head_stride + at) =
-                out;
+            store_values<R, N>(out + token * args.queries_out.token_stride, x);
         } else if (live && page < c.pages) {
-            Vector<C, N> out;
-#pragma unroll
-            for (uint32_t k = 0; k < N; ++k) {
-                out.v[k] = static_cast<C>(x[k]);
-            }
-            C *const pool = reinterpret_cast<C *>(kind == 1u ? c.keys : c.values);
-            *reinterpret_cast<Vector<C, N> *>(pool + page * c.page_stride +
-                                              (position & ((1u << c.page_shift) - 1u)) * c.entry_stride +
-                                              head * c.head_stride + at) = out;
-        }
-        if (args.half != 0u && gridDim.x < jobs) {
-            __syncthreads();  // the next token's sines
+            store_values<C, N>(pool + page * c.page_stride + (position & ((1u << c.page_shift) - 1u)) * c.entry_stride,
+                               x);
         }
     }
 }
 
-template <typename R, typename C>
-void launch_append(adi_hip_context *ctx, AppendArgs args, uint32_t head_size) {
-    const uint32_t lanes = head_size / (16u / sizeof(R)), rows = args.query_heads + 2u * args.c.heads;
-    args.parts = ceil_div(rows, kThreads / lanes);
+template <typename R, typename C, uint32_t D>
+void launch_append(adi_hip_context *ctx, AppendArgs args) {
+    constexpr uint32_t kRows = kThreads / (D / (16u / sizeof(R)));
+    args.parts = ceil_div(args.query_heads + 2u * args.c.heads, kRows);
+    // runs of tokens where there are more than six blocks a CU, what their registers
+    // let it hold (2,919 tokens: 17.6 us; 3, 4, 8 and 12 blocks 19.4, 17.8, 18.8, 19.0)
     const uint64_t jobs = static_cast<uint64_t>(args.c.tokens) * args.parts;
-    const dim3 grid(static_cast<uint32_t>(std::min<uint64_t>(jobs, 1u << 20)));
-    const auto kernel = head_size == 64    ? k_paged_append<R, C, 64>
-                        : head_size == 128 ? k_paged_append<R, C, 128>
-                                           : k_paged_append<R, C, 256>;
-    launch(ctx, "paged_append", kernel, grid, dim3(kThreads), 0, args);
+    args.run = std::max(ceil_div(jobs, 6u * static_cast<uint64_t>(ctx->cu_count)), 1u);
+    const uint64_t grid = static_cast<uint64_t>(ceil_div(args.c.tokens, args.run)) * args.parts;
+    require(grid < (1u << 23), "paged append: too many heads");
+    launch(ctx, "paged_append", k_paged_append<R, C, D>, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, args);
+}
+
+template <typename R, typename C>
+void launch_append(adi_hip_context *ctx, const AppendArgs &args, uint32_t head_size) {
+    if (head_size == 64) {
+        launch_append<R, C, 64>(ctx, args);
+    } else if (head_size == 128) {
+        launch_append<R, C, 128>(ctx, args);
+    } else {
+        launch_append<R, C, 256>(ctx, args);
+    }
 }
 
 }  // namespace
@@ -268,7 +353,7 @@ void paged_append(adi_hip_context *ctx, const adi_hip_paged_cache *cache, const 
     const bool weighted = a->query_heads != 0;
     AppendArgs args{paged_view(*cache, *batch), rows_view(a->keys), rows_view(a->values), rows_view(a->queries),
                     rows_view(a->queries_out), a->key_norm, weighted ? a->query_norm : nullptr, nullptr, sines,
-                    sines_half, 0, 1.0f, a->query_heads, 0, a->weight_offset, a->epsilon};
+                    sines_half, 0, 1.0f, a->query_heads, 0, 1, a->weight_offset, a->epsilon};
     if (a->rope != nullptr) {
         args.turns = a->rope->turns;
         args.half = a->rope->rotary / 2;

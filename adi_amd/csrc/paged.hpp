@@ -69,6 +69,48 @@ __device__ __forceinline__ SequenceRows sequence_rows(const PagedView &c, uint32
 
 __device__ __forceinline__ float bf16_of(uint32_t bits) { return __uint_as_float(bits << 16); }
 
+// Two floats rounded to nearest and packed.
+template <typename T>
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {x, y};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
+}
+
+// N floats (1, 2, 4 or 8) rounded to T and stored side by side in as few stores
+// as their bytes take (as an array of T the compiler stores them in pieces), `to`
+// aligned to them or to 16 bytes.
+template <typename T, uint32_t N>
+__device__ __forceinline__ void store_values(T *to, const float (&v)[N]) {
+    constexpr uint32_t kWords = N * sizeof(T) / 4u;
+    if constexpr (kWords == 0u) {
+        *to = static_cast<T>(v[0]);
+    } else {
+        uint32_t word[kWords];
+#pragma unroll
+        for (uint32_t i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4u) {
+                word[i] = __float_as_uint(v[i]);
+            } else {
+                word[i] = pack<T>(v[2u * i], v[2u * i + 1u]);
+            }
+        }
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        if constexpr (kWords == 1u) {
+            *reinterpret_cast<uint32_t *>(to) = word[0];
+        } else if constexpr (kWords == 2u) {
+            *reinterpret_cast<u32x2 *>(to) = u32x2{word[0], word[1]};
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kWords; i += 4u) {
+                reinterpret_cast<u32x4 *>(to)[i / 4u] = u32x4{word[i], word[i + 1u], word[i + 2u], word[i + 3u]};
+            }
+        }
+    }
+}
+
 // cos and sin of `position` times a frequency of `turns` a position: the
 // product and its whole quarter turns in 64 bits (exact to 2^-21 of a turn at
 // position 2^32, 2^-35 at 2^18), then the Taylor sums on an eighth of a turn

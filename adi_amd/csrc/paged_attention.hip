@@ -87,16 +87,6 @@ __device__ __forceinline__ float weight_of(float s, float m, float log2_scale) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack(float x, float y) {
-    const f32x2 v = {x, y};
-    if constexpr (std::is_same_v<T, _Float16>) {
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-    } else {
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-    }
-}
-
 // Two floats as pairs of 16-bit pieces: one, rounded to nearest; three bf16
 // pieces whose sum they are, exactly (an infinity gives NaN); or two f16 pieces,
 // 22 bits, of values scaled to f16's range.
@@ -241,13 +231,9 @@ __device__ __forceinline__ void store_output(const AttendArgs &a, uint32_t token
             v[k] *= 1.0f / (1.0f + expf(-static_cast<float>(g.v[k])));
         }
     }
-    Vector out;
-#pragma unroll
-    for (uint32_t k = 0; k < N; ++k) {
-        out.v[k] = static_cast<R>(v[k]);
-    }
-    *reinterpret_cast<Vector *>(reinterpret_cast<R *>(a.outputs.data) + token * a.outputs.token_stride +
-                                head * a.outputs.head_stride + at) = out;
+    store_values<R, N>(reinterpret_cast<R *>(a.outputs.data) + token * a.outputs.token_stride +
+                           head * a.outputs.head_stride + at,
+                       v);
 }
 
 // Rows of a sequence that nothing is computed for: NaN where it is over the

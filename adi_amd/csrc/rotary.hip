@@ -126,24 +126,24 @@ __global__ __launch_bounds__(kThreads) void k_rope_rows(RopeArgs args) {
             const uint32_t first = PAIRS ? 2u * unit * N : unit * N;
             const uint32_t second = PAIRS ? first + N : first + args.pairs;
             const V u = *reinterpret_cast<const V *>(x + first), v = *reinterpret_cast<const V *>(x + second);
-            V p, q;
+            float p[N], q[N];
 #pragma unroll
             for (uint32_t k = 0; k < N; ++k) {
                 const float2 w = wave[unit * N + k];
                 const auto element = [&](const V &lo, const V &hi, uint32_t i) { return i < N ? lo.v[i] : hi.v[i - N]; };
                 const float a = static_cast<float>(PAIRS ? element(u, v, 2u * k) : u.v[k]);
                 const float b = static_cast<float>(PAIRS ? element(u, v, 2u * k + 1u) : v.v[k]);
-                const T turned_a = static_cast<T>(a * w.x - b * w.y), turned_b = static_cast<T>(b * w.x + a * w.y);
+                const float turned_a = a * w.x - b * w.y, turned_b = b * w.x + a * w.y;
                 if constexpr (PAIRS) {
-                    (2u * k < N ? p.v[(2u * k) % N] : q.v[(2u * k) % N]) = turned_a;
-                    (2u * k + 1u < N ? p.v[(2u * k + 1u) % N] : q.v[(2u * k + 1u) % N]) = turned_b;
+                    (2u * k < N ? p[(2u * k) % N] : q[(2u * k) % N]) = turned_a;
+                    (2u * k + 1u < N ? p[(2u * k + 1u) % N] : q[(2u * k + 1u) % N]) = turned_b;
                 } else {
-                    p.v[k] = turned_a;
-                    q.v[k] = turned_b;
+                    p[k] = turned_a;
+                    q[k] = turned_b;
                 }
             }
-            *reinterpret_cast<V *>(y + first) = p;
-            *reinterpret_cast<V *>(y + second) = q;
+            store_values<T, N>(y + first, p);
+            store_values<T, N>(y + second, q);
         }
         __syncthreads();
     }

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -241,14 +242,14 @@ SIGNATURES = [
      [C.POINTER(RopeOptions), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     ("adi_hip_rope_create", C.c_int, [vp, C.POINTER(RopeOptions), C.POINTER(vp)]),
     ("adi_hip_rope_destroy", None, [vp]),
-    ("adi_hip_rope_rows", C.c_int, [vp, vp, C.POINTER(Rows), u32, u32, u32, vp, C.POINTER(Rows)]),
+    ("adi_hip_rope_rows", C.c_int, [vp, vp, vp, u32, u32, u32, vp, vp]),
     ("adi_hip_paged_check", C.c_int, [C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct)]),
     ("adi_hip_paged_append", C.c_int,
-     [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), C.POINTER(PagedAppendArguments)]),
+     [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), vp]),
     ("adi_hip_paged_workspace_create", C.c_int, [vp, C.c_size_t, C.POINTER(vp)]),
     ("adi_hip_paged_workspace_destroy", None, [vp]),
     ("adi_hip_paged_attention", C.c_int,
-     [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), C.POINTER(PagedAttentionArguments), vp]),
+     [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), vp, vp]),
     ("adi_hip_profiling_enable", C.c_int, [vp, C.c_int]),
     ("adi_hip_profiling_read", C.c_int, [vp, C.POINTER(KernelProfile), u32, C.POINTER(u32)]),
     # include/adi_hip_gguf.h
@@ -1154,43 +1155,59 @@ def _type_of(t) -> int:
     return code
 
 
-def _rows(ctx: Context, t, tokens: int, heads: Optional[int], head_size: int) -> Rows:
+# The calls of a decode step take some 10 us on the device, so their arguments
+# are packed as the structures' bytes (Rows, PagedAppendArguments,
+# PagedAttentionArguments), in a fraction of the time their fields take to set.
+_pack_rows = struct.Struct("=I4xQQQ").pack
+_pack_append = struct.Struct("=Q I4xQQQ I4xQQQ Q I4x I4xQQQ I4xQQQ Q f f").pack
+_pack_attention = struct.Struct("=I4x I4xQQQ I4xQQQ I4xQQQ f I").pack
+_no_rows = (0, 0, 0, 0)
+
+
+def _rows(ctx: Context, t, tokens: int, heads: Optional[int], head_size: int):
     """A tensor [tokens, heads, head size] (any strides of the first two) as
-    adi_hip_rows."""
-    shape, stride = t.shape, t.stride()
+    the fields of adi_hip_rows."""
+    shape = t.shape
     if len(shape) != 3 or shape[0] != tokens or shape[2] != head_size or (heads is not None and shape[1] != heads):
         _refuse(f"rows of shape {tuple(shape)}, expected [{tokens}, {heads or 'heads'}, {head_size}]")
-    if stride[2] != 1 and shape[2] > 1:
+    token_stride, head_stride, step = t.stride()
+    if step != 1 and head_size > 1:
         _refuse("a head's elements must be contiguous")
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         _refuse(f"rows on {t.device}, the context is on cuda:{ctx.device}")
-    if stride[0] == 0 and shape[0] > 1 or stride[1] == 0 and shape[1] > 1:
+    if (token_stride == 0 and shape[0] > 1) or (head_stride == 0 and shape[1] > 1):
         _refuse("broadcast rows are not supported")
-    return Rows(_type_of(t), t.data_ptr(), stride[0], stride[1])
+    return _type_codes.get(t.dtype) if t.dtype in _type_codes else _type_of(t), t.data_ptr(), token_stride, head_stride
 
 
 def _device_words(ctx: Context, t, name: str, *shape):
     """A contiguous int32 (or uint32) tensor of the context's device."""
-    if tuple(t.shape) != shape or not t.is_contiguous() or t.element_size() != 4 or t.is_floating_point():
+    if t.shape != shape or not t.is_contiguous() or _dtype_name(t) not in ("int32", "uint32"):
         _refuse(f"{name} must be a contiguous int32 tensor of shape {shape}")
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         _refuse(f"{name} on {t.device}, the context is on cuda:{ctx.device}")
     return t
 
 
-def _bf16_weight(ctx: Context, t, size: int) -> Optional[int]:
+def _bf16_weight(ctx: Context, t, size: int) -> int:
     if t is None:
-        return None
-    if tuple(t.shape) != (size,) or not t.is_contiguous() or t.element_size() != 2 or _dtype_name(t) not in (
-            "bfloat16", "int16"):
+        return 0
+    if t.shape != (size,) or t.stride(0) != 1 or _dtype_name(t) not in ("bfloat16", "int16"):
         _refuse(f"a norm weight must be {size} contiguous bf16 values")
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         _refuse(f"a norm weight on {t.device}, the context is on cuda:{ctx.device}")
     return t.data_ptr()
 
 
+_dtype_names: dict = {}
+
+
 def _dtype_name(t) -> str:
-    return str(t.dtype).replace("torch.", "")
+    dtype = t.dtype
+    name = _dtype_names.get(dtype)
+    if name is None:
+        name = _dtype_names[dtype] = str(dtype).replace("torch.", "")
+    return name
 
 
 def _rope_options(rotary, layout, theta, scaling, factor, original, fast, slow, magnitude) -> RopeOptions:
@@ -1247,7 +1264,8 @@ def rope_rows(ctx: Context, rope: Rope, x, positions, out) -> None:
     tokens, heads, size = x.shape
     a, b = _rows(ctx, x, tokens, heads, size), _rows(ctx, out, tokens, heads, size)
     _device_words(ctx, positions, "positions", tokens)
-    status = ctx.lib.adi_hip_rope_rows(ctx.handle, rope.handle, a, tokens, heads, size, positions.data_ptr(), b)
+    status = ctx.lib.adi_hip_rope_rows(ctx.handle, rope.handle, _pack_rows(*a), tokens, heads, size,
+                                       positions.data_ptr(), _pack_rows(*b))
     if status:
         ctx.check(status)
 
@@ -1261,7 +1279,7 @@ class PagedCache:
         if keys.dim() != 4 or keys.shape != values.shape or keys.stride() != values.stride() or \
                 keys.dtype != values.dtype or keys.stride(3) != 1:
             _refuse("a paged cache needs keys and values [pages, page size, heads, head size] of one type and layout")
-        if not keys.is_cuda or keys.device.index != ctx.device or values.device != keys.device:
+        if keys.get_device() != ctx.device or values.get_device() != ctx.device:
             _refuse(f"a paged cache on {keys.device}, the context is on cuda:{ctx.device}")
         pages, page_size, heads, size = keys.shape
         self.keys, self.values = keys, values
@@ -1325,9 +1343,6 @@ class PagedWorkspace:
             pass
 
 
-_no_rows = Rows()
-
-
 def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, keys, values, rope: Optional[Rope] = None,
                  key_norm=None, queries=None, query_norm=None, queries_out=None, weight_offset: float = 1.0,
                  epsilon: float = 1e-6) -> None:
@@ -1341,9 +1356,12 @@ def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, keys, value
         heads = queries.shape[1]
         q = _rows(ctx, queries, n, heads, size)
         o = q if queries_out is None else _rows(ctx, queries_out, n, heads, size)
-    a = PagedAppendArguments(rope.handle if rope is not None else None, _rows(ctx, keys, n, cache.heads, size),
-                             _rows(ctx, values, n, cache.heads, size), _bf16_weight(ctx, key_norm, size), heads, q, o,
-                             _bf16_weight(ctx, query_norm, size), weight_offset, epsilon)
+    a = _pack_append((rope.handle.value or 0) if rope is not None and rope.handle else 0,
+                     *_rows(ctx, keys, n, cache.heads, size), *_rows(ctx, values, n, cache.heads, size),
+                     _bf16_weight(ctx, key_norm, size), heads, *q, *o, _bf16_weight(ctx, query_norm, size),
+                     weight_offset, epsilon)
+    if rope is not None and not rope.handle:
+        _refuse("the rope is closed")
     status = ctx.lib.adi_hip_paged_append(ctx.handle, cache.struct, batch.struct, a)
     if status:
         ctx.check(status)
@@ -1355,8 +1373,10 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, queries,
     sequences' pages into out, times sigmoid(gate) where given; scale 0 is
     1 / sqrt(head size), window 0 none."""
     n, size, heads = batch.tokens, cache.head_size, queries.shape[1]
-    a = PagedAttentionArguments(heads, _rows(ctx, queries, n, heads, size), _rows(ctx, out, n, heads, size),
-                                _no_rows if gate is None else _rows(ctx, gate, n, heads, size), scale, window)
+    if not 0 <= window < 1 << 32:
+        _refuse("paged attention: window is out of range")
+    a = _pack_attention(heads, *_rows(ctx, queries, n, heads, size), *_rows(ctx, out, n, heads, size),
+                        *(_no_rows if gate is None else _rows(ctx, gate, n, heads, size)), scale, window)
     status = ctx.lib.adi_hip_paged_attention(ctx.handle, cache.struct, batch.struct, a, workspace.handle)
     if status:
         ctx.check(status)

@@ -42,6 +42,16 @@ def test_struct_layouts_match_header(tmp_path):
             assert want[(cname, field)] == getattr(ctype, field).offset, (cname, field)
 
 
+def test_packed_arguments_are_the_structures():
+    rows = [(i, 10 * i + 1, 10 * i + 2, 10 * i + 3) for i in range(5)]
+    assert hip._pack_rows(*rows[1]) == bytes(hip.Rows(*rows[1]))
+    assert hip._pack_append(77, *rows[0], *rows[1], 78, 79, *rows[2], *rows[3], 80, 1.5, 2.5) == bytes(
+        hip.PagedAppendArguments(77, hip.Rows(*rows[0]), hip.Rows(*rows[1]), 78, 79, hip.Rows(*rows[2]),
+                                 hip.Rows(*rows[3]), 80, 1.5, 2.5))
+    assert hip._pack_attention(9, *rows[1], *rows[2], *rows[3], 0.5, 6) == bytes(
+        hip.PagedAttentionArguments(9, hip.Rows(*rows[1]), hip.Rows(*rows[2]), hip.Rows(*rows[3]), 0.5, 6))
+
+
 # ---- frequencies --------------------------------------------------------------
 
 def close(got, want):
