@@ -30,6 +30,7 @@
 // reductions); results agree to float rounding.
 #include "attention.hpp"
 #include "dense.hpp"
+#include "paged_attention.hpp"
 #include "projection.hpp"
 
 #include <algorithm>
@@ -1545,6 +1546,58 @@ void full_attention_chunk(adi_hip_context *ctx, const adi_hip_full_attention *L,
     project_output(ctx, &L->output, attended, count, outputs, norm_tail);
 }
 
+// full_attention_forward for a batch of sequences whose entries lie in pages:
+// the projections over all rows, then norm, rotation (from the same table of the
+// reference's float angles as the contiguous caches') and append in one launch,
+// the gated attention, and the output projection.
+void full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *L, const adi_hip_paged_cache *cache,
+                          const adi_hip_paged_batch *batch, const float *inputs, float *outputs,
+                          adi_hip_paged_workspace *workspace) {
+    require_paged(cache, batch);
+    require(L != nullptr && workspace != nullptr, "paged full attention: null argument");
+    require(cache->heads == kKvHeads && cache->head_size == kHeadSize && cache->type != ADI_HIP_F16,
+            "paged full attention: the cache must hold 2 heads of 256 in f32 or bf16");
+    const uint32_t hidden = L->query.columns, count = batch->tokens;
+    require(ne_shaped(L->query, kQueryHeads * kQueryStride, hidden) &&
+                ne_shaped(L->key, kKvHeads * kHeadSize, hidden) &&
+                ne_shaped(L->value, kKvHeads * kHeadSize, hidden) &&
+                ne_shaped(L->output, hidden, kQueryHeads * kHeadSize) && L->query_norm != nullptr &&
+                L->key_norm != nullptr,
+            "full attention state or input shape mismatch");
+    if (count == 0 || batch->sequences == 0) {
+        return;
+    }
+    require(inputs != nullptr && outputs != nullptr, "full attention state or input shape mismatch");
+    auto &ws = ctx->layer_workspace;
+    ws.used = 0;
+    const size_t gates = size_t(count) * kQueryHeads * kQueryStride, heads = size_t(count) * kKvHeads * kHeadSize;
+    const size_t out = size_t(count) * kQueryHeads * kHeadSize;
+    ws.ensure(Workspace::round(gates * 4) + 2 * Workspace::round(heads * 4) + Workspace::round(out * 4));
+    float *query_gate = ws.take<float>(gates);
+    float *key = ws.take<float>(heads);
+    float *value = ws.take<float>(heads);
+    float *attended = ws.take<float>(out);
+    project_qkv(ctx, L, inputs, count, query_gate, key, value, nullptr);
+    const adi_hip_rows queries{ADI_HIP_F32, query_gate, kQueryHeads * kQueryStride, kQueryStride};
+    adi_hip_paged_append_arguments append{};
+    append.keys = {ADI_HIP_F32, key, kKvHeads * kHeadSize, kHeadSize};
+    append.values = {ADI_HIP_F32, value, kKvHeads * kHeadSize, kHeadSize};
+    append.key_norm = L->key_norm;
+    append.query_heads = kQueryHeads;
+    append.queries = append.queries_out = queries;
+    append.query_norm = L->query_norm;
+    append.weight_offset = 1.0f;
+    append.epsilon = kEpsilon;
+    paged_append(ctx, cache, batch, &append, rope_rows(ctx, std::max(batch->max_length, 1u)), kRopeHalf);
+    adi_hip_paged_attention_arguments attend{};
+    attend.query_heads = kQueryHeads;
+    attend.queries = queries;
+    attend.outputs = {ADI_HIP_F32, attended, kQueryHeads * kHeadSize, kHeadSize};
+    attend.gate = {ADI_HIP_F32, query_gate + kHeadSize, kQueryHeads * kQueryStride, kQueryStride};
+    paged_attention(ctx, cache, batch, &attend, workspace);
+    project_output(ctx, &L->output, attended, count, outputs, nullptr);
+}
+
 // Whether the Gated DeltaNet core launch computes alpha and beta itself from
 // the normalized rows x (8- or 16-lane order, rows of at most 2048 columns,
 // a multiple of 256, 16-byte aligned).
@@ -1933,6 +1986,12 @@ int adi_hip_full_attention_prefill(adi_hip_context *ctx, const adi_hip_full_atte
     return guarded(ctx, [&] {
         full_attention_chunk(ctx, L, position, count, inputs, outputs, keys, values, capacity);
     });
+}
+
+int adi_hip_full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *L,
+                                 const adi_hip_paged_cache *cache, const adi_hip_paged_batch *batch,
+                                 const float *inputs, float *outputs, adi_hip_paged_workspace *workspace) {
+    return guarded(ctx, [&] { full_attention_paged(ctx, L, cache, batch, inputs, outputs, workspace); });
 }
 
 int adi_hip_linear_attention_forward(adi_hip_context *ctx, const adi_hip_linear_attention *L,

@@ -250,6 +250,8 @@ SIGNATURES = [
     ("adi_hip_paged_workspace_destroy", None, [vp]),
     ("adi_hip_paged_attention", C.c_int,
      [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), vp, vp]),
+    ("adi_hip_full_attention_paged", C.c_int,
+     [vp, C.POINTER(FullAttentionStruct), C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), vp, vp, vp]),
     ("adi_hip_profiling_enable", C.c_int, [vp, C.c_int]),
     ("adi_hip_profiling_read", C.c_int, [vp, C.POINTER(KernelProfile), u32, C.POINTER(u32)]),
     # include/adi_hip_gguf.h
@@ -1380,3 +1382,16 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, queries,
     status = ctx.lib.adi_hip_paged_attention(ctx.handle, cache.struct, batch.struct, a, workspace.handle)
     if status:
         ctx.check(status)
+
+
+def full_attention_paged(ctx: Context, layer: DeviceFullAttention, cache: PagedCache, batch: PagedBatch, x, out,
+                         workspace: PagedWorkspace) -> None:
+    """The full-attention layer over a paged cache (KV heads 2 of 256, f32 or
+    bf16) for the batch's rows x [tokens, hidden] into out."""
+    hidden = layer.struct.query.columns
+    for t in (x, out):
+        if tuple(t.shape) != (batch.tokens, hidden) or not t.is_contiguous() or _type_of(t) != F32 or \
+                t.get_device() != ctx.device:
+            _refuse(f"rows must be contiguous f32 [{batch.tokens}, {hidden}] on cuda:{ctx.device}")
+    ctx.check(ctx.lib.adi_hip_full_attention_paged(ctx.handle, C.byref(layer.struct), cache.struct, batch.struct,
+                                                   x.data_ptr(), out.data_ptr(), workspace.handle))

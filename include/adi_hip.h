@@ -862,6 +862,20 @@ int adi_hip_paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cac
                             const adi_hip_paged_attention_arguments *arguments,
                             adi_hip_paged_workspace *workspace);
 
+/* full_attention_forward (src/executor.cpp:332-418) for a batch of sequences
+ * whose caches are pages: rows inputs[tokens][hidden], the new tokens of every
+ * sequence, through the q/k/v projections, adi_hip_paged_append with the
+ * layer's norms and rotation, the gated adi_hip_paged_attention and the
+ * output projection into outputs[tokens][hidden]. Chunks of prompts and
+ * decode tokens may share a batch. The cache holds 2 KV heads of 256 in f32 (the
+ * results of the contiguous entries, to float rounding) or bf16. Output rows of no
+ * sequence hold nothing of use. Unlike the two calls by themselves it uses
+ * the context's own workspaces, as the other layer entries do. */
+int adi_hip_full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *layer,
+                                 const adi_hip_paged_cache *cache,
+                                 const adi_hip_paged_batch *batch, const float *inputs,
+                                 float *outputs, adi_hip_paged_workspace *workspace);
+
 /* ---- kernel profiling ----------------------------------------------------- */
 
 /* Per-kernel timing with HIP events on the context stream, the counterpart

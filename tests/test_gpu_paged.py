@@ -744,3 +744,83 @@ def test_two_contexts_on_two_streams(gpu, workspace):
     for w, c in zip(spaces, contexts):
         w.close()
         c.close()
+
+
+# ---- the full-attention layer over pages -----------------------------------------------
+
+@pytest.fixture(scope="module")
+def layer(gpu):
+    from adi_amd import synthetic as syn
+    rng = syn.rng_for(40, 256)
+    tlut = syn.ne_tlut(rng)
+    host = syn.full_attention(rng, 256, tlut)
+    return host, hip.upload_full_attention(gpu, host, gpu.ne_codebook(tlut))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_layer_over_pages_is_the_layer_over_contiguous_caches(gpu, workspace, layer, kind):
+    """Three sequences' prompts in chunks and single tokens in shared batches
+    against full_attention_prefill of each over a contiguous cache. f32: the
+    same caches to the roundings of an RMS norm's sums in another order, and
+    outputs to 1e-4 of the largest (the layer tests' own bound). bf16: keys and
+    values are off by half a step each, 2^-9 of themselves, which scores, weights
+    and sums carry on linearly: 2^-5 of the largest output."""
+    from adi_amd import synthetic as syn
+    host, device = layer
+    total, hidden, page = [90, 33, 7], host.hidden, 16
+    x = [torch.from_numpy(syn.rms_normalized(syn.hidden_states(syn.rng_for(41, s), n, hidden))).cuda()
+         for s, n in enumerate(total)]
+    want, caches = [], []
+    for rows in x:
+        n = rows.shape[0]
+        k = torch.zeros(n, 2, 256, device="cuda")
+        v, out = torch.zeros_like(k), torch.empty(n, hidden, device="cuda")
+        hip.full_attention_prefill(gpu, device, 0, n, rows, out, k, v, n)
+        want.append(out)
+        caches.append((k, v))
+    pool = Pool(3, total, page, 2, 256, kind)
+    done, got = [0, 0, 0], [torch.empty_like(w) for w in want]
+    for counts in ([40, 0, 7], [1, 30, 0], [48, 1, 0], [1, 1, 0], [0, 1, 0]):
+        rows = torch.cat([x[s][done[s]:done[s] + counts[s]] for s in range(3)])
+        done = [d + c for d, c in zip(done, counts)]
+        batch = hip.PagedBatch(gpu, ints(np.concatenate([[0], np.cumsum(counts)])), ints(done), ints(pool.table),
+                               sum(counts), max(counts), 96)
+        out = torch.empty(sum(counts), hidden, device="cuda")
+        hip.full_attention_paged(gpu, device, pool.cache(gpu), batch, rows, out, workspace)
+        at = 0
+        for s in range(3):
+            got[s][done[s] - counts[s]:done[s]] = out[at:at + counts[s]]
+            at += counts[s]
+    assert done == total
+    limit = 1e-4 if kind == "f32" else 2.0 ** -5
+    step = 64 * U if kind == "f32" else half_step("bf16") + 64 * U
+    for s in range(3):
+        scale = want[s].abs().amax(-1, keepdim=True)
+        assert float(((got[s] - want[s]).abs() / scale).max()) <= limit, s
+        for p in range(total[s]):
+            at = int(pool.table[s, p // page]), p % page
+            for mine, theirs in ((pool.keys[at], caches[s][0][p]), (pool.values[at], caches[s][1][p])):
+                # turned pairs: relative to the pair, so to the head's largest
+                assert float(((mine.float() - theirs).abs() / theirs.abs().amax(-1, keepdim=True)).max()) <= step
+
+
+def test_layer_over_pages_refusals(gpu, workspace, layer):
+    _, device = layer
+    x = torch.zeros(2, 256, device="cuda")
+    out = torch.empty_like(x)
+    table = ints([[0, 1]])
+
+    def call(pool, rows=x, to=out, tokens=2):
+        cache = hip.PagedCache(gpu, pool, pool.clone())
+        batch = hip.PagedBatch(gpu, ints([0, tokens]), ints([tokens]), table, tokens, tokens, 32)
+        hip.full_attention_paged(gpu, device, cache, batch, rows, to, workspace)
+
+    call(normal(1, 2, 16, 2, 256))
+    for pool in (normal(1, 2, 16, 4, 256), normal(1, 2, 16, 2, 128), normal(1, 2, 16, 2, 256, kind="f16")):
+        with pytest.raises(hip.HipError, match="2 heads of 256") as info:
+            call(pool)
+        assert info.value.status == hip.INVALID_ARGUMENT
+    for rows, to in ((x[:1], out), (x.half(), out), (x, out.cpu()), (x, out.t())):
+        with pytest.raises(hip.HipError, match="rows must be contiguous f32"):
+            call(normal(1, 2, 16, 2, 256), rows, to)
+    gpu.synchronize()
