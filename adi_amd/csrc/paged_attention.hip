@@ -932,33 +932,39 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
 
 // The shapes of k_paged_chunk: rows of a wave (the columns of its matrix
 // products, 32 or 16), waves, keys of a tile, tiles in LDS at once, blocks a CU.
+// A wave alone issues a vector instruction every 7 cycles or so and two fill the
+// vector unit (16 multiply-adds a wave: 49 ns alone, 55 ns for both), so a SIMD
+// gets two waves at least. 32 rows a wave read half as much LDS for a product,
+// but a row's sums and queries then take D * 3 / 4 registers. Of what the
+// registers and the 160 KB of LDS leave room for, the fastest of a sweep; in us,
+// rows x keys (waves, tiles, blocks a CU), the kept one first:
+//   16 bits,  64, a prompt of 8192:  32x64 (4, 1, 3) 424, 16x128 (8, 1, 2) 428,
+//                                    16x64 (8, 1, 2) 482, 32x64 (8, 1, 1) 500
+//   16 bits, 128, 5 ragged chunks:   32x64 (8, 2, 1) 165, 32x64 (8, 1, 1) 170,
+//                                    32x32 (8, 2, 1) 186, 16x64 (8, 2, 1) 201
+// and for a chunk of 2048 behind 2048, 16 heads:
+//   16 bits, 256:         16x64 (8, 1, 1) 195, 16x32 (4, 1, 2) 220, 32x32 (4, 2, 1) 286
+//   f32 and f32,  64:     16x64 (4, 1, 2) 191, 16x64 (8, 1, 1) 197, 16x32 (8, 1, 1) 248
+//   f32 and f32, 128:     16x64 (8, 1, 1) 308, 16x32 (8, 1, 1) 348, 16x64 (4, 1, 2) 424
+//   f32 and bf16,  64:    16x64 (4, 1, 2) 113, 16x64 (8, 1, 1) 127, 16x32 (8, 1, 1) 169
+//   f32 and bf16, 128:    16x64 (4, 1, 2) 169, 16x64 (8, 1, 1) 185, 16x32 (8, 1, 1) 216
+//   f32 and bf16, 256:    16x32 (8, 1, 1) 367, 16x64 (8, 1, 1) 372, 16x32 (4, 1, 2) 477
+// f32 and f32 at 256 has LDS for one tile of 32 keys only (80 KB).
 template <uint32_t ROWS, uint32_t WAVES, uint32_t KEYS, uint32_t BUFFERS, uint32_t BLOCKS>
 struct ChunkShape {
     static constexpr uint32_t kRows = ROWS, kWaves = WAVES, kKeys = KEYS, kBuffers = BUFFERS, kBlocks = BLOCKS;
 };
 template <typename T, typename R, uint32_t D>
 struct ChunkOf {
-    // 16-bit rows: 32 rows a wave, so that an operand read from LDS feeds as
-    // many products as the LDS can keep up with
-#ifndef S64
-#define S64 ChunkShape<32, 4, 64, 1, 3>
-#endif
-#ifndef S128
-#define S128 ChunkShape<32, 8, 64, 2, 1>
-#endif
-    using Shape = std::conditional_t<D == 64, S64, std::conditional_t<D == 128, S128, ChunkShape<32, 4, 32, 2, 1>>>;
+    using Shape = std::conditional_t<
+        D == 64, ChunkShape<32, 4, 64, 1, 3>,
+        std::conditional_t<D == 128, ChunkShape<32, 8, 64, 2, 1>, ChunkShape<16, 8, 64, 1, 1>>>;
 };
 template <typename T, uint32_t D>
 struct ChunkOf<T, float, D> {
-    // f32 rows: three pieces of a query, of which 16 rows a wave leave room for
-    // two waves a SIMD
-#ifndef VAHEAD
-#define VAHEAD 2u
-#endif
-#ifndef SB
-#define SB ChunkShape<16, 8, 32, 1, 1>
-#endif
-    using Shape = std::conditional_t<std::is_same_v<T, float>, ChunkShape<16, 8, 32, 1, 1>, SB>;
+    using Shape = std::conditional_t<
+        D == 256, ChunkShape<16, 8, 32, 1, 1>,
+        std::conditional_t<D == 128 && std::is_same_v<T, float>, ChunkShape<16, 8, 64, 1, 1>, ChunkShape<16, 4, 64, 1, 2>>>;
 };
 template <typename T, typename R, uint32_t D>
 constexpr uint32_t chunk_rows() {
@@ -1359,52 +1365,52 @@ void k_paged_chunk(AttendArgs args) {
     };
     const auto scores = [&](uint32_t buffer, float (&score)[kSub][kHeld]) {
         const unsigned char *const key_lds = lds + buffer * kBuffer;
+        // with 16 rows a wave two products of 16 keys for every 32, interleaved so that
+        // a lane's eight results are eight keys in a row; a tile's turn by turn, as
+        // a product that adds to the one before it waits for it
+        constexpr uint32_t kHalves = W == 32u ? 1u : 2u, kProducts = kHalves * kSub;
+        Acc acc[kProducts], *to[kProducts];
 #pragma unroll
-        for (uint32_t b = 0; b < kSub; ++b) {
-            // with 16 rows a wave two products of 16 keys, interleaved so that
-            // a lane's eight results are eight keys in a row
-            constexpr uint32_t kProducts = W == 32u ? 1u : 2u;
-            Acc acc[kProducts], *to[kProducts];
+        for (uint32_t h = 0; h < kProducts; ++h) {
+#pragma unroll
+            for (uint32_t r = 0; r < kRegisters; ++r) {
+                acc[h][r] = 0.0f;
+            }
+            to[h] = &acc[h];
+        }
+        u32x4 k[2][kProducts][KP];
+        const auto read = [&](uint32_t j) {
 #pragma unroll
             for (uint32_t h = 0; h < kProducts; ++h) {
+                const uint32_t entry = 32u * (h / kHalves) +
+                                       (W == 32u ? column : 8u * (column / 4u) + 4u * (h % 2u) + column % 4u);
 #pragma unroll
-                for (uint32_t r = 0; r < kRegisters; ++r) {
-                    acc[h][r] = 0.0f;
-                }
-                to[h] = &acc[h];
-            }
-            u32x4 k[2][kProducts][KP];
-            const auto read = [&](uint32_t j) {
-#pragma unroll
-                for (uint32_t h = 0; h < kProducts; ++h) {
-                    const uint32_t entry = 32u * b + (W == 32u ? column : 8u * (column / 4u) + 4u * h + column % 4u);
-#pragma unroll
-                    for (uint32_t p = 0; p < KP; ++p) {
-                        k[j & 1u][h][p] = *reinterpret_cast<const u32x4 *>(
-                            key_lds + p * kPlane + key_place<D, W>(entry, kStepDims / 8u * j + side));
-                    }
-                }
-            };
-            read(0u);
-#pragma unroll
-            for (uint32_t j = 0; j < D / kStepDims; ++j) {
-                if (j + 1u < D / kStepDims) {
-                    read(j + 1u);
-                }
-                products<N>(k[j & 1u], query_pieces[j], to);
-                if constexpr (P == 3u) {
-                    __builtin_amdgcn_sched_barrier(0);
+                for (uint32_t p = 0; p < KP; ++p) {
+                    k[j & 1u][h][p] = *reinterpret_cast<const u32x4 *>(
+                        key_lds + p * kPlane + key_place<D, W>(entry, kStepDims / 8u * j + side));
                 }
             }
+        };
+        read(0u);
 #pragma unroll
-            for (uint32_t h = 0; h < kProducts; ++h) {
+        for (uint32_t j = 0; j < D / kStepDims; ++j) {
+            if (j + 1u < D / kStepDims) {
+                read(j + 1u);
+            }
+            products<N>(k[j & 1u], query_pieces[j], to);
+            if constexpr (P == 3u) {
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
 #pragma unroll
-                for (uint32_t r = 0; r < kRegisters; ++r) {
-                    score[b][h * kRegisters + r] = acc[h][r];
-                    if constexpr (kFloat) {
-                        score[b][h * kRegisters + r] =
-                            acc[h][r] * query_unscale * key_unscale[buffer * kKeys + 32u * b + key_of(h * kRegisters + r)];
-                    }
+        for (uint32_t h = 0; h < kProducts; ++h) {
+            const uint32_t sub = h / kHalves, at = h % kHalves * kRegisters;
+#pragma unroll
+            for (uint32_t r = 0; r < kRegisters; ++r) {
+                score[sub][at + r] = acc[h][r];
+                if constexpr (kFloat) {
+                    score[sub][at + r] =
+                        acc[h][r] * query_unscale * key_unscale[buffer * kKeys + 32u * sub + key_of(at + r)];
                 }
             }
         }
@@ -1484,7 +1490,7 @@ void k_paged_chunk(AttendArgs args) {
                 const uint32_t next = entry + (W == 32u ? 8u : 4u);
                 const uint32_t dimension = (W == 32u ? (lane >> 4 & 1u) * 16u : 0u) + (lane & 3u) * 4u;
                 // (two at a time, the next two on their way)
-                u32x4 v[VAHEAD][2][Q];
+                u32x4 v[2][2][Q];
                 const auto read = [&](uint32_t i) {
 #pragma unroll
                     for (uint32_t x = 0; x < 2u; ++x) {
@@ -1497,19 +1503,18 @@ void k_paged_chunk(AttendArgs args) {
                                 return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at));
                             };
                             const u32x2 lo = four(entry), hi = four(next);
-                            v[i % VAHEAD][x][p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                            v[i & 1u][x][p] = u32x4{lo.x, lo.y, hi.x, hi.y};
                         }
                     }
                 };
-                if (VAHEAD > 1u) read(0u);
+                read(0u);
 #pragma unroll
                 for (uint32_t i = 0; i < D / W / 2u; ++i) {
-                    if (VAHEAD == 1u) read(i); else
                     if (i + 1u < D / W / 2u) {
                         read(i + 1u);
                     }
                     Acc *to[2] = {&sums[2u * i], &sums[2u * i + 1u]};
-                    products<M>(v[i % VAHEAD], weights, to);
+                    products<M>(v[i & 1u], weights, to);
                     if constexpr (P == 3u) {
                         __builtin_amdgcn_sched_barrier(0);
                     }
