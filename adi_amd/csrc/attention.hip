@@ -1557,6 +1557,7 @@ void full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *L,
     require(L != nullptr && workspace != nullptr, "paged full attention: null argument");
     require(cache->heads == kKvHeads && cache->head_size == kHeadSize && cache->type != ADI_HIP_F16,
             "paged full attention: the cache must hold 2 heads of 256 in f32 or bf16");
+    require(batch->max_length <= (1u << 20), "paged full attention: max_length above 2^20");
     const uint32_t hidden = L->query.columns, count = batch->tokens;
     require(ne_shaped(L->query, kQueryHeads * kQueryStride, hidden) &&
                 ne_shaped(L->key, kKvHeads * kHeadSize, hidden) &&

@@ -20,6 +20,7 @@
 // it; what is left out is below 2^-22 of the largest.
 #include "paged_attention.hpp"
 
+#include <atomic>
 #include <type_traits>
 
 namespace adi_hip {
@@ -1721,7 +1722,6 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
     const bool many = uint64_t(c.sequences) * c.max_tokens == c.tokens || c.sequences == 1;
     args.mixed = !few && !many ? 1u : 0u;
     if (few || args.mixed != 0) {
-        require(c.heads < (1u << 16) && c.sequences < (1u << 16), "paged attention: too many heads or sequences");
         AttendArgs a = args;
         a.partial = partial;
         a.tickets = static_cast<uint32_t *>(workspace->base);
@@ -1770,8 +1770,13 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
     args.parts = ceil_div(extent, args.span);
     args.partial = partial;
     constexpr size_t lds = chunk_lds<T, R, D>();
-    static const bool raised = set_lds_limit(reinterpret_cast<const void *>(k_paged_chunk<T, R, D>), lds);
-    (void)raised;
+    // (once a device)
+    static std::atomic<uint64_t> raised{0};
+    const uint64_t device = uint64_t(1) << (static_cast<uint32_t>(ctx->device) & 63u);
+    if ((raised.load() & device) == 0) {
+        set_lds_limit(reinterpret_cast<const void *>(k_paged_chunk<T, R, D>), lds);
+        raised.fetch_or(device);
+    }
     const uint64_t pairs = uint64_t(c.heads) * args.parts;
     const uint64_t grid = (pairs < 8u ? pairs : (pairs + 7u) / 8u * 8u) * row_tiles;
     require(grid < (1u << 23), "paged attention: too many rows");
@@ -1808,8 +1813,10 @@ void paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache, con
             "paged attention: f32 rows read an f32 or bf16 cache, others their own type");
     require(a->query_heads >= 1 && a->query_heads % cache->heads == 0 && a->query_heads / cache->heads <= 256,
             "paged attention: query heads must be 1 to 256 times the cache's");
-    require(std::isfinite(a->scale) && a->scale >= 0.0f, "paged attention: scale must be positive, or 0");
-    if (batch->tokens == 0 || batch->sequences == 0 || batch->max_tokens == 0) {
+    require(cache->heads < (1u << 16) && batch->sequences < (1u << 16),
+            "paged attention: more than 65535 heads or sequences");
+    require(a->scale >= 0.0f && a->scale <= 1e38f, "paged attention: scale must be positive and at most 1e38, or 0");
+    if (batch->tokens == 0 || batch->sequences == 0) {
         return;
     }
     require_rows(a->queries, type, "paged attention: queries must be 16-byte aligned rows");

@@ -847,14 +847,14 @@ void adi_hip_paged_workspace_destroy(adi_hip_paged_workspace *workspace);
  * bf16 for both (queries, gate and outputs have one type). f32 rows get
  * products of 32-bit accuracy; f16 and bf16 rows round the weights w_j to the
  * type (sums in 32 bits). Scores must stay within a float. query_heads is a multiple
- * of heads, at most 256 times it. The outputs overlap neither queries nor gate. Rows of no sequence
- * stay as they are. */
+ * of heads, at most 256 times it. The outputs overlap neither queries nor gate. Rows
+ * of no sequence stay as they are. Sequences and KV heads: below 65536 each. */
 typedef struct {
     uint32_t query_heads;
     adi_hip_rows queries;  /* [tokens][query_heads][head_size] */
     adi_hip_rows outputs;
     adi_hip_rows gate;     /* data NULL: none */
-    float scale;           /* positive; 0: 1 / sqrt(head_size) */
+    float scale;           /* positive, at most 1e38; 0: 1 / sqrt(head_size) */
     uint32_t window;       /* 0: none */
 } adi_hip_paged_attention_arguments;
 int adi_hip_paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache,
@@ -868,9 +868,12 @@ int adi_hip_paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cac
  * layer's norms and rotation, the gated adi_hip_paged_attention and the
  * output projection into outputs[tokens][hidden]. Chunks of prompts and
  * decode tokens may share a batch. The cache holds 2 KV heads of 256 in f32 (the
- * results of the contiguous entries, to float rounding) or bf16. Output rows of no
- * sequence hold nothing of use. Unlike the two calls by themselves it uses
- * the context's own workspaces, as the other layer entries do. */
+ * results of the contiguous entries, to float rounding) or bf16; max_length is at
+ * most 2^20. Output rows of no sequence hold nothing of use. Unlike the two
+ * calls by themselves it uses the context's workspaces and its table of
+ * angles (max_length of them), which a call with more rows or a larger
+ * max_length grows, as the other layer entries do: a captured call takes a
+ * warm-up call of the largest sizes first and none of larger ones later. */
 int adi_hip_full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *layer,
                                  const adi_hip_paged_cache *cache,
                                  const adi_hip_paged_batch *batch, const float *inputs,

@@ -824,3 +824,88 @@ def test_layer_over_pages_refusals(gpu, workspace, layer):
         with pytest.raises(hip.HipError, match="rows must be contiguous f32"):
             call(normal(1, 2, 16, 2, 256), rows, to)
     gpu.synchronize()
+
+
+# ---- calls at the edges of what is allowed ------------------------------------------
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+def test_attention_of_more_sequences_than_lanes(gpu, workspace, rows, kind):
+    """Chunks behind the 64th and the 128th sequence, beside single tokens
+    and sequences without rows: a block finds its rows, a row its sequence."""
+    counts = [1] * 70 + [0] * 5 + [9, 1, 0, 21] + [1] * 60 + [5]
+    lengths = [7 + (11 * s) % 90 for s in range(len(counts))]
+    lengths[-1] = 400
+    check_attention(gpu, workspace, rows, kind, 64, 8, 2, 8, counts, lengths, padding=2)
+
+
+@pytest.mark.parametrize("heads", [4, 64])
+def test_a_bound_of_no_new_tokens(gpu, workspace, heads):
+    """max_tokens 0: any sequence with rows is over it, so NaN, and appended nowhere."""
+    pool = Pool(3, [20, 30], 16, 2, 64, "bf16", junk=None)
+    before = pool.keys.clone()
+    batch = hip.PagedBatch(gpu, ints([0, 3, 3]), ints([20, 30]), ints(pool.table), 4, 0, 32)
+    q, k = normal(1, 4, heads, 64, kind="bf16"), normal(2, 4, 2, 64, kind="bf16")
+    out = torch.full_like(q, 7.0)
+    hip.paged_append(gpu, pool.cache(gpu), batch, k, k)
+    hip.paged_attention(gpu, pool.cache(gpu), batch, q, out, workspace)
+    assert torch.equal(pool.keys, before)
+    assert bool(torch.isnan(out[:3]).all()) and bool((out[3:] == 7.0).all())
+
+
+@pytest.mark.parametrize("heads,counts", [(4, [2, 1]), (32, [2, 40])])
+def test_rows_before_the_first_sequence_stay(gpu, workspace, heads, counts):
+    """offsets[0] above 0: the rows before it belong to no sequence either."""
+    pool = Pool(4, [50, 90], 16, 2, 128, "f32", junk=None)
+    n = sum(counts)
+    offsets = np.concatenate([[0], np.cumsum(counts)])
+    q, k, v = normal(1, n + 3, heads, 128), normal(2, n + 3, 2, 128), normal(3, n + 3, 2, 128)
+    out = []
+    for shift in (0, 3):
+        keys, values = pool.keys.clone(), pool.values.clone()
+        cache = hip.PagedCache(gpu, keys, values)
+        batch = hip.PagedBatch(gpu, ints(offsets + shift), ints([50, 90]), ints(pool.table), n + 3, max(counts), 96)
+        rows = [torch.roll(x, shift, 0) for x in (q, k, v)]
+        turned_rows, attended = torch.full_like(q, 5.0), torch.full_like(q, 7.0)
+        hip.paged_append(gpu, cache, batch, rows[1], rows[2], queries=rows[0], queries_out=turned_rows)
+        hip.paged_attention(gpu, cache, batch, rows[0], attended, workspace)
+        out.append((keys, values, turned_rows[shift:shift + n], attended[shift:shift + n]))
+        others = torch.cat([turned_rows[:shift] - 5, turned_rows[shift + n:] - 5, attended[:shift] - 7,
+                            attended[shift + n:] - 7])
+        assert bool((others == 0).all())
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1, 30, 1]])
+def test_sequences_that_share_pages(gpu, workspace, rows, kind, counts):
+    """One prefix's pages in several tables, and one page twice in a table:
+    each row as if its sequence had copies of them."""
+    lengths, page = [70, 100, 75], 16
+    pool = Pool(6, lengths, page, 2, 64, kind, junk=None)
+    apart = pool.keys.clone(), pool.values.clone()
+    shared = pool.table.copy()
+    shared[1, :3] = shared[2, :3] = shared[0, :3]
+    shared[1, 3] = shared[1, 2]
+    for s in range(3):
+        for p in range(4):
+            for x in apart:
+                x[int(pool.table[s, p])] = x[int(shared[s, p])] if s else x[int(pool.table[s, p])]
+    n = sum(counts)
+    q = normal(7, n, 8, 64, kind=rows)
+    out = torch.empty_like(q), torch.empty_like(q)
+    pool.batch(gpu, counts)
+    for table, (keys, values), to in ((shared, (pool.keys, pool.values), out[0]), (pool.table, apart, out[1])):
+        batch = hip.PagedBatch(gpu, ints(np.concatenate([[0], np.cumsum(counts)])), ints(lengths), ints(table), n,
+                               max(counts), 112)
+        hip.paged_attention(gpu, hip.PagedCache(gpu, keys, values), batch, q, to, workspace)
+    assert torch.equal(*out)
+
+
+def test_attention_scale_refusals(gpu, workspace):
+    pool = Pool(1, [20], 16, 2, 64, "bf16", junk=None)
+    q = normal(1, 1, 4, 64, kind="bf16")
+    batch = pool.batch(gpu, [1])
+    for scale in (3e38, math.nan, -math.inf):
+        with pytest.raises(hip.HipError, match="scale"):
+            hip.paged_attention(gpu, pool.cache(gpu), batch, q, torch.empty_like(q), workspace, scale=scale)
