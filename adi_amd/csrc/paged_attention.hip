@@ -21,6 +21,7 @@
 #include "paged_attention.hpp"
 
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 namespace adi_hip {
@@ -1735,6 +1736,15 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
         // (one tile a wave at least)
         constexpr uint64_t kUnit = std::is_same_v<T, float> ? 64 : 128;
         a.span = span_of(std::max<uint64_t>(parts, 1u), kUnit);
+        // A part's tiles, and the parts that the last block joins, both go through
+        // one CU at about its rate, so a part takes at least the entries for which
+        // the two are even (a token of 16 heads on 2 behind 8000 entries: f32 of
+        // 256, spans of 64, 192 and 256 entries 37.0, 27.5 and 27.8 us; bf16 of 256
+        // under f32 rows, 128, 256 and 384 24.2, 19.9 and 22.2; bf16 of 128 15.0,
+        // 12.5 and 13.7).
+        const uint64_t rows = std::min<uint64_t>(uint64_t(c.max_tokens) * args.group, kStepRows);
+        const double even = std::sqrt(double(extent) * rows * (D + 4u) * sizeof(float) / (2.0 * D * sizeof(T)));
+        a.span = std::max(a.span, static_cast<uint32_t>(uint64_t(even / kUnit + 0.5) * kUnit));
         a.parts = ceil_div(extent, a.span);
         launch(ctx, "paged_step", k_paged_step<T, R, D>, dim3(a.parts * c.heads, c.sequences), dim3(kThreads), 0, a);
         if (few) {

@@ -1297,6 +1297,8 @@ class PagedBatch:
     rows, at most max_tokens new ones and max_length entries a sequence."""
 
     def __init__(self, ctx: Context, offsets, lengths, table, tokens: int, max_tokens: int, max_length: int):
+        if not all(0 <= x < 1 << 32 for x in (tokens, max_tokens, max_length)):
+            _refuse("paged batch: tokens, max_tokens or max_length is out of range")
         n = int(lengths.shape[0])
         _device_words(ctx, lengths, "lengths", n)
         _device_words(ctx, offsets, "offsets", n + 1)
