@@ -1759,10 +1759,14 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
                            uint64_t(c.tokens) * args.group / kBlockRows + c.sequences);
     const uint64_t likely = std::min<uint64_t>(row_tiles, ceil_div(uint64_t(c.tokens) * args.group, kBlockRows) +
                                                               (args.mixed != 0 ? 0u : c.sequences / 2u));
-    // The parts that end first, in units of 32 keys of a row tile (some 3 us):
-    // rounds of the blocks the chip holds (half a round more where there are
-    // several, for their uneven ends), a block's own start and end worth 6, and
-    // the parts' way through memory at 5 TB/s.
+    // The parts that end first, by us: 32 keys of a row tile about kTurn, rounds of
+    // the blocks the chip holds (half a round more where there are several, for
+    // their uneven ends), a block's own start and end as 6 turns; the parts' way
+    // through memory at 5 TB/s, and a join's launch and loop. Within 3% of the best
+    // number of parts for six chunks of 64 to 512 tokens behind 4000 and 8000
+    // entries (64 tokens, 16 heads of 128 on 2 in bf16: 16 parts 30.2 us, 8 32.8,
+    // 32 35.2).
+    constexpr double kTurn = D / 64.0 * (std::is_same_v<R, float> ? 0.8 : 0.5);
     const uint64_t part_bytes = uint64_t(c.tokens) * heads * (D + 4u) * sizeof(float);
     const uint64_t most = std::clamp<uint64_t>(room / part_bytes, 1u, 64u);
     const double resident = double(ctx->cu_count) * Shape::kBlocks;
@@ -1771,7 +1775,8 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
         const uint64_t span = span_of(parts, kSpanUnit), real = ceil_div(extent, span);
         const double count = double(likely * c.heads * real);
         const double rounds = count <= resident ? 1.0 : count / resident + 0.5;
-        const double cost = rounds * (span / 32.0 + 6.0) + (real > 1 ? 2.0 + 2.0 * part_bytes * real / 15.0e6 : 0.0);
+        const double cost = rounds * (span / 32.0 + 6.0) * kTurn +
+                            (real > 1 ? 4.0 + 0.3 * real + 2.0 * part_bytes * real / 5.0e6 : 0.0);
         if (parts == 1 || cost < least) {
             least = cost;
             args.span = static_cast<uint32_t>(span);
