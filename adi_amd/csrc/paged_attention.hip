@@ -12,12 +12,22 @@
 // Two kernels. k_paged_step: up to 16 rows a KV head (a decode step's tokens):
 // a wave streams its tiles from the cache straight into operands, the waves of
 // a block and the blocks of a long history are joined. k_paged_chunk: more rows,
-// 128 a block, over tiles staged in LDS.
+// 64 to 256 a block, over tiles staged in LDS, a long history's parts joined by
+// k_paged_join.
 //
-// Floats on the 16-bit matrix cores: an f32 value is the exact sum of three bf16
+// Floats on the 16-bit matrix cores (k_paged_chunk; the step's f32 products over
+// an f32 cache are the f32 ones): an f32 value is the exact sum of three bf16
 // pieces, each the leading 8 bits of what is left (truncated, so that none
 // overflows), and a product is the sum of the piece products down to 2^-16 of
-// it; what is left out is below 2^-22 of the largest.
+// it; what is left out is below 2^-22 of the largest. Scores over f32 keys take
+// two f16 pieces of 11 bits each instead, of queries and keys scaled by powers of
+// two that bring a row's or a key's largest element to 2^14 .. 2^15: three
+// products for six, and elements down to 2^-16 of the largest keep 22 bits.
+//
+// Rounding: scores, levels, sums and denominators are 32 bits. 16-bit rows'
+// weights are rounded once to the rows' type, as the products take them (the
+// denominator in k_paged_chunk is the sum of the rounded ones, which cancels
+// a part of it), and outputs once at the end.
 #include "paged_attention.hpp"
 
 #include <atomic>
@@ -320,6 +330,14 @@ constexpr uint32_t step_blocks() {
     return D == 256u ? (step_eager<T, R, D>() ? 1u : 2u) : 2u;
 }
 
+// Bound by the entries' bytes where there are many: two sequences behind 131,071
+// entries, 8 heads of 128 in bf16, 831 MB in 160 us, 5.2 TB/s, what a large copy
+// reaches; 32 sequences of up to 4,096 entries, 154 MB, 43 us (3.6 TB/s: their
+// lengths differ, and a block's start and end are some 8 us). Where there are few,
+// by its chain of latencies: one token behind 1,999 entries of 2 heads of 256 in
+// f32, 8.2 MB, 18 us: some 4 to start, page numbers, a tile's loads and products
+// 3, the join of 32 parts 7.
+//
 // Block (KV head, part, sequence): its four waves take the part's tiles in turn,
 // each straight from the cache into operands, the next tile's keys on their way
 // from the end of this one's scores and its values from the end of their
@@ -855,7 +873,9 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
 // ---- joining the parts of a history -------------------------------------------
 
 // A wave a row (token, query head) of more than one part: lane l takes the
-// factors of parts l, l + 64, ... and dimensions D / 64 l .. of every part.
+// factors of parts l, l + 64, ... and dimensions D / 64 l .. of every part. Bound
+// by the parts' bytes, which the chunks have just written: 8,192 rows of four
+// parts of 256, 34 MB, 12.5 us.
 template <typename R, uint32_t D, bool EXACT>
 __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
     constexpr uint32_t kSide = D / 64u;
@@ -982,6 +1002,17 @@ constexpr size_t chunk_lds() {
            Shape::kWaves * 64 * 4;
 }
 
+// Bound by matrix and vector phases that overlap in part: 8192 f16 tokens, 32
+// heads of 64 on 4, 275 GFLOP, 406 us (0.68 PFLOP/s; a large library product
+// reaches 1.29): the matrix cores are busy 44% of the cycles, the vector
+// units (of which half is exponentials) 54%, at a clock that such work takes down to
+// 1.8 GHz. Ragged chunks of 5 sequences in bf16, 32 heads of 128 on 8, 160 us (38%
+// and 44%); 512 f32 tokens behind 3584 over f32 heads of 256, 150 us and a join
+// of 12 (nine products an element: 47% of the matrix cores' cycles). Tried without gain:
+// the waves' halves a phase apart over two buffers of keys and three of values
+// (165 -> 185 us for the chunks), wave priorities for either phase (165 -> 170 and 175),
+// scores or weights kept apart from the products by scheduling barriers (171).
+//
 // Block (row tile, KV head, part, sequence). Lane l of a wave is row l % ROWS
 // of the wave's and piece l / ROWS of its keys.
 template <typename T, typename R, uint32_t D>
