@@ -1578,6 +1578,7 @@ void full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *L,
     float *key = ws.take<float>(heads);
     float *value = ws.take<float>(heads);
     float *attended = ws.take<float>(out);
+    const float *const angles = rope_rows(ctx, std::max(batch->max_length, 1u));
     project_qkv(ctx, L, inputs, count, query_gate, key, value, nullptr);
     const adi_hip_rows queries{ADI_HIP_F32, query_gate, kQueryHeads * kQueryStride, kQueryStride};
     adi_hip_paged_append_arguments append{};
@@ -1589,7 +1590,7 @@ void full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *L,
     append.query_norm = L->query_norm;
     append.weight_offset = 1.0f;
     append.epsilon = kEpsilon;
-    paged_append(ctx, cache, batch, &append, rope_rows(ctx, std::max(batch->max_length, 1u)), kRopeHalf);
+    paged_append(ctx, cache, batch, &append, angles, kRopeHalf);
     adi_hip_paged_attention_arguments attend{};
     attend.query_heads = kQueryHeads;
     attend.queries = queries;

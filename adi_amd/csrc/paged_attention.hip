@@ -50,7 +50,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kStepRows = 16;    // of a KV head, k_paged_step
-constexpr uint32_t kStepKeys = 32;    // a wave's tile
+
 constexpr uint32_t kSpanUnit = 128;   // parts of a history are multiples of this
 constexpr float kNegative = -__builtin_huge_valf();
 
@@ -91,11 +91,24 @@ constexpr float kSlack = 8.0f;
 // first, so that its rounding is relative to it; for 16-bit rows in one
 // multiply-add.
 template <bool EXACT>
-__device__ __forceinline__ float weight_of(float s, float m, float log2_scale) {
+__device__ __forceinline__ float factor_of(float s, float m, float log2_scale) {
     if constexpr (EXACT) {
         return __builtin_amdgcn_exp2f((s - m) * log2_scale);
     } else {
         return __builtin_amdgcn_exp2f(fmaf(s, log2_scale, -m * log2_scale));
+    }
+}
+
+// A score's weight at a level. f16 rows' are 2^7 of that (sums and denominators
+// alike, so outputs are not): up to 2^15 with the slack, and down to 2^-31 of the
+// level before one is rounded to nothing, so that it takes a history of 2^20
+// such entries to matter; bf16 has the range as it is.
+template <typename R>
+__device__ __forceinline__ float weight_of(float s, float m, float log2_scale) {
+    if constexpr (std::is_same_v<R, _Float16>) {
+        return __builtin_amdgcn_exp2f(fmaf(s, log2_scale, fmaf(-m, log2_scale, 7.0f)));
+    } else {
+        return factor_of<std::is_same_v<R, float>>(s, m, log2_scale);
     }
 }
 
@@ -188,6 +201,18 @@ __device__ __forceinline__ void products(const u32x4 (&a)[X][A], const u32x4 (&b
     }
 }
 
+// sum plus both values of a pair, in 32 bits.
+template <typename T>
+__device__ __forceinline__ float pair_sum(uint32_t pair, float sum) {
+    if constexpr (std::is_same_v<T, _Float16>) {
+        const f16x2 one = {1.0f, 1.0f};
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), one, sum, false);
+    } else {
+        const bf16x2 one = {1.0f, 1.0f};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), one, sum, false);
+    }
+}
+
 // Whether either 16-bit value of a pair is an infinity or NaN.
 template <typename T>
 __device__ __forceinline__ bool odd_pair(uint32_t v) {
@@ -216,7 +241,7 @@ __device__ __forceinline__ Page page_of(const PagedView &c, const uint32_t *tabl
 
 // The weight of an entry for a row at its maximum so far, outside the tiles' way:
 // for the few entries that hold values that are not finite.
-template <typename T, typename R, uint32_t D, bool EXACT>
+template <typename T, typename R, uint32_t D>
 __device__ __forceinline__ float odd_weight(const AttendArgs &a, const uint32_t *table, const T *keys, const R *query,
                                          uint32_t entry, float maximum) {
     const T *const key = keys + page_of(a.c, table, entry).at;
@@ -224,7 +249,7 @@ __device__ __forceinline__ float odd_weight(const AttendArgs &a, const uint32_t 
     for (uint32_t d = 0; d < D; ++d) {
         score = fmaf(static_cast<float>(query[d]), static_cast<float>(key[d]), score);
     }
-    return weight_of<EXACT>(score, maximum == kNegative ? 0.0f : maximum, a.log2_scale);
+    return weight_of<R>(score, maximum == kNegative ? 0.0f : maximum, a.log2_scale);
 }
 
 // N consecutive outputs of a row, gated.
@@ -621,7 +646,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         if (__any(top > limit)) {
             // (a row's level does not depend on the wave's other rows)
             const bool raised = top > limit;
-            const float factor = raised ? weight_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
+            const float factor = raised ? factor_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
             maximum = raised ? top : maximum;
             limit = raised ? top + args.slack : limit;
             denominator *= factor;
@@ -636,7 +661,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         const float level = maximum == kNegative ? 0.0f : maximum;
 #pragma unroll
         for (uint32_t k = 0; k < kHeld; ++k) {
-            score[k] = weight_of<P == 3>(score[k], level, args.log2_scale);
+            score[k] = weight_of<R>(score[k], level, args.log2_scale);
             denominator += score[k];
         }
         if constexpr (kFloat) {
@@ -690,7 +715,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         // part: the products left them out, the rows that see them get them.
         for (int32_t at = begin + static_cast<int32_t>(wave * kKeys); at < end; at += kTurn) {
             for (int32_t entry = at; edge_tile(at) && entry < min(at + static_cast<int32_t>(kKeys), end); ++entry) {
-                const float weight = odd_weight<T, R, D, P == 3>(args, table, keys, query, entry, maximum);
+                const float weight = odd_weight<T, R, D>(args, table, keys, query, entry, maximum);
                 const bool visible = entry <= position && entry >= oldest;
                 const Page page = page_of(cache, table, entry);
                 const T *const value = values + page.at;
@@ -717,14 +742,14 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         lds.denominator[wave][c] = denominator;
     }
     __syncthreads();
-    const auto factor_of = [&](float m, float top) {
-        return m == kNegative && top == kNegative ? 1.0f : weight_of<P == 3>(m, top, args.log2_scale);
+    const auto join_factor = [&](float m, float top) {
+        return m == kNegative && top == kNegative ? 1.0f : factor_of<P == 3>(m, top, args.log2_scale);
     };
     const auto top_of = [&](uint32_t r) {
         return fmaxf(fmaxf(lds.maximum[0][r], lds.maximum[1][r]), fmaxf(lds.maximum[2][r], lds.maximum[3][r]));
     };
     if (c < rows) {
-        const float factor = factor_of(maximum, top_of(c));
+        const float factor = join_factor(maximum, top_of(c));
 #pragma unroll
         for (uint32_t i = 0; i < kGroups; ++i) {
 #pragma unroll
@@ -756,7 +781,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t w = 0; w < 4u; ++w) {
-            total += lds.denominator[w][r] * factor_of(lds.maximum[w][r], top);
+            total += lds.denominator[w][r] * join_factor(lds.maximum[w][r], top);
             sum += *reinterpret_cast<const f32x4 *>(&lds.sums[w][r][at]);
         }
         if (live == 1u) {
@@ -810,7 +835,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
 #pragma unroll
         for (uint32_t i = 0; i < kStepParts / 64u; ++i) {
             if (64u * i + lane < live) {
-                const float factor = factor_of(m[i], top);
+                const float factor = join_factor(m[i], top);
                 total += lds.parts.total[64u * i + lane][r] * factor;
                 lds.parts.factor[64u * i + lane][r] = factor;
             }
@@ -934,7 +959,7 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
             const float *part = partial_row<D>(args, p, token, head);
             const float m = part[D], d = part[D + 1u];
             const Side v = *reinterpret_cast<const Side *>(part + kSide * lane);
-            const float factor = m == kNegative && top == kNegative ? 1.0f : weight_of<EXACT>(m, top, args.log2_scale);
+            const float factor = m == kNegative && top == kNegative ? 1.0f : factor_of<EXACT>(m, top, args.log2_scale);
             total += d * factor;
 #pragma unroll
             for (uint32_t k = 0; k < kSide; ++k) {
@@ -1383,15 +1408,6 @@ void k_paged_chunk(AttendArgs args) {
         return W == 32u ? 32u * m + 8u * (r / 4u) + 4u * side + r % 4u : 16u * m + 4u * side + r;
     };
 
-    // 16-bit rows add their rounded weights up on the matrix cores too, as a row of
-    // ones among the values (the vector units are the busier ones there)
-    Acc ones_sum;
-#pragma unroll
-    for (uint32_t r = 0; r < kRegisters; ++r) {
-        ones_sum[r] = 0.0f;
-    }
-    const uint32_t one = std::is_same_v<M, _Float16> ? 0x3C003C00u : 0x3F803F80u;
-
     // (a wave whose rows see nothing of a tile passes it by)
     const auto sees = [&](int32_t first) {
         return wave_live && first <= wave_high && first + static_cast<int32_t>(kKeys) > from(wave_low);
@@ -1479,7 +1495,7 @@ void k_paged_chunk(AttendArgs args) {
         if (__any(top > limit)) {
             // (a row's level does not depend on the wave's other rows)
             const bool raised = top > limit;
-            const float factor = raised ? weight_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
+            const float factor = raised ? factor_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
             maximum = raised ? top : maximum;
             limit = raised ? top + args.slack : limit;
             denominator *= factor;
@@ -1487,16 +1503,13 @@ void k_paged_chunk(AttendArgs args) {
             for (uint32_t m = 0; m < D / W; ++m) {
                 sums[m] *= factor;
             }
-            if constexpr (P == 1u) {
-                ones_sum *= factor;
-            }
         }
         const float level = maximum == kNegative ? 0.0f : maximum;
 #pragma unroll
         for (uint32_t b = 0; b < kSub; ++b) {
 #pragma unroll
             for (uint32_t r = 0; r < kHeld; ++r) {
-                score[b][r] = weight_of<P == 3>(score[b][r], level, args.log2_scale);
+                score[b][r] = weight_of<R>(score[b][r], level, args.log2_scale);
                 if constexpr (P == 3u) {
                     denominator += score[b][r];
                 }
@@ -1515,7 +1528,10 @@ void k_paged_chunk(AttendArgs args) {
                     }
                 }
                 if constexpr (P == 1u) {
-                    ones_sum = mfma<M>(u32x4{one, one, one, one}, weights[0], ones_sum);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k) {
+                        denominator = pair_sum<M>(weights[0][k], denominator);
+                    }
                 }
                 // the values transposed: lane i of 16 takes row i / 4 of four
                 // entries at dimension 4 (i % 4), and gets dimension i of the four
@@ -1670,7 +1686,7 @@ void k_paged_chunk(AttendArgs args) {
         // the products left them out, the rows that see them get them.
         for (int32_t first = begin; first < end; first += step) {
             for (int32_t entry = first; edge_tile(first) && entry < min(first + step, end); ++entry) {
-                const float weight = odd_weight<T, R, D, P == 3>(args, table, keys, query, entry, maximum);
+                const float weight = odd_weight<T, R, D>(args, table, keys, query, entry, maximum);
                 const bool visible = entry <= position && entry >= oldest;
                 const Page page = page_of(cache, table, entry);
                 const T *const value = values + page.at;
@@ -1686,14 +1702,10 @@ void k_paged_chunk(AttendArgs args) {
         }
     }
 
-    if constexpr (P == 1u) {
-        denominator = ones_sum[0];
-    } else {
-        if constexpr (W == 16u) {
-            denominator += lane_xor<16>(denominator);
-        }
-        denominator += lane_xor<32>(denominator);
+    if constexpr (W == 16u) {
+        denominator += lane_xor<16>(denominator);
     }
+    denominator += lane_xor<32>(denominator);
     if (!wave_live || wave_row + column >= rows) {
         return;
     }

@@ -846,7 +846,10 @@ void adi_hip_paged_workspace_destroy(adi_hip_paged_workspace *workspace);
  * Rows and cache types: f32 rows over an f32 or bf16 cache, else f16 or
  * bf16 for both (queries, gate and outputs have one type). f32 rows get
  * products of 32-bit accuracy; f16 and bf16 rows round the weights w_j to the
- * type (sums in 32 bits). Scores must stay within a float. query_heads is a multiple
+ * type (sums in 32 bits). Over an f32 cache, chunks (of more than 16 rows a KV
+ * head) take keys and queries to 2^-22 of each element or 2^-39 of
+ * the entry's or row's largest, whichever is more. Scores must stay within a float, and
+ * so must 2^8 times the sum of the values' magnitudes. query_heads is a multiple
  * of heads, at most 256 times it. The outputs overlap neither queries nor gate. Rows
  * of no sequence stay as they are. Sequences and KV heads: below 65536 each. */
 typedef struct {

@@ -909,3 +909,63 @@ def test_attention_scale_refusals(gpu, workspace):
     for scale in (3e38, math.nan, -math.inf):
         with pytest.raises(hip.HipError, match="scale"):
             hip.paged_attention(gpu, pool.cache(gpu), batch, q, torch.empty_like(q), workspace, scale=scale)
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("power", [12, 15, 20])
+@pytest.mark.parametrize("counts", [[1], [40]])
+def test_many_small_weights_add_up(gpu, workspace, rows, kind, power, counts):
+    """One entry of weight 1 and thousands of 2^-power, f16's subnormal
+    values among them (each exact in every type): none is lost, neither from the
+    sums nor from the denominator."""
+    def bend(pool, q):
+        pool.keys.zero_()
+        pool.values.fill_(1)
+        first = int(pool.table[0, 0])
+        pool.keys[first, 0, :, 0] = power
+        pool.values[first, 0] = 0
+        q.zero_()
+        q[..., 0] = 1
+
+    check_attention(gpu, workspace, rows, kind, 64, 4, 1, 64, counts, [6000], scale=math.log(2.0), bend=bend)
+    # (a group of 64: more than a step's rows)
+    check_attention(gpu, workspace, rows, kind, 128, 64, 1, 64, counts, [6000], scale=math.log(2.0), bend=bend)
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("heads", [4, 64])
+def test_weights_below_a_type_add_up_over_a_long_history(gpu, workspace, rows, kind, heads):
+    """130,000 weights of 2^-26, half of f16's least value: their sum is as near
+    as any other weights' are."""
+    def bend(pool, q):
+        pool.keys.zero_()
+        pool.values.fill_(1)
+        first = int(pool.table[0, 0])
+        pool.keys[first, 0, :, 0] = 26
+        pool.values[first, 0] = 0
+        q.zero_()
+        q[..., 0] = 1
+
+    check_attention(gpu, workspace, rows, kind, 64, heads, 1, 64, [1], [130000], scale=math.log(2.0), bend=bend)
+
+
+def test_layer_over_pages_keeps_bad_rows_to_themselves(gpu, workspace, layer):
+    """A sequence over the batch's bounds, one with a bad page, rows of no
+    sequence: NaN (or nothing of use) there, the others' rows as without them."""
+    _, device = layer
+    x = normal(5, 30, 256)
+    pool = Pool(2, [40, 60, 25, 33], 16, 2, 256, "f32", junk=None)
+
+    def call(lengths, table, pages):
+        out = torch.empty_like(x)
+        batch = hip.PagedBatch(gpu, ints([0, 9, 10, 21, 27]), ints(lengths), ints(table), 30, 12, 64)
+        hip.full_attention_paged(gpu, device, hip.PagedCache(gpu, *pages), batch, x, out, workspace)
+        return out
+
+    good = call(pool.lengths, pool.table, (pool.keys.clone(), pool.values.clone()))
+    table = pool.table.copy()
+    table[2, 0] = 1 << 20
+    bad = call([40, 65, 25, 33], table, (pool.keys.clone(), pool.values.clone()))
+    assert bool(torch.isnan(bad[9:21]).all()) and bool(torch.isfinite(good[:27]).all())
+    for rows in (slice(0, 9), slice(21, 27)):
+        assert torch.equal(bad[rows], good[rows])
