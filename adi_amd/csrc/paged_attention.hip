@@ -25,9 +25,9 @@
 // products for six, and elements down to 2^-16 of the largest keep 22 bits.
 //
 // Rounding: scores, levels, sums and denominators are 32 bits. 16-bit rows'
-// weights are rounded once to the rows' type, as the products take them (the
-// denominator in k_paged_chunk is the sum of the rounded ones, which cancels
-// a part of it), and outputs once at the end.
+// weights are rounded once to the rows' type, as the products take them (in
+// k_paged_chunk the denominator is the sum of the rounded ones, which cancels a
+// part of it), and outputs once at the end.
 #include "paged_attention.hpp"
 
 #include <atomic>
@@ -1028,15 +1028,18 @@ constexpr size_t chunk_lds() {
 }
 
 // Bound by matrix and vector phases that overlap in part: 8192 f16 tokens, 32
-// heads of 64 on 4, 275 GFLOP, 406 us (0.68 PFLOP/s; a large library product
-// reaches 1.29): the matrix cores are busy 44% of the cycles, the vector
-// units (of which half is exponentials) 54%, at a clock that such work takes down to
-// 1.8 GHz. Ragged chunks of 5 sequences in bf16, 32 heads of 128 on 8, 160 us (38%
-// and 44%); 512 f32 tokens behind 3584 over f32 heads of 256, 150 us and a join
-// of 12 (nine products an element: 47% of the matrix cores' cycles). Tried without gain:
-// the waves' halves a phase apart over two buffers of keys and three of values
-// (165 -> 185 us for the chunks), wave priorities for either phase (165 -> 170 and 175),
-// scores or weights kept apart from the products by scheduling barriers (171).
+// heads of 64 on 4, 275 GFLOP, 392 us (0.70 PFLOP/s; a large library product
+// reaches 1.29): the matrix cores are busy 36% of the cycles, the vector units
+// (a third of it exponentials) 58%, at a clock that such work takes down to 1.8
+// GHz. Ragged chunks of 5 sequences in bf16, 32 heads of 128 on 8, 155 us (35%
+// and 47%); 512 f32 tokens behind 3584 over f32 heads of 256, 150 us and a join
+// of 12 (nine products an element: 44% and 43%). Tried without gain: the waves' halves
+// a phase apart over two buffers of keys and three of values (165 -> 185 us for
+// the ragged chunks), the next tile's scores among a tile's exponentials over three
+// buffers (165 -> 209, the prompt 424 -> 562), wave priorities for either phase
+// (165 -> 170 and 175), weights kept apart from the products by scheduling
+// barriers (171); 16-bit denominators as a row of ones on the matrix cores (165, now
+// 161; the prompt 424 -> 415).
 //
 // Block (row tile, KV head, part, sequence). Lane l of a wave is row l % ROWS
 // of the wave's and piece l / ROWS of its keys.
