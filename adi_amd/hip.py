@@ -1166,20 +1166,20 @@ _pack_attention = struct.Struct("=I4x I4xQQQ I4xQQQ I4xQQQ f I").pack
 _no_rows = (0, 0, 0, 0)
 
 
-def _rows(ctx: Context, t, tokens: int, heads: Optional[int], head_size: int):
+def _rows(ctx: Context, t, tokens: int, heads: int, head_size: int):
     """A tensor [tokens, heads, head size] (any strides of the first two) as
     the fields of adi_hip_rows."""
-    shape = t.shape
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_size or (heads is not None and shape[1] != heads):
-        _refuse(f"rows of shape {tuple(shape)}, expected [{tokens}, {heads or 'heads'}, {head_size}]")
+    if t.shape != (tokens, heads, head_size):
+        _refuse(f"rows of shape {tuple(t.shape)}, expected [{tokens}, {heads}, {head_size}]")
     token_stride, head_stride, step = t.stride()
-    if step != 1 and head_size > 1:
-        _refuse("a head's elements must be contiguous")
     if t.get_device() != ctx.device:
         _refuse(f"rows on {t.device}, the context is on cuda:{ctx.device}")
-    if (token_stride == 0 and shape[0] > 1) or (head_stride == 0 and shape[1] > 1):
+    if step != 1 and head_size > 1:
+        _refuse("a head's elements must be contiguous")
+    if (token_stride == 0 and tokens > 1) or (head_stride == 0 and heads > 1):
         _refuse("broadcast rows are not supported")
-    return _type_codes.get(t.dtype) if t.dtype in _type_codes else _type_of(t), t.data_ptr(), token_stride, head_stride
+    code = _type_codes.get(t.dtype)
+    return _type_of(t) if code is None else code, t.data_ptr(), token_stride, head_stride
 
 
 def _device_words(ctx: Context, t, name: str, *shape):
