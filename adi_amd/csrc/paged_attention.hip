@@ -63,6 +63,7 @@ struct AttendArgs {
     uint32_t group;       // query heads of a KV head
     uint32_t span, parts; // entries of a part of a history, parts at most
     uint32_t mixed;       // nonzero: k_paged_step takes the sequences of few rows, k_paged_chunk the others
+    uint32_t slots;       // k_paged_step: blocks of a KV head that the sequences share by their lengths; 0: `parts` each
     uint32_t *tickets;    // [sequence][KV head], zero between calls (k_paged_step)
     float *partial;       // [part][token][head][D + 4]: sums, maximum, denominator (parts > 1)
 };
@@ -356,9 +357,9 @@ constexpr uint32_t step_blocks() {
 }
 
 // Bound by the entries' bytes where there are many: two sequences behind 131,071
-// entries, 8 heads of 128 in bf16, 831 MB in 160 us, 5.2 TB/s, what a large copy
-// reaches; 32 sequences of up to 4,096 entries, 154 MB, 43 us (3.6 TB/s: their
-// lengths differ, and a block's start and end are some 8 us). Where there are few,
+// entries, 8 heads of 128 in bf16, 832 MB in 155 us, 5.4 TB/s, what a large copy
+// reaches; 32 sequences of up to 4,096 entries, 153 MB, 35 us (4.4 TB/s: a
+// block's start and end are some 8 us). Where there are few,
 // by its chain of latencies: one token behind 1,999 entries of 2 heads of 256 in
 // f32, 8.2 MB, 18 us: some 4 to start, page numbers, a tile's loads and products
 // 3, the join of 32 parts 7.
@@ -380,15 +381,80 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
     constexpr uint32_t kSide = kFloat ? 4u : D == 64u ? 4u : 8u, kGroups = D / (16u * kSide);
     constexpr uint32_t kRegion = kStepRows * (D + 4u);
     constexpr bool kEager = step_eager<T, R, D>();
+    constexpr int32_t kTurn = 4 * kKeys;  // entries of the four waves' tiles
     static_assert(kRegion * sizeof(float) % 128u == 0u);
     __shared__ StepLds<D> lds;
     const PagedView &cache = args.c;
-    const uint32_t kv = blockIdx.x % cache.heads, part = blockIdx.x / cache.heads, sequence = blockIdx.y;
+    const uint32_t kv = blockIdx.x % cache.heads;
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const uint32_t c = lane & 15u, g = lane >> 4;
-    const SequenceRows s = sequence_rows(cache, sequence);
-    if (s.count == 0u || (args.mixed != 0u && s.count * args.group > kStepRows)) {
-        return;
+    const auto takes = [&](const SequenceRows &of) {
+        return of.count != 0u && (args.mixed == 0u || of.count * args.group <= kStepRows);
+    };
+    SequenceRows s;
+    uint32_t part = blockIdx.x / cache.heads, sequence = blockIdx.y, span = args.span;
+    // the regions of the workspace of this (sequence, KV head): the first, and
+    // how many lie from one part's to the next's
+    uint32_t region_base = (sequence * cache.heads + kv) * args.parts, region_step = 1u;
+    if (args.slots != 0u) {
+        // Up to 64 sequences, one a lane: a span with which their parts fit the
+        // slots. A sequence's last part is half empty on the average, so total /
+        // (slots - sequences / 2) entries; where that is too short total / (slots -
+        // sequences), which always fits, as a sequence has less than one part more
+        // than its share.
+        const SequenceRows own =
+            lane < cache.sequences ? sequence_rows(cache, lane) : SequenceRows{0u, 0u, 0u, false};
+        const bool taken = takes(own);
+        const int32_t own_first = static_cast<int32_t>(own.length) - static_cast<int32_t>(own.count);
+        const uint32_t extent = !taken                          ? 0u
+                                : own.over || own.length == 0u ? 1u
+                                                               : own.length - static_cast<uint32_t>(base_of(args, own_first));
+        float total = static_cast<float>(extent);
+        total += lane_xor<1>(total);
+        total += lane_xor<2>(total);
+        total += lane_xor<4>(total);
+        total += lane_xor<8>(total);
+        total += lane_xor<16>(total);
+        total += lane_xor<32>(total);
+        const float live_sequences = static_cast<float>(__popcll(__ballot(taken)));
+        uint32_t parts = 0, sum = 0;
+#pragma unroll 1
+        for (uint32_t attempt = 0; attempt < 2u; ++attempt) {
+            // (more slots than sequences; the sums' roundings are below 2^-17)
+            const float left = static_cast<float>(args.slots) - live_sequences * (attempt == 0u ? 0.5f : 1.0f);
+            const float wanted = total * 1.0001f / left;
+            span = max(args.span, (static_cast<uint32_t>(wanted) + kTurn) & ~(static_cast<uint32_t>(kTurn) - 1u));
+            parts = (extent + span - 1u) / span;
+            sum = parts;
+#pragma unroll
+            for (uint32_t d = 1; d < 64u; d *= 2u) {
+                const uint32_t below = __shfl_up(sum, d);
+                sum += lane >= d ? below : 0u;
+            }
+            if (__shfl(sum, 63) <= args.slots) {
+                break;
+            }
+        }
+        const uint64_t past = __ballot(sum > part);
+        if (past == 0u) {
+            return;
+        }
+        const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+        const auto of = [&](uint32_t v) {
+            return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), at));
+        };
+        sequence = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(at));
+        const uint32_t before = of(sum) - of(parts);
+        part -= before;
+        region_base = before * cache.heads + kv;
+        region_step = cache.heads;
+        s = {of(own.first), of(own.count), of(own.length), of(own.over ? 1u : 0u) != 0u};
+        span = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(span)));
+    } else {
+        s = sequence_rows(cache, sequence);
+        if (!takes(s)) {
+            return;
+        }
     }
     if (s.over || s.length == 0u) {
         if (part == 0u) {
@@ -404,12 +470,12 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
     const int32_t window = static_cast<int32_t>(args.window);
     const int32_t oldest = window == 0 ? 0 : max(0, position - window + 1);  // the row's first entry
     const int32_t base = base_of(args, first_position);
-    const int32_t begin = base + static_cast<int32_t>(part * args.span);
-    const int32_t end = min(begin + static_cast<int32_t>(args.span), static_cast<int32_t>(s.length));
+    const int32_t begin = base + static_cast<int32_t>(part * span);
+    const int32_t end = static_cast<int32_t>(min(static_cast<uint32_t>(begin) + span, s.length));
     if (begin >= end) {
         return;
     }
-    const uint32_t live = (s.length - static_cast<uint32_t>(base) + args.span - 1u) / args.span;
+    const uint32_t live = (s.length - static_cast<uint32_t>(base) + span - 1u) / span;
     // entries that some row sees, and those that every row sees
     const int32_t seen_from = window == 0 ? 0 : max(0, first_position - window + 1);
     const int32_t all_from = window == 0 ? 0 : max(0, static_cast<int32_t>(s.length) - window);
@@ -424,7 +490,6 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
     const uint32_t key_group = (kHeld * (c >> 2)) & ~7u, value_group = (kHeld * g) & ~7u;
     const uint64_t key_at = ((kHeld * (c >> 2) & 7u) + (c & 3u)) * cache.entry_stride;
     const uint64_t value_at = ((kHeld * g) & 7u) * cache.entry_stride;
-    constexpr int32_t kTurn = 4 * kKeys;  // entries of the four waves' tiles
     struct Numbers {
         uint32_t key, value;
     };
@@ -772,8 +837,8 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         }
         store_output<R, 4>(args, s.first + r / args.group, kv * args.group + r % args.group, at, out);
     };
-    // this part's region of the workspace
-    float *const joint = args.partial + (static_cast<uint64_t>(sequence) * cache.heads + kv) * args.parts * kRegion;
+    float *const joint = args.partial + static_cast<uint64_t>(region_base) * kRegion;
+    const uint32_t part_step = region_step * kRegion;
     for (uint32_t i = t; i < rows * (D / 4u); i += kThreads) {
         const uint32_t r = i / (D / 4u), at = i % (D / 4u) * 4u;
         const float top = top_of(r);
@@ -788,7 +853,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
             store_row(r, at, sum, total);
             continue;
         }
-        float *const region = joint + static_cast<uint64_t>(part) * kRegion;
+        float *const region = joint + static_cast<uint64_t>(part) * part_step;
         store_through(region, r * (D + 4u) + at, sum);
         if (at == 0u) {
             store_through(region, r * (D + 4u) + D, f32x4{top, total, 0.0f, 0.0f});
@@ -814,7 +879,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
     // top, factors and total by a wave
     for (uint32_t i = t; i < live * rows; i += kThreads) {
         const uint32_t p = i / rows, r = i % rows;
-        const f32x4 v = load_through(joint, p * kRegion + r * (D + 4u) + D);
+        const f32x4 v = load_through(joint, p * part_step + r * (D + 4u) + D);
         lds.parts.factor[p][r] = v[0];
         lds.parts.total[p][r] = v[1];
     }
@@ -862,7 +927,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
             f32x4 v[kAhead];
 #pragma unroll
             for (uint32_t u = 0; u < kAhead; ++u) {
-                v[u] = load_through(joint, min(p + u * step, live - 1u) * kRegion + at);
+                v[u] = load_through(joint, min(p + u * step, live - 1u) * part_step + at);
             }
 #pragma unroll
             for (uint32_t u = 0; u < kAhead; ++u) {
@@ -1774,14 +1839,8 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
         a.tickets = static_cast<uint32_t *>(workspace->base);
         const uint64_t blocks = uint64_t(c.sequences) * c.heads;
         const uint64_t region = uint64_t(kStepRows) * (D + 4u) * sizeof(float);
-        uint64_t parts = 1;
-        if (blocks <= kTickets) {
-            // as many as the chip holds blocks
-            parts = std::min<uint64_t>({uint64_t(step_blocks<T, R, D>()) * ctx->cu_count / blocks, room / (blocks * region), kStepParts});
-        }
         // (one tile a wave at least)
         constexpr uint64_t kUnit = std::is_same_v<T, float> ? 64 : 128;
-        a.span = span_of(std::max<uint64_t>(parts, 1u), kUnit);
         // A part's tiles, and the parts that the last block joins, both go through
         // one CU at about its rate, so a part takes at least the entries for which
         // the two are even (a token of 16 heads on 2 behind 8000 entries: f32 of
@@ -1790,9 +1849,29 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
         // 12.5 and 13.7).
         const uint64_t rows = std::min<uint64_t>(uint64_t(c.max_tokens) * args.group, kStepRows);
         const double even = std::sqrt(double(extent) * rows * (D + 4u) * sizeof(float) / (2.0 * D * sizeof(T)));
-        a.span = std::max(a.span, static_cast<uint32_t>(uint64_t(even / kUnit + 0.5) * kUnit));
-        a.parts = ceil_div(extent, a.span);
-        launch(ctx, "paged_step", k_paged_step<T, R, D>, dim3(a.parts * c.heads, c.sequences), dim3(kThreads), 0, a);
+        const uint32_t least = std::max(span_of(kStepParts, kUnit), static_cast<uint32_t>(uint64_t(even / kUnit + 0.5) * kUnit));
+        const uint64_t resident = uint64_t(step_blocks<T, R, D>()) * ctx->cu_count;
+        const uint64_t slots = std::min({resident / c.heads, room / (c.heads * region),
+                                         uint64_t(c.sequences) * ceil_div(extent, least)});
+        if (c.sequences > 1 && c.sequences <= 64 && slots > c.sequences && blocks <= kTickets) {
+            // As many blocks as the chip holds, shared by the lengths on the device.
+            // As many parts a sequence as if all were of max_length leave a
+            // third of the chip idle with lengths that are even up to it: 32
+            // sequences up to 4,096 of 16 f32 heads on 2 of 256 in bf16 43.1
+            // us, so 34.8; up to 8,000 of 32 heads on 8 of 128 146 and 130; 8
+            // sequences up to 4,000 of 2 f32 heads of 256 28.5 and 29.5.
+            a.span = least;
+            a.slots = static_cast<uint32_t>(slots);
+            launch(ctx, "paged_step", k_paged_step<T, R, D>, dim3(a.slots * c.heads), dim3(kThreads), 0, a);
+        } else {
+            uint64_t parts = 1;
+            if (blocks <= kTickets) {
+                parts = std::clamp<uint64_t>(std::min(resident / blocks, room / (blocks * region)), 1u, kStepParts);
+            }
+            a.span = std::max(span_of(parts, kUnit), parts > 1 ? least : 0u);
+            a.parts = ceil_div(extent, a.span);
+            launch(ctx, "paged_step", k_paged_step<T, R, D>, dim3(a.parts * c.heads, c.sequences), dim3(kThreads), 0, a);
+        }
         if (few) {
             return;
         }
@@ -1891,7 +1970,7 @@ void paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache, con
     const uint32_t window = std::min(a->window, 1u << 30);
     const AttendArgs args{paged_view(*cache, *batch), rows_view(a->queries), rows_view(a->outputs), rows_view(a->gate),
                           static_cast<float>(scale * 1.4426950408889634),
-                          static_cast<float>(kSlack / (scale * 1.4426950408889634)), window, a->query_heads / cache->heads, 0, 0, 0,
+                          static_cast<float>(kSlack / (scale * 1.4426950408889634)), window, a->query_heads / cache->heads, 0, 0, 0, 0,
                           nullptr, nullptr};
     if (type == ADI_HIP_F32 && cache->type == ADI_HIP_F32) {
         launch_attention<float, float>(ctx, args, workspace, cache->head_size);

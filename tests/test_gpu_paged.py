@@ -969,3 +969,16 @@ def test_layer_over_pages_keeps_bad_rows_to_themselves(gpu, workspace, layer):
     assert bool(torch.isnan(bad[9:21]).all()) and bool(torch.isfinite(good[:27]).all())
     for rows in (slice(0, 9), slice(21, 27)):
         assert torch.equal(bad[rows], good[rows])
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("window", [0, 300])
+def test_attention_of_steps_of_very_different_lengths(gpu, workspace, rows, kind, window):
+    """Blocks shared by the lengths on the device: one long history among short
+    and empty ones (whose one part each leaves few of the blocks), and
+    all about alike."""
+    for lengths in ([1 + s % 40 for s in range(29)] + [6000] + [0, 9, 0] + [5] * 26,
+                    [900 + 31 * s for s in range(24)], [4000, 3], [2] * 64):
+        counts = [1] * len(lengths)
+        check_attention(gpu, workspace, rows, kind, 64, 8, 8, 16, counts, lengths, window=window)
+    check_attention(gpu, workspace, rows, kind, 256, 4, 1, 64, [2, 0, 1, 3], [700, 50, 3000, 2], window=window)
