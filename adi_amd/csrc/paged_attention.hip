@@ -1826,13 +1826,65 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
     };
     const size_t room = workspace->bytes - kTickets * sizeof(uint32_t);
     float *const partial = reinterpret_cast<float *>(static_cast<char *>(workspace->base) + kTickets * sizeof(uint32_t));
+    using Shape = typename ChunkOf<T, R, D>::Shape;
+    constexpr uint32_t kBlockRows = chunk_rows<T, R, D>();
+    // A chunk's parts, those that end first, by us: 32 keys of a row tile about
+    // kTurn, rounds of the blocks the chip holds (half a round more where there
+    // are several, for their uneven ends), a block's own start and end as 6 turns;
+    // the parts' way through memory at 5 TB/s, and a join's launch and loop. Within
+    // 3% of the best number of parts for six chunks of 64 to 512 tokens behind 4000
+    // and 8000 entries (64 tokens, 16 heads of 128 on 2 in bf16: 16 parts 30.2 us,
+    // 8 32.8, 32 35.2).
+    constexpr double kTurn = D / 64.0 * (std::is_same_v<R, float> ? 0.8 : 0.5);
+    struct Parts {
+        uint32_t span;
+        double cost;
+    };
+    const uint64_t part_bytes = uint64_t(c.tokens) * heads * (D + 4u) * sizeof(float);
+    const auto parts_of = [&](uint64_t row_tiles) {
+        const uint64_t most = std::clamp<uint64_t>(room / part_bytes, 1u, 64u);
+        const double resident = double(ctx->cu_count) * Shape::kBlocks;
+        Parts best{0, 0.0};
+        for (uint64_t parts = 1; parts <= most; ++parts) {
+            const uint64_t span = span_of(parts, kSpanUnit), real = ceil_div(extent, span);
+            const double count = double(row_tiles * c.heads * real);
+            const double rounds = count <= resident ? 1.0 : count / resident + 0.5;
+            const double cost = rounds * (span / 32.0 + 6.0) * kTurn +
+                                (real > 1 ? 4.0 + 0.3 * real + 2.0 * part_bytes * real / 5.0e6 : 0.0);
+            if (parts == 1 || cost < best.cost) {
+                best = {static_cast<uint32_t>(span), cost};
+            }
+        }
+        return best;
+    };
     // Few rows of every sequence: k_paged_step. Many of every one (as many as
     // there may be): k_paged_chunk. Else both, each for its sequences: in the
     // chunk kernel a single token costs its block a tile's whole staging (31 of
-    // them beside 512 tokens: 62 us of 175).
+    // them beside 512 tokens: 62 us of 175). But where the single tokens' blocks have
+    // room beside the chunks' (4 us by the parts' estimate) it takes them too, as
+    // the other's launch, start and end are 8 us: 80 tokens beside two single ones, an
+    // f32 head of 256, 32.0 us, so 23.6; 200 beside 7 behind 500 entries, 32 bf16
+    // heads on 8 of 128, 34.7 and 27.5; 256 beside 7 behind 2000, 16 f32 heads on 2
+    // of 256 in bf16, 75.5 as two, 98.9 as one.
     const bool few = uint64_t(c.max_tokens) * args.group <= kStepRows;
     const bool many = uint64_t(c.sequences) * c.max_tokens == c.tokens || c.sequences == 1;
-    args.mixed = !few && !many ? 1u : 0u;
+    // row tiles at most, about how many, and with the single tokens'
+    const uint64_t row_tiles =
+        std::min<uint64_t>(ceil_div(uint64_t(c.max_tokens) * args.group, kBlockRows) * uint64_t(c.sequences),
+                           uint64_t(c.tokens) * args.group / kBlockRows + c.sequences);
+    const uint64_t full = ceil_div(uint64_t(c.tokens) * args.group, kBlockRows);
+    Parts chunk{};
+    if (!few) {
+        chunk = parts_of(std::min(row_tiles, full + (many ? c.sequences / 2u : 0u)));
+        if (!many) {
+            const Parts all = parts_of(std::min<uint64_t>(row_tiles, full + c.sequences - 1u));
+            args.mixed = all.cost > chunk.cost + 4.0 ? 1u : 0u;
+            chunk = args.mixed != 0 ? chunk : all;
+        }
+        args.span = chunk.span;
+        args.parts = ceil_div(extent, args.span);
+        require((uint64_t(c.heads) * args.parts + 7u) / 8u * 8u * row_tiles < (1u << 23), "paged attention: too many rows");
+    }
     if (few || args.mixed != 0) {
         AttendArgs a = args;
         a.partial = partial;
@@ -1876,38 +1928,6 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
             return;
         }
     }
-    using Shape = typename ChunkOf<T, R, D>::Shape;
-    constexpr uint32_t kBlockRows = chunk_rows<T, R, D>();
-    // row tiles at most, and about how many
-    const uint64_t row_tiles =
-        std::min<uint64_t>(ceil_div(uint64_t(c.max_tokens) * args.group, kBlockRows) * uint64_t(c.sequences),
-                           uint64_t(c.tokens) * args.group / kBlockRows + c.sequences);
-    const uint64_t likely = std::min<uint64_t>(row_tiles, ceil_div(uint64_t(c.tokens) * args.group, kBlockRows) +
-                                                              (args.mixed != 0 ? 0u : c.sequences / 2u));
-    // The parts that end first, by us: 32 keys of a row tile about kTurn, rounds of
-    // the blocks the chip holds (half a round more where there are several, for
-    // their uneven ends), a block's own start and end as 6 turns; the parts' way
-    // through memory at 5 TB/s, and a join's launch and loop. Within 3% of the best
-    // number of parts for six chunks of 64 to 512 tokens behind 4000 and 8000
-    // entries (64 tokens, 16 heads of 128 on 2 in bf16: 16 parts 30.2 us, 8 32.8,
-    // 32 35.2).
-    constexpr double kTurn = D / 64.0 * (std::is_same_v<R, float> ? 0.8 : 0.5);
-    const uint64_t part_bytes = uint64_t(c.tokens) * heads * (D + 4u) * sizeof(float);
-    const uint64_t most = std::clamp<uint64_t>(room / part_bytes, 1u, 64u);
-    const double resident = double(ctx->cu_count) * Shape::kBlocks;
-    double least = 0.0;
-    for (uint64_t parts = 1; parts <= most; ++parts) {
-        const uint64_t span = span_of(parts, kSpanUnit), real = ceil_div(extent, span);
-        const double count = double(likely * c.heads * real);
-        const double rounds = count <= resident ? 1.0 : count / resident + 0.5;
-        const double cost = rounds * (span / 32.0 + 6.0) * kTurn +
-                            (real > 1 ? 4.0 + 0.3 * real + 2.0 * part_bytes * real / 5.0e6 : 0.0);
-        if (parts == 1 || cost < least) {
-            least = cost;
-            args.span = static_cast<uint32_t>(span);
-        }
-    }
-    args.parts = ceil_div(extent, args.span);
     args.partial = partial;
     constexpr size_t lds = chunk_lds<T, R, D>();
     // (once a device)
@@ -1919,7 +1939,6 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
     }
     const uint64_t pairs = uint64_t(c.heads) * args.parts;
     const uint64_t grid = (pairs < 8u ? pairs : (pairs + 7u) / 8u * 8u) * row_tiles;
-    require(grid < (1u << 23), "paged attention: too many rows");
     launch(ctx, "paged_chunk", k_paged_chunk<T, R, D>, dim3(static_cast<uint32_t>(grid)), dim3(Shape::kWaves * 64u),
            lds, args);
     if (args.parts > 1) {

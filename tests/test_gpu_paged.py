@@ -982,3 +982,20 @@ def test_attention_of_steps_of_very_different_lengths(gpu, workspace, rows, kind
         counts = [1] * len(lengths)
         check_attention(gpu, workspace, rows, kind, 64, 8, 8, 16, counts, lengths, window=window)
     check_attention(gpu, workspace, rows, kind, 256, 4, 1, 64, [2, 0, 1, 3], [700, 50, 3000, 2], window=window)
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("size", [64, 256])
+def test_attention_of_both_kernels_in_one_call(gpu, workspace, rows, kind, size):
+    """More single tokens than have room beside a chunk's blocks: those of
+    large heads take the other kernel, of small ones a second round of the chunk's;
+    with pages, windows and rows of no sequence as ever."""
+    counts = [1] * 30 + [0, 40] + [1] * 30 + [2]
+    lengths = [3 + (17 * s) % 150 for s in range(len(counts))]
+    lengths[31], lengths[40], lengths[41] = 700, 1500, 0
+    for window in (0, 60):
+        gpu.profiling(True)
+        check_attention(gpu, workspace, rows, kind, size, 32, 16, 16, counts, lengths, window=window, padding=3)
+        ran = gpu.profile()
+        gpu.profiling(False)
+        assert "paged_chunk" in ran and ("paged_step" in ran or size == 64)
