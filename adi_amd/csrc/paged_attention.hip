@@ -364,7 +364,8 @@ constexpr uint32_t step_blocks() {
 // f32, 8.2 MB, 18 us: some 4 to start, page numbers, a tile's loads and products
 // 3, the join of 32 parts 7.
 //
-// Block (KV head, part, sequence): its four waves take the part's tiles in turn,
+// Block (KV head, part, sequence), the parts of up to 64 sequences by their
+// lengths: its four waves take the part's tiles in turn,
 // each straight from the cache into operands, the next tile's keys on their way
 // from the end of this one's scores and its values from the end of their
 // products. Lane l is column c = l % 16 (a row), quarter g = l / 16. The blocks
