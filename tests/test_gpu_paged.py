@@ -999,3 +999,36 @@ def test_attention_of_both_kernels_in_one_call(gpu, workspace, rows, kind, size)
         ran = gpu.profile()
         gpu.profiling(False)
         assert "paged_chunk" in ran and ("paged_step" in ran or size == 64)
+
+
+def test_captured_layer_replays_with_new_lengths(gpu, workspace, layer):
+    """The layer over pages captured after a warm-up call, its replays against
+    eager calls on a copy of the pool while the lengths grow."""
+    _, device = layer
+    stores = [[normal(i, 24, 16, 2, 256) for i in (1, 2)] for _ in range(2)]
+    caches = [hip.PagedCache(gpu, *s) for s in stores]
+    lengths, x = ints([5, 20, 9]), normal(3, 3, 256)
+    table = ints(np.random.default_rng(2).permutation(24).reshape(3, 8))
+    batch = hip.PagedBatch(gpu, ints([0, 1, 2, 3]), lengths, table, 3, 1, 128)
+    out, want = torch.empty_like(x), torch.empty_like(x)
+    own = hip.PagedWorkspace(gpu, 8 << 20)
+    hip.full_attention_paged(gpu, device, caches[0], batch, x, out, own)
+    hip.full_attention_paged(gpu, device, caches[1], batch, x, want, workspace)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            gpu.use_stream(torch.cuda.current_stream())
+            hip.full_attention_paged(gpu, device, caches[0], batch, x, out, own)
+    finally:
+        gpu.use_stream(torch.cuda.current_stream())
+    for growth in (1, 1, 40, 60):
+        lengths += growth
+        x.copy_(normal(10 + growth, 3, 256))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        hip.full_attention_paged(gpu, device, caches[1], batch, x, want, workspace)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and bool(torch.isfinite(out).all())
+        assert all(torch.equal(a, b) for a, b in zip(*stores))
