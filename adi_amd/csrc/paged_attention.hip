@@ -58,7 +58,7 @@ struct AttendArgs {
     PagedView c;
     RowsView queries, outputs, gate;
     float log2_scale;     // scale log2 e
-    float slack;          // kSlack / log2_scale
+    float slack, far;     // kSlack, kFar / log2_scale
     uint32_t window;
     uint32_t group;       // query heads of a KV head
     uint32_t span, parts; // entries of a part of a history, parts at most
@@ -88,28 +88,84 @@ __device__ __forceinline__ int32_t base_of(const AttendArgs &a, int32_t first_po
 // vector work; a weight of 2^8 is as exact as one of 1.
 constexpr float kSlack = 8.0f;
 
-// exp2(log2_scale (s - m)), s at most kSlack above m: for f32 rows the difference is taken
-// first, so that its rounding is relative to it; for 16-bit rows in one
-// multiply-add.
-template <bool EXACT>
-__device__ __forceinline__ float factor_of(float s, float m, float log2_scale) {
-    if constexpr (EXACT) {
-        return __builtin_amdgcn_exp2f((s - m) * log2_scale);
+// How far from 0 (in powers of two of a weight) a row's level may lie for that
+// slack, and for a 16-bit row's exponents in one multiply-add: beyond it a
+// float's step at the level (2^-3 here) comes near the slack, and passes it.
+constexpr float kFar = 1048576.0f;
+
+__device__ __forceinline__ bool far_level(const AttendArgs &a, float m) { return fabsf(m) > a.far; }
+
+// exp2(log2_scale (s - m)): what sums at level s are multiplied by at level m.
+__device__ __forceinline__ float factor_of(const AttendArgs &a, float s, float m) {
+    return __builtin_amdgcn_exp2f((s - m) * a.log2_scale);
+}
+
+// A score s has the exponent log2_scale (s - minus) + offset at a row's level m. f32
+// rows take the difference first (minus = m), so that its rounding is relative to
+// it. 16-bit rows do with one multiply-add, and -m log2_scale rounded once as
+// the offset: as good as exact, as their sums are held at the level of that
+// offset, until settle_of takes them to m's. Far levels take the difference.
+// f16 rows' exponents are 7 more (sums and denominators alike, so outputs are
+// not): weights are up to 2^15 with the slack, and down to 2^-31 of the level
+// before one is rounded to nothing, so that it takes a history of 2^20 such
+// entries to matter; bf16 has the range as it is.
+struct Level {
+    float minus, offset;
+};
+template <typename R>
+constexpr float kLift = std::is_same_v<R, _Float16> ? 7.0f : 0.0f;
+template <typename R>
+__device__ __forceinline__ Level near_level_of(const AttendArgs &a, float maximum) {
+    const float m = maximum == kNegative ? 0.0f : maximum;
+    if constexpr (std::is_same_v<R, float>) {
+        return {m, 0.0f};
     } else {
-        return __builtin_amdgcn_exp2f(fmaf(s, log2_scale, -m * log2_scale));
+        return {0.0f, fmaf(-m, a.log2_scale, kLift<R>)};
+    }
+}
+template <typename R>
+__device__ __forceinline__ Level level_of(const AttendArgs &a, float maximum) {
+    if constexpr (!std::is_same_v<R, float>) {
+        if (maximum != kNegative && far_level(a, maximum)) {
+            return {maximum, kLift<R>};
+        }
+    }
+    return near_level_of<R>(a, maximum);
+}
+
+// The exponent of a score that `minus` is taken from already.
+template <typename R>
+__device__ __forceinline__ float exponent_of(const AttendArgs &a, float s, const Level &level) {
+    return std::is_same_v<R, float> ? s * a.log2_scale : fmaf(s, a.log2_scale, level.offset);
+}
+template <typename R>
+__device__ __forceinline__ float weight_of(const AttendArgs &a, float s, const Level &level) {
+    return __builtin_amdgcn_exp2f(exponent_of<R>(a, s, level));
+}
+
+// What a row's sums are multiplied by when its level rises from `from` to `to`.
+template <typename R>
+__device__ __forceinline__ float raise_of(const AttendArgs &a, float from, float to) {
+    if constexpr (std::is_same_v<R, float>) {
+        return factor_of(a, from, to);
+    } else {
+        const Level was = level_of<R>(a, from), is = level_of<R>(a, to);
+        return from == kNegative ? 0.0f
+                                 : __builtin_amdgcn_exp2f(exponent_of<R>(a, to - is.minus, is) -
+                                                          exponent_of<R>(a, to - was.minus, was));
     }
 }
 
-// A score's weight at a level. f16 rows' are 2^7 of that (sums and denominators
-// alike, so outputs are not): up to 2^15 with the slack, and down to 2^-31 of the
-// level before one is rounded to nothing, so that it takes a history of 2^20
-// such entries to matter; bf16 has the range as it is.
+// What takes a row's sums from its offset's level to `maximum` itself, by which
+// they are joined with others.
 template <typename R>
-__device__ __forceinline__ float weight_of(float s, float m, float log2_scale) {
-    if constexpr (std::is_same_v<R, _Float16>) {
-        return __builtin_amdgcn_exp2f(fmaf(s, log2_scale, fmaf(-m, log2_scale, 7.0f)));
+__device__ __forceinline__ float settle_of(const AttendArgs &a, float maximum) {
+    if constexpr (std::is_same_v<R, float>) {
+        return 1.0f;
     } else {
-        return factor_of<std::is_same_v<R, float>>(s, m, log2_scale);
+        const Level level = level_of<R>(a, maximum);
+        const float m = maximum == kNegative ? 0.0f : maximum;
+        return __builtin_amdgcn_exp2f(kLift<R> - exponent_of<R>(a, m - level.minus, level));
     }
 }
 
@@ -250,7 +306,8 @@ __device__ __forceinline__ float odd_weight(const AttendArgs &a, const uint32_t 
     for (uint32_t d = 0; d < D; ++d) {
         score = fmaf(static_cast<float>(query[d]), static_cast<float>(key[d]), score);
     }
-    return weight_of<R>(score, maximum == kNegative ? 0.0f : maximum, a.log2_scale);
+    const Level level = level_of<R>(a, maximum);
+    return weight_of<R>(a, score - level.minus, level);
 }
 
 // N consecutive outputs of a row, gated.
@@ -612,6 +669,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
     // the level of the row's weights (kNegative before its first score), and the
     // score from which it is raised
     float maximum = kNegative, limit = kNegative, denominator = 0.0f;
+    bool far = false;  // some row's level is
     // a tile that some row does not see whole
     const auto edge_tile = [&](int32_t at) {
         return at + static_cast<int32_t>(kKeys) > first_position + 1 || at < all_from;
@@ -712,9 +770,10 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         if (__any(top > limit)) {
             // (a row's level does not depend on the wave's other rows)
             const bool raised = top > limit;
-            const float factor = raised ? factor_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
+            const float factor = raised ? raise_of<R>(args, maximum, top) : 1.0f;
             maximum = raised ? top : maximum;
-            limit = raised ? top + args.slack : limit;
+            limit = raised ? top + (far_level(args, top) ? 0.0f : args.slack) : limit;
+            far = __any(maximum != kNegative && far_level(args, maximum)) != 0;
             denominator *= factor;
 #pragma unroll
             for (uint32_t i = 0; i < kGroups; ++i) {
@@ -724,10 +783,17 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
                 }
             }
         }
-        const float level = maximum == kNegative ? 0.0f : maximum;
+        Level level = near_level_of<R>(args, maximum);
+        if (P == 1u && far) {
+            level = level_of<R>(args, maximum);
+#pragma unroll
+            for (uint32_t k = 0; k < kHeld; ++k) {
+                score[k] -= level.minus;
+            }
+        }
 #pragma unroll
         for (uint32_t k = 0; k < kHeld; ++k) {
-            score[k] = weight_of<R>(score[k], level, args.log2_scale);
+            score[k] = weight_of<R>(args, P == 3u ? score[k] - level.minus : score[k], level);
             denominator += score[k];
         }
         if constexpr (kFloat) {
@@ -803,19 +869,21 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
     // the row's lanes' parts of the denominator, then the waves
     denominator += lane_xor<16>(denominator);
     denominator += lane_xor<32>(denominator);
+    const float settle = settle_of<R>(args, maximum);
+    denominator *= settle;
     if (g == 0u) {
         lds.maximum[wave][c] = maximum;
         lds.denominator[wave][c] = denominator;
     }
     __syncthreads();
     const auto join_factor = [&](float m, float top) {
-        return m == kNegative && top == kNegative ? 1.0f : factor_of<P == 3>(m, top, args.log2_scale);
+        return m == kNegative && top == kNegative ? 1.0f : factor_of(args, m, top);
     };
     const auto top_of = [&](uint32_t r) {
         return fmaxf(fmaxf(lds.maximum[0][r], lds.maximum[1][r]), fmaxf(lds.maximum[2][r], lds.maximum[3][r]));
     };
     if (c < rows) {
-        const float factor = join_factor(maximum, top_of(c));
+        const float factor = join_factor(maximum, top_of(c)) * settle;
 #pragma unroll
         for (uint32_t i = 0; i < kGroups; ++i) {
 #pragma unroll
@@ -967,7 +1035,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
 // factors of parts l, l + 64, ... and dimensions D / 64 l .. of every part. Bound
 // by the parts' bytes, which the chunks have just written: 8,192 rows of four
 // parts of 256, 34 MB, 12.5 us.
-template <typename R, uint32_t D, bool EXACT>
+template <typename R, uint32_t D>
 __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
     constexpr uint32_t kSide = D / 64u;
     const PagedView &cache = args.c;
@@ -1025,7 +1093,7 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
             const float *part = partial_row<D>(args, p, token, head);
             const float m = part[D], d = part[D + 1u];
             const Side v = *reinterpret_cast<const Side *>(part + kSide * lane);
-            const float factor = m == kNegative && top == kNegative ? 1.0f : factor_of<EXACT>(m, top, args.log2_scale);
+            const float factor = m == kNegative && top == kNegative ? 1.0f : factor_of(args, m, top);
             total += d * factor;
 #pragma unroll
             for (uint32_t k = 0; k < kSide; ++k) {
@@ -1469,6 +1537,7 @@ void k_paged_chunk(AttendArgs args) {
     // the level of the row's weights (kNegative before its first score), and the
     // score from which it is raised
     float maximum = kNegative, limit = kNegative, denominator = 0.0f;
+    bool far = false;  // some row's level is
     // a lane's keys of 32, and register r of sums[m]
     const auto key_of = [&](uint32_t r) {
         return W == 32u ? 8u * (r / 4u) + 4u * side + r % 4u : 8u * side + r;
@@ -1564,21 +1633,32 @@ void k_paged_chunk(AttendArgs args) {
         if (__any(top > limit)) {
             // (a row's level does not depend on the wave's other rows)
             const bool raised = top > limit;
-            const float factor = raised ? factor_of<P == 3>(maximum, top, args.log2_scale) : 1.0f;
+            const float factor = raised ? raise_of<R>(args, maximum, top) : 1.0f;
             maximum = raised ? top : maximum;
-            limit = raised ? top + args.slack : limit;
+            limit = raised ? top + (far_level(args, top) ? 0.0f : args.slack) : limit;
+            far = __any(maximum != kNegative && far_level(args, maximum)) != 0;
             denominator *= factor;
 #pragma unroll
             for (uint32_t m = 0; m < D / W; ++m) {
                 sums[m] *= factor;
             }
         }
-        const float level = maximum == kNegative ? 0.0f : maximum;
+        Level level = near_level_of<R>(args, maximum);
+        if (P == 1u && far) {
+            level = level_of<R>(args, maximum);
+#pragma unroll
+            for (uint32_t b = 0; b < kSub; ++b) {
+#pragma unroll
+                for (uint32_t r = 0; r < kHeld; ++r) {
+                    score[b][r] -= level.minus;
+                }
+            }
+        }
 #pragma unroll
         for (uint32_t b = 0; b < kSub; ++b) {
 #pragma unroll
             for (uint32_t r = 0; r < kHeld; ++r) {
-                score[b][r] = weight_of<R>(score[b][r], level, args.log2_scale);
+                score[b][r] = weight_of<R>(args, P == 3u ? score[b][r] - level.minus : score[b][r], level);
                 if constexpr (P == 3u) {
                     denominator += score[b][r];
                 }
@@ -1786,7 +1866,7 @@ void k_paged_chunk(AttendArgs args) {
         return;  // the part holds nothing the row sees
     }
     float *const to = whole ? nullptr : partial_row<D>(args, part, token, head);
-    const float scale = none ? 0.0f : 1.0f / denominator;
+    const float scale = none ? 0.0f : whole ? 1.0f / denominator : settle_of<R>(args, maximum);
 #pragma unroll
     for (uint32_t m = 0; m < D / W; ++m) {
 #pragma unroll
@@ -1801,13 +1881,13 @@ void k_paged_chunk(AttendArgs args) {
                 }
                 store_output<R, 4>(args, token, head, at, out);
             } else {
-                *reinterpret_cast<f32x4 *>(to + at) = v;
+                *reinterpret_cast<f32x4 *>(to + at) = P == 3u ? v : v * scale;
             }
         }
     }
     if (!whole && side == 0u) {
         to[D] = maximum;
-        to[D + 1u] = denominator;
+        to[D + 1u] = P == 3u ? denominator : denominator * scale;
     }
 }
 
@@ -1944,7 +2024,7 @@ void launch_attention(adi_hip_context *ctx, AttendArgs args, const adi_hip_paged
            lds, args);
     if (args.parts > 1) {
         const uint64_t rows = uint64_t(c.tokens) * heads;
-        launch(ctx, "paged_join", k_paged_join<R, D, std::is_same_v<R, float>>,
+        launch(ctx, "paged_join", k_paged_join<R, D>,
                dim3(static_cast<uint32_t>(std::min<uint64_t>((rows + 3) / 4, 1u << 20))), dim3(kThreads), 0, args);
     }
 }
@@ -1988,10 +2068,11 @@ void paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache, con
     }
     const double scale = a->scale == 0.0f ? 1.0 / std::sqrt(double(cache->head_size)) : double(a->scale);
     const uint32_t window = std::min(a->window, 1u << 30);
+    const double log2_scale = scale * 1.4426950408889634;
+    const auto in_scores = [&](float powers) { return static_cast<float>(std::min(powers / log2_scale, 3e38)); };
     const AttendArgs args{paged_view(*cache, *batch), rows_view(a->queries), rows_view(a->outputs), rows_view(a->gate),
-                          static_cast<float>(scale * 1.4426950408889634),
-                          static_cast<float>(kSlack / (scale * 1.4426950408889634)), window, a->query_heads / cache->heads, 0, 0, 0, 0,
-                          nullptr, nullptr};
+                          static_cast<float>(log2_scale), in_scores(kSlack), in_scores(kFar), window,
+                          a->query_heads / cache->heads, 0, 0, 0, 0, nullptr, nullptr};
     if (type == ADI_HIP_F32 && cache->type == ADI_HIP_F32) {
         launch_attention<float, float>(ctx, args, workspace, cache->head_size);
     } else if (type == ADI_HIP_F32) {

@@ -1,0 +1,123 @@
+"""Paged attention where scores are far from 0: results have the same bounds
+there as for scores near it, as long as a score stays within a float.
+
+The scores of these cases are exact in a float, so a weight's error is that of
+its exponent. An exponent passes at most four roundings (from its score, to a
+new level, to its part's level, to the row's), each half a step of at most 64
+(what lies below weighs less than 2^-64): 4 * 64 * 2^-24 * ln 2 < 2^-16. The
+exponential and the joins' factors add at most 16 half steps of a float, and a
+16-bit weight half a step of its type, in the numerator and (k_paged_chunk) in the
+denominator."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from adi_amd import hip
+from test_gpu_paged import PAIRS, TYPES, U, Pool, half_step, normal, within
+
+pytestmark = pytest.mark.gpu
+
+STEP = [1, 1, 3]            # rows of k_paged_step (8 query heads on 2)
+CHUNK = [40, 1, 9]          # k_paged_chunk
+LENGTHS = [130, 1, 3000]    # one part and several
+
+
+@pytest.fixture(scope="module")
+def workspace(gpu):
+    w = hip.PagedWorkspace(gpu)
+    yield w
+    gpu.synchronize()
+    w.close()
+
+
+def weighted(pool, scores, counts, lengths, heads, values, kind, scale):
+    """(outputs, bound) [tokens, heads, size] in double of exact scores
+    scores(row, entries) -> [heads, entries]."""
+    out, bound = [], []
+    for s, (a, length) in enumerate(zip(pool.offsets, lengths)):
+        at = np.arange(length)
+        pages = torch.tensor(pool.table[s, at // pool.page], device="cuda")
+        v = values[pages, torch.tensor(at % pool.page, device="cuda")].double()
+        v = v.repeat_interleave(heads // v.shape[1], 1).permute(1, 0, 2)  # [heads, entries, size]
+        for i in range(counts[s]):
+            n = max(length - counts[s] + i + 1, 0)
+            w = torch.softmax(scores(a + i, s)[:, :n] * scale, -1)
+            o = torch.bmm(w[:, None], v[:, :n].contiguous())[:, 0] if n else torch.zeros_like(v[:, 0])
+            spread = torch.bmm(w[:, None], v[:, :n].abs().contiguous())[:, 0] if n else torch.zeros_like(o)
+            error = 2 * (2.0 ** -16 + 16 * U) + (0 if kind == "f32" else 2 * half_step(kind)) + 3 * (n + 16) * U
+            out.append(o)
+            bound.append(spread * error + half_step(kind) * (o.abs() + spread * error) + torch.finfo(TYPES[kind]).tiny)
+    return torch.stack(out), torch.stack(bound)
+
+
+FAR = {  # far, near dimensions of a query and a key's far one; the near ones' unit; scale
+    # scores near 2^26 with steps of 8, 2^23 scaled: weights within a few of each other
+    "f16": [(2048.0, 1.0, 32960.0, 16.0, 1 / 8), (32768.0, 2.0, 32768.0, 64.0, 2.0 ** -7),
+            # near 2^31 in steps of 256, scaled 2^28: all of the weight on the largest
+            (49152.0, 1.0, 49152.0, 256.0, 1 / 8)],
+    "bf16": [(2.0 ** 20, 1.0, 2.0 ** 20, 2.0 ** 17, 2.0 ** -17), (2.0 ** 40, 2.0 ** 40, 2.0 ** 40, 2.0 ** 17, 2.0 ** -57),
+             (2.0 ** 50, 2.0 ** 50, 2.0 ** 50, 2.0 ** 27, 1 / 8)],
+}
+FAR["f32"] = FAR["bf16"]
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("counts", [STEP, CHUNK])
+@pytest.mark.parametrize("size", [64, 128, 256])
+def test_exact_scores_far_from_zero(gpu, workspace, rows, kind, which, counts, size):
+    """Scores a b + c u: a b (or its negative, or 0, by row) beside which a float
+    has few bits left, u from 0 to 7."""
+    far, near, key, unit, scale = FAR[rows][which]
+    heads, kv = 8, 2
+    pool = Pool(5 + which, LENGTHS, 16, kv, size, kind)
+    batch = pool.batch(gpu, counts)
+    n = pool.tokens
+    rng = np.random.default_rng(which)
+    small = [torch.tensor(rng.integers(0, 8, length), device="cuda").double() for length in LENGTHS]
+    for s, length in enumerate(LENGTHS):
+        for p in range(-(-length // 16)):
+            page, held = int(pool.table[s, p]), min(16, length - 16 * p)
+            pool.keys[page, :held] = 0
+            pool.keys[page, :held, :, 3] = key
+            pool.keys[page, :held, :, size - 5] = (small[s][16 * p:16 * p + held] * unit)[:, None].to(pool.keys.dtype)
+    sign = torch.tensor(rng.choice([1.0, 1.0, -1.0, 0.0], (n, heads)), device="cuda")
+    q = torch.zeros(n, heads, size, dtype=TYPES[rows], device="cuda")
+    q[..., 3] = (sign * far).to(q.dtype)
+    q[..., size - 5] = near
+    assert torch.equal(q[..., 3].double(), sign * far) and float(pool.keys[int(pool.table[0, 0]), 0, 0, 3]) == key
+
+    def scores(row, s):
+        score = sign[row][:, None] * (far * key) + near * unit * small[s][None, :]
+        assert torch.equal(score.float().double(), score)
+        return score
+
+    out = torch.empty_like(q)
+    hip.paged_attention(gpu, pool.cache(gpu), batch, q, out, workspace, scale=scale)
+    want, bound = weighted(pool, scores, counts, LENGTHS, heads, pool.values, rows, scale)
+    within(out, want, bound)
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("magnitude", [300.0, 5000.0, 20000.0])
+@pytest.mark.parametrize("counts", [STEP, CHUNK])
+@pytest.mark.parametrize("heads", [8, 64])
+def test_equal_keys_of_any_magnitude_weigh_the_same(gpu, workspace, rows, kind, magnitude, counts, heads):
+    """Every key of a head the same random row, so that its scores, however
+    rounded, are one number: outputs are the values' means, one entry's its value."""
+    size, kv = 64, 2
+    pool = Pool(9, LENGTHS, 16, kv, size, kind)
+    # (f16's largest is 65504)
+    key = normal(4, kv, size, scale=magnitude).clamp(-60000, 60000).to(TYPES[kind])
+    for s, length in enumerate(LENGTHS):
+        for p in range(-(-length // 16)):
+            pool.keys[int(pool.table[s, p]), :min(16, length - 16 * p)] = key
+    batch = pool.batch(gpu, counts)
+    q = normal(5, pool.tokens, heads, size, scale=magnitude).clamp(-60000, 60000).to(TYPES[rows])
+    out = torch.empty_like(q)
+    hip.paged_attention(gpu, pool.cache(gpu), batch, q, out, workspace)
+    even = [torch.zeros(heads, length, dtype=torch.float64, device="cuda") for length in LENGTHS]
+    want, bound = weighted(pool, lambda row, s: even[s], counts, LENGTHS, heads, pool.values, rows, 1.0)
+    within(out, want, bound)
