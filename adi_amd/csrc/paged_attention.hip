@@ -193,10 +193,12 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[N]) {
 }
 
 // The power of two that brings values of a largest magnitude of these float bits
-// to 2^14 .. 2^15, as an exponent (2^126 at most), and what takes it back.
+// to 2^14 .. 2^15, as an exponent (2^126 at most), and the power that takes it
+// back. A score's two powers are added before they are applied: by itself either
+// may pass a float's range where the score does not.
 __device__ __forceinline__ uint32_t scale_exponent(uint32_t largest) { return min(268u - (largest >> 23), 253u); }
 __device__ __forceinline__ float scale_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
-__device__ __forceinline__ float unscale_of(uint32_t exponent) { return __uint_as_float((254u - exponent) << 23); }
+__device__ __forceinline__ int32_t unscale_of(uint32_t exponent) { return 127 - static_cast<int32_t>(exponent); }
 __device__ __forceinline__ uint32_t magnitude(uint32_t largest, float v) {
     return max(largest, __float_as_uint(v) & 0x7FFFFFFFu);
 }
@@ -1207,8 +1209,8 @@ void k_paged_chunk(AttendArgs args) {
     // pointer waited for every load in flight)
     uint32_t *const marks = reinterpret_cast<uint32_t *>(lds + kBuffers * kBuffer);
     uint32_t *const bad_key = marks + 4u;                             // [2][kKeys]
-    // what takes the scores of a key back from its scale
-    float *const key_unscale = reinterpret_cast<float *>(lds + kBuffers * kBuffer) + 4u + 2u * kKeys;  // [2][kKeys]
+    // the power of two that takes the scores of a key back from its scale
+    int32_t *const key_unscale = reinterpret_cast<int32_t *>(lds + kBuffers * kBuffer) + 4u + 2u * kKeys;  // [2][kKeys]
     uint32_t *const page_ids = reinterpret_cast<uint32_t *>(key_unscale + 2u * kKeys);
     const PagedView &cache = args.c;
     // the blocks of one (KV head, part) of a sequence read the same entries: where
@@ -1489,7 +1491,8 @@ void k_paged_chunk(AttendArgs args) {
 
     // the row's query: step j holds dimensions kStepDims j + 8 side + 0 .. 7
     u32x4 query_pieces[D / kStepDims][QP];
-    float query_scale = 1.0f, query_unscale = 1.0f;
+    float query_scale = 1.0f;
+    int32_t query_unscale = 0;
     if constexpr (kFloat) {
         uint32_t largest = 0;
 #pragma unroll
@@ -1597,7 +1600,7 @@ void k_paged_chunk(AttendArgs args) {
                 score[sub][at + r] = acc[h][r];
                 if constexpr (kFloat) {
                     score[sub][at + r] =
-                        acc[h][r] * query_unscale * key_unscale[buffer * kKeys + 32u * sub + key_of(at + r)];
+                        ldexpf(acc[h][r], query_unscale + key_unscale[buffer * kKeys + 32u * sub + key_of(at + r)]);
                 }
             }
         }

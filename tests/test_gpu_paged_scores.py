@@ -15,7 +15,7 @@ import pytest
 import torch
 
 from adi_amd import hip
-from test_gpu_paged import PAIRS, TYPES, U, Pool, half_step, normal, within
+from test_gpu_paged import PAIRS, TYPES, U, Pool, check_attention, half_step, normal, within
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +121,38 @@ def test_equal_keys_of_any_magnitude_weigh_the_same(gpu, workspace, rows, kind, 
     even = [torch.zeros(heads, length, dtype=torch.float64, device="cuda") for length in LENGTHS]
     want, bound = weighted(pool, lambda row, s: even[s], counts, LENGTHS, heads, pool.values, rows, 1.0)
     within(out, want, bound)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("up,down", [(115, -115), (-100, 100), (-115, 115), (105, -112), (-125, 10)])
+@pytest.mark.parametrize("counts,lengths", [([1], [100]), ([33], [100]), ([33, 2], [90, 2000])])
+def test_queries_and_keys_at_both_ends_of_a_float(gpu, workspace, kind, up, down, counts, lengths):
+    """f32 queries of 2^up and keys of 2^down: ordinary scores, or nothing."""
+    def bend(pool, q):
+        pool.keys.mul_(2.0 ** down)
+        q.mul_(2.0 ** up)
+
+    for size in (64, 128, 256):
+        check_attention(gpu, workspace, "f32", kind, size, 4, 2, 32, counts, lengths, bend=bend)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("counts", [[1], [33]])
+def test_large_queries_across_large_keys(gpu, workspace, kind, counts):
+    """Queries and keys whose largest elements' product is past a float while their
+    scores are 0, and keys whose elements are 2^220 apart."""
+    def across(pool, q):
+        pool.keys[..., 32:].mul_(2.0 ** 110)
+        pool.keys[..., :32] = 0
+        q[..., :32].mul_(2.0 ** 110)
+        q[..., 32:] = 0
+
+    def apart(pool, q):
+        pool.keys[..., :32].mul_(2.0 ** -110)
+        pool.keys[..., 32:].mul_(2.0 ** 110)
+        q[..., :32] = 0
+        q[..., 32:].mul_(2.0 ** -100)
+        q.mul_(2.0 ** -10)
+
+    for b in (across, apart):
+        check_attention(gpu, workspace, "f32", kind, 64, 4, 2, 32, counts, [100], bend=b)
