@@ -6,8 +6,12 @@
 namespace adi_hip {
 namespace {
 
+// The last failed adi_hip_context_create of any thread, and the last failed call
+// without a context of this one, whose text stays where it is while other threads
+// fail theirs.
 std::mutex g_create_error_mutex;
 std::string g_create_error;
+thread_local std::string t_error;
 
 // f32 -> f16 bits, round to nearest even with subnormals, the rounding of the
 // reference's f32_to_f16 (src/kernels.cpp:336-379).
@@ -74,10 +78,7 @@ adi_hip_codebook *upload(adi_hip_context *ctx, adi_hip_codebook::Kind kind,
 
 }  // namespace
 
-void record_error(std::string message) {
-    std::lock_guard<std::mutex> lock(g_create_error_mutex);
-    g_create_error = std::move(message);
-}
+void record_error(std::string message) { t_error = std::move(message); }
 
 KernelStat &stat_for(adi_hip_context *ctx, const char *name) {
     for (auto &stat : ctx->stats) {
@@ -96,7 +97,13 @@ using namespace adi_hip;
 extern "C" {
 
 int adi_hip_context_create(int device, adi_hip_context **out) {
-    const auto record = [](std::string message) { record_error(std::move(message)); };
+    const auto record = [](std::string message) {
+        {
+            std::lock_guard<std::mutex> lock(g_create_error_mutex);
+            g_create_error = message;
+        }
+        record_error(std::move(message));
+    };
     if (out == nullptr) {
         record("adi_hip_context_create: null output pointer");
         return ADI_HIP_INVALID_ARGUMENT;
@@ -201,8 +208,11 @@ void adi_hip_context_destroy(adi_hip_context *ctx) {
 
 const char *adi_hip_last_error(const adi_hip_context *ctx) {
     if (ctx == nullptr) {
-        std::lock_guard<std::mutex> lock(g_create_error_mutex);
-        return g_create_error.c_str();
+        if (t_error.empty()) {
+            std::lock_guard<std::mutex> lock(g_create_error_mutex);
+            t_error = g_create_error;
+        }
+        return t_error.c_str();
     }
     return const_cast<adi_hip_context *>(ctx)->last_error_cstr();
 }

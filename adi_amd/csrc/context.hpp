@@ -210,7 +210,7 @@ int guarded(adi_hip_context *ctx, F &&function) {
     }
 }
 
-// Leaves a message for adi_hip_last_error(NULL).
+// Leaves a message for this thread's adi_hip_last_error(NULL).
 void record_error(std::string message);
 
 // guarded() for calls that take no context and touch no device.

@@ -49,9 +49,10 @@ int adi_hip_context_create(int device, adi_hip_context **out);
 void adi_hip_context_destroy(adi_hip_context *ctx);
 
 /* Message of the last failed call on this context ("" if none). A NULL
- * context gives the message of the last failed adi_hip_context_create, or
- * of the last failed call that takes no context (adi_hip_rope_frequencies,
- * adi_hip_paged_check) where that came later. */
+ * context gives the message of this thread's last failed call without one
+ * (adi_hip_context_create, adi_hip_rope_frequencies, adi_hip_paged_check),
+ * and to a thread that had none the last failed adi_hip_context_create's of
+ * any; the text stays until this thread's next such call fails. */
 const char *adi_hip_last_error(const adi_hip_context *ctx);
 
 /* Stream the context launches on (a hipStream_t; NULL = the null stream). */

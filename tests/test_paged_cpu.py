@@ -1,6 +1,7 @@
 """The rotary and paged-cache entry points without a GPU: their structures
 against the header, the frequencies of every scaling against their formulas in
 double, the refusals of both, and adi_hip_paged_check over host arrays."""
+import concurrent.futures
 import ctypes as C
 import math
 import os
@@ -216,3 +217,39 @@ def test_null_context_and_descriptors():
     assert lib.adi_hip_rope_rows(None, None, None, 0, 0, 0, None, None) == hip.INVALID_ARGUMENT
     lib.adi_hip_rope_destroy(None)
     lib.adi_hip_paged_workspace_destroy(None)
+
+
+def test_threads_keep_their_own_messages():
+    """Two threads whose checks fail differently, one of them many times while
+    the other holds its message's address."""
+    raw = C.CDLL(hip.load()._name)
+    raw.adi_hip_last_error.restype = C.c_void_p
+    raw.adi_hip_last_error.argtypes = [C.c_void_p]
+    address = []
+
+    def fail(change, message):
+        with pytest.raises(hip.HipError, match=message):
+            hip.paged_check(cache(**change), **batch())
+
+    def other():
+        for heads in (0, 70000):
+            for _ in range(200):
+                fail(dict(heads=heads), "heads must be")
+                assert C.string_at(raw.adi_hip_last_error(None)).endswith(b"heads must be 1 to 65536")
+
+    fail(dict(page_size=24), "page size")
+    address.append(raw.adi_hip_last_error(None))
+    held = C.string_at(address[0])
+    assert b"page size" in held
+    with concurrent.futures.ThreadPoolExecutor(3) as pool:
+        for done in [pool.submit(other) for _ in range(3)]:
+            done.result()
+    assert C.string_at(address[0]) == held and raw.adi_hip_last_error(None) == address[0]
+
+
+def test_a_thread_without_a_message_reads_the_last_failed_creation():
+    lib = hip.load()
+    with concurrent.futures.ThreadPoolExecutor(1) as pool:
+        assert pool.submit(lib.adi_hip_context_create, 4096, None).result() == hip.INVALID_ARGUMENT
+    with concurrent.futures.ThreadPoolExecutor(1) as pool:
+        assert pool.submit(lib.adi_hip_last_error, None).result() == b"adi_hip_context_create: null output pointer"
