@@ -312,14 +312,15 @@ __device__ __forceinline__ float odd_weight(const AttendArgs &a, const uint32_t 
     return weight_of<R>(a, score - level.minus, level);
 }
 
-// N consecutive outputs of a row, gated.
+// N consecutive outputs of a row, gated unless the row sees nothing (whose gate
+// may be whatever a padded row holds).
 template <typename R, uint32_t N>
 __device__ __forceinline__ void store_output(const AttendArgs &a, uint32_t token, uint32_t head, uint32_t at,
-                                             float (&v)[N]) {
+                                             float (&v)[N], bool none = false) {
     struct alignas(sizeof(R) * N) Vector {
         R v[N];
     };
-    if (a.gate.data != nullptr) {
+    if (a.gate.data != nullptr && !none) {
         const Vector g = *reinterpret_cast<const Vector *>(reinterpret_cast<const R *>(a.gate.data) +
                                                            token * a.gate.token_stride + head * a.gate.head_stride +
                                                            at);
@@ -342,7 +343,7 @@ __device__ __forceinline__ void fill_rows(const AttendArgs &a, const SequenceRow
         const uint32_t row = static_cast<uint32_t>(i / (D / 4u)), at = static_cast<uint32_t>(i % (D / 4u)) * 4u;
         const float v = s.over ? __builtin_nanf("") : 0.0f;
         float out[4] = {v, v, v, v};
-        store_output<R, 4>(a, s.first + row / a.group, kv * a.group + row % a.group, at, out);
+        store_output<R, 4>(a, s.first + row / a.group, kv * a.group + row % a.group, at, out, true);
     }
 }
 
@@ -906,7 +907,7 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         for (uint32_t k = 0; k < 4u; ++k) {
             out[k] = none ? 0.0f : sum[k] / total;
         }
-        store_output<R, 4>(args, s.first + r / args.group, kv * args.group + r % args.group, at, out);
+        store_output<R, 4>(args, s.first + r / args.group, kv * args.group + r % args.group, at, out, none);
     };
     float *const joint = args.partial + static_cast<uint64_t>(region_base) * kRegion;
     const uint32_t part_step = region_step * kRegion;
@@ -1882,7 +1883,7 @@ void k_paged_chunk(AttendArgs args) {
                 for (uint32_t k = 0; k < 4u; ++k) {
                     out[k] = none ? 0.0f : v[k] * scale;
                 }
-                store_output<R, 4>(args, token, head, at, out);
+                store_output<R, 4>(args, token, head, at, out, none);
             } else {
                 *reinterpret_cast<f32x4 *>(to + at) = P == 3u ? v : v * scale;
             }

@@ -156,3 +156,25 @@ def test_large_queries_across_large_keys(gpu, workspace, kind, counts):
 
     for b in (across, apart):
         check_attention(gpu, workspace, "f32", kind, 64, 4, 2, 32, counts, [100], bend=b)
+
+
+@pytest.mark.parametrize("rows,kind", PAIRS)
+@pytest.mark.parametrize("heads", [4, 64])
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
+def test_rows_that_see_nothing_are_zero_whatever_they_hold(gpu, workspace, rows, kind, heads, junk):
+    """Front padding and empty sequences whose queries and gates were never
+    written: 0, and the other rows as with ordinary padding."""
+    counts, lengths = [3, 4, 2, 40], [1, 0, 50, 37]
+    pool = Pool(3, lengths, 16, 2, 64, kind)
+    batch = pool.batch(gpu, counts)
+    q, gate = (normal(i, pool.tokens, heads, 64, kind=rows) for i in (1, 2))
+    blank = torch.zeros(pool.tokens, dtype=torch.bool, device="cuda")
+    for a, n, length in zip(pool.offsets, counts, lengths):
+        blank[a:a + max(n - length, 0)] = True
+    assert int(blank.sum()) == 2 + 4 + 3
+    out = torch.empty_like(q), torch.empty_like(q)
+    hip.paged_attention(gpu, pool.cache(gpu), batch, q, out[0], workspace, gate=gate)
+    q[blank], gate[blank] = junk, junk
+    hip.paged_attention(gpu, pool.cache(gpu), batch, q, out[1], workspace, gate=gate)
+    assert bool((out[1][blank] == 0).all()) and torch.equal(*out)
+    assert bool((out[1][~blank] != 0).any(-1).all())
