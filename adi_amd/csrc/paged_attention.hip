@@ -483,7 +483,9 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
         for (uint32_t attempt = 0; attempt < 2u; ++attempt) {
             // (more slots than sequences; the sums' roundings are below 2^-17)
             const float left = static_cast<float>(args.slots) - live_sequences * (attempt == 0u ? 0.5f : 1.0f);
-            const float wanted = total * 1.0001f / left;
+            // (2^28 entries hold any history whole, and are an integer that has room
+            // to be rounded up)
+            const float wanted = fminf(total * 1.0001f / left, 268435456.0f);
             span = max(args.span, (static_cast<uint32_t>(wanted) + kTurn) & ~(static_cast<uint32_t>(kTurn) - 1u));
             parts = (extent + span - 1u) / span;
             sum = parts;

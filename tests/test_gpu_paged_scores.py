@@ -178,3 +178,27 @@ def test_rows_that_see_nothing_are_zero_whatever_they_hold(gpu, workspace, rows,
     hip.paged_attention(gpu, pool.cache(gpu), batch, q, out[1], workspace, gate=gate)
     assert bool((out[1][blank] == 0).all()) and torch.equal(*out)
     assert bool((out[1][~blank] != 0).any(-1).all())
+
+
+def test_a_step_of_more_than_2_to_32_entries(gpu, workspace):
+    """Twenty histories of 2^28 - 1 entries among 43 of one, all of one page, on 8
+    heads: one block more than sequences, so a part is a whole history. Value
+    (e, head, d) is head + 1 where e % 64 = d, so every sum is exact."""
+    n, page, heads, size, longest = 63, 4096, 8, 64, (1 << 28) - 1
+    lengths = [longest if s % 3 == 1 and s < 60 else 1 for s in range(n)]
+    keys = torch.zeros(1, page, heads, size, dtype=torch.bfloat16, device="cuda")
+    values = torch.eye(size, dtype=torch.bfloat16, device="cuda").repeat(page // size, 1)[None, :, None, :]
+    values = values * torch.arange(1, heads + 1, device="cuda").to(torch.bfloat16)[:, None]
+    table = torch.zeros(n, 1 << 16, dtype=torch.int32, device="cuda")
+    batch = hip.PagedBatch(gpu, torch.arange(n + 1, dtype=torch.int32, device="cuda"),
+                           torch.tensor(lengths, dtype=torch.int32, device="cuda"), table, n, 1, longest)
+    q = normal(1, n, heads, size, kind="bf16")
+    out = torch.full_like(q, 7.0)
+    hip.paged_attention(gpu, hip.PagedCache(gpu, keys, values), batch, q, out, workspace)
+    scale = torch.arange(1, heads + 1, device="cuda").double()[:, None]
+    at = torch.arange(size, device="cuda")
+    for s, length in enumerate(lengths):
+        want = scale * ((length - at + size - 1) // size).double() / length
+        within(out[s], want, want * (half_step("bf16") + 16 * U), s)
+    # the workspace as it was: a call after it gives what it gives alone
+    check_attention(gpu, workspace, "bf16", "bf16", 64, 8, 8, 16, [1] * 8, [4000] * 8)
