@@ -1565,6 +1565,8 @@ void full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attention *L,
                 ne_shaped(L->output, hidden, kQueryHeads * kHeadSize) && L->query_norm != nullptr &&
                 L->key_norm != nullptr,
             "full attention state or input shape mismatch");
+    // (before the first launch: a refused call appends nothing)
+    require_attention(ctx, cache, batch, kQueryHeads, workspace);
     if (count == 0 || batch->sequences == 0) {
         return;
     }

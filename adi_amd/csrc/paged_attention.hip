@@ -2049,18 +2049,24 @@ void launch_attention(adi_hip_context *ctx, const AttendArgs &args, const adi_hi
 
 }  // namespace
 
-void paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache, const adi_hip_paged_batch *batch,
-                     const adi_hip_paged_attention_arguments *a, adi_hip_paged_workspace *workspace) {
+void require_attention(const adi_hip_context *ctx, const adi_hip_paged_cache *cache, const adi_hip_paged_batch *batch,
+                       uint32_t query_heads, const adi_hip_paged_workspace *workspace) {
     require_paged(cache, batch);
-    require(a != nullptr && workspace != nullptr, "paged attention: null argument");
+    require(workspace != nullptr, "paged attention: null argument");
     require(workspace->device == ctx->device, "paged attention: the workspace is on another device");
-    const uint32_t type = a->queries.type;
-    require(known_type(type) && (type == cache->type || (type == ADI_HIP_F32 && cache->type == ADI_HIP_BF16)),
-            "paged attention: f32 rows read an f32 or bf16 cache, others their own type");
-    require(a->query_heads >= 1 && a->query_heads % cache->heads == 0 && a->query_heads / cache->heads <= 256,
+    require(query_heads >= 1 && query_heads % cache->heads == 0 && query_heads / cache->heads <= 256,
             "paged attention: query heads must be 1 to 256 times the cache's");
     require(cache->heads < (1u << 16) && batch->sequences < (1u << 16),
             "paged attention: more than 65535 heads or sequences");
+}
+
+void paged_attention(adi_hip_context *ctx, const adi_hip_paged_cache *cache, const adi_hip_paged_batch *batch,
+                     const adi_hip_paged_attention_arguments *a, adi_hip_paged_workspace *workspace) {
+    require(a != nullptr, "paged attention: null argument");
+    require_attention(ctx, cache, batch, a->query_heads, workspace);
+    const uint32_t type = a->queries.type;
+    require(known_type(type) && (type == cache->type || (type == ADI_HIP_F32 && cache->type == ADI_HIP_BF16)),
+            "paged attention: f32 rows read an f32 or bf16 cache, others their own type");
     require(a->scale >= 0.0f && a->scale <= 1e38f, "paged attention: scale must be positive and at most 1e38, or 0");
     if (batch->tokens == 0 || batch->sequences == 0) {
         return;

@@ -1,5 +1,7 @@
-"""Paged attention where scores are far from 0: results have the same bounds
-there as for scores near it, as long as a score stays within a float.
+"""Paged attention at the edges of what its documentation allows.
+
+Where scores are far from 0, results have the same bounds as for scores near it,
+as long as a score stays within a float.
 
 The scores of these cases are exact in a float, so a weight's error is that of
 its exponent. An exponent passes at most four roundings (from its score, to a
@@ -202,3 +204,23 @@ def test_a_step_of_more_than_2_to_32_entries(gpu, workspace):
         within(out[s], want, want * (half_step("bf16") + 16 * U), s)
     # the workspace as it was: a call after it gives what it gives alone
     check_attention(gpu, workspace, "bf16", "bf16", 64, 8, 8, 16, [1] * 8, [4000] * 8)
+
+
+def test_a_refused_layer_call_appends_nothing(gpu, workspace):
+    """More sequences than the attention takes (the append takes them)."""
+    from adi_amd import synthetic as syn
+    rng = syn.rng_for(40, 256)
+    tlut = syn.ne_tlut(rng)
+    layer = hip.upload_full_attention(gpu, syn.full_attention(rng, 256, tlut), gpu.ne_codebook(tlut))
+    keys = normal(1, 2, 16, 2, 256)
+    before, x = keys.clone(), normal(2, 1, 256)
+    n = 1 << 16
+    offsets, lengths = (torch.ones(k, dtype=torch.int32, device="cuda") for k in (n + 1, n))
+    offsets[0] = 0
+    batch = hip.PagedBatch(gpu, offsets, lengths, torch.zeros(n, 1, dtype=torch.int32, device="cuda"), 1, 1, 16)
+    cache = hip.PagedCache(gpu, keys, keys.clone())
+    with pytest.raises(hip.HipError, match="65535") as info:
+        hip.full_attention_paged(gpu, layer, cache, batch, x, torch.empty_like(x), workspace)
+    assert info.value.status == hip.INVALID_ARGUMENT
+    gpu.synchronize()
+    assert torch.equal(keys, before)
