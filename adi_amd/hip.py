@@ -1144,6 +1144,12 @@ def _refuse(message: str):
     raise HipError(INVALID_ARGUMENT, message)
 
 
+def _words(message: str, *values) -> None:
+    """Refuses what ctypes would cut to 32 bits."""
+    if not all(0 <= x < 1 << 32 for x in values):
+        _refuse(message)
+
+
 _type_codes: dict = {}
 
 
@@ -1215,6 +1221,7 @@ def _dtype_name(t) -> str:
 def _rope_options(rotary, layout, theta, scaling, factor, original, fast, slow, magnitude) -> RopeOptions:
     if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
         _refuse(f"rope: unknown layout {layout!r} or scaling {scaling!r}")
+    _words("rope: rotary must be even, 2 to 1024", rotary)
     return RopeOptions(rotary, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], theta, factor, original, fast, slow,
                        magnitude)
 
@@ -1297,8 +1304,7 @@ class PagedBatch:
     rows, at most max_tokens new ones and max_length entries a sequence."""
 
     def __init__(self, ctx: Context, offsets, lengths, table, tokens: int, max_tokens: int, max_length: int):
-        if not all(0 <= x < 1 << 32 for x in (tokens, max_tokens, max_length)):
-            _refuse("paged batch: tokens, max_tokens or max_length is out of range")
+        _words("paged batch: tokens, max_tokens or max_length is out of range", tokens, max_tokens, max_length)
         n = int(lengths.shape[0])
         _device_words(ctx, lengths, "lengths", n)
         _device_words(ctx, offsets, "offsets", n + 1)
@@ -1312,8 +1318,14 @@ class PagedBatch:
 def paged_check(cache: PagedCacheStruct, offsets, lengths, table, tokens: int, max_tokens: int,
                 max_length: int) -> None:
     """adi_hip_paged_check of a batch's host arrays (numpy) against a cache's
-    descriptor; needs no GPU."""
-    held = [np.ascontiguousarray(a).astype(np.uint32, casting="unsafe") for a in (offsets, lengths, table)]
+    descriptor; needs no GPU. Integers of any type; a negative one is the
+    unsigned one of its bits, as the device arrays' are."""
+    _words("paged batch: tokens, max_tokens or max_length is out of range", tokens, max_tokens, max_length)
+    held = [np.ascontiguousarray(a) for a in (offsets, lengths, table)]
+    for a in held:
+        if a.size and (a.dtype.kind not in "iu" or a.min() < -(1 << 31) or a.max() >= 1 << 32):
+            _refuse("paged batch: offsets, lengths and table must be 32-bit integers")
+    held = [a.astype(np.uint32, casting="unsafe") for a in held]
     n = held[1].size
     if held[0].shape != (n + 1,) or held[2].ndim != 2 or held[2].shape[0] != n:
         _refuse("paged batch: offsets, lengths and table do not fit each other")
@@ -1360,10 +1372,13 @@ def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, keys, value
         heads = queries.shape[1]
         q = _rows(ctx, queries, n, heads, size)
         o = q if queries_out is None else _rows(ctx, queries_out, n, heads, size)
-    a = _pack_append((rope.handle.value or 0) if rope is not None and rope.handle else 0,
-                     *_rows(ctx, keys, n, cache.heads, size), *_rows(ctx, values, n, cache.heads, size),
-                     _bf16_weight(ctx, key_norm, size), heads, *q, *o, _bf16_weight(ctx, query_norm, size),
-                     weight_offset, epsilon)
+    k, v = _rows(ctx, keys, n, cache.heads, size), _rows(ctx, values, n, cache.heads, size)
+    try:
+        a = _pack_append((rope.handle.value or 0) if rope is not None and rope.handle else 0, *k, *v,
+                         _bf16_weight(ctx, key_norm, size), heads, *q, *o, _bf16_weight(ctx, query_norm, size),
+                         weight_offset, epsilon)
+    except OverflowError:
+        _refuse("paged append: weight offset or epsilon is past a float")
     if rope is not None and not rope.handle:
         _refuse("the rope is closed")
     status = ctx.lib.adi_hip_paged_append(ctx.handle, cache.struct, batch.struct, a)
@@ -1379,8 +1394,12 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, queries,
     n, size, heads = batch.tokens, cache.head_size, queries.shape[1]
     if not 0 <= window < 1 << 32:
         _refuse("paged attention: window is out of range")
-    a = _pack_attention(heads, *_rows(ctx, queries, n, heads, size), *_rows(ctx, out, n, heads, size),
-                        *(_no_rows if gate is None else _rows(ctx, gate, n, heads, size)), scale, window)
+    rows = (*_rows(ctx, queries, n, heads, size), *_rows(ctx, out, n, heads, size),
+            *(_no_rows if gate is None else _rows(ctx, gate, n, heads, size)))
+    try:
+        a = _pack_attention(heads, *rows, scale, window)
+    except OverflowError:
+        _refuse("paged attention: scale is past a float")
     status = ctx.lib.adi_hip_paged_attention(ctx.handle, cache.struct, batch.struct, a, workspace.handle)
     if status:
         ctx.check(status)

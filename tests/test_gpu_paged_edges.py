@@ -224,3 +224,15 @@ def test_a_refused_layer_call_appends_nothing(gpu, workspace):
     assert info.value.status == hip.INVALID_ARGUMENT
     gpu.synchronize()
     assert torch.equal(keys, before)
+
+
+def test_numbers_past_a_float_are_refused(gpu, workspace):
+    pool = Pool(1, [20], 16, 2, 64, "bf16", junk=None)
+    q, k = normal(1, 1, 4, 64, kind="bf16"), normal(2, 1, 2, 64, kind="bf16")
+    cache, batch = pool.cache(gpu), pool.batch(gpu, [1])
+    for call in (lambda: hip.paged_attention(gpu, cache, batch, q, torch.empty_like(q), workspace, scale=1e39),
+                 lambda: hip.paged_append(gpu, cache, batch, k, k, epsilon=1e39),
+                 lambda: hip.paged_append(gpu, cache, batch, k, k, weight_offset=-1e39)):
+        with pytest.raises(hip.HipError, match="past a float") as info:
+            call()
+        assert info.value.status == hip.INVALID_ARGUMENT

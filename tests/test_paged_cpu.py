@@ -253,3 +253,25 @@ def test_a_thread_without_a_message_reads_the_last_failed_creation():
         assert pool.submit(lib.adi_hip_context_create, 4096, None).result() == hip.INVALID_ARGUMENT
     with concurrent.futures.ThreadPoolExecutor(1) as pool:
         assert pool.submit(lib.adi_hip_last_error, None).result() == b"adi_hip_context_create: null output pointer"
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(tokens=(1 << 32) + 6), "out of range"),
+    (dict(max_tokens=(1 << 32) + 3), "out of range"),
+    (dict(max_length=(1 << 32) + 48), "out of range"),
+    (dict(offsets=np.array([0, 3, 3, (1 << 32) + 4])), "32-bit"),
+    (dict(lengths=np.array([40, 1 << 40, 16])), "32-bit"),
+    (dict(table=np.array([[7, 1 << 32, 9], [-1, -1, -1], [3, -1, -1]])), "32-bit"),
+    (dict(lengths=np.array([40.5, 0, 16])), "32-bit"),
+])
+def test_check_refuses_what_32_bits_cannot_hold(change, message):
+    """Each of these, cut to 32 bits, is the accepted batch."""
+    with pytest.raises(hip.HipError, match=message) as info:
+        hip.paged_check(cache(), **batch(**change))
+    assert info.value.status == hip.INVALID_ARGUMENT
+
+
+def test_rotary_dimensions_past_32_bits():
+    with pytest.raises(hip.HipError, match="rotary") as info:
+        hip.rope_frequencies((1 << 32) + 64)
+    assert info.value.status == hip.INVALID_ARGUMENT
