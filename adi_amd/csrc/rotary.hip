@@ -24,7 +24,9 @@ Frequencies frequencies_of(const adi_hip_rope_options *o) {
     require(o->layout <= ADI_HIP_ROPE_PAIRS, "rope: unknown layout");
     require(o->scaling <= ADI_HIP_ROPE_BANDS, "rope: unknown scaling");
     require(std::isfinite(o->theta) && o->theta > 1.0, "rope: theta must be above 1");
-    require(std::isfinite(o->magnitude) && o->magnitude >= 0.0, "rope: magnitude must not be negative");
+    // (the kernels' is a float)
+    require(o->magnitude == 0.0 || (o->magnitude >= 0x1p-100 && o->magnitude <= 0x1p100),
+            "rope: magnitude must be 2^-100 to 2^100, or 0");
     const bool stretched = o->scaling != ADI_HIP_ROPE_PLAIN;
     require(!stretched || (std::isfinite(o->factor) && o->factor >= 1.0), "rope: factor must be at least 1");
     const bool bounded = o->scaling == ADI_HIP_ROPE_YARN || o->scaling == ADI_HIP_ROPE_BANDS;

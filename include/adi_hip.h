@@ -693,8 +693,8 @@ int adi_hip_batcher_force_failure(adi_hip_batcher *batcher, int where);
  *   YaRN     between the pairs that turn `fast` and `slow` times over the
  *            original context, i_t = rotary ln(original / (2 pi t)) /
  *            (2 ln theta) rounded outwards and kept within 0 .. rotary - 1, a
- *            linear ramp from f_i to f_i / factor; rows are multiplied by
- *            0.1 ln(factor) + 1
+ *            linear ramp from f_i to f_i / factor; turned dimensions are
+ *            multiplied by 0.1 ln(factor) + 1
  *   bands    by the turns t_i = original f_i / (2 pi): f_i where
  *            t_i >= fast, f_i / factor where t_i <= slow, between them
  *            linear in t_i. */
@@ -712,7 +712,7 @@ typedef struct {
     double factor;     /* at least 1 (not read for plain) */
     double original;   /* YaRN, bands: at least 1 */
     double fast, slow; /* YaRN, bands: turns, fast > slow > 0; both 0: 32 and 1, 4 and 1 */
-    double magnitude;  /* what turned dimensions are multiplied by; 0: the scaling's own */
+    double magnitude;  /* what turned dimensions are multiplied by, 2^-100 to 2^100; 0: the scaling's own */
 } adi_hip_rope_options;
 
 /* On the host, no GPU needed: the rotary / 2 frequencies (radians a position)

@@ -275,3 +275,10 @@ def test_rotary_dimensions_past_32_bits():
     with pytest.raises(hip.HipError, match="rotary") as info:
         hip.rope_frequencies((1 << 32) + 64)
     assert info.value.status == hip.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("magnitude", [1e39, 1e300, 1e-46, float("inf"), float("nan"), -0.5])
+def test_magnitudes_that_a_float_cannot_hold(magnitude):
+    with pytest.raises(hip.HipError, match="magnitude") as info:
+        hip.rope_frequencies(64, magnitude=magnitude)
+    assert info.value.status == hip.INVALID_ARGUMENT
