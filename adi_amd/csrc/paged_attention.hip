@@ -684,19 +684,21 @@ __global__ __launch_bounds__(kThreads, (step_blocks<T, R, D>())) void k_paged_st
     for (; first < end; first += kTurn) {
         float score[kHeld];
         if constexpr (kFloat) {
-            f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            // (four sums of 64 dimensions at most: with two the scores' roundings were twice
+            // those of a plain 32-bit product)
+            f32x4 acc[4] = {};
 #pragma unroll
             for (uint32_t j = 0; j < D / 16u; ++j) {
                 const f32x4 q = *reinterpret_cast<const f32x4 *>(lds.query + query_place(4u * j + g));
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i) {
-                    acc[j & 1u] =
-                        __builtin_amdgcn_mfma_f32_16x16x4f32(key_float[j][i], q[i], acc[j & 1u], 0, 0, 0);
+                    acc[j & 3u] =
+                        __builtin_amdgcn_mfma_f32_16x16x4f32(key_float[j][i], q[i], acc[j & 3u], 0, 0, 0);
                 }
             }
 #pragma unroll
             for (uint32_t r = 0; r < 4u; ++r) {
-                score[r] = acc[0][r] + acc[1][r];
+                score[r] = (acc[0][r] + acc[1][r]) + (acc[2][r] + acc[3][r]);
             }
         } else {
             f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
