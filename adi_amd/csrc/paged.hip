@@ -93,9 +93,9 @@ constexpr uint32_t kAhead = 2;  // tokens whose rows are on their way
 // a block, a head's partner dimensions through the wave's own piece of LDS.
 //
 // Bound by a block's chain of loads (offsets and lengths, page, store) where the
-// tokens are few (4.1 us for one, 4.3 for 32), by the rows' bytes where they are
-// many: 2,919 tokens of 32 + 8 + 8 heads of 128 in bf16, 72 MB, take 17.6 us, 4.1
-// TB/s. A block a token and part waited out that chain and its sines for every
+// tokens are few (3.8 us for one, 4.3 for 32), by the rows' bytes where they are
+// many: 2,919 tokens of 32 + 8 + 8 heads of 128 in bf16, 72 MB, take 16.1 us, 4.5
+// TB/s (19 where none of it is in the last-level cache). A block a token and part waited out that chain and its sines for every
 // one, and read its partners from LDS by the element: 28.9.
 template <typename R, typename C, uint32_t D>
 __global__ __launch_bounds__(kThreads) void k_paged_append(AppendArgs args) {
@@ -305,7 +305,7 @@ void launch_append(adi_hip_context *ctx, AppendArgs args) {
     constexpr uint32_t kRows = kThreads / (D / (16u / sizeof(R)));
     args.parts = ceil_div(args.query_heads + 2u * args.c.heads, kRows);
     // runs of tokens where there are more than six blocks a CU, what their registers
-    // let it hold (2,919 tokens: 17.6 us; 3, 4, 8 and 12 blocks 19.4, 17.8, 18.8, 19.0)
+    // let it hold (2,919 tokens, of an earlier form: 17.6 us; 3, 4, 8 and 12 blocks 19.4, 17.8, 18.8, 19.0)
     const uint64_t jobs = static_cast<uint64_t>(args.c.tokens) * args.parts;
     args.run = std::max(ceil_div(jobs, 6u * static_cast<uint64_t>(ctx->cu_count)), 1u);
     const uint64_t grid = static_cast<uint64_t>(ceil_div(args.c.tokens, args.run)) * args.parts;

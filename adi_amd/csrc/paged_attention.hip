@@ -406,7 +406,9 @@ __device__ __forceinline__ f32x4 load_through(const float *base, uint32_t at) {
 }
 
 // Whether a tile's values are on their way beside its keys, or take the keys'
-// registers when its scores are done; and the blocks a CU holds, by registers.
+// registers when its scores are done; and the blocks a CU holds, by registers
+// (which at heads of 64 and 128 have room for three or four: more than two have
+// been timed at 256 only).
 template <typename T, typename R, uint32_t D>
 constexpr bool step_eager() {
     return D < 256u || sizeof(R) > sizeof(T);
@@ -417,15 +419,16 @@ constexpr uint32_t step_blocks() {
 }
 
 // Bound by the entries' bytes where there are many: two sequences behind 131,071
-// entries, 8 heads of 128 in bf16, 832 MB in 155 us, 5.4 TB/s, what a large copy
-// reaches; 32 sequences of up to 4,096 entries, 153 MB, 35 us (4.4 TB/s: a
-// block's start and end are some 8 us). Where there are few,
+// entries, 8 heads of 128 in bf16, 832 MB in 148 us, 5.6 TB/s, above a large copy's
+// 5.1; 32 sequences of up to 4,096 entries, 153 MB, 40 us from HBM, 3.8 TB/s (a
+// block's start and end are some 8 us; 34 where the last call left them in the
+// last-level cache). Where there are few,
 // by its chain of latencies: one token behind 1,999 entries of 2 heads of 256 in
 // f32, 8.2 MB, 18 us: some 4 to start, page numbers, a tile's loads and products
 // 3, the join of 32 parts 7.
 //
-// Block (KV head, part, sequence), the parts of up to 64 sequences by their
-// lengths: its four waves take the part's tiles in turn,
+// Block (KV head, part, sequence), the parts of 2 to 64 sequences by their lengths,
+// of others by max_length: its four waves take the part's tiles in turn,
 // each straight from the cache into operands, the next tile's keys on their way
 // from the end of this one's scores and its values from the end of their
 // products. Lane l is column c = l % 16 (a row), quarter g = l / 16. The blocks
@@ -1124,8 +1127,9 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
 // vector unit (16 multiply-adds a wave: 49 ns alone, 55 ns for both), so a SIMD
 // gets two waves at least. 32 rows a wave read half as much LDS for a product,
 // but a row's sums and queries then take D * 3 / 4 registers. Of what the
-// registers and the 160 KB of LDS leave room for, the fastest of a sweep; in us,
-// rows x keys (waves, tiles, blocks a CU), the kept one first:
+// registers and the 160 KB of LDS leave room for, the fastest of a sweep; in us of
+// the kernels as they were then (10 to 15% above the present ones'), rows x
+// keys (waves, tiles, blocks a CU), the kept one first:
 //   16 bits,  64, a prompt of 8192:  32x64 (4, 1, 3) 424, 16x128 (8, 1, 2) 428,
 //                                    16x64 (8, 1, 2) 482, 32x64 (8, 1, 1) 500
 //   16 bits, 128, 5 ragged chunks:   32x64 (8, 2, 1) 165, 32x64 (8, 1, 1) 170,
@@ -1137,7 +1141,9 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(AttendArgs args) {
 //   f32 and bf16,  64:    16x64 (4, 1, 2) 113, 16x64 (8, 1, 1) 127, 16x32 (8, 1, 1) 169
 //   f32 and bf16, 128:    16x64 (4, 1, 2) 169, 16x64 (8, 1, 1) 185, 16x32 (8, 1, 1) 216
 //   f32 and bf16, 256:    16x32 (8, 1, 1) 367, 16x64 (8, 1, 1) 372, 16x32 (4, 1, 2) 477
-// f32 and f32 at 256 has LDS for one tile of 32 keys only (80 KB).
+// f32 and f32 at 256 has LDS for one tile of 32 keys only (80 KB). Both shapes of f32
+// rows at 256 are short of registers by 14 and 16 a lane, some of which are
+// read back from memory (60 and 68 bytes a lane) for every tile.
 template <uint32_t ROWS, uint32_t WAVES, uint32_t KEYS, uint32_t BUFFERS, uint32_t BLOCKS>
 struct ChunkShape {
     static constexpr uint32_t kRows = ROWS, kWaves = WAVES, kKeys = KEYS, kBuffers = BUFFERS, kBlocks = BLOCKS;
@@ -1169,12 +1175,13 @@ constexpr size_t chunk_lds() {
 }
 
 // Bound by matrix and vector phases that overlap in part: 8192 f16 tokens, 32
-// heads of 64 on 4, 275 GFLOP, 392 us (0.70 PFLOP/s; a large library product
+// heads of 64 on 4, 275 GFLOP, 374 us (0.73 PFLOP/s; a large library product
 // reaches 1.29): the matrix cores are busy 36% of the cycles, the vector units
 // (a third of it exponentials) 58%, at a clock that such work takes down to 1.8
-// GHz. Ragged chunks of 5 sequences in bf16, 32 heads of 128 on 8, 155 us (35%
-// and 47%); 512 f32 tokens behind 3584 over f32 heads of 256, 150 us and a join
-// of 12 (nine products an element: 44% and 43%). Tried without gain: the waves' halves
+// GHz. Ragged chunks of 5 sequences in bf16, 32 heads of 128 on 8, 145 us (35%
+// and 46%); 512 f32 tokens behind 3584 over f32 heads of 256, 153 us and a join
+// of 12 (three products of pieces for a score's, six for a value's: 44% and 42%).
+// Tried without gain on earlier forms of the kernel: the waves' halves
 // a phase apart over two buffers of keys and three of values (165 -> 185 us for
 // the ragged chunks), the next tile's scores among a tile's exponentials over three
 // buffers (165 -> 209, the prompt 424 -> 562), wave priorities for either phase

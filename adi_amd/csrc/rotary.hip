@@ -98,7 +98,7 @@ struct alignas(sizeof(T) * N) Vector {
 // bytes), and units of N dimensions behind them copied. Bound by the rows'
 // bytes where there are many: 4,099 tokens of 32 heads of 128 in bf16, 67 MB,
 // 13.6 us, 4.9 TB/s (a large copy: 5.1); by the launch where there are few (16
-// tokens: 3.2 us). With sines per head and pair they would be the work (60
+// tokens: 3.3 us). With sines per head and pair they would be the work (60
 // instructions a pair).
 template <typename T, uint32_t N, bool PAIRS>
 __global__ __launch_bounds__(kThreads) void k_rope_rows(RopeArgs args) {
