@@ -1,0 +1,747 @@
+// pages.hip -- the pages of a paged cache: tables forked, grown and given back
+// with their reference counts, pages copied, and a pool compacted.
+//
+// Nothing here reads a count on the host: pages are found, counted and moved by
+// the kernels, the lowest free ones first, so results do not depend on the order
+// of blocks and a captured call replays with the tables it finds.
+#include "paged_attention.hpp"
+
+#include <algorithm>
+
+namespace adi_hip {
+namespace {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWaves = kThreads / kWave;
+constexpr uint32_t kNone = 0xFFFFFFFFu;
+constexpr uint32_t kMaxBeams = 64;
+constexpr uint32_t kCaches = 64, kMaxCaches = 1024;  // of a launch, of a pool
+constexpr uint32_t kMaxPages = 1u << 22;
+// pages of a segment: what a block counts
+constexpr uint32_t kSegment = 2048, kSegments = kMaxPages / kSegment;
+constexpr uint32_t kOwn = kSegment / kThreads;  // pages of a thread
+
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+
+// ---- copies of pages ---------------------------------------------------------
+
+// The keys and values of every cache of a pool, and how a page of them lies: its
+// first n entries are `heads` runs of n entries (heads outermost) or n runs of
+// `heads`, in units of 16 bytes.
+struct CachesView {
+    char *data[2u * kCaches];  // keys, values, keys, ...
+    uint64_t page_stride, entry_stride, head_stride;  // bytes
+    uint32_t arrays, heads, head_units, page_size, pages;
+    uint32_t heads_first;
+};
+
+CachesView caches_view(const adi_hip_paged_pool &pool, uint32_t first) {
+    CachesView v{};
+    const adi_hip_paged_cache *const caches = pool.cache + first;
+    const uint32_t count = std::min(pool.caches - first, kCaches);
+    const adi_hip_paged_cache &c = caches[0];
+    const uint32_t size = type_bytes(c.type);
+    for (uint32_t i = 0; i < count; ++i) {
+        v.data[2u * i] = static_cast<char *>(caches[i].keys);
+        v.data[2u * i + 1u] = static_cast<char *>(caches[i].values);
+    }
+    v.page_stride = c.page_stride * size;
+    v.entry_stride = c.entry_stride * size;
+    v.head_stride = c.head_stride * size;
+    v.arrays = 2u * count;
+    v.heads = c.heads;
+    v.head_units = c.head_size * size / 16u;
+    v.page_size = c.page_size;
+    v.pages = c.pages;
+    v.heads_first = c.entry_stride < c.head_stride ? 1u : 0u;
+    return v;
+}
+
+// Where unit u of a page's first `entries` lies: vectors of a head counted entry by
+// entry, or head by head where `heads_first` (the order of the copy's source).
+__device__ __forceinline__ uint64_t unit_at(const CachesView &v, uint32_t heads_first, uint32_t entries, uint32_t u) {
+    const uint32_t run = heads_first != 0u ? entries : v.heads;
+    const uint32_t vector = u / v.head_units, d = u - vector * v.head_units;
+    const uint32_t outer = vector / run, inner = vector - outer * run;
+    return outer * (heads_first != 0u ? v.head_stride : v.entry_stride) +
+           inner * (heads_first != 0u ? v.entry_stride : v.head_stride) + d * 16u;
+}
+
+// Units of a piece: what a block copies at once.
+constexpr uint32_t kAhead = 4, kPiece = kThreads * kAhead;
+
+// Piece `piece` of the first `entries` of a page of array n into another's.
+__device__ __forceinline__ void copy_piece(const CachesView &from, const CachesView &to, uint32_t n, uint32_t source,
+                                           uint32_t target, uint32_t entries, uint32_t piece) {
+    const uint32_t units = entries * from.heads * from.head_units;
+    const char *const a = from.data[n] + source * from.page_stride;
+    char *const b = to.data[n] + target * to.page_stride;
+    u32x4 x[kAhead];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) {
+        const uint32_t u = piece * kPiece + i * kThreads + threadIdx.x;
+        if (u < units) {
+            x[i] = *reinterpret_cast<const u32x4 *>(a + unit_at(from, from.heads_first, entries, u));
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) {
+        const uint32_t u = piece * kPiece + i * kThreads + threadIdx.x;
+        if (u < units) {
+            *reinterpret_cast<u32x4 *>(b + unit_at(to, from.heads_first, entries, u)) = x[i];
+        }
+    }
+}
+
+struct CopyArgs {
+    CachesView from, to;
+    const uint32_t *sources, *targets, *entries;
+    uint32_t pieces;
+};
+
+__global__ __launch_bounds__(kThreads) void k_paged_copy(CopyArgs args) {
+    const uint32_t piece = blockIdx.x % args.pieces, rest = blockIdx.x / args.pieces;
+    const uint32_t n = rest % args.from.arrays, i = rest / args.from.arrays;
+    const uint32_t source = args.sources[i], target = args.targets[i];
+    uint32_t entries = args.from.page_size;
+    if (args.entries != nullptr) {
+        entries = min(entries, args.entries[i]);
+    }
+    if (source < args.from.pages && target < args.to.pages) {
+        copy_piece(args.from, args.to, n, source, target, entries, piece);
+    }
+}
+
+// ---- counts of a pool's segments -----------------------------------------------
+
+// The sum of `own` over the threads below this one, and in `all` over the block.
+// `sums`: kWaves words of LDS, free for use when every thread is here.
+__device__ __forceinline__ uint32_t block_before(uint32_t own, uint32_t *sums, uint32_t &all) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / kWave;
+    uint32_t sum = own;
+#pragma unroll
+    for (uint32_t step = 1; step < 64u; step <<= 1) {
+        const uint32_t below = static_cast<uint32_t>(__shfl_up(static_cast<int>(sum), step));
+        sum += lane >= step ? below : 0u;
+    }
+    __syncthreads();
+    if (lane == 63u) {
+        sums[wave] = sum;
+    }
+    __syncthreads();
+    uint32_t before = sum - own;
+    all = 0u;
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        before += w < wave ? sums[w] : 0u;
+        all += sums[w];
+    }
+    return before;
+}
+
+// What a fork's first launch leaves for its second, of each row: the entries that
+// it and its parent held (0: no parent), its new ones, the parent's row; the page
+// of which the first entries are copied (kNone: none), and how many pages rows
+// before it take.
+struct RowPlan {
+    uint32_t held, parents, added, parent;
+    uint32_t source, before, demand, over;
+};
+
+struct ForkArgs {
+    const uint32_t *old_lengths, *old_table, *old_references;
+    uint32_t old_stride;
+    uint32_t *lengths, *table, *references;
+    uint32_t stride, max_length;
+    const uint32_t *offsets, *parents;
+    uint32_t rows, beams, page_shift, pages, segments;
+    uint32_t tokens, max_tokens;
+    uint32_t *lacking;
+    // workspace
+    RowPlan *plan;
+    uint32_t *free_count, *free_page;  // [segments], [segments][kSegment]
+    uint32_t *demand;                  // of all rows
+};
+
+__device__ __forceinline__ uint32_t pages_of(uint32_t entries, uint32_t shift) {
+    return (entries >> shift) + ((entries & ((1u << shift) - 1u)) != 0u ? 1u : 0u);
+}
+
+// The free pages of a segment a block, and the rows' plans by the last one.
+__global__ __launch_bounds__(kThreads) void k_fork_plan(ForkArgs args) {
+    __shared__ uint32_t sums[kWaves];
+    const uint32_t t = threadIdx.x;
+    if (blockIdx.x < args.segments) {
+        const uint32_t first = blockIdx.x * kSegment + t * kOwn;
+        uint32_t count[kOwn], own = 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            count[i] = first + i < args.pages ? args.old_references[first + i] : 1u;
+            own += count[i] == 0u ? 1u : 0u;
+        }
+        uint32_t all = 0u, at = block_before(own, sums, all);
+        uint32_t *const list = args.free_page + blockIdx.x * kSegment;
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            if (count[i] == 0u) {
+                list[at++] = first + i;
+            }
+            if (args.references != args.old_references && first + i < args.pages) {
+                args.references[first + i] = count[i];
+            }
+        }
+        if (t == 0u) {
+            args.free_count[blockIdx.x] = all;
+        }
+        return;
+    }
+    const uint32_t page_mask = (1u << args.page_shift) - 1u;
+    uint32_t taken = 0u;
+    for (uint32_t base = 0; base < args.rows; base += kThreads) {
+        const uint32_t row = base + t;
+        RowPlan plan{0u, 0u, 0u, kNone, kNone, 0u, 0u, 0u};
+        if (row < args.rows) {
+            const uint32_t group = row / args.beams * args.beams, parent = args.parents[row];
+            const uint32_t a = min(args.offsets[row], args.tokens), b = min(args.offsets[row + 1u], args.tokens);
+            plan.held = args.old_lengths[row];
+            plan.added = b > a ? b - a : 0u;
+            if (parent < args.beams) {
+                plan.parent = group + parent;
+                plan.parents = args.old_lengths[plan.parent];
+            }
+            const uint64_t next = static_cast<uint64_t>(plan.parents) + plan.added;
+            plan.over = plan.added > args.max_tokens || next > args.max_length ? 1u : 0u;
+            if (plan.over == 0u) {
+                plan.demand = pages_of(plan.parents + plan.added, args.page_shift) -
+                              pages_of(plan.parents, args.page_shift);
+                const uint32_t last = plan.parents >> args.page_shift;
+                if ((plan.parents & page_mask) != 0u && plan.added != 0u && last < args.old_stride) {
+                    const uint32_t page = args.old_table[static_cast<uint64_t>(plan.parent) * args.old_stride + last];
+                    bool eldest = true;
+                    for (uint32_t other = group; other < row; ++other) {
+                        eldest = eldest && args.parents[other] != parent;
+                    }
+                    if (page < args.pages && !(eldest && args.old_references[page] == 1u)) {
+                        plan.source = page;
+                        plan.demand += 1u;
+                    }
+                }
+            }
+        }
+        uint32_t all = 0u;
+        plan.before = taken + block_before(plan.demand, sums, all);
+        taken += all;
+        if (row < args.rows) {
+            args.plan[row] = plan;
+        }
+    }
+    if (t == 0u) {
+        *args.demand = taken;
+    }
+}
+
+// The free pages before every segment's, in LDS (`before`, kSegments + 1 words).
+__device__ __forceinline__ void segments_before(const uint32_t *count, uint32_t segments, uint32_t *before,
+                                                uint32_t *sums) {
+    uint32_t done = 0u;
+    for (uint32_t base = 0; base < segments; base += kThreads) {
+        const uint32_t s = base + threadIdx.x;
+        uint32_t all = 0u;
+        const uint32_t at = done + block_before(s < segments ? count[s] : 0u, sums, all);
+        if (s < segments) {
+            before[s] = at;
+        }
+        done += all;
+    }
+    if (threadIdx.x == 0u) {
+        before[segments] = done;
+    }
+    __syncthreads();
+}
+
+// The n-th free page, kNone where there are not as many.
+__device__ __forceinline__ uint32_t nth_free(const ForkArgs &args, const uint32_t *before, uint32_t n) {
+    if (n >= before[args.segments]) {
+        return kNone;
+    }
+    uint32_t low = 0u, high = args.segments;  // before[low] <= n < before[high]
+    while (high - low > 1u) {
+        const uint32_t middle = (low + high) / 2u;
+        if (before[middle] <= n) {
+            low = middle;
+        } else {
+            high = middle;
+        }
+    }
+    return args.free_page[low * kSegment + (n - before[low])];
+}
+
+struct ForkCopyArgs {
+    CachesView caches;
+    uint32_t pieces, table_blocks, column_blocks;
+    uint64_t work;  // pieces of all rows and arrays
+};
+
+// The tables, a column of a request's rows a thread (each entry is read before any
+// is written, so that the old table may be the new one), and the copies.
+template <uint32_t K>
+__global__ __launch_bounds__(kThreads) void k_fork_apply(ForkArgs args, ForkCopyArgs copy) {
+    __shared__ uint32_t before[kSegments + 1u];
+    __shared__ uint32_t sums[kWaves];
+    __shared__ RowPlan plans[K];
+    const uint32_t t = threadIdx.x;
+    segments_before(args.free_count, args.segments, before, sums);
+    const uint32_t free = before[args.segments];
+    if (blockIdx.x >= copy.table_blocks) {
+        for (uint64_t w = blockIdx.x - copy.table_blocks; w < copy.work; w += gridDim.x - copy.table_blocks) {
+            const uint32_t piece = static_cast<uint32_t>(w % copy.pieces);
+            const uint64_t rest = w / copy.pieces;
+            const uint32_t n = static_cast<uint32_t>(rest % copy.caches.arrays);
+            const RowPlan plan = args.plan[rest / copy.caches.arrays];
+            if (plan.source != kNone) {
+                const uint32_t target = nth_free(args, before, plan.before);
+                if (target != kNone) {
+                    copy_piece(copy.caches, copy.caches, n, plan.source, target,
+                               plan.parents & ((1u << args.page_shift) - 1u), piece);
+                }
+            }
+        }
+        return;
+    }
+    if (blockIdx.x == 0u && t == 0u && args.lacking != nullptr) {
+        *args.lacking = *args.demand > free ? *args.demand - free : 0u;
+    }
+    const uint32_t group = blockIdx.x / copy.column_blocks * args.beams;
+    const uint32_t c = blockIdx.x % copy.column_blocks * kThreads + t;
+    if (t < args.beams) {
+        plans[t] = args.plan[group + t];
+    }
+    __syncthreads();
+    uint32_t x[K], kept[K];
+#pragma unroll
+    for (uint32_t q = 0; q < K; ++q) {
+        x[q] = kNone;
+        kept[q] = 0u;
+        if (q < args.beams && c < min(pages_of(plans[q].held, args.page_shift), args.old_stride)) {
+            x[q] = args.old_table[static_cast<uint64_t>(group + q) * args.old_stride + c];
+        }
+    }
+    for (uint32_t s = 0; s < args.beams; ++s) {
+        const RowPlan plan = plans[s];
+        const uint32_t held = pages_of(plan.parents, args.page_shift);
+        const uint32_t end = static_cast<uint32_t>(
+            min((static_cast<uint64_t>(plan.parents) + plan.added + (1u << args.page_shift) - 1u) >> args.page_shift,
+                static_cast<uint64_t>(args.stride)));
+        if (c < end) {
+            const bool copies = plan.source != kNone && c == plan.parents >> args.page_shift;
+            uint32_t page = kNone;
+            if (copies || (c >= held && plan.over == 0u)) {
+                page = nth_free(args, before, plan.before + (copies ? 0u : c - held + (plan.source != kNone ? 1u : 0u)));
+                if (page != kNone) {
+                    args.references[page] = 1u;
+                }
+            } else if (c < held) {
+#pragma unroll
+                for (uint32_t q = 0; q < K; ++q) {
+                    if (group + q == plan.parent) {
+                        page = x[q];
+                        kept[q] += 1u;
+                    }
+                }
+            }
+            args.table[static_cast<uint64_t>(group + s) * args.stride + c] = page;
+        }
+        if (blockIdx.x % copy.column_blocks == 0u && t == 0u) {
+            args.lengths[group + s] =
+                static_cast<uint32_t>(min(static_cast<uint64_t>(plan.parents) + plan.added, uint64_t(kNone)));
+        }
+    }
+    // a page's holders of the request, counted once where they follow each other
+    uint32_t page = kNone, change = 0u;
+#pragma unroll
+    for (uint32_t q = 0; q < K; ++q) {
+        if (x[q] < args.pages) {
+            if (x[q] != page) {
+                if (change != 0u) {
+                    atomicAdd(&args.references[page], change);
+                }
+                page = x[q];
+                change = 0u;
+            }
+            change += kept[q] - 1u;
+        }
+    }
+    if (change != 0u) {
+        atomicAdd(&args.references[page], change);
+    }
+}
+
+// ---- compaction -----------------------------------------------------------------
+
+struct CompactArgs {
+    const uint32_t *old_references, *old_table, *lengths;
+    uint32_t *references, *table;
+    uint32_t rows, stride, columns, page_shift, pages, segments;
+    uint32_t *live;
+    // workspace
+    uint32_t *count;                     // live pages of each segment
+    uint32_t *sources, *targets, *rank;  // [pages / 2] twice, [pages]
+    uint32_t *moves;
+};
+
+__global__ __launch_bounds__(kThreads) void k_compact_count(CompactArgs args) {
+    __shared__ uint32_t sums[kWaves];
+    const uint32_t first = blockIdx.x * kSegment + threadIdx.x * kOwn;
+    uint32_t own = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+        if (first + i < args.pages) {
+            const uint32_t count = args.old_references[first + i];
+            own += count != 0u ? 1u : 0u;
+            if (args.references != args.old_references) {
+                args.references[first + i] = count;
+            }
+        }
+    }
+    uint32_t all = 0u;
+    (void)block_before(own, sums, all);
+    if (threadIdx.x == 0u) {
+        args.count[blockIdx.x] = all;
+    }
+}
+
+// The n-th live page behind the first `live` moves to the n-th free one below it.
+__global__ __launch_bounds__(kThreads) void k_compact_plan(CompactArgs args) {
+    __shared__ uint32_t before[kSegments + 1u];
+    __shared__ uint32_t sums[kWaves];
+    segments_before(args.count, args.segments, before, sums);
+    const uint32_t live = before[args.segments];
+    const uint32_t first = blockIdx.x * kSegment + threadIdx.x * kOwn;
+    uint32_t holds[kOwn], own = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+        holds[i] = first + i < args.pages && args.old_references[first + i] != 0u ? 1u : 0u;
+        own += holds[i];
+    }
+    uint32_t all = 0u, at = before[blockIdx.x] + block_before(own, sums, all);
+    // live pages below `live`: of the segments before its own, and in that
+    const uint32_t border = live / kSegment, edge = border * kSegment + threadIdx.x * kOwn;
+    uint32_t below = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+        below += edge + i < live && args.old_references[edge + i] != 0u ? 1u : 0u;
+    }
+    uint32_t in_border = 0u;
+    (void)block_before(below, sums, in_border);
+    const uint32_t kept = before[border] + in_border;
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+        const uint32_t page = first + i;
+        if (page < args.pages) {
+            if (page >= live) {
+                // (held, but counted as free: it has no new number)
+                args.rank[page] = holds[i] != 0u ? at - kept : kNone;
+                if (holds[i] != 0u) {
+                    args.sources[at - kept] = page;
+                }
+            } else if (holds[i] == 0u) {
+                args.targets[page - at] = page;
+            }
+        }
+        at += holds[i];
+    }
+    if (blockIdx.x == 0u && threadIdx.x == 0u) {
+        *args.moves = live - kept;
+        *args.live = live;
+    }
+}
+
+struct CompactCopyArgs {
+    CachesView caches;
+    uint32_t pieces, table_blocks;
+};
+
+__global__ __launch_bounds__(kThreads) void k_compact_apply(CompactArgs args, CompactCopyArgs copy) {
+    const uint32_t moves = *args.moves, live = *args.live;
+    if (blockIdx.x >= copy.table_blocks) {
+        const uint64_t work = static_cast<uint64_t>(moves) * copy.caches.arrays * copy.pieces;
+        for (uint64_t w = blockIdx.x - copy.table_blocks; w < work; w += gridDim.x - copy.table_blocks) {
+            const uint32_t piece = static_cast<uint32_t>(w % copy.pieces);
+            const uint64_t rest = w / copy.pieces;
+            const uint32_t n = static_cast<uint32_t>(rest % copy.caches.arrays);
+            const uint64_t i = rest / copy.caches.arrays;
+            copy_piece(copy.caches, copy.caches, n, args.sources[i], args.targets[i], 1u << args.page_shift, piece);
+        }
+        return;
+    }
+    const uint32_t step = copy.table_blocks * kThreads;
+    for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < moves; i += step) {
+        const uint32_t source = args.sources[i], target = args.targets[i];
+        args.references[target] = args.references[source];
+        args.references[source] = 0u;
+    }
+    for (uint64_t i = blockIdx.x * kThreads + threadIdx.x; i < static_cast<uint64_t>(args.rows) * args.columns;
+         i += step) {
+        const uint32_t row = static_cast<uint32_t>(i / args.columns), c = static_cast<uint32_t>(i % args.columns);
+        if (c < pages_of(args.lengths[row], args.page_shift)) {
+            const uint64_t at = static_cast<uint64_t>(row) * args.stride + c;
+            const uint32_t page = args.old_table[at];
+            const uint32_t rank = page >= live && page < args.pages ? args.rank[page] : kNone;
+            args.table[at] = rank != kNone ? args.targets[rank] : page;
+        }
+    }
+}
+
+// ---- checks and launches ----------------------------------------------------------
+
+void require_caches(const adi_hip_paged_cache *caches, uint32_t count) {
+    require(caches != nullptr && count >= 1 && count <= kMaxCaches, "paged pool: caches must be 1 to 1024");
+    adi_hip_paged_batch none{};
+    for (uint32_t i = 0; i < count; ++i) {
+        require_paged(&caches[i], &none);
+        const adi_hip_paged_cache &a = caches[0], &b = caches[i];
+        require(a.type == b.type && a.heads == b.heads && a.head_size == b.head_size && a.page_size == b.page_size &&
+                    a.pages == b.pages && a.page_stride == b.page_stride && a.entry_stride == b.entry_stride &&
+                    a.head_stride == b.head_stride,
+                "paged pool: the caches of a pool must be of one type and layout");
+    }
+    require(caches[0].pages <= kMaxPages, "paged pool: more than 2^22 pages");
+    // (a page's units are counted in 32 bits)
+    require(uint64_t(caches[0].heads) * caches[0].head_size * caches[0].page_size < (1u << 30),
+            "paged pool: a page of 2^30 elements or more");
+}
+
+void require_pool(const adi_hip_paged_pool *pool) {
+    require(pool != nullptr, "paged pool: null descriptor");
+    require_caches(pool->cache, pool->caches);
+}
+
+void require_counted(const adi_hip_paged_pool *pool) {
+    require_pool(pool);
+    require(pool->references != nullptr && aligned_to(pool->references, 4) && aligned_to(pool->lacking, 4),
+            "paged pool: null or unaligned references");
+}
+
+uint32_t pieces_of(const adi_hip_paged_cache &c, uint32_t entries) {
+    return ceil_div(uint64_t(entries) * c.heads * c.head_size * type_bytes(c.type) / 16u, kPiece);
+}
+
+void require_fork(const adi_hip_paged_pool *pool, const adi_hip_paged_batch *batch,
+                  const adi_hip_paged_fork_arguments *a) {
+    require_counted(pool);
+    require_paged(&pool->cache[0], batch);
+    require(a != nullptr, "paged fork: null arguments");
+    require(a->beams >= 1 && a->beams <= kMaxBeams && batch->sequences % a->beams == 0,
+            "paged fork: beams must be 1 to 64, and sequences a multiple of them");
+    if (batch->sequences == 0) {
+        return;
+    }
+    require(a->parents != nullptr && a->lengths != nullptr && a->table != nullptr && a->references != nullptr &&
+                batch->table != nullptr && batch->table_stride >= 1 && a->table_stride >= 1,
+            "paged fork: null argument");
+    require(aligned_to(a->parents, 4) && aligned_to(a->lengths, 4) && aligned_to(a->table, 4) &&
+                aligned_to(a->references, 4),
+            "paged fork: unaligned argument");
+    require(a->table != batch->table || a->table_stride == batch->table_stride,
+            "paged fork: the tables overlap with different strides");
+    require(uint64_t(batch->sequences / a->beams) * ceil_div(std::max(a->table_stride, batch->table_stride), kThreads) <
+                (1u << 22),
+            "paged fork: the tables are too large");
+}
+
+struct Scratch {
+    char *at;
+    uint64_t left;
+    template <typename T>
+    T *take(uint64_t count) {
+        const uint64_t bytes = (count * sizeof(T) + 255u) & ~uint64_t(255);
+        if (bytes > left) {
+            fail(ADI_HIP_OUT_OF_MEMORY, "paged pool: the workspace is too small for the pool's pages and rows");
+        }
+        T *const p = reinterpret_cast<T *>(at);
+        at += bytes;
+        left -= bytes;
+        return p;
+    }
+};
+
+Scratch scratch_of(adi_hip_context *ctx, const adi_hip_paged_workspace *workspace) {
+    require(workspace != nullptr, "paged pool: null workspace");
+    require(workspace->device == ctx->device, "paged pool: the workspace is on another device");
+    return {static_cast<char *>(workspace->base) + kTickets * sizeof(uint32_t),
+            workspace->bytes - kTickets * sizeof(uint32_t)};
+}
+
+void paged_fork(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const adi_hip_paged_batch *batch,
+                const adi_hip_paged_fork_arguments *a, const adi_hip_paged_workspace *workspace) {
+    require_fork(pool, batch, a);
+    Scratch scratch = scratch_of(ctx, workspace);
+    if (batch->sequences == 0) {
+        return;
+    }
+    const adi_hip_paged_cache &c = pool->cache[0];
+    ForkArgs args{};
+    args.old_lengths = a->lengths;
+    args.old_table = a->table;
+    args.old_references = a->references;
+    args.old_stride = a->table_stride;
+    args.lengths = const_cast<uint32_t *>(batch->lengths);
+    args.table = const_cast<uint32_t *>(batch->table);
+    args.references = pool->references;
+    args.stride = batch->table_stride;
+    args.max_length = batch->max_length;
+    args.offsets = batch->offsets;
+    args.parents = a->parents;
+    args.rows = batch->sequences;
+    args.beams = a->beams;
+    args.page_shift = log2_of(c.page_size);
+    args.pages = c.pages;
+    args.segments = ceil_div(c.pages, kSegment);
+    args.tokens = batch->tokens;
+    args.max_tokens = batch->max_tokens;
+    args.lacking = pool->lacking;
+    args.plan = scratch.take<RowPlan>(args.rows);
+    args.free_count = scratch.take<uint32_t>(args.segments);
+    args.free_page = scratch.take<uint32_t>(uint64_t(args.segments) * kSegment);
+    args.demand = scratch.take<uint32_t>(1);
+    ForkCopyArgs copy{};
+    copy.pieces = pieces_of(c, c.page_size - 1u);
+    copy.column_blocks = ceil_div(std::max(args.old_stride, args.stride), kThreads);
+    copy.table_blocks = args.rows / args.beams * copy.column_blocks;
+    launch(ctx, "fork_plan", k_fork_plan, dim3(args.segments + 1u), dim3(kThreads), 0, args);
+    for (uint32_t first = 0; first < pool->caches; first += kCaches) {
+        copy.caches = caches_view(*pool, first);
+        copy.work = uint64_t(args.rows) * copy.caches.arrays * copy.pieces;
+        const uint32_t copiers = static_cast<uint32_t>(std::min<uint64_t>(copy.work, 16u * ctx->cu_count));
+        const dim3 grid(copy.table_blocks + copiers), block(kThreads);
+        if (args.beams <= 4) {
+            launch(ctx, "fork_apply", k_fork_apply<4>, grid, block, 0, args, copy);
+        } else if (args.beams <= 16) {
+            launch(ctx, "fork_apply", k_fork_apply<16>, grid, block, 0, args, copy);
+        } else {
+            launch(ctx, "fork_apply", k_fork_apply<64>, grid, block, 0, args, copy);
+        }
+        copy.table_blocks = 0;
+    }
+}
+
+void require_copy(const adi_hip_paged_pool *from, const adi_hip_paged_pool *to, const uint32_t *sources,
+                  const uint32_t *targets, const uint32_t *entries, uint32_t count) {
+    require_pool(from);
+    require_pool(to);
+    const adi_hip_paged_cache &a = from->cache[0], &b = to->cache[0];
+    require(from->caches == to->caches && a.type == b.type && a.heads == b.heads && a.head_size == b.head_size &&
+                a.page_size == b.page_size,
+            "paged copy: pools of different caches");
+    require(count <= kMaxPages, "paged copy: more than 2^22 pages");
+    require(count == 0 || (sources != nullptr && targets != nullptr && aligned_to(sources, 4) &&
+                           aligned_to(targets, 4) && aligned_to(entries, 4)),
+            "paged copy: null or unaligned argument");
+}
+
+void paged_copy(adi_hip_context *ctx, const adi_hip_paged_pool *from, const adi_hip_paged_pool *to,
+                const uint32_t *sources, const uint32_t *targets, const uint32_t *entries, uint32_t count) {
+    require_copy(from, to, sources, targets, entries, count);
+    CopyArgs args{};
+    args.pieces = pieces_of(from->cache[0], from->cache[0].page_size);
+    for (uint32_t first = 0; first < from->caches; first += kCaches) {
+        args.from = caches_view(*from, first);
+        args.to = caches_view(*to, first);
+        const uint64_t each = uint64_t(args.from.arrays) * args.pieces;
+        const uint64_t at_once = std::max<uint64_t>((1u << 23) / each, 1u);
+        for (uint64_t done = 0; done < count; done += at_once) {
+            const uint64_t n = std::min<uint64_t>(at_once, count - done);
+            args.sources = sources + done;
+            args.targets = targets + done;
+            args.entries = entries != nullptr ? entries + done : nullptr;
+            launch(ctx, "paged_copy", k_paged_copy, dim3(static_cast<uint32_t>(n * each)), dim3(kThreads), 0, args);
+        }
+    }
+}
+
+void require_compact(const adi_hip_paged_pool *pool, const adi_hip_paged_compact_arguments *a) {
+    require_counted(pool);
+    require(a != nullptr && a->references != nullptr && a->live != nullptr && aligned_to(a->references, 4) &&
+                aligned_to(a->live, 4),
+            "paged compact: null or unaligned argument");
+    require(a->rows <= (1u << 20), "paged compact: more than 2^20 rows");
+    require(a->rows == 0 || (a->lengths != nullptr && a->table != nullptr && a->next_table != nullptr &&
+                             a->table_stride >= 1 && aligned_to(a->lengths, 4) && aligned_to(a->table, 4) &&
+                             aligned_to(a->next_table, 4)),
+            "paged compact: null or unaligned table");
+}
+
+void paged_compact(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const adi_hip_paged_compact_arguments *a,
+                   const adi_hip_paged_workspace *workspace) {
+    require_compact(pool, a);
+    Scratch scratch = scratch_of(ctx, workspace);
+    const adi_hip_paged_cache &c = pool->cache[0];
+    CompactArgs args{};
+    args.old_references = a->references;
+    args.old_table = a->table;
+    args.lengths = a->lengths;
+    args.references = pool->references;
+    args.table = a->next_table;
+    args.rows = a->rows;
+    args.stride = a->table_stride;
+    args.columns = a->table_stride;
+    args.page_shift = log2_of(c.page_size);
+    args.pages = c.pages;
+    args.segments = ceil_div(c.pages, kSegment);
+    args.live = a->live;
+    args.count = scratch.take<uint32_t>(args.segments);
+    args.sources = scratch.take<uint32_t>(c.pages / 2u + 1u);
+    args.targets = scratch.take<uint32_t>(c.pages / 2u + 1u);
+    args.rank = scratch.take<uint32_t>(c.pages);
+    args.moves = scratch.take<uint32_t>(1);
+    CompactCopyArgs copy{};
+    copy.pieces = pieces_of(c, c.page_size);
+    const uint64_t words = std::max<uint64_t>(uint64_t(a->rows) * args.columns, c.pages / 2u + 1u);
+    copy.table_blocks = static_cast<uint32_t>(std::min<uint64_t>((words + kThreads - 1) / kThreads, ctx->cu_count));
+    launch(ctx, "compact_count", k_compact_count, dim3(args.segments), dim3(kThreads), 0, args);
+    launch(ctx, "compact_plan", k_compact_plan, dim3(args.segments), dim3(kThreads), 0, args);
+    for (uint32_t first = 0; first < pool->caches; first += kCaches) {
+        copy.caches = caches_view(*pool, first);
+        const uint64_t work = uint64_t(c.pages / 2u) * copy.caches.arrays * copy.pieces;
+        const uint32_t copiers = static_cast<uint32_t>(std::min<uint64_t>(work, 16u * ctx->cu_count));
+        launch(ctx, "compact_apply", k_compact_apply, dim3(copy.table_blocks + copiers), dim3(kThreads), 0, args, copy);
+        copy.table_blocks = 0;
+    }
+}
+
+}  // namespace
+}  // namespace adi_hip
+
+using namespace adi_hip;
+
+extern "C" {
+
+int adi_hip_paged_fork(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const adi_hip_paged_batch *batch,
+                       const adi_hip_paged_fork_arguments *arguments, adi_hip_paged_workspace *workspace) {
+    return guarded(ctx, [&] { paged_fork(ctx, pool, batch, arguments, workspace); });
+}
+
+int adi_hip_paged_copy(adi_hip_context *ctx, const adi_hip_paged_pool *from, const adi_hip_paged_pool *to,
+                       const uint32_t *sources, const uint32_t *targets, const uint32_t *entries, uint32_t count) {
+    return guarded(ctx, [&] { paged_copy(ctx, from, to, sources, targets, entries, count); });
+}
+
+int adi_hip_paged_compact(adi_hip_context *ctx, const adi_hip_paged_pool *pool,
+                          const adi_hip_paged_compact_arguments *arguments, adi_hip_paged_workspace *workspace) {
+    return guarded(ctx, [&] { paged_compact(ctx, pool, arguments, workspace); });
+}
+
+int adi_hip_paged_fork_check(const adi_hip_paged_pool *pool, const adi_hip_paged_batch *batch,
+                             const adi_hip_paged_fork_arguments *arguments) {
+    return guarded_host([&] { require_fork(pool, batch, arguments); });
+}
+
+int adi_hip_paged_copy_check(const adi_hip_paged_pool *from, const adi_hip_paged_pool *to, const uint32_t *sources,
+                             const uint32_t *targets, const uint32_t *entries, uint32_t count) {
+    return guarded_host([&] { require_copy(from, to, sources, targets, entries, count); });
+}
+
+int adi_hip_paged_compact_check(const adi_hip_paged_pool *pool, const adi_hip_paged_compact_arguments *arguments) {
+    return guarded_host([&] { require_compact(pool, arguments); });
+}
+
+}  // extern "C"

@@ -151,6 +151,31 @@ class PagedAttentionArguments(C.Structure):
                 ("scale", f32), ("window", u32)]
 
 
+class BeamArguments(C.Structure):
+    _fields_ = [("type", u32), ("logits", vp), ("request_stride", u64), ("beam_stride", u64), ("requests", u32),
+                ("beams", u32), ("vocabulary", u32), ("choices", u32), ("scores", vp), ("weights", vp),
+                ("ended", vp), ("ended_token", u32), ("settle", u32), ("out_scores", vp), ("parents", vp),
+                ("tokens", vp)]
+
+
+class RowArray(C.Structure):
+    _fields_ = [("data", vp), ("request_stride", u64), ("row_stride", u64), ("row_bytes", u64)]
+
+
+class PagedPoolStruct(C.Structure):
+    _fields_ = [("caches", u32), ("cache", C.POINTER(PagedCacheStruct)), ("references", vp), ("lacking", vp)]
+
+
+class PagedForkArguments(C.Structure):
+    _fields_ = [("beams", u32), ("parents", vp), ("lengths", vp), ("table", vp), ("table_stride", u32),
+                ("references", vp)]
+
+
+class PagedCompactArguments(C.Structure):
+    _fields_ = [("references", vp), ("rows", u32), ("lengths", vp), ("table", vp), ("next_table", vp),
+                ("table_stride", u32), ("live", vp)]
+
+
 class KernelProfile(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("launches", C.c_uint64), ("total_ms", C.c_double)]
 
@@ -252,6 +277,19 @@ SIGNATURES = [
      [vp, C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), vp, vp]),
     ("adi_hip_full_attention_paged", C.c_int,
      [vp, C.POINTER(FullAttentionStruct), C.POINTER(PagedCacheStruct), C.POINTER(PagedBatchStruct), vp, vp, vp]),
+    ("adi_hip_beam_select", C.c_int, [vp, vp, vp]),
+    ("adi_hip_beam_check", C.c_int, [C.POINTER(BeamArguments)]),
+    ("adi_hip_reorder_rows", C.c_int, [vp, vp, u32, u32, u32, vp]),
+    ("adi_hip_reorder_check", C.c_int, [C.POINTER(RowArray), u32, u32, u32, vp]),
+    ("adi_hip_paged_fork", C.c_int, [vp, C.POINTER(PagedPoolStruct), C.POINTER(PagedBatchStruct), vp, vp]),
+    ("adi_hip_paged_fork_check", C.c_int,
+     [C.POINTER(PagedPoolStruct), C.POINTER(PagedBatchStruct), C.POINTER(PagedForkArguments)]),
+    ("adi_hip_paged_copy", C.c_int,
+     [vp, C.POINTER(PagedPoolStruct), C.POINTER(PagedPoolStruct), vp, vp, vp, u32]),
+    ("adi_hip_paged_copy_check", C.c_int,
+     [C.POINTER(PagedPoolStruct), C.POINTER(PagedPoolStruct), vp, vp, vp, u32]),
+    ("adi_hip_paged_compact", C.c_int, [vp, C.POINTER(PagedPoolStruct), vp, vp]),
+    ("adi_hip_paged_compact_check", C.c_int, [C.POINTER(PagedPoolStruct), C.POINTER(PagedCompactArguments)]),
     ("adi_hip_profiling_enable", C.c_int, [vp, C.c_int]),
     ("adi_hip_profiling_read", C.c_int, [vp, C.POINTER(KernelProfile), u32, C.POINTER(u32)]),
     # include/adi_hip_gguf.h
@@ -1416,3 +1454,170 @@ def full_attention_paged(ctx: Context, layer: DeviceFullAttention, cache: PagedC
             _refuse(f"rows must be contiguous f32 [{batch.tokens}, {hidden}] on cuda:{ctx.device}")
     ctx.check(ctx.lib.adi_hip_full_attention_paged(ctx.handle, C.byref(layer.struct), cache.struct, batch.struct,
                                                    x.data_ptr(), out.data_ptr(), workspace.handle))
+
+
+# ---- beam search, and the pages of a cache ------------------------------------
+
+# As the calls above: the structures' bytes (BeamArguments, PagedForkArguments,
+# PagedCompactArguments).
+_pack_beam = struct.Struct("=I4xQQQ IIII QQQ II QQQ").pack
+_pack_fork = struct.Struct("=I4xQQQ I4xQ").pack
+_pack_compact = struct.Struct("=Q I4xQQQ I4xQ").pack
+
+
+def _device_floats(ctx: Context, t, name: str, *shape):
+    if t.shape != shape or not t.is_contiguous() or _dtype_name(t) != "float32":
+        _refuse(f"{name} must be a contiguous float32 tensor of shape {shape}")
+    if t.get_device() != ctx.device:
+        _refuse(f"{name} on {t.device}, the context is on cuda:{ctx.device}")
+    return t
+
+
+def beam_select(ctx: Context, logits, scores, out_scores, parents, tokens, workspace: PagedWorkspace, weights=None,
+                ended=None, ended_token: int = 0, settle: bool = False) -> None:
+    """The best candidates of every request over its beams and the vocabulary:
+    logits [requests, beams, vocabulary] (f32, f16 or bf16, any strides of the first
+    two) behind the beams' scores [requests, beams] into out_scores, parents and
+    tokens [requests, choices]; `weights` of a beam's scores in the order, beams
+    that have `ended` (nonzero; int32) stand for ended_token alone. settle: a
+    parent's first child in the parent's row (adi_hip_beam_select)."""
+    if logits.dim() != 3:
+        _refuse("logits must be of shape [requests, beams, vocabulary]")
+    n, k, v = logits.shape
+    if logits.get_device() != ctx.device:
+        _refuse(f"logits on {logits.device}, the context is on cuda:{ctx.device}")
+    request_stride, beam_stride, step = logits.stride()
+    if step != 1 and v > 1:
+        _refuse("a row's logits must be contiguous")
+    if not 0 <= ended_token < 1 << 32:
+        _refuse("beam select: ended_token is out of range")
+    _device_floats(ctx, scores, "scores", n, k)
+    if out_scores.dim() != 2:
+        _refuse("out_scores must be of shape [requests, choices]")
+    choices = out_scores.shape[1]
+    _device_floats(ctx, out_scores, "out_scores", n, choices)
+    _device_words(ctx, parents, "parents", n, choices)
+    _device_words(ctx, tokens, "tokens", n, choices)
+    a = _pack_beam(_type_of(logits), logits.data_ptr(), request_stride, beam_stride, n, k, v, choices,
+                   scores.data_ptr(), 0 if weights is None else _device_floats(ctx, weights, "weights", n, k).data_ptr(),
+                   0 if ended is None else _device_words(ctx, ended, "ended", n, k).data_ptr(), ended_token,
+                   1 if settle else 0, out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr())
+    status = ctx.lib.adi_hip_beam_select(ctx.handle, a, workspace.handle)
+    if status:
+        ctx.check(status)
+
+
+class StateRows:
+    """Tensors [requests, beams, ...] of one request and beam count, for
+    reorder_rows; what follows a row's two dimensions is contiguous."""
+
+    def __init__(self, ctx: Context, arrays):
+        self.arrays = list(arrays)
+        if any(t.dim() < 2 for t in self.arrays):
+            _refuse("state rows: arrays must be of shape [requests, beams, ...], one for all")
+        self.requests, self.beams = (int(x) for x in self.arrays[0].shape[:2]) if self.arrays else (0, 1)
+        rows = (RowArray * max(len(self.arrays), 1))()
+        for i, t in enumerate(self.arrays):
+            if tuple(t.shape[:2]) != (self.requests, self.beams):
+                _refuse("state rows: arrays must be of shape [requests, beams, ...], one for all")
+            if t.get_device() != ctx.device:
+                _refuse(f"state rows on {t.device}, the context is on cuda:{ctx.device}")
+            if t.numel() and not t[0, 0].is_contiguous():
+                _refuse("state rows: a row must be contiguous")
+            size = t.element_size()
+            each = t.numel() // max(self.requests * self.beams, 1)
+            rows[i] = RowArray(t.data_ptr(), t.stride(0) * size, t.stride(1) * size, each * size)
+        self.struct = rows
+
+
+def reorder_rows(ctx: Context, rows: StateRows, parents) -> None:
+    """Row b of every request becomes row parents[request, b] (int32 [requests,
+    beams]) of the same request, in place, in all the arrays; others stay."""
+    _device_words(ctx, parents, "parents", rows.requests, rows.beams)
+    status = ctx.lib.adi_hip_reorder_rows(ctx.handle, rows.struct, len(rows.arrays), rows.requests, rows.beams,
+                                          parents.data_ptr())
+    if status:
+        ctx.check(status)
+
+
+class PagedPool:
+    """The caches (PagedCache, one a layer) whose pages are handed out together,
+    with their reference counts (int32 [pages]; 0: free) and, where given, the
+    number of pages that the last fork lacked (int32 [1])."""
+
+    def __init__(self, ctx: Context, caches, references=None, lacking=None):
+        self.caches = list(caches)
+        if not self.caches:
+            _refuse("paged pool: caches must be 1 to 1024")
+        self.pages, self.page_size = self.caches[0].pages, self.caches[0].page_size
+        self.references, self.lacking = references, lacking
+        if references is not None:
+            _device_words(ctx, references, "references", self.pages)
+        if lacking is not None:
+            _device_words(ctx, lacking, "lacking", 1)
+        self._array = (PagedCacheStruct * len(self.caches))(*(c.struct for c in self.caches))
+        self.struct = PagedPoolStruct(len(self.caches), self._array, _addr(references), _addr(lacking))
+
+
+def paged_fork(ctx: Context, pool: PagedPool, batch: PagedBatch, parents, workspace: PagedWorkspace, lengths=None,
+               table=None, references=None) -> None:
+    """The tables and lengths of a batch's next step, written into batch.table,
+    batch.lengths and pool.references: sequence s becomes its parent (parents int32
+    [requests, beams], a row of its request, -1: none) with the batch's new tokens
+    behind, pages shared, copied where two would write into one, taken and given
+    back. The old lengths, table and references are the batch's and the pool's own, in
+    place, or those given (adi_hip_paged_fork)."""
+    lengths = batch.lengths if lengths is None else lengths
+    table = batch.table if table is None else table
+    references = pool.references if references is None else references
+    if references is None:
+        _refuse("paged fork: the pool has no references")
+    if parents.dim() != 2:
+        _refuse("parents must be of shape [requests, beams]")
+    n, k = parents.shape
+    if n * k != batch.lengths.shape[0]:
+        _refuse(f"parents of {n * k} rows, the batch has {batch.lengths.shape[0]}")
+    _device_words(ctx, parents, "parents", n, k)
+    _device_words(ctx, lengths, "lengths", n * k)
+    _device_words(ctx, table, "table", n * k, int(table.shape[-1]))
+    _device_words(ctx, references, "references", pool.pages)
+    a = _pack_fork(k, parents.data_ptr(), lengths.data_ptr(), table.data_ptr(), table.shape[1], references.data_ptr())
+    status = ctx.lib.adi_hip_paged_fork(ctx.handle, pool.struct, batch.struct, a, workspace.handle)
+    if status:
+        ctx.check(status)
+
+
+def paged_copy(ctx: Context, source: PagedPool, target: PagedPool, sources, targets, entries=None) -> None:
+    """Pages sources[i] of a pool to pages targets[i] of another or the same (int32
+    [count]), in every cache, the first entries[i] of their entries where given."""
+    n = int(sources.shape[0])
+    _device_words(ctx, sources, "sources", n)
+    _device_words(ctx, targets, "targets", n)
+    if entries is not None:
+        _device_words(ctx, entries, "entries", n)
+    status = ctx.lib.adi_hip_paged_copy(ctx.handle, source.struct, target.struct, sources.data_ptr(),
+                                        targets.data_ptr(), _addr(entries), n)
+    if status:
+        ctx.check(status)
+
+
+def paged_compact(ctx: Context, pool: PagedPool, lengths, next_table, live, workspace: PagedWorkspace, table=None,
+                  references=None) -> None:
+    """Moves a pool's held pages to the lowest numbers, `live` (int32 [1]) of them:
+    the rows' table [rows, columns] (default: next_table, in place) into next_table,
+    the old references (default: the pool's own) into the pool's."""
+    table = next_table if table is None else table
+    references = pool.references if references is None else references
+    if references is None:
+        _refuse("paged compact: the pool has no references")
+    n = int(lengths.shape[0])
+    _device_words(ctx, lengths, "lengths", n)
+    _device_words(ctx, table, "table", n, int(table.shape[-1]))
+    _device_words(ctx, next_table, "next_table", *table.shape)
+    _device_words(ctx, references, "references", pool.pages)
+    _device_words(ctx, live, "live", 1)
+    a = _pack_compact(references.data_ptr(), n, lengths.data_ptr(), table.data_ptr(), next_table.data_ptr(),
+                      table.shape[1], live.data_ptr())
+    status = ctx.lib.adi_hip_paged_compact(ctx.handle, pool.struct, a, workspace.handle)
+    if status:
+        ctx.check(status)

@@ -883,6 +883,162 @@ int adi_hip_full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attent
                                  const adi_hip_paged_batch *batch, const float *inputs,
                                  float *outputs, adi_hip_paged_workspace *workspace);
 
+/* ---- beam search, and the pages of a cache -------------------------------- */
+
+/* One step's choice for `requests` requests of `beams` beams each: beam b of
+ * request r has the score scores[r][b] (a sum of log-probabilities) and the logits
+ * of its next token, and a request takes the `choices` best of its candidates
+ *   score(b, v) = scores[b] + (logit[b][v] - log sum_u exp(logit[b][u]))
+ * by rank = weights[b] score(b, v) (no weights: 1; say 1 / length^a), best
+ * first, ranks in 64 bits of exact logarithms; equal ranks: the lower beam, then
+ * the larger logit, then the lower token. A beam that has `ended` (nonzero) is one
+ * candidate, ended_token with the score it has; its logits are not read. Outputs
+ * are the candidates' scores (rounded to float), beams and tokens. It follows
+ * sample_token (src/generation.cpp:161-225) where that keeps one token of a row.
+ *
+ * Never chosen: tokens whose logit is -infinity, and anything of a beam whose
+ * score is -infinity (as the other beams' of a first step), whatever its
+ * logits, weight or mark hold. Places without a candidate get score
+ * -infinity and 0xFFFFFFFF for beam and token. A NaN or +infinity among a
+ * beam's logits or as its score, or a weight that is not positive and finite,
+ * makes all the request's scores NaN, its beams and tokens 0xFFFFFFFF.
+ *
+ * With `settle` (choices = beams) the candidates are placed so that states move
+ * least: a parent's first child goes to the parent's row, the others, in their
+ * order, and then places without a candidate, to the rows of beams without a
+ * child, ascending.
+ *
+ * The workspace (adi_hip_paged_workspace) holds 12 + 8 choices bytes for each
+ * 8192 logits of a row, 2048 where there are few, and takes requests one after
+ * another where it cannot hold all; ADI_HIP_OUT_OF_MEMORY where it cannot hold
+ * one. Nothing is allocated, so a call may be captured. */
+typedef struct {
+    uint32_t type;                        /* of the logits: ADI_HIP_F32, _F16, _BF16 */
+    const void *logits;                   /* [requests][beams][vocabulary] */
+    uint64_t request_stride, beam_stride; /* elements */
+    uint32_t requests;                    /* up to 2^20 */
+    uint32_t beams;                       /* 1 to 64 */
+    uint32_t vocabulary;                  /* 1 to 2^24 */
+    uint32_t choices;                     /* 1 to 128 */
+    const float *scores;                  /* [requests][beams] */
+    const float *weights;                 /* [requests][beams] or NULL */
+    const uint32_t *ended;                /* [requests][beams] or NULL */
+    uint32_t ended_token;
+    uint32_t settle;
+    float *out_scores;                    /* [requests][choices]; not the scores */
+    uint32_t *parents, *tokens;           /* [requests][choices] */
+} adi_hip_beam_arguments;
+int adi_hip_beam_select(adi_hip_context *ctx, const adi_hip_beam_arguments *arguments,
+                        adi_hip_paged_workspace *workspace);
+/* The call's checks alone, on the host, no GPU needed (message:
+ * adi_hip_last_error(NULL)). So are the other _check entries below. */
+int adi_hip_beam_check(const adi_hip_beam_arguments *arguments);
+
+/* Per-beam states that follow their parents, in place: in every array, row b of a
+ * request becomes what row parents[request][b] (DEVICE) was; a parent that is
+ * not below `beams` leaves the row as it is. Row b of request r is the row_bytes
+ * bytes at data + r request_stride + b row_stride (all in bytes, of any size and
+ * alignment; rows must not overlap). Rows that stay, and bytes between rows, are
+ * not written. For sequence states as adi_hip_layer_state, token histories, and
+ * the arrays of a search. beams: 1 to 64. */
+typedef struct {
+    void *data;
+    uint64_t request_stride, row_stride, row_bytes;
+} adi_hip_row_array;
+int adi_hip_reorder_rows(adi_hip_context *ctx, const adi_hip_row_array *arrays, uint32_t count,
+                         uint32_t requests, uint32_t beams, const uint32_t *parents);
+int adi_hip_reorder_check(const adi_hip_row_array *arrays, uint32_t count, uint32_t requests,
+                          uint32_t beams, const uint32_t *parents);
+
+/* The caches (a layer's each) whose pages a server hands out together: one type,
+ * layout and number of pages (up to 2^22), keys and values of their own; a page
+ * number is a page of each. references[p] is the number of table entries, of
+ * rows' lengths, that hold page p; 0: free. */
+typedef struct {
+    uint32_t caches;                  /* 1 to 1024 */
+    const adi_hip_paged_cache *cache; /* HOST [caches] */
+    uint32_t *references;             /* DEVICE [pages] (not read by adi_hip_paged_copy) */
+    uint32_t *lacking;                /* DEVICE [1] or NULL: see adi_hip_paged_fork */
+} adi_hip_paged_pool;
+
+/* Page tables for a batch's next step. Its sequences are rows of requests of
+ * `beams` each (1: no search). Row s was arguments->lengths[s] entries long, with
+ * pages in arguments->table[s]; now it becomes its parent, row
+ * parents[s] of its request as it was, with the batch's new tokens of s (offsets)
+ * behind: batch->lengths[s] = lengths[parent] + new, and batch->table[s] holds
+ *   - the parent's pages, shared;
+ *   - instead of a partly filled last page that new entries go into, a page of its
+ *     own with the parent's entries copied, in every cache of the pool; the first
+ *     row of a parent keeps the page itself where no other row held it;
+ *   - pages for the new tokens.
+ * A parent that is not below `beams` is none: what the row held is given back, and
+ * new tokens begin a sequence. So one call forks, grows, admits and frees, and
+ * adi_hip_paged_append may follow with the same batch. New pages are the
+ * lowest of those free before the call (pages given back are free for the next),
+ * handed out to rows in order; pool->references becomes arguments->references
+ * with all of it counted. Entries of the tables behind a row's pages are neither
+ * read nor written.
+ *
+ * Where too few pages are free, *pool->lacking (else 0) is the number that lacks,
+ * and the last rows' table entries for them are 0xFFFFFFFF: nothing is appended
+ * there, and rows that see them are NaN. A row over the batch's bounds
+ * (max_tokens, max_length) takes no pages; its length says so, its entries for
+ * them are 0xFFFFFFFF. Page numbers that are not the pool's are not counted.
+ *
+ * The old lengths, table and references may be the batch's and the pool's own
+ * (in place, one stride), or others, which stay valid until the next call: a step
+ * may be dropped by going on with the old ones. Other overlaps are not allowed.
+ * batch->lengths and table are written. The workspace holds 4 bytes a page
+ * (rounded up to 2048) and 32 a row; ADI_HIP_OUT_OF_MEMORY where it cannot. */
+typedef struct {
+    uint32_t beams;            /* 1 to 64; the batch's sequences a multiple */
+    const uint32_t *parents;   /* DEVICE [sequences] */
+    const uint32_t *lengths;   /* DEVICE [sequences] */
+    const uint32_t *table;     /* DEVICE [sequences][table_stride] */
+    uint32_t table_stride;
+    const uint32_t *references; /* DEVICE [pages] */
+} adi_hip_paged_fork_arguments;
+int adi_hip_paged_fork(adi_hip_context *ctx, const adi_hip_paged_pool *pool,
+                       const adi_hip_paged_batch *batch,
+                       const adi_hip_paged_fork_arguments *arguments,
+                       adi_hip_paged_workspace *workspace);
+int adi_hip_paged_fork_check(const adi_hip_paged_pool *pool, const adi_hip_paged_batch *batch,
+                             const adi_hip_paged_fork_arguments *arguments);
+
+/* Copies pages sources[i] of `from` to pages targets[i] of `to` (DEVICE [count]), in
+ * every cache, the first entries[i] of a page's entries (NULL, or more than a
+ * page's: all). The pools may be one; their caches are as many, of one type, heads
+ * and page size, of any layouts. Pairs with a number that is not a page are
+ * skipped. No target is another's, nor a source (but a page onto itself). */
+int adi_hip_paged_copy(adi_hip_context *ctx, const adi_hip_paged_pool *from,
+                       const adi_hip_paged_pool *to, const uint32_t *sources,
+                       const uint32_t *targets, const uint32_t *entries, uint32_t count);
+int adi_hip_paged_copy_check(const adi_hip_paged_pool *from, const adi_hip_paged_pool *to,
+                             const uint32_t *sources, const uint32_t *targets,
+                             const uint32_t *entries, uint32_t count);
+
+/* Moves the pages that are held (arguments->references above 0), *live of them,
+ * to the numbers below *live: the n-th of those from there on to the n-th
+ * free one below, in every cache. pool->references and next_table hold the
+ * counts and the numbers after it (next_table only where the rows' lengths reach);
+ * they may be the old arrays. Every table that holds pages of the pool has to be
+ * part of the call. The workspace holds 8 bytes a page; ADI_HIP_OUT_OF_MEMORY
+ * where it cannot. */
+typedef struct {
+    const uint32_t *references; /* DEVICE [pages] */
+    uint32_t rows;
+    const uint32_t *lengths;    /* DEVICE [rows], entries */
+    const uint32_t *table;      /* DEVICE [rows][table_stride] */
+    uint32_t *next_table;       /* of the same stride */
+    uint32_t table_stride;
+    uint32_t *live;             /* DEVICE [1] */
+} adi_hip_paged_compact_arguments;
+int adi_hip_paged_compact(adi_hip_context *ctx, const adi_hip_paged_pool *pool,
+                          const adi_hip_paged_compact_arguments *arguments,
+                          adi_hip_paged_workspace *workspace);
+int adi_hip_paged_compact_check(const adi_hip_paged_pool *pool,
+                                const adi_hip_paged_compact_arguments *arguments);
+
 /* ---- kernel profiling ----------------------------------------------------- */
 
 /* Per-kernel timing with HIP events on the context stream, the counterpart
