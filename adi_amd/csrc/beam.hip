@@ -3,7 +3,7 @@
 //
 // Selection: a beam of score s whose logits are l has the candidates
 //   s + (l_v - lse),  lse = m + log sum_v exp(l_v - m),
-// and a request takes the best of its beams'. One pass over the logits: a block
+// and a request takes the best of its beams'. One pass over the logits: a wave
 // holds a tile of a row in registers, adds up its exponentials and finds its best
 // logits (a row's candidates are in the order of its logits, whatever lse is); a
 // block a request then joins the sums and ranks the tiles' candidates.
@@ -19,21 +19,24 @@ constexpr uint32_t kWaves = kThreads / kWave;
 constexpr uint32_t kMaxBeams = 64, kMaxChoices = 128;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
+using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 
 struct BeamArgs {
     const char *logits;
     uint64_t request_stride, beam_stride;  // elements
-    uint32_t beams, vocabulary, choices, parts;
+    uint32_t beams, vocabulary, choices;
+    uint32_t span, parts, arrivals;  // logits of a part, a row's parts, a request's blocks
     const float *scores, *weights;
     const uint32_t *ended;
     uint32_t ended_token, settle;
     float *out_scores;
     uint32_t *parents, *tokens;
-    // of each row's tiles: largest logit, sum of exp(logit - largest), best logits
+    // of each row's parts: largest logit, sum of exponentials (reference_of), best logits
     float *most;
     double *sum;
     uint64_t *best;
+    uint32_t *tickets;  // of each request, zero between calls
 };
 
 // Ascending with the float, -0 as +0.
@@ -72,267 +75,265 @@ struct Piece {
     }
 };
 
+// The larger, or a NaN where either is one.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+using adi_hip::lane_xor;
+
 __device__ __forceinline__ float wave_most(float v) {
-    v = fmaxf(v, lane_xor<1>(v));
-    v = fmaxf(v, lane_xor<2>(v));
-    v = fmaxf(v, lane_xor<4>(v));
-    v = fmaxf(v, lane_xor<8>(v));
-    v = fmaxf(v, lane_xor<16>(v));
-    return fmaxf(v, lane_xor<32>(v));
+    v = larger(v, lane_xor<1>(v));
+    v = larger(v, lane_xor<2>(v));
+    v = larger(v, lane_xor<4>(v));
+    v = larger(v, lane_xor<8>(v));
+    v = larger(v, lane_xor<16>(v));
+    return larger(v, lane_xor<32>(v));
+}
+
+template <int MASK>
+__device__ __forceinline__ double lane_xor(double v) {
+    u32x2 bits = __builtin_bit_cast(u32x2, v);
+    bits[0] = lane_xor_bits<MASK>(bits[0]);
+    bits[1] = lane_xor_bits<MASK>(bits[1]);
+    return __builtin_bit_cast(double, bits);
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int offset = 1; offset < 64; offset <<= 1) {
-        v += __shfl_xor(v, offset);
-    }
-    return v;
+    v += lane_xor<1>(v);
+    v += lane_xor<2>(v);
+    v += lane_xor<4>(v);
+    v += lane_xor<8>(v);
+    v += lane_xor<16>(v);
+    return v + lane_xor<32>(v);
 }
 
-// The largest key that at least `count` (1 to 64) of the wave's lanes reach.
-__device__ __forceinline__ uint32_t reached_by(uint32_t key, uint32_t count) {
+// A lane's kPieces pieces of a wave's tile, `from` its first logit. Rows of 16-bit
+// logits may begin in the middle of a word, where loads of 16 bytes are split by
+// their bytes: such a piece is put together from the words around it, each of
+// which holds a logit of the piece.
+template <typename T, uint32_t PIECES>
+__device__ __forceinline__ void load_tile(Piece<T> (&x)[PIECES], const char *from, uint32_t lane) {
+    if (sizeof(T) == 4u || (reinterpret_cast<uintptr_t>(from) & 2u) == 0u) {
+#pragma unroll
+        for (uint32_t j = 0; j < PIECES; ++j) {
+            x[j].load(from + (j * kWave + lane) * 16u);
+        }
+        return;
+    }
+    u32x4 head[PIECES];
+    uint32_t tail[PIECES];
+#pragma unroll
+    for (uint32_t j = 0; j < PIECES; ++j) {
+        const uint32_t *const words = reinterpret_cast<const uint32_t *>(from - 2 + (j * kWave + lane) * 16u);
+        __builtin_memcpy(&head[j], words, 16);
+        tail[j] = words[4];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < PIECES; ++j) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            x[j].raw[i] = __builtin_amdgcn_alignbit(i < 3u ? head[j][i + 1u] : tail[j], head[j][i], 16u);
+        }
+    }
+}
+
+// The same of a tile of which only the first `live` logits are the row's: -infinity
+// behind them. (No branches, so that all loads are on their way at once.)
+template <typename T, uint32_t PIECES>
+__device__ __forceinline__ void load_last(Piece<T> (&x)[PIECES], const char *from, uint32_t lane, uint32_t live) {
+    constexpr uint32_t kCount = Piece<T>::kCount;
+    T v[PIECES][kCount];
+#pragma unroll
+    for (uint32_t j = 0; j < PIECES; ++j) {
+#pragma unroll
+        for (uint32_t i = 0; i < kCount; ++i) {
+            v[j][i] = reinterpret_cast<const T *>(from)[min((j * kWave + lane) * kCount + i, live - 1u)];
+        }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < PIECES; ++j) {
+#pragma unroll
+        for (uint32_t i = 0; i < kCount; ++i) {
+            x[j].set(i, (j * kWave + lane) * kCount + i < live ? v[j][i] : static_cast<T>(-__builtin_huge_valf()));
+        }
+    }
+}
+
+// The largest key of 16 bits, 0s behind, that at least `count` of the two of each
+// of the wave's lanes reach (0 where fewer are not 0).
+__device__ __forceinline__ uint32_t reached_by(uint32_t a, uint32_t b, uint32_t count) {
     uint32_t reached = 0u;
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1) {
+#pragma unroll 4
+    for (uint32_t bit = 0x80000000u; bit != 0x8000u; bit >>= 1) {
         const uint32_t more = reached | bit;
-        reached = static_cast<uint32_t>(__popcll(__ballot(key >= more))) >= count ? more : reached;
+        const uint32_t reach = static_cast<uint32_t>(__popcll(__ballot(a >= more)) + __popcll(__ballot(b >= more)));
+        reached = reach >= count ? more : reached;
     }
     return reached;
 }
 
-// A tile of kThreads x N logits of a row. Its best: every wave's lanes hold their
-// own largest logits, of which the choices / 4 best bound the tile's `choices` best
-// from below; what reaches the least of the waves' bounds goes to a list in LDS,
-// a little more than `choices` long, and each entry's place is the number of
-// entries before it. Where many are equal (a masked run of ids) the list may not
-// hold them, and the last taken is found bit by bit.
-template <typename T, uint32_t N>
-__global__ __launch_bounds__(kThreads) void k_beam_tiles(BeamArgs args) {
-    constexpr uint32_t kCount = Piece<T>::kCount, kPieces = N / kCount, kTile = kThreads * N;
-    constexpr uint32_t kList = 512;
-    __shared__ uint64_t list[kList];
-    __shared__ uint32_t listed, bound[kWaves];
-    __shared__ float wave_top[kWaves];
-    __shared__ double wave_total[kWaves];
-    const uint32_t row = blockIdx.x / args.parts, part = blockIdx.x % args.parts;
-    const float score = args.scores[row];
-    if (score == -__builtin_huge_valf() || (args.ended != nullptr && args.ended[row] != 0u)) {
-        return;
-    }
-    const uint32_t t = threadIdx.x, wave = t / kWave;
-    const uint32_t first = part * kTile, live = min(args.vocabulary - first, kTile);
-    const char *const from = args.logits + (row / args.beams * args.request_stride +
-                                            row % args.beams * args.beam_stride + first) * sizeof(T);
-    if (t == 0u) {
-        listed = 0u;
-    }
-    Piece<T> x[kPieces];
-    if (live == kTile) {
-#pragma unroll
-        for (uint32_t j = 0; j < kPieces; ++j) {
-            x[j].load(from + (j * kThreads + t) * 16u);
-        }
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < kPieces; ++j) {
-            const uint32_t at = (j * kThreads + t) * kCount;
-            if (at + kCount <= live) {
-                x[j].load(from + at * sizeof(T));
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < kCount; ++i) {
-                    T v = static_cast<T>(-__builtin_huge_valf());
-                    if (at + i < live) {
-                        v = reinterpret_cast<const T *>(from)[at + i];
-                    }
-                    x[j].set(i, v);
-                }
-            }
-        }
-    }
-    float own = -__builtin_huge_valf();
-#pragma unroll
-    for (uint32_t j = 0; j < kPieces; ++j) {
-#pragma unroll
-        for (uint32_t i = 0; i < kCount; ++i) {
-            own = fmaxf(own, x[j].get(i));
-        }
-    }
-    const float top = wave_most(own);
-    // (nothing but -infinity: all of its exponentials are 0)
-    const double level = top == -__builtin_huge_valf() ? 0.0 : static_cast<double>(top);
-    double total = 0.0;
-#pragma unroll
-    for (uint32_t j = 0; j < kPieces; ++j) {
-#pragma unroll
-        for (uint32_t i = 0; i < kCount; ++i) {
-            total += exp(static_cast<double>(x[j].get(i)) - level);
-        }
-    }
-    total = wave_sum(total);
-    const uint32_t reached = reached_by(ascending_key(own), (args.choices + kWaves - 1u) / kWaves);
-    if ((t & 63u) == 0u) {
-        bound[wave] = reached;
-        wave_top[wave] = top;
-        wave_total[wave] = total;
-    }
-    __syncthreads();
-    const uint32_t least = max(min(min(bound[0], bound[1]), min(bound[2], bound[3])), kLowestKey + 1u);
-    const auto place_of = [&](uint32_t j, uint32_t i) { return (j * kThreads + t) * kCount + i; };
-#pragma unroll
-    for (uint32_t j = 0; j < kPieces; ++j) {
-#pragma unroll
-        for (uint32_t i = 0; i < kCount; ++i) {
-            const uint32_t key = ascending_key(x[j].get(i));
-            if (key >= least) {
-                const uint32_t at = atomicAdd(&listed, 1u);
-                if (at < kList) {
-                    list[at] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~(first + place_of(j, i)));
-                }
-            }
-        }
-    }
-    __syncthreads();
-    uint32_t entries = listed;
-    if (entries > kList) {
-        // the last taken, in the order of the keys and then of the places
-        uint64_t last = 0u;
-        constexpr uint32_t kPlaceBits = 13;
-        static_assert(kTile <= 1u << kPlaceBits, "a tile's places fit their bits");
-        const auto whole = [&](uint32_t j, uint32_t i) {
-            return static_cast<uint64_t>(ascending_key(x[j].get(i))) << kPlaceBits |
-                   ((1u << kPlaceBits) - 1u - place_of(j, i));
-        };
-#pragma unroll 1
-        for (uint64_t bit = 1ull << (31u + kPlaceBits); bit != 0u; bit >>= 1) {
-            const uint64_t more = last | bit;
-            uint32_t reach = 0u;
-#pragma unroll
-            for (uint32_t j = 0; j < kPieces; ++j) {
-#pragma unroll
-                for (uint32_t i = 0; i < kCount; ++i) {
-                    reach += static_cast<uint32_t>(__popcll(__ballot(whole(j, i) >= more)));
-                }
-            }
-            __syncthreads();  // the last round's bounds are read
-            if ((t & 63u) == 0u) {
-                bound[wave] = reach;
-            }
-            __syncthreads();
-            last = bound[0] + bound[1] + bound[2] + bound[3] >= args.choices ? more : last;
-        }
-        if (t == 0u) {
-            listed = 0u;
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t j = 0; j < kPieces; ++j) {
-#pragma unroll
-            for (uint32_t i = 0; i < kCount; ++i) {
-                const uint32_t key = ascending_key(x[j].get(i));
-                if (key >= least && whole(j, i) >= last) {
-                    list[atomicAdd(&listed, 1u)] =
-                        static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~(first + place_of(j, i)));
-                }
-            }
-        }
-        __syncthreads();
-        entries = listed;  // `choices` of them
-    }
-    uint64_t *const best = args.best + static_cast<uint64_t>(blockIdx.x) * args.choices;
-    for (uint32_t e = t; e < entries; e += kThreads) {
-        const uint64_t key = list[e];
-        uint32_t before = 0u;
-        for (uint32_t o = 0; o < entries; ++o) {
-            before += list[o] > key ? 1u : 0u;
-        }
-        if (before < args.choices) {
-            best[before] = key;
-        }
-    }
-    for (uint32_t e = entries + t; e < args.choices; e += kThreads) {
-        best[e] = 0u;
-    }
-    if (t == 0u) {
-        float most = -__builtin_huge_valf();
-        for (uint32_t w = 0; w < kWaves; ++w) {
-            most = fmaxf(most, wave_top[w]);
-        }
-        double sum = 0.0;
-        for (uint32_t w = 0; w < kWaves; ++w) {
-            sum += wave_top[w] == -__builtin_huge_valf()
-                       ? wave_total[w]
-                       : wave_total[w] * exp(static_cast<double>(wave_top[w]) - static_cast<double>(most));
-        }
-        args.most[blockIdx.x] = most;
-        args.sum[blockIdx.x] = sum;
-    }
-}
+// e^v / 2^whole for floats of which the largest is about whole ln 2 (-65536 for
+// those below). In 64 bits, since the sums' logarithms decide between beams: v log2 e
+// = n + r with |r| <= 1/2 by two fused products, 2^r by the polynomial of degree 7
+// that is nearest on that interval (2^-34.5 of it; solved for by exchange), n - whole
+// added to its exponent. Values more than 1000 powers of two below count as 2^-1000.
+constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
+constexpr float kFar = 65536.0f;
 
-struct Candidate {
-    double rank;
-    uint64_t key;   // its logit's key, then ~token; 0: none
-    uint32_t beam;
+struct Exponentials {
+    static constexpr double kRound = 6755399441055744.0;  // 1.5 2^52
+    double rounding;
+    float least;
+
+    // From here on for `top`; returns whole before - whole now.
+    __device__ __forceinline__ int32_t raise(float top) {
+        const double whole = rint(static_cast<double>(fmaxf(top, -kFar)) * kLog2e), before = rounding;
+        rounding = kRound - whole;
+        least = static_cast<float>((whole - 1000.0) * kLn2);
+        return static_cast<int32_t>(rounding - before);
+    }
+    __device__ __forceinline__ double of(float v) const {
+        const double x = static_cast<double>(larger(v, least));
+        const double moved = fma(x, kLog2e, rounding);
+        const double r = fma(x, kLog2e, -(moved - rounding));
+        double p = fma(r, 1.520192398382284e-05, 0.00015469291034881546);
+        p = fma(r, p, 0.0013333922552474853);
+        p = fma(r, p, 0.0096180272541093615);
+        p = fma(r, p, 0.055504103534627078);
+        p = fma(r, p, 0.24022651198153328);
+        p = fma(r, p, 0.6931471807284425);
+        p = fma(r, p, 0.99999999996168243);
+        u32x2 bits = __builtin_bit_cast(u32x2, p);
+        bits[1] += __builtin_bit_cast(u32x2, moved)[0] << 20;
+        return __builtin_bit_cast(double, bits);
+    }
 };
 
-// The order of candidates: rank, then the lower beam, then the larger logit, then
-// the lower token.
-__device__ __forceinline__ bool precedes(const Candidate &a, const Candidate &b) {
-    return a.rank != b.rank ? a.rank > b.rank : a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
+// What a part's sum is to be multiplied by, as a logarithm (beam_part).
+__device__ __forceinline__ double reference_of(float top) {
+    return fabsf(top) < kFar ? rint(static_cast<double>(top) * kLog2e) * kLn2 : static_cast<double>(top);
 }
 
-// Joins a request's tiles.
-__global__ __launch_bounds__(kThreads) void k_beam_join(BeamArgs args) {
-    constexpr uint32_t kList = 1024;
-    __shared__ double lse[kMaxBeams], score[kMaxBeams], weight[kMaxBeams];
-    __shared__ uint32_t kind[kMaxBeams];  // 0: no candidates, 1: its logits', 2: ended
-    __shared__ Candidate list[kList];
-    __shared__ Candidate taken[kMaxChoices];
-    __shared__ uint32_t listed, bad, bound[kWaves];
-    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t / kWave, request = blockIdx.x;
-    const uint32_t k = args.beams, choices = args.choices, of_beam = args.parts * choices;
+using adi_hip::coherent_load;
+using adi_hip::coherent_store;
+__device__ __forceinline__ uint64_t coherent_load(const uint64_t *p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double coherent_load(const double *p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void coherent_store(uint64_t *p, uint64_t v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void coherent_store(double *p, double v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A candidate in the order of candidates: the larger rank (as a whole number), then
+// the larger tie: the lower beam, then the larger logit, then the lower token.
+// A rank of 0 is no candidate's (it would be a NaN's).
+struct Candidate {
+    uint64_t rank, tie;
+};
+__device__ __forceinline__ bool precedes(const Candidate &a, const Candidate &b) {
+    return a.rank > b.rank || (a.rank == b.rank && a.tie > b.tie);
+}
+__device__ __forceinline__ Candidate choose(bool first, const Candidate &a, const Candidate &b) {
+    return Candidate{first ? a.rank : b.rank, first ? a.tie : b.tie};
+}
+__device__ __forceinline__ uint64_t ascending_key(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v + 0.0);
+    return bits ^ (bits >> 63 != 0u ? ~0ull : 1ull << 63);
+}
+constexpr uint32_t kTokenBits = 24;
+__device__ __forceinline__ uint64_t tie_of(uint32_t beam, uint64_t key) {
+    return static_cast<uint64_t>(kMaxBeams - 1u - beam) << 56 | key >> 32 << kTokenBits |
+           (key & ((1u << kTokenBits) - 1u));
+}
+
+constexpr uint32_t kJoinList = 512;
+
+struct JoinShared {
+    double lse[kMaxBeams], score[kMaxBeams], weight[kMaxBeams];
+    uint32_t kind[kMaxBeams];  // 0: no candidates, 1: its logits', 2: ended
+    uint64_t rank[kJoinList], tie[kJoinList];
+    uint64_t taken[kMaxChoices];  // ties
+    alignas(16) uint32_t keys[kThreads];
+    uint32_t listed, bad;
+};
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, uint32_t lane) {
+    const u32x2 bits = __builtin_bit_cast(u32x2, v);
+    const u32x2 of = {static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits[0]), static_cast<int>(lane))),
+                      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits[1]), static_cast<int>(lane)))};
+    return __builtin_bit_cast(uint64_t, of);
+}
+
+// Joins a request's parts: the beams' logarithms, 64 / `group` beams a wave, then the
+// candidates. The heads of the parts' lists (all candidates, where the lists are few)
+// bound what is taken from below, and of each list what reaches that bound goes to
+// a list in LDS, whose entries find their places by counting.
+__device__ __forceinline__ void join_request(const BeamArgs &args, uint32_t request, JoinShared &lds) {
+    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t / kWave;
+    const uint32_t k = args.beams, choices = args.choices, parts = args.parts;
+    const uint64_t *const best = args.best + static_cast<uint64_t>(request) * k * parts * choices;
+    // items: the lists, or their candidates one by one; then the ended beams
+    const uint32_t depth = k * parts >= 4u * choices ? choices : 1u;
+    const uint32_t of_beam = parts * (choices / depth), items = k * of_beam;
+    // (on its way while the logarithms are made)
+    const uint64_t head = t < items ? coherent_load(best + static_cast<uint64_t>(t) * depth) : 0u;
     if (t == 0u) {
-        listed = 0u;
-        bad = 0u;
+        lds.listed = 0u;
+        lds.bad = 0u;
     }
-    for (uint32_t i = t; i < choices; i += kThreads) {
-        taken[i].key = 0u;
-        taken[i].beam = kNone;
+    if (t < choices) {
+        lds.taken[t] = 0u;
     }
     __syncthreads();
-    for (uint32_t b = wave; b < k; b += kWaves) {
-        const uint32_t row = request * k + b;
+    // lanes of a beam: the power of two from the parts on, at most a wave
+    const uint32_t group = min(1u << (32u - static_cast<uint32_t>(__builtin_clz(2u * parts - 1u)) - 1u), kWave);
+    for (uint32_t base = wave * (kWave / group); base < k; base += kWaves * (kWave / group)) {
+        const uint32_t b = base + lane / group, within = lane % group;
+        const uint32_t row = request * k + min(b, k - 1u);
+        const float *const most = args.most + static_cast<uint64_t>(row) * parts;
+        const double *const sum = args.sum + static_cast<uint64_t>(row) * parts;
+        // (its last part again, where a lane has none)
         const float s = args.scores[row], w = args.weights != nullptr ? args.weights[row] : 1.0f;
-        uint32_t what = s == -__builtin_huge_valf() ? 0u : args.ended != nullptr && args.ended[row] != 0u ? 2u : 1u;
+        const uint32_t gone = args.ended != nullptr ? args.ended[row] : 0u;
+        const float first_most = coherent_load(most + min(within, parts - 1u));
+        const double first_sum = coherent_load(sum + min(within, parts - 1u));
+        uint32_t what = b >= k || s == -__builtin_huge_valf() ? 0u : gone != 0u ? 2u : 1u;
         bool wrong = what != 0u && !(__builtin_isfinite(s) && w > 0.0f && __builtin_isfinite(w));
-        double normal = 0.0;
-        if (what == 1u) {
-            const float *const most = args.most + static_cast<uint64_t>(row) * args.parts;
-            const double *const sum = args.sum + static_cast<uint64_t>(row) * args.parts;
-            float top = -__builtin_huge_valf();
-            for (uint32_t p = lane; p < args.parts; p += kWave) {
-                top = fmaxf(top, most[p]);
-            }
-            top = wave_most(top);
-            double total = 0.0;
-            for (uint32_t p = lane; p < args.parts; p += kWave) {
-                total += most[p] == -__builtin_huge_valf()
-                             ? sum[p]
-                             : sum[p] * exp(static_cast<double>(most[p]) - static_cast<double>(top));
-            }
-            total = wave_sum(total);
-            // a NaN or +infinity among the logits leaves a NaN in the sum
-            wrong = wrong || total != total;
-            what = top == -__builtin_huge_valf() ? 0u : what;
-            normal = static_cast<double>(top) + log(total);
+        float top = first_most;
+        for (uint32_t p = within + group; p < parts; p += group) {
+            top = larger(top, coherent_load(most + p));
         }
-        if (lane == 0u) {
-            lse[b] = normal;
-            score[b] = s;
-            weight[b] = w;
-            kind[b] = what;
+        const auto over_group = [&](auto &&join) {
+            if (group > 1u) { join(std::integral_constant<int, 1>()); }
+            if (group > 2u) { join(std::integral_constant<int, 2>()); }
+            if (group > 4u) { join(std::integral_constant<int, 4>()); }
+            if (group > 8u) { join(std::integral_constant<int, 8>()); }
+            if (group > 16u) { join(std::integral_constant<int, 16>()); }
+            if (group > 32u) { join(std::integral_constant<int, 32>()); }
+        };
+        over_group([&](auto step) { top = larger(top, lane_xor<decltype(step)::value>(top)); });
+        const auto part = [&](float own, double value) {
+            return own == -__builtin_huge_valf() ? 0.0 : value * exp(reference_of(own) - static_cast<double>(top));
+        };
+        double total = within < parts ? part(first_most, first_sum) : 0.0;
+        for (uint32_t p = within + group; p < parts; p += group) {
+            total += part(coherent_load(most + p), coherent_load(sum + p));
+        }
+        over_group([&](auto step) { total += lane_xor<decltype(step)::value>(total); });
+        // a NaN or +infinity among the logits leaves a NaN in the sum
+        wrong = wrong || (what == 1u && total != total);
+        what = what == 1u && top == -__builtin_huge_valf() ? 0u : what;
+        if (within == 0u && b < k) {
+            lds.lse[b] = static_cast<double>(top) + log(total);
+            lds.score[b] = s;
+            lds.weight[b] = w;
+            lds.kind[b] = what;
             if (wrong) {
-                bad = 1u;
+                lds.bad = 1u;
             }
         }
     }
@@ -340,171 +341,475 @@ __global__ __launch_bounds__(kThreads) void k_beam_join(BeamArgs args) {
     float *const out_scores = args.out_scores + static_cast<uint64_t>(request) * choices;
     uint32_t *const parents = args.parents + static_cast<uint64_t>(request) * choices;
     uint32_t *const tokens = args.tokens + static_cast<uint64_t>(request) * choices;
-    if (bad != 0u) {
-        for (uint32_t i = t; i < choices; i += kThreads) {
-            out_scores[i] = __builtin_nanf("");
-            parents[i] = kNone;
-            tokens[i] = kNone;
+    if (lds.bad != 0u) {
+        if (t < choices) {
+            out_scores[t] = __builtin_nanf("");
+            parents[t] = kNone;
+            tokens[t] = kNone;
         }
         return;
     }
-    const uint64_t *const best = args.best + static_cast<uint64_t>(request) * k * of_beam;
-    // candidate i: of the tiles' lists, then one of each ended beam
-    const uint32_t candidates = k * of_beam + k;
-    const auto candidate = [&](uint32_t i) {
-        Candidate c{0.0, 0u, 0u};
-        if (i < k * of_beam) {
-            c.beam = i / of_beam;
-            if (kind[c.beam] == 1u) {
-                c.key = best[i];
-                const double logit = of_ascending_key(static_cast<uint32_t>(c.key >> 32));
-                c.rank = (score[c.beam] + (logit - lse[c.beam])) * weight[c.beam];
-            }
-        } else {
-            c.beam = i - k * of_beam;
-            if (kind[c.beam] == 2u) {
-                c.key = ~0ull;
-                c.rank = score[c.beam] * weight[c.beam];
-            }
+    const auto of_key = [&](uint32_t beam, uint64_t key) {
+        Candidate c{0u, 0u};
+        if (key != 0u && lds.kind[beam] == 1u) {
+            const double logit = of_ascending_key(static_cast<uint32_t>(key >> 32));
+            c.rank = ascending_key((lds.score[beam] + (logit - lds.lse[beam])) * lds.weight[beam]);
+            c.tie = tie_of(beam, key);
         }
         return c;
     };
-    // of the rank: ascending with it, equal for ranks next to each other
-    const auto coarse = [](const Candidate &c) {
-        const uint64_t bits = __builtin_bit_cast(uint64_t, c.rank + 0.0);
-        const uint32_t high = static_cast<uint32_t>(bits >> 32);
-        return c.key == 0u ? 0u : high ^ ((high & 0x80000000u) != 0u ? 0xFFFFFFFFu : 0x80000000u);
+    const auto ended = [&](uint32_t beam) {
+        Candidate c{0u, 0u};
+        if (lds.kind[beam] == 2u) {
+            c.rank = ascending_key(lds.score[beam] * lds.weight[beam]);
+            c.tie = tie_of(beam, ~0ull);
+        }
+        return c;
+    };
+    // item i's candidate j
+    const auto candidate = [&](uint32_t i, uint32_t j) {
+        Candidate c{0u, 0u};
+        if (i >= items) {
+            c = ended(i - items);
+        } else {
+            uint64_t key = head;
+            if (i != t || j != 0u) {
+                key = coherent_load(best + static_cast<uint64_t>(i) * depth + j);
+            }
+            c = of_key(i / of_beam, key);
+        }
+        return c;
     };
     uint32_t own = 0u;
-    for (uint32_t i = t; i < candidates; i += kThreads) {
-        own = max(own, coarse(candidate(i)));
+    for (uint32_t i = t; i < items + k; i += kThreads) {
+        own = max(own, static_cast<uint32_t>(candidate(i, 0u).rank >> 32));
     }
-    const uint32_t reached = reached_by(own, (choices + kWaves - 1u) / kWaves);
-    if (lane == 0u) {
-        bound[wave] = reached;
-    }
+    lds.keys[t] = own;
     __syncthreads();
-    const uint32_t least = max(min(min(bound[0], bound[1]), min(bound[2], bound[3])), 1u);
-    for (uint32_t i = t; i < candidates; i += kThreads) {
-        const Candidate c = candidate(i);
-        if (coarse(c) >= least) {
-            const uint32_t at = atomicAdd(&listed, 1u);
-            if (at < kList) {
-                list[at] = c;
+    const u32x4 four = *reinterpret_cast<const u32x4 *>(lds.keys + 4u * lane);
+    uint32_t least = 0u;
+#pragma unroll 4
+    for (uint32_t bit = 0x80000000u; bit != 0x80u; bit >>= 1) {
+        const uint32_t more = least | bit;
+        const uint32_t reach =
+            static_cast<uint32_t>(__popcll(__ballot(four[0] >= more)) + __popcll(__ballot(four[1] >= more)) +
+                                  __popcll(__ballot(four[2] >= more)) + __popcll(__ballot(four[3] >= more)));
+        least = reach >= choices ? more : least;
+    }
+    least = max(least, 1u);
+    for (uint32_t i = t; i < items + k; i += kThreads) {
+        for (uint32_t j = 0; j < (i < items ? depth : 1u); ++j) {
+            const Candidate c = candidate(i, j);
+            if (static_cast<uint32_t>(c.rank >> 32) < least) {
+                break;
+            }
+            const uint32_t at = atomicAdd(&lds.listed, 1u);
+            if (at < kJoinList) {
+                lds.rank[at] = c.rank;
+                lds.tie[at] = c.tie;
             }
         }
     }
     __syncthreads();
-    const uint32_t entries = listed;
-    if (entries <= kList) {
-        for (uint32_t e = t; e < entries; e += kThreads) {
-            const Candidate c = list[e];
+    const uint32_t entries = lds.listed;
+    if (entries <= kJoinList) {
+        // (entries are read from lanes: read from LDS, each of them is a wait)
+        for (uint32_t e = t; e < (entries + 63u) / 64u * 64u; e += kThreads) {
+            const Candidate c{e < entries ? lds.rank[e] : 0u, e < entries ? lds.tie[e] : 0u};
             uint32_t before = 0u;
-            for (uint32_t o = 0; o < entries; ++o) {
-                before += precedes(list[o], c) ? 1u : 0u;
+            for (uint32_t from = 0; from < entries; from += kWave) {
+                const uint32_t held = min(entries - from, kWave);
+                const uint32_t at = min(from + lane, entries - 1u);
+                const Candidate h{lds.rank[at], lds.tie[at]};
+                for (uint32_t o = 0; o < held; ++o) {
+                    const Candidate other{read_lane(h.rank, o), read_lane(h.tie, o)};
+                    before += precedes(other, c) ? 1u : 0u;
+                }
             }
-            if (before < choices) {
-                taken[before] = c;
+            if (e < entries && before < choices) {
+                lds.taken[before] = c.tie;
             }
         }
     } else {
         // so many near each other: one after another
+        Candidate last{~0ull, ~0ull};
         for (uint32_t n = 0; n < choices; ++n) {
-            Candidate next{0.0, 0u, 0u};
-            for (uint32_t i = t; i < candidates; i += kThreads) {
-                const Candidate c = candidate(i);
-                if (c.key != 0u && (n == 0u || precedes(taken[n - 1u], c)) && (next.key == 0u || precedes(c, next))) {
-                    next = c;
-                }
-            }
-            list[t] = next;
-            __syncthreads();
-            if (t == 0u) {
-                for (uint32_t o = 1; o < kThreads; ++o) {
-                    if (list[o].key != 0u && (next.key == 0u || precedes(list[o], next))) {
-                        next = list[o];
+            Candidate next{0u, 0u};
+            for (uint32_t i = t; i < items + k; i += kThreads) {
+                for (uint32_t j = 0; j < (i < items ? depth : 1u); ++j) {
+                    const Candidate c = candidate(i, j);
+                    if (c.rank == 0u) {
+                        break;
                     }
-                }
-                if (next.key != 0u) {
-                    taken[n] = next;
+                    next = choose(precedes(last, c) && precedes(c, next), c, next);
                 }
             }
+            lds.rank[t] = next.rank;
+            lds.tie[t] = next.tie;
             __syncthreads();
-            if (taken[n].key == 0u) {
+            last = Candidate{0u, 0u};
+            for (uint32_t o = 0; o < kThreads; ++o) {
+                const Candidate c{lds.rank[o], lds.tie[o]};
+                last = choose(precedes(c, last), c, last);
+            }
+            if (t == 0u) {
+                lds.taken[n] = last.tie;
+            }
+            __syncthreads();
+            if (last.rank == 0u) {
                 break;
             }
         }
     }
     __syncthreads();
-    uint64_t children = 0u;  // beams with one
-    if (args.settle != 0u) {
-        for (uint32_t i = 0; i < choices; ++i) {
-            children |= taken[i].key != 0u ? 1ull << taken[i].beam : 0u;
-        }
-    }
-    for (uint32_t i = t; i < choices; i += kThreads) {
-        const Candidate c = taken[i];
-        uint32_t place = i;
+    if (t < choices) {
+        const uint64_t tie = lds.taken[t];
+        const bool some = tie != 0u;
+        const uint32_t beam = kMaxBeams - 1u - static_cast<uint32_t>(tie >> 56);
+        uint32_t place = t;
         if (args.settle != 0u) {
-            // the parent's row for its first child; the others' rows, and those of
-            // places without a candidate, are the rows without one, in turn
-            const auto is_first = [&](uint32_t n) {
-                bool first = taken[n].key != 0u;
-                for (uint32_t o = 0; o < n; ++o) {
-                    first = first && taken[o].beam != taken[n].beam;
-                }
-                return first;
-            };
-            if (is_first(i)) {
-                place = c.beam;
-            } else {
-                uint32_t nth = 0u;
-                for (uint32_t o = 0; o < i; ++o) {
-                    nth += is_first(o) ? 0u : 1u;
-                }
-                uint64_t rows = ~children;
-                for (; nth != 0u; --nth) {
-                    rows &= rows - 1u;
-                }
-                place = static_cast<uint32_t>(__builtin_ctzll(rows));
+            // (choices = beams <= 64: the lanes of the first wave.) The parent's row
+            // for its first child; the others' rows, and those of places without a
+            // candidate, are the rows without one, in turn
+            bool first = some;
+            uint64_t children = 0u;
+            for (uint32_t o = 0; o < choices; ++o) {
+                const uint32_t parent = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(beam), static_cast<int>(o)));
+                const bool lives = __builtin_amdgcn_readlane(some ? 1 : 0, static_cast<int>(o)) != 0;
+                first = first && (o >= t || parent != beam);
+                children |= lives ? 1ull << parent : 0u;
             }
+            const uint64_t others = __ballot(!first) & ((1ull << t) - 1u);
+            uint64_t rows = ~children;
+            for (uint32_t nth = static_cast<uint32_t>(__popcll(others)); nth != 0u; --nth) {
+                rows &= rows - 1u;
+            }
+            place = first ? beam : static_cast<uint32_t>(__builtin_ctzll(rows | 1ull << 63));
         }
-        const bool some = c.key != 0u;
-        const double logit = of_ascending_key(static_cast<uint32_t>(c.key >> 32));
         double value = -__builtin_huge_val();
-        if (some) {
-            value = kind[c.beam] == 2u ? score[c.beam] : score[c.beam] + (logit - lse[c.beam]);
+        uint32_t token = kNone;
+        if (some && lds.kind[beam] == 2u) {
+            value = lds.score[beam];
+            token = args.ended_token;
+        } else if (some) {
+            value = lds.score[beam] + (of_ascending_key(static_cast<uint32_t>(tie >> kTokenBits)) - lds.lse[beam]);
+            token = ~static_cast<uint32_t>(tie) & ((1u << kTokenBits) - 1u);
         }
         out_scores[place] = static_cast<float>(value);
-        parents[place] = some ? c.beam : kNone;
-        tokens[place] = !some ? kNone : kind[c.beam] == 2u ? args.ended_token : ~static_cast<uint32_t>(c.key);
+        parents[place] = some ? beam : kNone;
+        tokens[place] = token;
     }
 }
 
+// The next float below a key's (the key below that of 0 is that of -0, which is
+// not below 0).
+__device__ __forceinline__ float below(uint32_t key) {
+    return of_ascending_key(key - (key == 0x80000000u ? 2u : 1u));
+}
+
+// The best of a wave's part so far, in LDS: keys as Candidate's. `edge`: a logit is
+// among the best only if it is larger.
+constexpr uint32_t kPartList = 256;
+
+__device__ __forceinline__ void wave_lds() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// Keeps the `choices` first of the list's entries, in order: an entry's place is
+// the number of entries before it. (Entries are held by lanes and read from
+// there: read from LDS, each of them is a wait.)
+__device__ __forceinline__ void keep_best(uint64_t *list, uint32_t &entries, uint32_t choices, uint32_t lane) {
+    constexpr uint32_t kHeld = kPartList / kWave;
+    wave_lds();
+    uint64_t own[kHeld];
+    uint32_t before[kHeld];
+#pragma unroll
+    for (uint32_t q = 0; q < kHeld; ++q) {
+        own[q] = q * kWave + lane < entries ? list[q * kWave + lane] : 0u;
+        before[q] = 0u;
+    }
+    if (entries <= kWave) {
+        for (uint32_t o = 0; o < entries; ++o) {
+            before[0] += read_lane(own[0], o) > own[0] ? 1u : 0u;
+        }
+    } else {
+#pragma unroll
+        for (uint32_t p = 0; p < kHeld; ++p) {
+            const uint32_t held = entries > p * kWave ? min(entries - p * kWave, kWave) : 0u;
+#pragma unroll 1
+            for (uint32_t o = 0; o < held; ++o) {
+                const uint64_t other = read_lane(own[p], o);
+#pragma unroll
+                for (uint32_t q = 0; q < kHeld; ++q) {
+                    before[q] += other > own[q] ? 1u : 0u;
+                }
+            }
+        }
+    }
+    wave_lds();
+#pragma unroll
+    for (uint32_t q = 0; q < kHeld; ++q) {
+        if (q * kWave + lane < entries && before[q] < choices) {
+            list[before[q]] = own[q];
+        }
+    }
+    entries = min(entries, choices);
+    wave_lds();
+}
+
+// Drops entries from a list of up to 64 that are not among its `choices` best: those
+// below the key of 16 bits that `choices` of them reach, which is returned. Not all
+// of them and in no order, but in a sixth of keep_best's instructions.
+__device__ __forceinline__ uint32_t trim(uint64_t *list, uint32_t &entries, uint32_t choices, uint32_t lane) {
+    wave_lds();
+    const uint64_t own = lane < entries ? list[lane] : 0u;
+    const uint32_t key = static_cast<uint32_t>(own >> 32), reached = reached_by(key, 0u, choices);
+    const uint64_t stays = __ballot(key >= reached && lane < entries);
+    wave_lds();
+    if (key >= reached && lane < entries) {
+        list[__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(stays >> 32),
+                                       __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(stays), 0u))] = own;
+    }
+    entries = static_cast<uint32_t>(__popcll(stays));
+    wave_lds();
+    return reached;
+}
+
+// A wave's part of a row: tiles of 64 x N logits, each held in registers, the next on
+// its way. A lane adds up its own exponentials, in powers of two below its own
+// largest logit so far. The best: in a first tile, the `choices` best of the lanes'
+// own two largest (of their pieces' halves) bound what is taken from below, later the
+// last of those taken so far, so that `choices` / m are taken of tile m, about.
+template <typename T, uint32_t N>
+__device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, uint32_t row, const char *from,
+                                          uint64_t *list) {
+    constexpr uint32_t kCount = Piece<T>::kCount, kPieces = N / kCount, kTile = kWave * N;
+    const uint32_t lane = threadIdx.x & 63u, choices = args.choices;
+    const uint32_t first = part * args.span, end = min(first + args.span, args.vocabulary);
+    uint32_t entries = 0u;
+    uint64_t least = 0u;  // keys above it are taken
+    float edge = -__builtin_huge_valf(), top = -__builtin_huge_valf();
+    Exponentials e;
+    e.rounding = Exponentials::kRound;
+    (void)e.raise(-kFar);
+    double total = 0.0;
+    const auto load = [&](Piece<T> (&x)[kPieces], uint32_t at) {
+        const char *const tile = from + static_cast<uint64_t>(at) * sizeof(T);
+        if (end - at >= kTile) {
+            load_tile(x, tile, lane);
+        } else {
+            load_last(x, tile, lane, end - at);
+        }
+    };
+    Piece<T> next[kPieces];
+    load(next, first);
+#pragma unroll 1
+    for (uint32_t at = first; at < end; at += kTile) {
+        Piece<T> x[kPieces];
+#pragma unroll
+        for (uint32_t j = 0; j < kPieces; ++j) {
+            x[j] = next[j];
+        }
+        if (end - at > kTile) {
+            load(next, at + kTile);
+        }
+        float half[2] = {-__builtin_huge_valf(), -__builtin_huge_valf()};
+#pragma unroll
+        for (uint32_t j = 0; j < kPieces; ++j) {
+#pragma unroll
+            for (uint32_t i = 0; i < kCount; i += 2u) {
+                float &own = half[(j * kCount + i) * 2u / N];
+                own = larger(own, larger(x[j].get(i), x[j].get(i + 1u)));
+            }
+        }
+        const float own = larger(half[0], half[1]);
+        top = larger(top, own);
+        total = ldexp(total, e.raise(top));
+        if (entries < choices) {
+            const uint32_t reached =
+                max(reached_by(ascending_key(half[0]), ascending_key(half[1]), choices), kLowestKey + 1u);
+            least = static_cast<uint64_t>(reached) << 32;
+            edge = below(reached);
+        }
+        if (__ballot(own > edge) != 0u) {
+            const uint32_t held = entries;
+#pragma unroll
+            for (uint32_t j = 0; j < kPieces; ++j) {
+#pragma unroll
+                for (uint32_t i = 0; i < kCount; ++i) {
+                    const float v = x[j].get(i);
+                    const uint64_t takes = __ballot(v > edge);
+                    if (takes != 0u) {
+                        const uint32_t place =
+                            entries + __builtin_amdgcn_mbcnt_hi(
+                                          static_cast<uint32_t>(takes >> 32),
+                                          __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(takes), 0u));
+                        if (v > edge && place < kPartList) {
+                            list[place] = static_cast<uint64_t>(ascending_key(v)) << 32 |
+                                          static_cast<uint32_t>(~(at + (j * kWave + lane) * kCount + i));
+                        }
+                        entries += static_cast<uint32_t>(__popcll(takes));
+                    }
+                }
+            }
+            if (entries > kPartList) {
+                // more than the list holds (many equal ones, or all in few lanes): again
+                // lane by lane, read from memory, with only the best kept
+                entries = held;
+                for (uint64_t holders = __ballot(own > edge); holders != 0u; holders &= holders - 1u) {
+                    const uint32_t i = lane % N, holder = static_cast<uint32_t>(__builtin_ctzll(holders));
+                    const uint32_t place = at + (i / kCount * kWave + holder) * kCount + i % kCount;
+                    float v = -__builtin_huge_valf();
+                    if (lane < N && place < end) {
+                        v = static_cast<float>(reinterpret_cast<const T *>(from)[place]);
+                    }
+                    const uint64_t key = static_cast<uint64_t>(ascending_key(v)) << 32 | static_cast<uint32_t>(~place);
+                    const bool takes = v > -__builtin_huge_valf() && key > least;
+                    const uint64_t taken = __ballot(takes);
+                    if (takes) {
+                        list[entries + __builtin_amdgcn_mbcnt_hi(
+                                           static_cast<uint32_t>(taken >> 32),
+                                           __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(taken), 0u))] = key;
+                    }
+                    entries += static_cast<uint32_t>(__popcll(taken));
+                    if (entries > kPartList - kWave) {
+                        keep_best(list, entries, choices, lane);
+                        least = entries == choices ? list[choices - 1u] : least;
+                    }
+                }
+            }
+            if (end - at > kTile && entries >= choices + choices / 2u + 4u) {
+                if (entries <= kWave) {
+                    const uint32_t reached = trim(list, entries, choices, lane);
+                    least = max(least, static_cast<uint64_t>(reached) << 32);
+                    edge = fmaxf(edge, below(reached));
+                } else {
+                    keep_best(list, entries, choices, lane);
+                    least = list[choices - 1u];
+                    edge = of_ascending_key(static_cast<uint32_t>(least >> 32));
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kPieces; ++j) {
+#pragma unroll
+            for (uint32_t i = 0; i < kCount; ++i) {
+                total += e.of(x[j].get(i));
+            }
+        }
+    }
+    const float most = wave_most(top);
+    if (fabsf(most) < kFar) {
+        Exponentials whole;
+        whole.rounding = e.rounding;
+        total = ldexp(total, whole.raise(most));
+    } else {
+        // too far from 0 for that, or a NaN or an infinity, which give a NaN
+        total = 0.0;
+        if (most != -__builtin_huge_valf()) {
+#pragma unroll 1
+            for (uint32_t at = first + lane; at < end; at += kWave) {
+                total += exp(static_cast<double>(static_cast<float>(reinterpret_cast<const T *>(from)[at])) -
+                             static_cast<double>(most));
+            }
+        }
+    }
+    total = wave_sum(total);
+    keep_best(list, entries, choices, lane);
+    const uint64_t place = static_cast<uint64_t>(row) * args.parts + part;
+    for (uint32_t i = lane; i < choices; i += kWave) {
+        coherent_store(args.best + place * choices + i, i < entries ? list[i] : uint64_t(0));
+    }
+    if (lane == 0u) {
+        coherent_store(args.most + place, most);
+        coherent_store(args.sum + place, total);
+    }
+}
+
+// A wave a part; where the launch joins, the last block of a request's through its
+// ticket does.
+// (Waves a SIMD that the registers are held to: bf16 rows fit in five without
+// spills, 512 rows of 248,320 115 us in place of 125; f32 and f16 rows spill.)
 template <typename T>
-void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const adi_hip_paged_workspace &workspace) {
-    constexpr uint32_t N = 32;
-    BeamArgs args{static_cast<const char *>(a.logits), a.request_stride, a.beam_stride, a.beams, a.vocabulary,
-                  a.choices, ceil_div(a.vocabulary, kThreads * N), a.scores, a.weights, a.ended, a.ended_token, a.settle,
-                  a.out_scores, a.parents, a.tokens, nullptr, nullptr, nullptr};
+constexpr int kResident = std::is_same_v<T, __bf16> ? 5 : 4;
+
+template <typename T, uint32_t N, bool JOINS>
+__global__ __launch_bounds__(kThreads, kResident<T>) void k_beam_select(BeamArgs args) {
+    __shared__ union Shared {
+        uint64_t list[kWaves][kPartList];
+        std::conditional_t<JOINS, JoinShared, uint32_t> join;
+    } lds;
+    __shared__ uint32_t last;
+    const uint32_t row = blockIdx.z * args.beams + blockIdx.y;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), part = blockIdx.x * kWaves + wave;
+    if (part < args.parts && args.scores[row] != -__builtin_huge_valf() &&
+        (args.ended == nullptr || args.ended[row] == 0u)) {
+        const char *const from =
+            args.logits + (blockIdx.z * args.request_stride + blockIdx.y * args.beam_stride) * sizeof(T);
+        beam_part<T, N>(args, part, row, from, lds.list[wave]);
+    }
+    if constexpr (JOINS) {
+        wait_stores();
+        __syncthreads();
+        if (threadIdx.x == 0u) {
+            uint32_t *const ticket = args.tickets + blockIdx.z;
+            last = coherent_add(ticket, 1u) + 1u == args.arrivals ? 1u : 0u;
+            if (last != 0u) {
+                coherent_store(ticket, 0u);
+            }
+        }
+        __syncthreads();
+        if (last != 0u) {
+            join_request(args, blockIdx.z, lds.join);
+        }
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void k_beam_join(BeamArgs args) {
+    __shared__ JoinShared lds;
+    join_request(args, blockIdx.x, lds);
+}
+
+template <typename T, uint32_t N, bool JOINS>
+void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const adi_hip_paged_workspace &workspace,
+                   uint32_t tiles) {
+    BeamArgs args{};
+    args.logits = static_cast<const char *>(a.logits);
+    args.request_stride = a.request_stride;
+    args.beam_stride = a.beam_stride;
+    args.beams = a.beams;
+    args.vocabulary = a.vocabulary;
+    args.choices = a.choices;
+    args.span = tiles * kWave * N;
+    args.parts = ceil_div(a.vocabulary, args.span);
+    args.arrivals = ceil_div(args.parts, kWaves) * a.beams;
+    args.scores = a.scores;
+    args.weights = a.weights;
+    args.ended = a.ended;
+    args.ended_token = a.ended_token;
+    args.settle = a.settle;
+    args.out_scores = a.out_scores;
+    args.parents = a.parents;
+    args.tokens = a.tokens;
+    args.tickets = static_cast<uint32_t *>(workspace.base);
     // as many requests at once as the workspace holds
-    const uint64_t tiles = uint64_t(a.beams) * args.parts;
-    const uint64_t bytes = tiles * (sizeof(double) + sizeof(uint64_t) * a.choices + sizeof(float));
+    const uint64_t parts = uint64_t(a.beams) * args.parts;
+    const uint64_t bytes = parts * (sizeof(double) + sizeof(uint64_t) * a.choices + sizeof(float));
     const uint64_t room = workspace.bytes - kTickets * sizeof(uint32_t);
-    const uint64_t at_once = std::min<uint64_t>({room / bytes, a.requests, (1u << 23) / tiles});
+    const uint64_t at_once = std::min<uint64_t>({room / bytes, a.requests, (1u << 23) / parts, kTickets - 1u});
     if (at_once == 0) {
         fail(ADI_HIP_OUT_OF_MEMORY, "beam select: a request needs a workspace of " +
                                         std::to_string(bytes + kTickets * sizeof(uint32_t)) + " bytes");
     }
     char *const base = static_cast<char *>(workspace.base) + kTickets * sizeof(uint32_t);
     args.sum = reinterpret_cast<double *>(base);
-    args.best = reinterpret_cast<uint64_t *>(args.sum + at_once * tiles);
-    args.most = reinterpret_cast<float *>(args.best + at_once * tiles * a.choices);
+    args.best = reinterpret_cast<uint64_t *>(args.sum + at_once * parts);
+    args.most = reinterpret_cast<float *>(args.best + at_once * parts * a.choices);
     for (uint64_t done = 0; done < a.requests; done += at_once) {
         const uint32_t requests = static_cast<uint32_t>(std::min<uint64_t>(at_once, a.requests - done));
-        launch(ctx, "beam_tiles", k_beam_tiles<T, N>, dim3(static_cast<uint32_t>(requests * tiles)), dim3(kThreads), 0,
-               args);
-        launch(ctx, "beam_join", k_beam_join, dim3(requests), dim3(kThreads), 0, args);
+        const dim3 grid(ceil_div(args.parts, kWaves), a.beams, requests), block(kThreads);
+        launch(ctx, "beam_select", k_beam_select<T, N, JOINS>, grid, block, 0, args);
+        if (!JOINS) {
+            launch(ctx, "beam_join", k_beam_join, dim3(requests), block, 0, args);
+        }
         args.logits += requests * args.request_stride * sizeof(T);
         args.scores += requests * a.beams;
         args.weights += args.weights != nullptr ? requests * a.beams : 0;
@@ -512,6 +817,33 @@ void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const 
         args.out_scores += requests * a.choices;
         args.parents += requests * a.choices;
         args.tokens += requests * a.choices;
+    }
+}
+
+// Tiles of 512 logits where that makes at most a wave a CU, else of 2048, and as
+// many a part as leave 32 waves a CU, about (one request of 4 x 248,320 f32 logits:
+// 14.4 us, with tiles of 1024 and 512 16.4 and 23.6, as more parts are joined; of 4 x
+// 32,000 in 512s 10.5, in 1024s 11.2). Up to half a block a CU joins within the
+// launch (4 x 512 logits: 8.4 us, with a launch of its own 9.4); more blocks wait
+// for each other at the tickets (16 requests of 4 x 248,320: 28.3 us, and 25.3).
+template <typename T>
+void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const adi_hip_paged_workspace &workspace) {
+    const uint64_t rows = uint64_t(a.requests) * a.beams, cus = static_cast<uint64_t>(ctx->cu_count);
+    const auto go = [&](auto n) {
+        constexpr uint32_t N = decltype(n)::value;
+        const uint64_t waves = rows * ceil_div(a.vocabulary, kWave * N);
+        const uint32_t tiles = static_cast<uint32_t>(std::clamp<uint64_t>(waves / (32u * cus), 1u, 16u));
+        const uint64_t blocks = rows * ceil_div(ceil_div(a.vocabulary, kWave * N * tiles), kWaves);
+        if (blocks <= cus / 2u) {
+            launch_select<T, N, true>(ctx, a, workspace, tiles);
+        } else {
+            launch_select<T, N, false>(ctx, a, workspace, tiles);
+        }
+    };
+    if (rows * ceil_div(a.vocabulary, kWave * 8u) <= cus) {
+        go(std::integral_constant<uint32_t, 8>());
+    } else {
+        go(std::integral_constant<uint32_t, 32>());
     }
 }
 
