@@ -876,10 +876,10 @@ constexpr uint32_t kArrays = 64;  // of a launch
 struct RowArray {
     char *data;
     uint64_t request_stride, row_stride;  // bytes
-    uint64_t row_units;
+    uint64_t units;        // of 16 bytes in a row
     uint64_t first_block;  // of the array's
     uint32_t blocks;       // of a request
-    uint32_t unit;         // bytes
+    uint32_t tail;         // bytes behind them
 };
 struct ReorderArgs {
     RowArray array[kArrays];
@@ -887,37 +887,24 @@ struct ReorderArgs {
     const uint32_t *parents;
 };
 
-// One unit of every row of a request a thread: the rows that others take are
-// loaded, then stored where they go, so no order of the moves matters, and what
-// stays is neither read nor written.
+typedef uint32_t loose_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
+
+// 16 bytes of every row of a request, at any address, or one of the bytes behind
+// them: the rows that others take are loaded, then stored where they go, so no order of
+// the moves matters, and what stays is neither read nor written.
 template <typename U, uint32_t K>
-__device__ __forceinline__ void reorder_units(const RowArray &array, uint32_t request, uint32_t block, uint32_t beams,
-                                              const uint32_t *parents) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t parent = lane < beams ? parents[static_cast<uint64_t>(request) * beams + lane] : kNone;
-    // of each row, the other rows that take it (uniform)
-    const bool moves = parent < beams && parent != lane;
-    uint64_t takers[K];
-#pragma unroll
-    for (uint32_t p = 0; p < K; ++p) {
-        takers[p] = __ballot(moves && parent == p);
-    }
-    const uint64_t unit = static_cast<uint64_t>(block) * kThreads + threadIdx.x;
-    if (unit >= array.row_units) {
-        return;
-    }
-    char *const base = array.data + request * array.request_stride + unit * sizeof(U);
+__device__ __forceinline__ void reorder_unit(char *base, uint64_t row_stride, const uint64_t (&takers)[K]) {
     U v[K];
 #pragma unroll
     for (uint32_t p = 0; p < K; ++p) {
         if (takers[p] != 0u) {
-            v[p] = *reinterpret_cast<const U *>(base + p * array.row_stride);
+            v[p] = *reinterpret_cast<const U *>(base + p * row_stride);
         }
     }
 #pragma unroll
     for (uint32_t p = 0; p < K; ++p) {
         for (uint64_t left = takers[p]; left != 0u; left &= left - 1u) {
-            *reinterpret_cast<U *>(base + static_cast<uint32_t>(__builtin_ctzll(left)) * array.row_stride) = v[p];
+            *reinterpret_cast<U *>(base + static_cast<uint32_t>(__builtin_ctzll(left)) * row_stride) = v[p];
         }
     }
 }
@@ -931,12 +918,21 @@ __global__ __launch_bounds__(kThreads) void k_reorder_rows(ReorderArgs args) {
     const RowArray &array = args.array[n];
     const uint32_t at = static_cast<uint32_t>(blockIdx.x - array.first_block);
     const uint32_t request = at / array.blocks, block = at % array.blocks;
-    if (array.unit == 16u) {
-        reorder_units<u32x4, K>(array, request, block, args.beams, args.parents);
-    } else if (array.unit == 4u) {
-        reorder_units<uint32_t, K>(array, request, block, args.beams, args.parents);
-    } else {
-        reorder_units<uint8_t, K>(array, request, block, args.beams, args.parents);
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t parent = lane < args.beams ? args.parents[static_cast<uint64_t>(request) * args.beams + lane] : kNone;
+    // of each row, the other rows that take it (uniform)
+    const bool moves = parent < args.beams && parent != lane;
+    uint64_t takers[K];
+#pragma unroll
+    for (uint32_t p = 0; p < K; ++p) {
+        takers[p] = __ballot(moves && parent == p);
+    }
+    const uint64_t unit = static_cast<uint64_t>(block) * kThreads + threadIdx.x;
+    char *const base = array.data + request * array.request_stride;
+    if (unit < array.units) {
+        reorder_unit<loose_u32x4, K>(base + unit * 16u, array.row_stride, takers);
+    } else if (unit - array.units < array.tail) {
+        reorder_unit<uint8_t, K>(base + array.units * 16u + (unit - array.units), array.row_stride, takers);
     }
 }
 
@@ -990,11 +986,9 @@ void reorder_rows(adi_hip_context *ctx, const adi_hip_row_array *arrays, uint32_
         if (a.row_bytes == 0) {
             continue;
         }
-        const uint64_t all = reinterpret_cast<uintptr_t>(a.data) | a.row_stride | a.request_stride | a.row_bytes;
-        RowArray r{static_cast<char *>(a.data), a.request_stride, a.row_stride, 0, 0, 0, 0};
-        r.unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
-        r.row_units = a.row_bytes / r.unit;
-        const uint64_t per = (r.row_units + kThreads - 1) / kThreads;
+        RowArray r{static_cast<char *>(a.data), a.request_stride, a.row_stride, a.row_bytes / 16, 0, 0,
+                   static_cast<uint32_t>(a.row_bytes % 16)};
+        const uint64_t per = (r.units + r.tail + kThreads - 1) / kThreads;
         require(per * requests < (1u << 23), "reorder rows: too many rows of such a size");
         r.blocks = static_cast<uint32_t>(per);
         if (args.arrays == kArrays || blocks + per * requests >= (1u << 23)) {

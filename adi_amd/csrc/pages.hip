@@ -20,6 +20,9 @@ constexpr uint32_t kMaxPages = 1u << 22;
 // pages of a segment: what a block counts
 constexpr uint32_t kSegment = 2048, kSegments = kMaxPages / kSegment;
 constexpr uint32_t kOwn = kSegment / kThreads;  // pages of a thread
+// pools of which one block finds the free pages (fork), or every block counts all
+// live ones (compaction)
+constexpr uint32_t kSmallPages = 4096;
 
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 
@@ -31,7 +34,7 @@ using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 struct CachesView {
     char *data[2u * kCaches];  // keys, values, keys, ...
     uint64_t page_stride, entry_stride, head_stride;  // bytes
-    uint32_t arrays, heads, head_units, page_size, pages;
+    uint32_t arrays, heads, head_shift, page_size, pages;  // head_shift: log2 of a head's units
     uint32_t heads_first;
 };
 
@@ -50,7 +53,7 @@ CachesView caches_view(const adi_hip_paged_pool &pool, uint32_t first) {
     v.head_stride = c.head_stride * size;
     v.arrays = 2u * count;
     v.heads = c.heads;
-    v.head_units = c.head_size * size / 16u;
+    v.head_shift = log2_of(c.head_size * size / 16u);
     v.page_size = c.page_size;
     v.pages = c.pages;
     v.heads_first = c.entry_stride < c.head_stride ? 1u : 0u;
@@ -61,8 +64,8 @@ CachesView caches_view(const adi_hip_paged_pool &pool, uint32_t first) {
 // entry, or head by head where `heads_first` (the order of the copy's source).
 __device__ __forceinline__ uint64_t unit_at(const CachesView &v, uint32_t heads_first, uint32_t entries, uint32_t u) {
     const uint32_t run = heads_first != 0u ? entries : v.heads;
-    const uint32_t vector = u / v.head_units, d = u - vector * v.head_units;
-    const uint32_t outer = vector / run, inner = vector - outer * run;
+    const uint32_t vector = u >> v.head_shift, d = u - (vector << v.head_shift);
+    const uint32_t outer = run == 1u ? vector : vector / run, inner = vector - outer * run;
     return outer * (heads_first != 0u ? v.head_stride : v.entry_stride) +
            inner * (heads_first != 0u ? v.entry_stride : v.head_stride) + d * 16u;
 }
@@ -70,28 +73,36 @@ __device__ __forceinline__ uint64_t unit_at(const CachesView &v, uint32_t heads_
 // Units of a piece: what a block copies at once.
 constexpr uint32_t kAhead = 4, kPiece = kThreads * kAhead;
 
-// Piece `piece` of the first `entries` of a page of array n into another's.
-__device__ __forceinline__ void copy_piece(const CachesView &from, const CachesView &to, uint32_t n, uint32_t source,
-                                           uint32_t target, uint32_t entries, uint32_t piece) {
-    const uint32_t units = entries * from.heads * from.head_units;
-    const char *const a = from.data[n] + source * from.page_stride;
-    char *const b = to.data[n] + target * to.page_stride;
+// Piece `piece` of the first `entries` of a page of array n.
+struct PieceOfPage {
     u32x4 x[kAhead];
+
+    __device__ __forceinline__ void load(const CachesView &from, uint32_t n, uint32_t page, uint32_t entries,
+                                         uint32_t piece) {
+        const uint32_t units = entries * from.heads << from.head_shift;
+        const char *const a = from.data[n] + page * from.page_stride;
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) {
-        const uint32_t u = piece * kPiece + i * kThreads + threadIdx.x;
-        if (u < units) {
-            x[i] = *reinterpret_cast<const u32x4 *>(a + unit_at(from, from.heads_first, entries, u));
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t u = piece * kPiece + i * kThreads + threadIdx.x;
+            if (u < units) {
+                x[i] = *reinterpret_cast<const u32x4 *>(a + unit_at(from, from.heads_first, entries, u));
+            }
         }
     }
+    // (in the order of the source's)
+    __device__ __forceinline__ void store(const CachesView &from, const CachesView &to, uint32_t n, uint32_t page,
+                                          uint32_t entries, uint32_t piece) const {
+        const uint32_t units = entries * from.heads << from.head_shift;
+        char *const b = to.data[n] + page * to.page_stride;
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) {
-        const uint32_t u = piece * kPiece + i * kThreads + threadIdx.x;
-        if (u < units) {
-            *reinterpret_cast<u32x4 *>(b + unit_at(to, from.heads_first, entries, u)) = x[i];
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t u = piece * kPiece + i * kThreads + threadIdx.x;
+            if (u < units) {
+                *reinterpret_cast<u32x4 *>(b + unit_at(to, from.heads_first, entries, u)) = x[i];
+            }
         }
     }
-}
+};
 
 struct CopyArgs {
     CachesView from, to;
@@ -108,7 +119,9 @@ __global__ __launch_bounds__(kThreads) void k_paged_copy(CopyArgs args) {
         entries = min(entries, args.entries[i]);
     }
     if (source < args.from.pages && target < args.to.pages) {
-        copy_piece(args.from, args.to, n, source, target, entries, piece);
+        PieceOfPage x;
+        x.load(args.from, n, source, entries, piece);
+        x.store(args.from, args.to, n, target, entries, piece);
     }
 }
 
@@ -158,41 +171,65 @@ struct ForkArgs {
     uint32_t *lacking;
     // workspace
     RowPlan *plan;
-    uint32_t *free_count, *free_page;  // [segments], [segments][kSegment]
+    uint32_t *free_count, *free_page;  // [segments], [segments][kSegment]; in a small pool [1], [pages]
     uint32_t *demand;                  // of all rows
+    uint32_t small;
 };
 
 __device__ __forceinline__ uint32_t pages_of(uint32_t entries, uint32_t shift) {
     return (entries >> shift) + ((entries & ((1u << shift) - 1u)) != 0u ? 1u : 0u);
 }
 
-// The free pages of a segment a block, and the rows' plans by the last one.
+// The rows' plans by the first block. Of a small pool (kSmallPages) it counts the
+// free pages too, a run of them a thread, and lists the first of them, as many as
+// rows take; of others every block but the first lists a segment's. The others
+// copy the counts, where the new ones are apart from the old.
 __global__ __launch_bounds__(kThreads) void k_fork_plan(ForkArgs args) {
     __shared__ uint32_t sums[kWaves];
     const uint32_t t = threadIdx.x;
-    if (blockIdx.x < args.segments) {
-        const uint32_t first = blockIdx.x * kSegment + t * kOwn;
+    if (blockIdx.x != 0u) {
+        const uint32_t segment = blockIdx.x - 1u, first = segment * kSegment + t * kOwn;
         uint32_t count[kOwn], own = 0u;
 #pragma unroll
         for (uint32_t i = 0; i < kOwn; ++i) {
             count[i] = first + i < args.pages ? args.old_references[first + i] : 1u;
             own += count[i] == 0u ? 1u : 0u;
         }
+        if (args.references != args.old_references) {
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i) {
+                if (first + i < args.pages) {
+                    args.references[first + i] = count[i];
+                }
+            }
+        }
+        if (args.small != 0u) {
+            return;
+        }
         uint32_t all = 0u, at = block_before(own, sums, all);
-        uint32_t *const list = args.free_page + blockIdx.x * kSegment;
+        uint32_t *const list = args.free_page + segment * kSegment;
 #pragma unroll
         for (uint32_t i = 0; i < kOwn; ++i) {
             if (count[i] == 0u) {
                 list[at++] = first + i;
             }
-            if (args.references != args.old_references && first + i < args.pages) {
-                args.references[first + i] = count[i];
-            }
         }
         if (t == 0u) {
-            args.free_count[blockIdx.x] = all;
+            args.free_count[segment] = all;
         }
         return;
+    }
+    // (on its way while the rows are planned; a run past the pool's end has no free ones)
+    constexpr uint32_t kRun = kSmallPages / kThreads;
+    uint32_t count[kRun];
+    const uint32_t run = (args.pages + kThreads - 1u) / kThreads;
+    if (args.small != 0u) {
+#pragma unroll
+        for (uint32_t i = 0; i < kRun; ++i) {
+            if (i < run) {
+                count[i] = args.old_references[min(t * run + i, args.pages - 1u)];
+            }
+        }
     }
     const uint32_t page_mask = (1u << args.page_shift) - 1u;
     uint32_t taken = 0u;
@@ -237,43 +274,80 @@ __global__ __launch_bounds__(kThreads) void k_fork_plan(ForkArgs args) {
     if (t == 0u) {
         *args.demand = taken;
     }
-}
-
-// The free pages before every segment's, in LDS (`before`, kSegments + 1 words).
-__device__ __forceinline__ void segments_before(const uint32_t *count, uint32_t segments, uint32_t *before,
-                                                uint32_t *sums) {
-    uint32_t done = 0u;
-    for (uint32_t base = 0; base < segments; base += kThreads) {
-        const uint32_t s = base + threadIdx.x;
-        uint32_t all = 0u;
-        const uint32_t at = done + block_before(s < segments ? count[s] : 0u, sums, all);
-        if (s < segments) {
-            before[s] = at;
-        }
-        done += all;
+    if (args.small == 0u) {
+        return;
     }
-    if (threadIdx.x == 0u) {
-        before[segments] = done;
-    }
-    __syncthreads();
-}
-
-// The n-th free page, kNone where there are not as many.
-__device__ __forceinline__ uint32_t nth_free(const ForkArgs &args, const uint32_t *before, uint32_t n) {
-    if (n >= before[args.segments]) {
-        return kNone;
-    }
-    uint32_t low = 0u, high = args.segments;  // before[low] <= n < before[high]
-    while (high - low > 1u) {
-        const uint32_t middle = (low + high) / 2u;
-        if (before[middle] <= n) {
-            low = middle;
-        } else {
-            high = middle;
+    uint32_t own = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        if (i < run) {
+            count[i] = t * run + i < args.pages ? count[i] : 1u;
+            own += count[i] == 0u ? 1u : 0u;
         }
     }
-    return args.free_page[low * kSegment + (n - before[low])];
+    uint32_t all = 0u, at = block_before(own, sums, all);
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        if (i < run && count[i] == 0u) {
+            if (at < taken) {
+                args.free_page[at] = t * run + i;
+            }
+            ++at;
+        }
+    }
+    if (t == 0u) {
+        args.free_count[0] = all;
+    }
 }
+
+// A pool's free pages as a wave finds them: a lane counts those of a run of
+// segments, and knows the number up to its run's end.
+struct FreePages {
+    uint32_t up_to, run, all;
+
+    __device__ __forceinline__ explicit FreePages(const ForkArgs &args) {
+        const uint32_t lane = threadIdx.x & 63u;
+        if (args.small != 0u) {
+            run = 1u;
+            up_to = all = args.free_count[0];
+            return;
+        }
+        run = (args.segments + kWave - 1u) / kWave;
+        up_to = 0u;
+        for (uint32_t s = lane * run; s < min(lane * run + run, args.segments); ++s) {
+            up_to += args.free_count[s];
+        }
+#pragma unroll
+        for (uint32_t step = 1; step < kWave; step <<= 1) {
+            const uint32_t below = static_cast<uint32_t>(__shfl_up(static_cast<int>(up_to), step));
+            up_to += lane >= step ? below : 0u;
+        }
+        all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(up_to), kWave - 1));
+    }
+    // The n-th of them, kNone where there are not as many. Every lane is here.
+    __device__ __forceinline__ uint32_t nth(const ForkArgs &args, uint32_t n) const {
+        if (args.small != 0u) {
+            return n < all ? args.free_page[n] : kNone;
+        }
+        // the first lane whose run ends beyond it
+        uint32_t owner = 0u;
+#pragma unroll
+        for (uint32_t step = kWave / 2u; step != 0u; step >>= 1) {
+            const uint32_t end = static_cast<uint32_t>(__shfl(static_cast<int>(up_to), static_cast<int>(owner + step - 1u)));
+            owner += end <= n ? step : 0u;
+        }
+        const uint32_t before = static_cast<uint32_t>(__shfl(static_cast<int>(up_to), static_cast<int>(owner == 0u ? 0u : owner - 1u)));
+        if (n >= all) {
+            return kNone;
+        }
+        uint32_t left = n - (owner == 0u ? 0u : before), s = owner * run;
+        while (run > 1u && left >= args.free_count[s]) {
+            left -= args.free_count[s];
+            ++s;
+        }
+        return args.free_page[s * kSegment + left];
+    }
+};
 
 struct ForkCopyArgs {
     CachesView caches;
@@ -282,33 +356,33 @@ struct ForkCopyArgs {
 };
 
 // The tables, a column of a request's rows a thread (each entry is read before any
-// is written, so that the old table may be the new one), and the copies.
+// is written, so that the old table may be the new one), and the copies: what a
+// block copies is on its way before it knows where it goes.
 template <uint32_t K>
 __global__ __launch_bounds__(kThreads) void k_fork_apply(ForkArgs args, ForkCopyArgs copy) {
-    __shared__ uint32_t before[kSegments + 1u];
-    __shared__ uint32_t sums[kWaves];
     __shared__ RowPlan plans[K];
     const uint32_t t = threadIdx.x;
-    segments_before(args.free_count, args.segments, before, sums);
-    const uint32_t free = before[args.segments];
     if (blockIdx.x >= copy.table_blocks) {
         for (uint64_t w = blockIdx.x - copy.table_blocks; w < copy.work; w += gridDim.x - copy.table_blocks) {
             const uint32_t piece = static_cast<uint32_t>(w % copy.pieces);
             const uint64_t rest = w / copy.pieces;
             const uint32_t n = static_cast<uint32_t>(rest % copy.caches.arrays);
             const RowPlan plan = args.plan[rest / copy.caches.arrays];
+            const uint32_t entries = plan.parents & ((1u << args.page_shift) - 1u);
             if (plan.source != kNone) {
-                const uint32_t target = nth_free(args, before, plan.before);
+                PieceOfPage x;
+                x.load(copy.caches, n, plan.source, entries, piece);
+                const uint32_t target = FreePages(args).nth(args, plan.before);
                 if (target != kNone) {
-                    copy_piece(copy.caches, copy.caches, n, plan.source, target,
-                               plan.parents & ((1u << args.page_shift) - 1u), piece);
+                    x.store(copy.caches, copy.caches, n, target, entries, piece);
                 }
             }
         }
         return;
     }
+    const FreePages free(args);
     if (blockIdx.x == 0u && t == 0u && args.lacking != nullptr) {
-        *args.lacking = *args.demand > free ? *args.demand - free : 0u;
+        *args.lacking = *args.demand > free.all ? *args.demand - free.all : 0u;
     }
     const uint32_t group = blockIdx.x / copy.column_blocks * args.beams;
     const uint32_t c = blockIdx.x % copy.column_blocks * kThreads + t;
@@ -331,11 +405,17 @@ __global__ __launch_bounds__(kThreads) void k_fork_apply(ForkArgs args, ForkCopy
         const uint32_t end = static_cast<uint32_t>(
             min((static_cast<uint64_t>(plan.parents) + plan.added + (1u << args.page_shift) - 1u) >> args.page_shift,
                 static_cast<uint64_t>(args.stride)));
+        const bool copies = c < end && plan.source != kNone && c == plan.parents >> args.page_shift;
+        const bool takes = copies || (c < end && c >= held && plan.over == 0u);
+        uint32_t taken = kNone;
+        if (__ballot(takes) != 0u) {
+            const uint32_t n = plan.before + (copies ? 0u : c - held + (plan.source != kNone ? 1u : 0u));
+            taken = free.nth(args, takes ? n : kNone);
+        }
         if (c < end) {
-            const bool copies = plan.source != kNone && c == plan.parents >> args.page_shift;
             uint32_t page = kNone;
-            if (copies || (c >= held && plan.over == 0u)) {
-                page = nth_free(args, before, plan.before + (copies ? 0u : c - held + (plan.source != kNone ? 1u : 0u)));
+            if (takes) {
+                page = taken;
                 if (page != kNone) {
                     args.references[page] = 1u;
                 }
@@ -388,19 +468,14 @@ struct CompactArgs {
     uint32_t *moves;
 };
 
+// The free and live pages of long pools, a segment a block.
 __global__ __launch_bounds__(kThreads) void k_compact_count(CompactArgs args) {
     __shared__ uint32_t sums[kWaves];
     const uint32_t first = blockIdx.x * kSegment + threadIdx.x * kOwn;
     uint32_t own = 0u;
 #pragma unroll
     for (uint32_t i = 0; i < kOwn; ++i) {
-        if (first + i < args.pages) {
-            const uint32_t count = args.old_references[first + i];
-            own += count != 0u ? 1u : 0u;
-            if (args.references != args.old_references) {
-                args.references[first + i] = count;
-            }
-        }
+        own += first + i < args.pages && args.old_references[first + i] != 0u ? 1u : 0u;
     }
     uint32_t all = 0u;
     (void)block_before(own, sums, all);
@@ -409,26 +484,101 @@ __global__ __launch_bounds__(kThreads) void k_compact_count(CompactArgs args) {
     }
 }
 
+// The live pages before every segment's, in LDS (`before`, kSegments + 1 words).
+__device__ __forceinline__ void segments_before(const uint32_t *count, uint32_t segments, uint32_t *before,
+                                                uint32_t *sums) {
+    uint32_t done = 0u;
+    for (uint32_t base = 0; base < segments; base += kThreads) {
+        const uint32_t s = base + threadIdx.x;
+        uint32_t all = 0u;
+        const uint32_t at = done + block_before(s < segments ? count[s] : 0u, sums, all);
+        if (s < segments) {
+            before[s] = at;
+        }
+        done += all;
+    }
+    if (threadIdx.x == 0u) {
+        before[segments] = done;
+    }
+    __syncthreads();
+}
+
 // The n-th live page behind the first `live` moves to the n-th free one below it.
+// (Of a small pool every block reads all counts, so that no launch before it has to.)
 __global__ __launch_bounds__(kThreads) void k_compact_plan(CompactArgs args) {
+    constexpr uint32_t kSmall = kSmallPages / kSegment;
     __shared__ uint32_t before[kSegments + 1u];
     __shared__ uint32_t sums[kWaves];
-    segments_before(args.count, args.segments, before, sums);
-    const uint32_t live = before[args.segments];
-    const uint32_t first = blockIdx.x * kSegment + threadIdx.x * kOwn;
-    uint32_t holds[kOwn], own = 0u;
+    const uint32_t t = threadIdx.x;
+    // of each segment, a bit for each of the thread's pages that is held
+    uint32_t holds = 0u, first_below = 0u, border = 0u;
+    uint32_t mine[kOwn];
+    const uint32_t first = blockIdx.x * kSegment + t * kOwn;
+    if (args.pages <= kSmallPages) {
+        uint32_t held[kSmall], count[kSmall][kOwn];
 #pragma unroll
-    for (uint32_t i = 0; i < kOwn; ++i) {
-        holds[i] = first + i < args.pages && args.old_references[first + i] != 0u ? 1u : 0u;
-        own += holds[i];
+        for (uint32_t s = 0; s < kSmall; ++s) {
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i) {
+                count[s][i] = args.old_references[min(s * kSegment + t * kOwn + i, args.pages - 1u)];
+            }
+        }
+        uint32_t done = 0u;
+#pragma unroll
+        for (uint32_t s = 0; s < kSmall; ++s) {
+            held[s] = 0u;
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i) {
+                held[s] |= s * kSegment + t * kOwn + i < args.pages && count[s][i] != 0u ? 1u << i : 0u;
+            }
+            uint32_t all = 0u;
+            (void)block_before(static_cast<uint32_t>(__popc(held[s])), sums, all);
+            if (t == 0u) {
+                before[s] = done;
+            }
+            done += all;
+        }
+        if (t == 0u) {
+            before[kSmall] = done;
+            before[args.segments] = done;
+        }
+        border = done / kSegment;
+#pragma unroll
+        for (uint32_t s = 0; s < kSmall; ++s) {
+            holds = s == blockIdx.x ? held[s] : holds;
+            first_below = s == border ? held[s] : first_below;
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i) {
+                mine[i] = s == blockIdx.x ? count[s][i] : mine[i];
+            }
+        }
+        __syncthreads();
+    } else {
+        segments_before(args.count, args.segments, before, sums);
+        border = before[args.segments] / kSegment;
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            mine[i] = first + i < args.pages ? args.old_references[first + i] : 0u;
+            holds |= mine[i] != 0u ? 1u << i : 0u;
+            const uint32_t edge = border * kSegment + t * kOwn + i;
+            first_below |= edge < args.pages && args.old_references[edge] != 0u ? 1u << i : 0u;
+        }
     }
-    uint32_t all = 0u, at = before[blockIdx.x] + block_before(own, sums, all);
+    const uint32_t live = before[args.segments];
+    if (args.references != args.old_references) {
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            if (first + i < args.pages) {
+                args.references[first + i] = mine[i];
+            }
+        }
+    }
+    uint32_t all = 0u, at = before[blockIdx.x] + block_before(static_cast<uint32_t>(__popc(holds)), sums, all);
     // live pages below `live`: of the segments before its own, and in that
-    const uint32_t border = live / kSegment, edge = border * kSegment + threadIdx.x * kOwn;
     uint32_t below = 0u;
 #pragma unroll
     for (uint32_t i = 0; i < kOwn; ++i) {
-        below += edge + i < live && args.old_references[edge + i] != 0u ? 1u : 0u;
+        below += border * kSegment + t * kOwn + i < live ? first_below >> i & 1u : 0u;
     }
     uint32_t in_border = 0u;
     (void)block_before(below, sums, in_border);
@@ -436,20 +586,21 @@ __global__ __launch_bounds__(kThreads) void k_compact_plan(CompactArgs args) {
 #pragma unroll
     for (uint32_t i = 0; i < kOwn; ++i) {
         const uint32_t page = first + i;
+        const bool lives = (holds >> i & 1u) != 0u;
         if (page < args.pages) {
             if (page >= live) {
                 // (held, but counted as free: it has no new number)
-                args.rank[page] = holds[i] != 0u ? at - kept : kNone;
-                if (holds[i] != 0u) {
+                args.rank[page] = lives ? at - kept : kNone;
+                if (lives) {
                     args.sources[at - kept] = page;
                 }
-            } else if (holds[i] == 0u) {
+            } else if (!lives) {
                 args.targets[page - at] = page;
             }
         }
-        at += holds[i];
+        at += lives ? 1u : 0u;
     }
-    if (blockIdx.x == 0u && threadIdx.x == 0u) {
+    if (blockIdx.x == 0u && t == 0u) {
         *args.moves = live - kept;
         *args.live = live;
     }
@@ -469,7 +620,10 @@ __global__ __launch_bounds__(kThreads) void k_compact_apply(CompactArgs args, Co
             const uint64_t rest = w / copy.pieces;
             const uint32_t n = static_cast<uint32_t>(rest % copy.caches.arrays);
             const uint64_t i = rest / copy.caches.arrays;
-            copy_piece(copy.caches, copy.caches, n, args.sources[i], args.targets[i], 1u << args.page_shift, piece);
+            const uint32_t source = args.sources[i], target = args.targets[i];
+            PieceOfPage x;
+            x.load(copy.caches, n, source, 1u << args.page_shift, piece);
+            x.store(copy.caches, copy.caches, n, target, 1u << args.page_shift, piece);
         }
         return;
     }
@@ -607,7 +761,9 @@ void paged_fork(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const adi_
     copy.pieces = pieces_of(c, c.page_size - 1u);
     copy.column_blocks = ceil_div(std::max(args.old_stride, args.stride), kThreads);
     copy.table_blocks = args.rows / args.beams * copy.column_blocks;
-    launch(ctx, "fork_plan", k_fork_plan, dim3(args.segments + 1u), dim3(kThreads), 0, args);
+    args.small = c.pages <= kSmallPages ? 1u : 0u;
+    const uint32_t others = args.small != 0u && args.references == args.old_references ? 0u : args.segments;
+    launch(ctx, "fork_plan", k_fork_plan, dim3(1u + others), dim3(kThreads), 0, args);
     for (uint32_t first = 0; first < pool->caches; first += kCaches) {
         copy.caches = caches_view(*pool, first);
         copy.work = uint64_t(args.rows) * copy.caches.arrays * copy.pieces;
@@ -697,7 +853,9 @@ void paged_compact(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const a
     copy.pieces = pieces_of(c, c.page_size);
     const uint64_t words = std::max<uint64_t>(uint64_t(a->rows) * args.columns, c.pages / 2u + 1u);
     copy.table_blocks = static_cast<uint32_t>(std::min<uint64_t>((words + kThreads - 1) / kThreads, ctx->cu_count));
-    launch(ctx, "compact_count", k_compact_count, dim3(args.segments), dim3(kThreads), 0, args);
+    if (c.pages > kSmallPages) {
+        launch(ctx, "compact_count", k_compact_count, dim3(args.segments), dim3(kThreads), 0, args);
+    }
     launch(ctx, "compact_plan", k_compact_plan, dim3(args.segments), dim3(kThreads), 0, args);
     for (uint32_t first = 0; first < pool->caches; first += kCaches) {
         copy.caches = caches_view(*pool, first);
