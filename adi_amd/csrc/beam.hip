@@ -871,7 +871,8 @@ void require_select(const adi_hip_beam_arguments *a) {
 
 // ---- states that follow their parents -------------------------------------------
 
-constexpr uint32_t kArrays = 64;  // of a launch
+// arrays of a launch; few of them, so that its arguments are few bytes
+constexpr uint32_t kArrays = 64, kFewArrays = 4;
 
 struct RowArray {
     char *data;
@@ -881,10 +882,11 @@ struct RowArray {
     uint32_t blocks;       // of a request
     uint32_t tail;         // bytes behind them
 };
+template <uint32_t ARRAYS>
 struct ReorderArgs {
-    RowArray array[kArrays];
-    uint32_t arrays, beams;
     const uint32_t *parents;
+    uint32_t arrays, beams;
+    RowArray array[ARRAYS];
 };
 
 typedef uint32_t loose_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
@@ -909,8 +911,8 @@ __device__ __forceinline__ void reorder_unit(char *base, uint64_t row_stride, co
     }
 }
 
-template <uint32_t K>
-__global__ __launch_bounds__(kThreads) void k_reorder_rows(ReorderArgs args) {
+template <uint32_t K, uint32_t ARRAYS>
+__global__ __launch_bounds__(kThreads) void k_reorder_rows(ReorderArgs<ARRAYS> args) {
     uint32_t n = 0u;
     while (n + 1u < args.arrays && args.array[n + 1u].first_block <= blockIdx.x) {
         ++n;
@@ -963,20 +965,26 @@ void reorder_rows(adi_hip_context *ctx, const adi_hip_row_array *arrays, uint32_
     if (requests == 0 || beams == 1) {
         return;
     }
-    ReorderArgs args{};
-    args.beams = beams;
-    args.parents = parents;
+    ReorderArgs<kArrays> args{parents, 0, beams, {}};
     uint64_t blocks = 0;
+    const auto launch_of = [&](auto &&of) {
+        constexpr uint32_t kOf = sizeof(of.array) / sizeof(RowArray);
+        const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
+        if (beams <= 4) {
+            launch(ctx, "reorder_rows", k_reorder_rows<4, kOf>, grid, block, 0, of);
+        } else if (beams <= 16) {
+            launch(ctx, "reorder_rows", k_reorder_rows<16, kOf>, grid, block, 0, of);
+        } else {
+            launch(ctx, "reorder_rows", k_reorder_rows<64, kOf>, grid, block, 0, of);
+        }
+    };
     const auto go = [&] {
-        if (args.arrays != 0) {
-            const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
-            if (beams <= 4) {
-                launch(ctx, "reorder_rows", k_reorder_rows<4>, grid, block, 0, args);
-            } else if (beams <= 16) {
-                launch(ctx, "reorder_rows", k_reorder_rows<16>, grid, block, 0, args);
-            } else {
-                launch(ctx, "reorder_rows", k_reorder_rows<64>, grid, block, 0, args);
-            }
+        if (args.arrays > kFewArrays) {
+            launch_of(args);
+        } else if (args.arrays != 0) {
+            ReorderArgs<kFewArrays> few{parents, args.arrays, beams, {}};
+            std::copy_n(args.array, kFewArrays, few.array);
+            launch_of(few);
         }
         args.arrays = 0;
         blocks = 0;

@@ -1540,6 +1540,55 @@ def reorder_rows(ctx: Context, rows: StateRows, parents) -> None:
         ctx.check(status)
 
 
+class BeamRow(Sequence):
+    """A sequence whose states are a row of BeamStates."""
+
+    def __init__(self, layers, capacity: int):
+        self.tensors, self._layers, self.capacity = [], layers, capacity
+        self.struct = DecoderStateStruct(0, layers)
+
+
+class BeamStates:
+    """The decoder states of one request's beams, side by side in arrays [1, beams,
+    ...], so that one call lets them follow their parents; `sequences` are its
+    rows for prefill, decode_batch and DecodeGraph. `more`: further arrays [1, beams,
+    ...] that follow along."""
+
+    def __init__(self, ctx: Context, model: Model, beams: int, capacity: int, more=()):
+        import torch
+        kind = dict(dtype=torch.float32, device=f"cuda:{ctx.device}")
+        self.ctx, self.capacity, self.arrays, self.caches, self.linear = ctx, capacity, [], [], []
+        layers = [(LayerState * len(model.layers))() for _ in range(beams)]
+        for i in range(len(model.layers)):
+            if model.full_attention(i):
+                pair = [torch.zeros((1, beams, capacity, 2, 256), **kind) for _ in range(2)]
+                self.caches += range(len(self.arrays), len(self.arrays) + 2)
+                for b in range(beams):
+                    layers[b][i] = LayerState(pair[0][0, b].data_ptr(), pair[1][0, b].data_ptr(), capacity, None, None)
+            else:
+                pair = [torch.zeros((1, beams, 8192 * 3), **kind), torch.zeros((1, beams, 32 * 128 * 128), **kind)]
+                self.linear += pair
+                for b in range(beams):
+                    layers[b][i] = LayerState(None, None, 0, pair[0][0, b].data_ptr(), pair[1][0, b].data_ptr())
+            self.arrays += pair
+        self.sequences = [BeamRow(s, capacity) for s in layers]
+        self.rows = StateRows(ctx, [*self.arrays, *more])
+
+    def start(self) -> None:
+        """Row 0 begins a new sequence."""
+        for t in self.linear:
+            t[0, 0].zero_()
+        self.sequences[0].struct.position = 0
+
+    def follow(self, parents, position: int) -> None:
+        """Every row becomes its parent (int32 [1, beams]), `position` entries long."""
+        for i in self.caches:
+            self.rows.struct[i].row_bytes = position * 2 * 256 * 4
+        reorder_rows(self.ctx, self.rows, parents)
+        for s in self.sequences:
+            s.struct.position = position
+
+
 class PagedPool:
     """The caches (PagedCache, one a layer) whose pages are handed out together,
     with their reference counts (int32 [pages]; 0: free) and, where given, the

@@ -188,3 +188,120 @@ class ContinuousBatcher:
             self.close()
         except Exception:
             pass
+
+
+@dataclass
+class Hypothesis:
+    """One result of a beam search: its tokens without the stop token, the sum of
+    their log-probabilities (the stop token's included), and that divided by
+    length^length_penalty, which results are ordered by."""
+    tokens: list
+    log_probability: float
+    score: float
+    finish_reason: str  # "stop_token" or "length"
+
+
+class BeamSearch:
+    """Beam search over the model, with token ids, beside the batcher's one token a
+    row (sample_token, src/generation.cpp:161-225): each step takes the best
+    `beams` of beams x vocabulary on the device (hip.beam_select), the decoder
+    states follow their parents in place (hip.BeamStates), and the beams decode
+    as a batch, recorded once as a HIP graph and replayed (replay_steps=False
+    launches every step directly; both give the same bits). Beams that have ended stay as
+    one candidate each; candidates are compared by sum / length^length_penalty. One
+    search at a time; the context must not be used otherwise meanwhile."""
+
+    def __init__(self, ctx: hip.Context, model: hip.Model, beams: int = 4, capacity: int = 4096,
+                 length_penalty: float = 0.0, stop_tokens: Sequence[int] = (), masked_tokens: Sequence[int] = (),
+                 prefill_ubatch: int = 128, replay_steps: bool = True):
+        if not 1 <= beams <= 64:
+            raise GenerationError("beams must be 1 to 64")
+        if not 1 <= capacity <= model.struct.context:
+            raise GenerationError("capacity exceeds model context")
+        if any(not 0 <= t < model.vocabulary for t in (*stop_tokens, *masked_tokens)):
+            raise GenerationError("a stop or masked token is outside the vocabulary")
+        torch = ctx.torch
+        self.ctx, self.model, self.beams, self.capacity = ctx, model, beams, capacity
+        self.length_penalty, self.ubatch, self.replay_steps = float(length_penalty), prefill_ubatch, replay_steps
+        device = f"cuda:{ctx.device}"
+        self._stop = torch.tensor(list(stop_tokens), dtype=torch.int32, device=device)
+        self._ended_token = int(stop_tokens[0]) if len(stop_tokens) else 0
+        self._masked = torch.tensor(list(masked_tokens), dtype=torch.int64, device=device)
+        self._logits = torch.empty((1, beams, model.vocabulary), dtype=torch.float32, device=device)
+        self._history = torch.zeros((1, beams, capacity), dtype=torch.int32, device=device)
+        self._tokens = torch.zeros((1, beams), dtype=torch.int32, device=device)
+        self._parents = torch.zeros((1, beams), dtype=torch.int32, device=device)
+        self._scores = [torch.zeros((1, beams), dtype=torch.float32, device=device) for _ in range(2)]
+        self._workspace = hip.PagedWorkspace(ctx)
+        self._states = hip.BeamStates(ctx, model, beams, capacity, more=[self._history])
+        self._graph: Optional[hip.DecodeGraph] = None
+
+    def _decode(self) -> None:
+        if not self.replay_steps:
+            tokens = [max(t, 0) for t in self._tokens[0].tolist()]  # -1: a row without a beam
+            hip.decode_batch(self.ctx, self.model, tokens, self._states.sequences, self._logits)
+            return
+        if self._graph is None:
+            self._graph = hip.DecodeGraph(self.ctx, self.model, self._states.sequences, self._tokens, self._logits)
+        self._graph.launch()
+
+    def search(self, prompt: Sequence[int], max_output_tokens: int) -> list:
+        """The beams' hypotheses, best first."""
+        if max_output_tokens < 1:
+            raise GenerationError("max_output_tokens must be positive")
+        if len(prompt) < 1 or len(prompt) + max_output_tokens > self.capacity:
+            raise GenerationError("the prompt and its output exceed the capacity")
+        torch, states = self.ctx.torch, self._states
+        scores, other = self._scores
+        states.start()
+        hip.prefill(self.ctx, self.model, prompt, states.sequences[0], self._logits[0, 0], ubatch=self.ubatch)
+        # the prompt is one beam; the first step's children are all its own
+        scores.fill_(-torch.inf)
+        scores[0, 0] = 0.0
+        ended = torch.zeros_like(self._tokens)
+        lengths = torch.zeros_like(scores)
+        position = len(prompt)
+        for n in range(1, max_output_tokens + 1):
+            if self._masked.numel():
+                self._logits.index_fill_(2, self._masked, torch.finfo(torch.float32).min)
+            # (a live beam's candidates have n tokens)
+            lengths = torch.where(ended != 0, lengths, float(n))
+            hip.beam_select(self.ctx, self._logits, scores, other, self._parents, self._tokens, self._workspace,
+                            weights=lengths.pow(-self.length_penalty) if self.length_penalty else None, ended=ended,
+                            ended_token=self._ended_token, settle=True)
+            scores, other = other, scores
+            states.follow(self._parents, position)
+            self._history[:, :, n - 1] = self._tokens
+            # (rows without a beam, of a vocabulary smaller than the beams, have no parent)
+            parents = self._parents.clamp(min=0).long()
+            lengths = lengths.gather(1, parents)
+            ended = ended.gather(1, parents)
+            if self._stop.numel():
+                ended = ((ended != 0) | torch.isin(self._tokens, self._stop)).int()
+            if n == max_output_tokens or bool(((ended != 0) | torch.isneginf(scores)).all()):
+                break
+            self._decode()
+            position += 1
+        found = []
+        for row, total, length, gone in zip(self._history[0].tolist(), scores[0].tolist(), lengths[0].tolist(),
+                                            ended[0].tolist()):
+            if total == float("-inf"):
+                continue
+            length = int(length)
+            found.append(Hypothesis(row[:length - 1 if gone else length], total, total / length ** self.length_penalty,
+                                    "stop_token" if gone else "length"))
+        return sorted(found, key=lambda h: -h.score)
+
+    def close(self) -> None:
+        if getattr(self, "_graph", None) is not None:
+            self._graph.close()
+            self._graph = None
+        if getattr(self, "_workspace", None) is not None:
+            self._workspace.close()
+            self._workspace = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
