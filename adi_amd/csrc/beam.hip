@@ -577,10 +577,10 @@ __device__ __forceinline__ uint32_t trim(uint64_t *list, uint32_t &entries, uint
 // its way. A lane adds up its own exponentials, in powers of two below its own
 // largest logit so far. The best: in a first tile, the `choices` best of the lanes'
 // own two largest (of their pieces' halves) bound what is taken from below, later the
-// last of those taken so far, so that `choices` / m are taken of tile m, about.
+// last of those taken so far, by any wave of the block.
 template <typename T, uint32_t N>
 __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, uint32_t row, const char *from,
-                                          uint64_t *list) {
+                                          uint64_t *list, uint32_t *shared) {
     constexpr uint32_t kCount = Piece<T>::kCount, kPieces = N / kCount, kTile = kWave * N;
     const uint32_t lane = threadIdx.x & 63u, choices = args.choices;
     const uint32_t first = part * args.span, end = min(first + args.span, args.vocabulary);
@@ -597,6 +597,12 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
             load_tile(x, tile, lane);
         } else {
             load_last(x, tile, lane, end - at);
+        }
+    };
+    // a key that `choices` logits of the row reach is the other waves' bound too
+    const auto share = [&](uint32_t reached) {
+        if (lane == 0u) {
+            atomicMax(shared, reached);
         }
     };
     Piece<T> next[kPieces];
@@ -628,6 +634,12 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
                 max(reached_by(ascending_key(half[0]), ascending_key(half[1]), choices), kLowestKey + 1u);
             least = static_cast<uint64_t>(reached) << 32;
             edge = below(reached);
+            share(reached);
+        }
+        if (at != first) {
+            const uint32_t reached = *static_cast<volatile uint32_t *>(shared);
+            least = max(least, static_cast<uint64_t>(reached) << 32);
+            edge = fmaxf(edge, below(max(reached, kLowestKey + 1u)));
         }
         if (__ballot(own > edge) != 0u) {
             const uint32_t held = entries;
@@ -681,10 +693,12 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
                     const uint32_t reached = trim(list, entries, choices, lane);
                     least = max(least, static_cast<uint64_t>(reached) << 32);
                     edge = fmaxf(edge, below(reached));
+                    share(reached);
                 } else {
                     keep_best(list, entries, choices, lane);
                     least = list[choices - 1u];
                     edge = of_ascending_key(static_cast<uint32_t>(least >> 32));
+                    share(static_cast<uint32_t>(least >> 32));
                 }
             }
         }
@@ -737,14 +751,18 @@ __global__ __launch_bounds__(kThreads, kResident<T>) void k_beam_select(BeamArgs
         uint64_t list[kWaves][kPartList];
         std::conditional_t<JOINS, JoinShared, uint32_t> join;
     } lds;
-    __shared__ uint32_t last;
+    __shared__ uint32_t last, reached;
+    if (threadIdx.x == 0u) {
+        reached = 0u;
+    }
+    __syncthreads();
     const uint32_t row = blockIdx.z * args.beams + blockIdx.y;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), part = blockIdx.x * kWaves + wave;
     if (part < args.parts && args.scores[row] != -__builtin_huge_valf() &&
         (args.ended == nullptr || args.ended[row] == 0u)) {
         const char *const from =
             args.logits + (blockIdx.z * args.request_stride + blockIdx.y * args.beam_stride) * sizeof(T);
-        beam_part<T, N>(args, part, row, from, lds.list[wave]);
+        beam_part<T, N>(args, part, row, from, lds.list[wave], &reached);
     }
     if constexpr (JOINS) {
         wait_stores();
