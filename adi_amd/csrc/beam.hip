@@ -279,8 +279,17 @@ __device__ __forceinline__ void join_request(const BeamArgs &args, uint32_t requ
     // items: the lists, or their candidates one by one; then the ended beams
     const uint32_t depth = k * parts >= 4u * choices ? choices : 1u;
     const uint32_t of_beam = parts * (choices / depth), items = k * of_beam;
-    // (on its way while the logarithms are made)
-    const uint64_t head = t < items ? coherent_load(best + static_cast<uint64_t>(t) * depth) : 0u;
+    // (on their way while the logarithms are made: two items' first two candidates)
+    constexpr uint32_t kHeld = 2;
+    uint64_t head[kHeld][kHeld];
+#pragma unroll
+    for (uint32_t q = 0; q < kHeld; ++q) {
+#pragma unroll
+        for (uint32_t j = 0; j < kHeld; ++j) {
+            head[q][j] = coherent_load(best + static_cast<uint64_t>(min(q * kThreads + t, items - 1u)) * depth +
+                                       min(j, depth - 1u));
+        }
+    }
     if (t == 0u) {
         lds.listed = 0u;
         lds.bad = 0u;
@@ -299,12 +308,17 @@ __device__ __forceinline__ void join_request(const BeamArgs &args, uint32_t requ
         // (its last part again, where a lane has none)
         const float s = args.scores[row], w = args.weights != nullptr ? args.weights[row] : 1.0f;
         const uint32_t gone = args.ended != nullptr ? args.ended[row] : 0u;
-        const float first_most = coherent_load(most + min(within, parts - 1u));
-        const double first_sum = coherent_load(sum + min(within, parts - 1u));
+        float most_of[kHeld];
+        double sum_of[kHeld];
+#pragma unroll
+        for (uint32_t q = 0; q < kHeld; ++q) {
+            most_of[q] = coherent_load(most + min(within + q * group, parts - 1u));
+            sum_of[q] = coherent_load(sum + min(within + q * group, parts - 1u));
+        }
         uint32_t what = b >= k || s == -__builtin_huge_valf() ? 0u : gone != 0u ? 2u : 1u;
         bool wrong = what != 0u && !(__builtin_isfinite(s) && w > 0.0f && __builtin_isfinite(w));
-        float top = first_most;
-        for (uint32_t p = within + group; p < parts; p += group) {
+        float top = larger(most_of[0], most_of[1]);
+        for (uint32_t p = within + kHeld * group; p < parts; p += group) {
             top = larger(top, coherent_load(most + p));
         }
         const auto over_group = [&](auto &&join) {
@@ -319,8 +333,9 @@ __device__ __forceinline__ void join_request(const BeamArgs &args, uint32_t requ
         const auto part = [&](float own, double value) {
             return own == -__builtin_huge_valf() ? 0.0 : value * exp(reference_of(own) - static_cast<double>(top));
         };
-        double total = within < parts ? part(first_most, first_sum) : 0.0;
-        for (uint32_t p = within + group; p < parts; p += group) {
+        double total = within < parts ? part(most_of[0], sum_of[0]) : 0.0;
+        total += within + group < parts ? part(most_of[1], sum_of[1]) : 0.0;
+        for (uint32_t p = within + kHeld * group; p < parts; p += group) {
             total += part(coherent_load(most + p), coherent_load(sum + p));
         }
         over_group([&](auto step) { total += lane_xor<decltype(step)::value>(total); });
@@ -368,21 +383,26 @@ __device__ __forceinline__ void join_request(const BeamArgs &args, uint32_t requ
     };
     // item i's candidate j
     const auto candidate = [&](uint32_t i, uint32_t j) {
-        Candidate c{0u, 0u};
-        if (i >= items) {
-            c = ended(i - items);
-        } else {
-            uint64_t key = head;
-            if (i != t || j != 0u) {
-                key = coherent_load(best + static_cast<uint64_t>(i) * depth + j);
-            }
-            c = of_key(i / of_beam, key);
-        }
-        return c;
+        return i >= items ? ended(i - items)
+                          : of_key(i / of_beam, coherent_load(best + static_cast<uint64_t>(i) * depth + j));
     };
+    // the items held: candidates of ended beams come after them
+    Candidate held[kHeld][kHeld];
     uint32_t own = 0u;
-    for (uint32_t i = t; i < items + k; i += kThreads) {
+#pragma unroll
+    for (uint32_t q = 0; q < kHeld; ++q) {
+        const uint32_t i = q * kThreads + t;
+#pragma unroll
+        for (uint32_t j = 0; j < kHeld; ++j) {
+            held[q][j] = of_key(min(i, items - 1u) / of_beam, i < items && j < depth ? head[q][j] : 0u);
+        }
+        own = max(own, static_cast<uint32_t>(held[q][0].rank >> 32));
+    }
+    for (uint32_t i = kHeld * kThreads + t; i < items; i += kThreads) {
         own = max(own, static_cast<uint32_t>(candidate(i, 0u).rank >> 32));
+    }
+    if (t < k) {
+        own = max(own, static_cast<uint32_t>(ended(t).rank >> 32));
     }
     lds.keys[t] = own;
     __syncthreads();
@@ -397,18 +417,31 @@ __device__ __forceinline__ void join_request(const BeamArgs &args, uint32_t requ
         least = reach >= choices ? more : least;
     }
     least = max(least, 1u);
-    for (uint32_t i = t; i < items + k; i += kThreads) {
-        for (uint32_t j = 0; j < (i < items ? depth : 1u); ++j) {
-            const Candidate c = candidate(i, j);
-            if (static_cast<uint32_t>(c.rank >> 32) < least) {
-                break;
-            }
+    const auto take = [&](const Candidate &c) {
+        const bool takes = static_cast<uint32_t>(c.rank >> 32) >= least;
+        if (takes) {
             const uint32_t at = atomicAdd(&lds.listed, 1u);
             if (at < kJoinList) {
                 lds.rank[at] = c.rank;
                 lds.tie[at] = c.tie;
             }
         }
+        return takes;
+    };
+#pragma unroll
+    for (uint32_t q = 0; q < kHeld; ++q) {
+        bool takes = take(held[q][0]);
+        takes = takes && take(held[q][1]);
+        for (uint32_t j = kHeld; takes && j < depth; ++j) {
+            takes = take(candidate(q * kThreads + t, j));
+        }
+    }
+    for (uint32_t i = kHeld * kThreads + t; i < items; i += kThreads) {
+        for (uint32_t j = 0; j < depth && take(candidate(i, j)); ++j) {
+        }
+    }
+    if (t < k) {
+        (void)take(ended(t));
     }
     __syncthreads();
     const uint32_t entries = lds.listed;
@@ -607,6 +640,10 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
     };
     Piece<T> next[kPieces];
     load(next, first);
+    // (asked for after the first tile, so as not to wait for one before the other)
+    if (args.scores[row] == -__builtin_huge_valf() || (args.ended != nullptr && args.ended[row] != 0u)) {
+        return;
+    }
 #pragma unroll 1
     for (uint32_t at = first; at < end; at += kTile) {
         Piece<T> x[kPieces];
@@ -758,8 +795,7 @@ __global__ __launch_bounds__(kThreads, kResident<T>) void k_beam_select(BeamArgs
     __syncthreads();
     const uint32_t row = blockIdx.z * args.beams + blockIdx.y;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), part = blockIdx.x * kWaves + wave;
-    if (part < args.parts && args.scores[row] != -__builtin_huge_valf() &&
-        (args.ended == nullptr || args.ended[row] == 0u)) {
+    if (part < args.parts) {
         const char *const from =
             args.logits + (blockIdx.z * args.request_stride + blockIdx.y * args.beam_stride) * sizeof(T);
         beam_part<T, N>(args, part, row, from, lds.list[wave], &reached);
@@ -841,9 +877,10 @@ void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const 
 // Tiles of 512 logits where that makes at most a wave a CU, else of 2048, and as
 // many a part as leave 32 waves a CU, about (one request of 4 x 248,320 f32 logits:
 // 14.4 us, with tiles of 1024 and 512 16.4 and 23.6, as more parts are joined; of 4 x
-// 32,000 in 512s 10.5, in 1024s 11.2). Up to half a block a CU joins within the
-// launch (4 x 512 logits: 8.4 us, with a launch of its own 9.4); more blocks wait
-// for each other at the tickets (16 requests of 4 x 248,320: 28.3 us, and 25.3).
+// 32,000 in 512s 10.5, in 1024s 11.2). Few blocks join within the launch (4 x 512
+// logits: 8.3 us, with a launch of its own 8.8); more wait for each other at the
+// ticket, and the launch's end for the join (4 x 248,320: 14.5 and 13.8, 16 requests
+// of them 31 and 25.8).
 template <typename T>
 void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const adi_hip_paged_workspace &workspace) {
     const uint64_t rows = uint64_t(a.requests) * a.beams, cus = static_cast<uint64_t>(ctx->cu_count);
@@ -852,7 +889,7 @@ void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const 
         const uint64_t waves = rows * ceil_div(a.vocabulary, kWave * N);
         const uint32_t tiles = static_cast<uint32_t>(std::clamp<uint64_t>(waves / (32u * cus), 1u, 16u));
         const uint64_t blocks = rows * ceil_div(ceil_div(a.vocabulary, kWave * N * tiles), kWaves);
-        if (blocks <= cus / 2u) {
+        if (blocks <= cus / 8u) {
             launch_select<T, N, true>(ctx, a, workspace, tiles);
         } else {
             launch_select<T, N, false>(ctx, a, workspace, tiles);

@@ -892,7 +892,7 @@ int adi_hip_full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attent
  * by rank = weights[b] score(b, v) (no weights: 1; say 1 / length^a), best
  * first, ranks in 64 bits of exact logarithms; equal ranks: the lower beam, then
  * the larger logit, then the lower token. A beam that has `ended` (nonzero) is one
- * candidate, ended_token with the score it has; its logits are not read. Outputs
+ * candidate, ended_token with the score it has, whatever its logits hold. Outputs
  * are the candidates' scores (rounded to float), beams and tokens. It follows
  * sample_token (src/generation.cpp:161-225) where that keeps one token of a row.
  *
