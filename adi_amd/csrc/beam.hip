@@ -949,22 +949,41 @@ typedef uint32_t loose_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
 // 16 bytes of every row of a request, at any address, or one of the bytes behind
 // them: the rows that others take are loaded, then stored where they go, so no order of
 // the moves matters, and what stays is neither read nor written.
-template <typename U, uint32_t K>
-__device__ __forceinline__ void reorder_unit(char *base, uint64_t row_stride, const uint64_t (&takers)[K]) {
-    U v[K];
+template <typename U, uint32_t K, uint32_t N>
+__device__ __forceinline__ void reorder_units(char *base, uint64_t row_stride, const uint64_t (&takers)[K], uint64_t step,
+                                              uint32_t count) {
+    U v[K][N];
 #pragma unroll
     for (uint32_t p = 0; p < K; ++p) {
         if (takers[p] != 0u) {
-            v[p] = *reinterpret_cast<const U *>(base + p * row_stride);
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                if (i < count) {
+                    v[p][i] = *reinterpret_cast<const U *>(base + p * row_stride + i * step);
+                }
+            }
         }
     }
 #pragma unroll
     for (uint32_t p = 0; p < K; ++p) {
         for (uint64_t left = takers[p]; left != 0u; left &= left - 1u) {
-            *reinterpret_cast<U *>(base + static_cast<uint32_t>(__builtin_ctzll(left)) * row_stride) = v[p];
+            char *const to = base + static_cast<uint32_t>(__builtin_ctzll(left)) * row_stride;
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                if (i < count) {
+                    *reinterpret_cast<U *>(to + i * step) = v[p][i];
+                }
+            }
         }
     }
 }
+
+// Units of a row that a thread moves, a block's threads apart: as many as the
+// registers hold, as rows lie far apart and one unit of each leaves most of the memory's
+// channels idle (4 rows of 4 requests' 30 states, 1.05 GB: 254 us with one unit, 191
+// with four, 5.5 TB/s; 8 rows 415 with one, 198 with two and with four; 16 213 and 205).
+template <uint32_t K>
+constexpr uint32_t kUnits = K <= 4u ? 4u : K <= 16u ? 2u : 1u;
 
 template <uint32_t K, uint32_t ARRAYS>
 __global__ __launch_bounds__(kThreads) void k_reorder_rows(ReorderArgs<ARRAYS> args) {
@@ -984,12 +1003,16 @@ __global__ __launch_bounds__(kThreads) void k_reorder_rows(ReorderArgs<ARRAYS> a
     for (uint32_t p = 0; p < K; ++p) {
         takers[p] = __ballot(moves && parent == p);
     }
-    const uint64_t unit = static_cast<uint64_t>(block) * kThreads + threadIdx.x;
+    constexpr uint32_t N = kUnits<K>;
+    const uint64_t unit = static_cast<uint64_t>(block) * (N * kThreads) + threadIdx.x;
     char *const base = array.data + request * array.request_stride;
     if (unit < array.units) {
-        reorder_unit<loose_u32x4, K>(base + unit * 16u, array.row_stride, takers);
-    } else if (unit - array.units < array.tail) {
-        reorder_unit<uint8_t, K>(base + array.units * 16u + (unit - array.units), array.row_stride, takers);
+        const uint64_t more = (array.units - 1u - unit) / kThreads;
+        reorder_units<loose_u32x4, K, N>(base + unit * 16u, array.row_stride, takers, 16u * kThreads,
+                                         more < N ? static_cast<uint32_t>(more) + 1u : N);
+    }
+    if (block == 0u && threadIdx.x < array.tail) {
+        reorder_units<uint8_t, K, 1>(base + array.units * 16u + threadIdx.x, array.row_stride, takers, 0u, 1u);
     }
 }
 
@@ -1027,6 +1050,8 @@ void reorder_rows(adi_hip_context *ctx, const adi_hip_row_array *arrays, uint32_
         const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
         if (beams <= 4) {
             launch(ctx, "reorder_rows", k_reorder_rows<4, kOf>, grid, block, 0, of);
+        } else if (beams <= 8) {
+            launch(ctx, "reorder_rows", k_reorder_rows<8, kOf>, grid, block, 0, of);
         } else if (beams <= 16) {
             launch(ctx, "reorder_rows", k_reorder_rows<16, kOf>, grid, block, 0, of);
         } else {
@@ -1051,7 +1076,11 @@ void reorder_rows(adi_hip_context *ctx, const adi_hip_row_array *arrays, uint32_
         }
         RowArray r{static_cast<char *>(a.data), a.request_stride, a.row_stride, a.row_bytes / 16, 0, 0,
                    static_cast<uint32_t>(a.row_bytes % 16)};
-        const uint64_t per = (r.units + r.tail + kThreads - 1) / kThreads;
+        const uint64_t each = kThreads * (beams <= 4    ? kUnits<4>
+                                          : beams <= 8  ? kUnits<8>
+                                          : beams <= 16 ? kUnits<16>
+                                                        : kUnits<64>);
+        const uint64_t per = std::max<uint64_t>((r.units + each - 1) / each, 1);
         require(per * requests < (1u << 23), "reorder rows: too many rows of such a size");
         r.blocks = static_cast<uint32_t>(per);
         if (args.arrays == kArrays || blocks + per * requests >= (1u << 23)) {

@@ -1522,11 +1522,13 @@ class StateRows:
                 _refuse("state rows: arrays must be of shape [requests, beams, ...], one for all")
             if t.get_device() != ctx.device:
                 _refuse(f"state rows on {t.device}, the context is on cuda:{ctx.device}")
-            if t.numel() and not t[0, 0].is_contiguous():
-                _refuse("state rows: a row must be contiguous")
+            shape, strides, each = t.shape, t.stride(), 1
+            for n, step in zip(reversed(shape[2:]), reversed(strides[2:])):
+                if n > 1 and step != each:
+                    _refuse("state rows: a row must be contiguous")
+                each *= n
             size = t.element_size()
-            each = t.numel() // max(self.requests * self.beams, 1)
-            rows[i] = RowArray(t.data_ptr(), t.stride(0) * size, t.stride(1) * size, each * size)
+            rows[i] = RowArray(t.data_ptr(), strides[0] * size, strides[1] * size, each * size)
         self.struct = rows
 
 
