@@ -238,8 +238,7 @@ class BeamSearch:
 
     def _decode(self) -> None:
         if not self.replay_steps:
-            tokens = [max(t, 0) for t in self._tokens[0].tolist()]  # -1: a row without a beam
-            hip.decode_batch(self.ctx, self.model, tokens, self._states.sequences, self._logits)
+            hip.decode_batch(self.ctx, self.model, self._tokens[0].tolist(), self._states.sequences, self._logits)
             return
         if self._graph is None:
             self._graph = hip.DecodeGraph(self.ctx, self.model, self._states.sequences, self._tokens, self._logits)
@@ -278,8 +277,12 @@ class BeamSearch:
             ended = ended.gather(1, parents)
             if self._stop.numel():
                 ended = ((ended != 0) | torch.isin(self._tokens, self._stop)).int()
-            if n == max_output_tokens or bool(((ended != 0) | torch.isneginf(scores)).all()):
+            done, wrong = torch.stack([((ended != 0) | torch.isneginf(scores)).all(), scores.isnan().any()]).tolist()
+            if wrong:
+                raise GenerationError("the model's logits hold a NaN or an infinity")
+            if n == max_output_tokens or done:
                 break
+            self._tokens.clamp_(min=0)  # (of rows without a beam)
             self._decode()
             position += 1
         found = []

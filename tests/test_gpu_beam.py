@@ -179,6 +179,35 @@ def test_sorted_logits_and_spikes(gpu, workspace):
     check(gpu, workspace, far, torch.tensor([[-3.0, -3.5]], device="cuda"), 20)
 
 
+@pytest.mark.parametrize("v", [300, 9000, 70001])
+def test_logits_far_from_0(gpu, workspace, v):
+    """Every float is a logit: large ones of both signs, rows around the edges of what
+    the kernel's own exponentials take (65536), parts of a row on either side of it."""
+    for shift, scale in [(65536.0, 3.0), (-65536.0, 3.0), (7e4, 3.0), (-7e4, 3.0), (0.0, 3e4), (0.0, 1e30), (1e38, 1e37),
+                         (-1e38, 1e37)]:
+        logits = normal(v, 2, 2, v) * scale + shift
+        check(gpu, workspace, logits, running(4, 2, 2), 9)
+    half = normal(v, 1, 2, v)
+    half[:, :, v // 2:] += 65536.0
+    half[:, 1] -= 65530.0
+    check(gpu, workspace, half, running(4, 1, 2), 9)
+    for kind, shift in (("f16", 65000.0), ("f16", -65000.0), ("bf16", 3e38), ("bf16", -3e38)):
+        check(gpu, workspace, (normal(v, 2, 2, v, scale=2.0) + shift).to(TYPES[kind]), running(4, 2, 2), 9)
+    tiny = (normal(v, 2, 2, v) * 1e-39)  # below the normal floats
+    check(gpu, workspace, tiny, running(4, 2, 2), 9)
+
+
+def test_many_requests_of_few_tokens(gpu, workspace):
+    n = 70000  # more than a launch takes
+    out = torch.zeros(n, 2, device="cuda"), ints(np.zeros((n, 2))), ints(np.zeros((n, 2)))
+    logits, scores = normal(1, n, 2, 5), running(1, n, 2)
+    hip.beam_select(gpu, logits, scores, *out, workspace)
+    x = (scores[..., None].double() + torch.log_softmax(logits.double(), -1)).reshape(n, 10)
+    best = x.topk(2, -1)
+    assert torch.equal(out[1], (best.indices // 5).int()) and torch.equal(out[2], (best.indices % 5).int())
+    assert bool(((out[0].double() - best.values).abs() <= U * best.values.abs() + 2.0 ** -32).all())
+
+
 def test_wrong_logits_and_scores(gpu, workspace):
     """A NaN or +infinity makes its request NaN, and no other; what a dead beam
     holds does not matter."""

@@ -187,7 +187,7 @@ def test_beams_and_requests(gpu, workspace, beams, requests, in_place):
         b.step(parents, np.minimum(added, 6 * 8 - grown), in_place=in_place)
 
 
-@pytest.mark.parametrize("pages", [4095, 4096, 4097, 30011])
+@pytest.mark.parametrize("pages", [4095, 4096, 4097, 30011, 140001])
 def test_pools_of_many_segments(gpu, workspace, pages):
     """The lowest free pages, wherever in a long pool they lie."""
     b = Books(gpu, workspace, 8, 4, 400, pages, 8, caches=1, heads=1)
@@ -430,7 +430,7 @@ def compacted(count, lengths, table, page):
 @pytest.mark.parametrize("pages,rows,page,share,layout", [
     (1, 1, 8, 1.0, {}), (1, 1, 8, 0.0, {}), (7, 2, 16, 0.5, {}), (100, 5, 8, 0.3, dict(heads_first=True)),
     (2047, 20, 8, 0.7, {}), (2048, 20, 8, 0.5, {}), (2049, 30, 8, 0.02, {}), (4096, 30, 8, 1.0, {}),
-    (9001, 100, 8, 0.4, dict(wide=8)), (6000, 3, 8, 0.999, {})])
+    (9001, 100, 8, 0.4, dict(wide=8)), (6000, 3, 8, 0.999, {}), (140001, 90, 8, 0.6, {})])
 def test_compaction(gpu, workspace, in_place, pages, rows, page, share, layout):
     g = np.random.default_rng(pages + rows)
     live = int(pages * share)
