@@ -610,8 +610,10 @@ __device__ __forceinline__ uint32_t trim(uint64_t *list, uint32_t &entries, uint
 // its way. A lane adds up its own exponentials, in powers of two below its own
 // largest logit so far. The best: in a first tile, the `choices` best of the lanes'
 // own two largest (of their pieces' halves) bound what is taken from below, later the
-// last of those taken so far, by any wave of the block.
-template <typename T, uint32_t N>
+// last of those taken so far, by any wave of the block. A part of ONE tile is the same
+// without the next tile and the bounds for it (16 x 4 rows of 248,320 f32 logits 22.9
+// us in place of 24.2, 32 x 4 39.4 and 41.8).
+template <typename T, uint32_t N, bool ONE>
 __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, uint32_t row, const char *from,
                                           uint64_t *list, uint32_t *shared) {
     constexpr uint32_t kCount = Piece<T>::kCount, kPieces = N / kCount, kTile = kWave * N;
@@ -651,7 +653,7 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
         for (uint32_t j = 0; j < kPieces; ++j) {
             x[j] = next[j];
         }
-        if (end - at > kTile) {
+        if (!ONE && end - at > kTile) {
             load(next, at + kTile);
         }
         float half[2] = {-__builtin_huge_valf(), -__builtin_huge_valf()};
@@ -671,9 +673,11 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
                 max(reached_by(ascending_key(half[0]), ascending_key(half[1]), choices), kLowestKey + 1u);
             least = static_cast<uint64_t>(reached) << 32;
             edge = below(reached);
-            share(reached);
+            if (!ONE) {
+                share(reached);
+            }
         }
-        if (at != first) {
+        if (!ONE && at != first) {
             const uint32_t reached = *static_cast<volatile uint32_t *>(shared);
             least = max(least, static_cast<uint64_t>(reached) << 32);
             edge = fmaxf(edge, below(max(reached, kLowestKey + 1u)));
@@ -725,7 +729,7 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
                     }
                 }
             }
-            if (end - at > kTile && entries >= choices + choices / 2u + 4u) {
+            if (!ONE && end - at > kTile && entries >= choices + choices / 2u + 4u) {
                 if (entries <= kWave) {
                     const uint32_t reached = trim(list, entries, choices, lane);
                     least = max(least, static_cast<uint64_t>(reached) << 32);
@@ -745,6 +749,9 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
             for (uint32_t i = 0; i < kCount; ++i) {
                 total += e.of(x[j].get(i));
             }
+        }
+        if constexpr (ONE) {
+            break;
         }
     }
     const float most = wave_most(top);
@@ -777,13 +784,14 @@ __device__ __forceinline__ void beam_part(const BeamArgs &args, uint32_t part, u
 
 // A wave a part; where the launch joins, the last block of a request's through its
 // ticket does.
-// (Waves a SIMD that the registers are held to: bf16 rows fit in five without
-// spills, 512 rows of 248,320 115 us in place of 125; f32 and f16 rows spill.)
-template <typename T>
-constexpr int kResident = std::is_same_v<T, __bf16> ? 5 : 4;
+// (Waves a SIMD that the registers are held to: long parts of bf16 rows fit in five
+// without spills, 512 rows of 248,320 115 us in place of 125; f32 and f16 rows spill.
+// Parts of ONE tile take 69 to 75 registers either way.)
+template <typename T, bool ONE>
+constexpr int kResident = !ONE && std::is_same_v<T, __bf16> ? 5 : 4;
 
-template <typename T, uint32_t N, bool JOINS>
-__global__ __launch_bounds__(kThreads, kResident<T>) void k_beam_select(BeamArgs args) {
+template <typename T, uint32_t N, bool ONE, bool JOINS>
+__global__ __launch_bounds__(kThreads, (kResident<T, ONE>)) void k_beam_select(BeamArgs args) {
     __shared__ union Shared {
         uint64_t list[kWaves][kPartList];
         std::conditional_t<JOINS, JoinShared, uint32_t> join;
@@ -798,7 +806,7 @@ __global__ __launch_bounds__(kThreads, kResident<T>) void k_beam_select(BeamArgs
     if (part < args.parts) {
         const char *const from =
             args.logits + (blockIdx.z * args.request_stride + blockIdx.y * args.beam_stride) * sizeof(T);
-        beam_part<T, N>(args, part, row, from, lds.list[wave], &reached);
+        beam_part<T, N, ONE>(args, part, row, from, lds.list[wave], &reached);
     }
     if constexpr (JOINS) {
         wait_stores();
@@ -822,7 +830,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_join(BeamArgs args) {
     join_request(args, blockIdx.x, lds);
 }
 
-template <typename T, uint32_t N, bool JOINS>
+template <typename T, uint32_t N, bool ONE, bool JOINS>
 void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const adi_hip_paged_workspace &workspace,
                    uint32_t tiles) {
     BeamArgs args{};
@@ -860,7 +868,7 @@ void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const 
     for (uint64_t done = 0; done < a.requests; done += at_once) {
         const uint32_t requests = static_cast<uint32_t>(std::min<uint64_t>(at_once, a.requests - done));
         const dim3 grid(ceil_div(args.parts, kWaves), a.beams, requests), block(kThreads);
-        launch(ctx, "beam_select", k_beam_select<T, N, JOINS>, grid, block, 0, args);
+        launch(ctx, "beam_select", k_beam_select<T, N, ONE, JOINS>, grid, block, 0, args);
         if (!JOINS) {
             launch(ctx, "beam_join", k_beam_join, dim3(requests), block, 0, args);
         }
@@ -884,21 +892,21 @@ void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const 
 template <typename T>
 void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const adi_hip_paged_workspace &workspace) {
     const uint64_t rows = uint64_t(a.requests) * a.beams, cus = static_cast<uint64_t>(ctx->cu_count);
-    const auto go = [&](auto n) {
+    const auto single = [&](auto n) {
         constexpr uint32_t N = decltype(n)::value;
-        const uint64_t waves = rows * ceil_div(a.vocabulary, kWave * N);
-        const uint32_t tiles = static_cast<uint32_t>(std::clamp<uint64_t>(waves / (32u * cus), 1u, 16u));
-        const uint64_t blocks = rows * ceil_div(ceil_div(a.vocabulary, kWave * N * tiles), kWaves);
-        if (blocks <= cus / 8u) {
-            launch_select<T, N, true>(ctx, a, workspace, tiles);
+        if (rows * ceil_div(ceil_div(a.vocabulary, kWave * N), kWaves) <= cus / 8u) {
+            launch_select<T, N, true, true>(ctx, a, workspace, 1u);
         } else {
-            launch_select<T, N, false>(ctx, a, workspace, tiles);
+            launch_select<T, N, true, false>(ctx, a, workspace, 1u);
         }
     };
-    if (rows * ceil_div(a.vocabulary, kWave * 8u) <= cus) {
-        go(std::integral_constant<uint32_t, 8>());
+    const uint64_t tiles = std::min<uint64_t>(rows * ceil_div(a.vocabulary, kWave * 32u) / (32u * cus), 16u);
+    if (tiles > 1u) {
+        launch_select<T, 32, false, false>(ctx, a, workspace, static_cast<uint32_t>(tiles));
+    } else if (rows * ceil_div(a.vocabulary, kWave * 8u) <= cus) {
+        single(std::integral_constant<uint32_t, 8>());
     } else {
-        go(std::integral_constant<uint32_t, 32>());
+        single(std::integral_constant<uint32_t, 32>());
     }
 }
 
