@@ -882,19 +882,19 @@ void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const 
     }
 }
 
-// Tiles of 512 logits where that makes at most a wave a CU, else of 2048, and as
-// many a part as leave 32 waves a CU, about (one request of 4 x 248,320 f32 logits:
-// 14.4 us, with tiles of 1024 and 512 16.4 and 23.6, as more parts are joined; of 4 x
-// 32,000 in 512s 10.5, in 1024s 11.2). Few blocks join within the launch (4 x 512
-// logits: 8.3 us, with a launch of its own 8.8); more wait for each other at the
-// ticket, and the launch's end for the join (4 x 248,320: 14.5 and 13.8, 16 requests
-// of them 31 and 25.8).
+// Tiles of 512 logits where that makes at most a wave a CU, else of 2048 (one request
+// of 4 x 248,320 f32 logits: 12.5 us, with tiles of 1024 and 512 15.0 and 20.5, as
+// more parts are joined; of 4 x 512 in 512s 8.0, in 2048s 9.4), and as many a part as
+// leave 32 waves a CU, about. Up to half a block a CU the last of a request's blocks
+// joins within the launch (4 x 512 logits 8.0 us, by a launch of its own 9.5; 4 x
+// 32,000 9.8 and 10.5); more wait for each other at the ticket, and the launch's end
+// for the join (2 x 4 x 248,320: 13.9 and 12.5, 16 requests of them 36.7 and 23.2).
 template <typename T>
 void launch_select(adi_hip_context *ctx, const adi_hip_beam_arguments &a, const adi_hip_paged_workspace &workspace) {
     const uint64_t rows = uint64_t(a.requests) * a.beams, cus = static_cast<uint64_t>(ctx->cu_count);
     const auto single = [&](auto n) {
         constexpr uint32_t N = decltype(n)::value;
-        if (rows * ceil_div(ceil_div(a.vocabulary, kWave * N), kWaves) <= cus / 8u) {
+        if (rows * ceil_div(ceil_div(a.vocabulary, kWave * N), kWaves) <= cus / 2u) {
             launch_select<T, N, true, true>(ctx, a, workspace, 1u);
         } else {
             launch_select<T, N, true, false>(ctx, a, workspace, 1u);
