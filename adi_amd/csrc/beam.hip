@@ -936,6 +936,7 @@ void require_select(const adi_hip_beam_arguments *a) {
 
 // arrays of a launch; few of them, so that its arguments are few bytes
 constexpr uint32_t kArrays = 64, kFewArrays = 4;
+constexpr uint32_t kReorderBlocks = 1u << 23;  // of a launch
 
 struct RowArray {
     char *data;
@@ -1024,6 +1025,15 @@ __global__ __launch_bounds__(kThreads) void k_reorder_rows(ReorderArgs<ARRAYS> a
     }
 }
 
+// Blocks of a request's rows in an array.
+uint64_t reorder_blocks(uint64_t row_bytes, uint32_t beams) {
+    const uint64_t units = beams <= 4    ? kUnits<4>
+                           : beams <= 8  ? kUnits<8>
+                           : beams <= 16 ? kUnits<16>
+                                         : kUnits<64>;
+    return std::max<uint64_t>((row_bytes / 16u + kThreads * units - 1u) / (kThreads * units), 1u);
+}
+
 void require_reorder(const adi_hip_row_array *arrays, uint32_t count, uint32_t requests, uint32_t beams,
                      const uint32_t *parents) {
     require(beams >= 1 && beams <= kMaxBeams, "reorder rows: beams must be 1 to 64");
@@ -1042,6 +1052,8 @@ void require_reorder(const adi_hip_row_array *arrays, uint32_t count, uint32_t r
                     (requests == 1 || a.request_stride >= (beams - 1) * a.row_stride + a.row_bytes ||
                      (a.request_stride >= a.row_bytes && a.row_stride >= (requests - 1) * a.request_stride + a.row_bytes)),
                 "reorder rows: an array's rows overlap");
+        require(reorder_blocks(a.row_bytes, beams) * requests < kReorderBlocks,
+                "reorder rows: too many rows of such a size");
     }
 }
 
@@ -1084,14 +1096,9 @@ void reorder_rows(adi_hip_context *ctx, const adi_hip_row_array *arrays, uint32_
         }
         RowArray r{static_cast<char *>(a.data), a.request_stride, a.row_stride, a.row_bytes / 16, 0, 0,
                    static_cast<uint32_t>(a.row_bytes % 16)};
-        const uint64_t each = kThreads * (beams <= 4    ? kUnits<4>
-                                          : beams <= 8  ? kUnits<8>
-                                          : beams <= 16 ? kUnits<16>
-                                                        : kUnits<64>);
-        const uint64_t per = std::max<uint64_t>((r.units + each - 1) / each, 1);
-        require(per * requests < (1u << 23), "reorder rows: too many rows of such a size");
+        const uint64_t per = reorder_blocks(a.row_bytes, beams);
         r.blocks = static_cast<uint32_t>(per);
-        if (args.arrays == kArrays || blocks + per * requests >= (1u << 23)) {
+        if (args.arrays == kArrays || blocks + per * requests >= kReorderBlocks) {
             go();
         }
         r.first_block = blocks;

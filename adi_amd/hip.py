@@ -1376,8 +1376,9 @@ def paged_check(cache: PagedCacheStruct, offsets, lengths, table, tokens: int, m
 
 class PagedWorkspace:
     """Device memory in which attention calls join the parts of long
-    histories (adi_hip_paged_workspace); one for calls that may run at once
-    each."""
+    histories, and beam selection and the calls on a pool's pages keep what
+    they join and plan (adi_hip_paged_workspace); one for calls that may run
+    at once each."""
 
     def __init__(self, ctx: Context, size: int = 0):
         self.handle = None
@@ -1600,6 +1601,9 @@ class PagedPool:
         self.caches = list(caches)
         if not self.caches:
             _refuse("paged pool: caches must be 1 to 1024")
+        for c in self.caches:
+            if c.keys.get_device() != ctx.device:
+                _refuse(f"a paged pool on {c.keys.device}, the context is on cuda:{ctx.device}")
         self.pages, self.page_size = self.caches[0].pages, self.caches[0].page_size
         self.references, self.lacking = references, lacking
         if references is not None:

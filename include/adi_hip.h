@@ -824,7 +824,8 @@ int adi_hip_paged_append(adi_hip_context *ctx, const adi_hip_paged_cache *cache,
                          const adi_hip_paged_batch *batch,
                          const adi_hip_paged_append_arguments *arguments);
 
-/* Device memory in which attention calls join the parts of a long history:
+/* Device memory in which attention calls join the parts of a long history, and
+ * the calls of a beam search and on pages (below) keep what they join and plan:
  * `bytes` (0: 64 MiB; at least 1 MiB), allocated here, so that a call never
  * allocates and may be captured. Calls with one workspace run one after another
  * (one stream, or ordered by the caller): two captured graphs that may run at
@@ -890,10 +891,13 @@ int adi_hip_full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attent
  * of its next token, and a request takes the `choices` best of its candidates
  *   score(b, v) = scores[b] + (logit[b][v] - log sum_u exp(logit[b][u]))
  * by rank = weights[b] score(b, v) (no weights: 1; say 1 / length^a), best
- * first, ranks in 64 bits of exact logarithms; equal ranks: the lower beam, then
- * the larger logit, then the lower token. A beam that has `ended` (nonzero) is one
+ * first. Sums, logarithms (good to about 2^-32) and ranks are held in 64 bits;
+ * equal ranks: the lower beam, then the larger logit, then the lower token. Which
+ * of a beam's tokens comes first goes by their logits alone, and the outputs of
+ * a call are the same each time. A beam that has `ended` (nonzero) is one
  * candidate, ended_token with the score it has, whatever its logits hold. Outputs
- * are the candidates' scores (rounded to float), beams and tokens. It follows
+ * are the candidates' scores (rounded to float), beams and tokens; none overlaps an
+ * input or another. It follows
  * sample_token (src/generation.cpp:161-225) where that keeps one token of a row.
  *
  * Never chosen: tokens whose logit is -infinity, and anything of a beam whose
@@ -909,9 +913,10 @@ int adi_hip_full_attention_paged(adi_hip_context *ctx, const adi_hip_full_attent
  * child, ascending.
  *
  * The workspace (adi_hip_paged_workspace) holds 12 + 8 choices bytes for each
- * 8192 logits of a row, 2048 where there are few, and takes requests one after
- * another where it cannot hold all; ADI_HIP_OUT_OF_MEMORY where it cannot hold
- * one. Nothing is allocated, so a call may be captured. */
+ * part of a row: 2048 logits, 512 in calls of few logits, up to 32768 in those of
+ * many. Where it cannot hold all requests they are taken in turns;
+ * ADI_HIP_OUT_OF_MEMORY where it cannot hold one. Nothing is allocated, so a call
+ * may be captured. */
 typedef struct {
     uint32_t type;                        /* of the logits: ADI_HIP_F32, _F16, _BF16 */
     const void *logits;                   /* [requests][beams][vocabulary] */
@@ -925,7 +930,7 @@ typedef struct {
     const uint32_t *ended;                /* [requests][beams] or NULL */
     uint32_t ended_token;
     uint32_t settle;
-    float *out_scores;                    /* [requests][choices]; not the scores */
+    float *out_scores;                    /* [requests][choices] */
     uint32_t *parents, *tokens;           /* [requests][choices] */
 } adi_hip_beam_arguments;
 int adi_hip_beam_select(adi_hip_context *ctx, const adi_hip_beam_arguments *arguments,
@@ -938,9 +943,10 @@ int adi_hip_beam_check(const adi_hip_beam_arguments *arguments);
  * request becomes what row parents[request][b] (DEVICE) was; a parent that is
  * not below `beams` leaves the row as it is. Row b of request r is the row_bytes
  * bytes at data + r request_stride + b row_stride (all in bytes, of any size and
- * alignment; rows must not overlap). Rows that stay, and bytes between rows, are
- * not written. For sequence states as adi_hip_layer_state, token histories, and
- * the arrays of a search. beams: 1 to 64. */
+ * alignment; no row overlaps another, of its array or of the others, nor the
+ * parents). Rows that stay, and bytes between rows, are not written. For sequence
+ * states as adi_hip_layer_state, token histories, and the arrays of a search. beams:
+ * 1 to 64. */
 typedef struct {
     void *data;
     uint64_t request_stride, row_stride, row_bytes;

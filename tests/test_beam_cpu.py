@@ -131,6 +131,12 @@ def test_reorder_refusals():
     refused(lib.adi_hip_reorder_check(None, 1, 2, 4, 4), "null")
     refused(lib.adi_hip_reorder_check((hip.RowArray * 1)(hip.RowArray(None, 400, 100, 100)), 1, 2, 4, 4), "null array")
     refused(lib.adi_hip_reorder_check((hip.RowArray * 1)(hip.RowArray(4, 0, 1 << 46, 1 << 36)), 1, 1, 4, 4), "2^36")
+    # (a block moves 4 KB of 64 rows, 16 of four; all are checked before any is moved)
+    small, large = hip.RowArray(4, 1 << 30, 1 << 20, 16), hip.RowArray(4, 1 << 30, 1 << 20, 1 << 16)
+    both = (hip.RowArray * 2)(small, large)
+    refused(lib.adi_hip_reorder_check(both, 2, 1 << 19, 64, 4), "too many rows")
+    assert lib.adi_hip_reorder_check(both, 2, (1 << 19) - 1, 64, 4) == hip.OK
+    assert lib.adi_hip_reorder_check(both, 2, 1 << 19, 4, 4) == hip.OK
     assert lib.adi_hip_reorder_check(None, 0, 2, 4, None) == hip.OK
 
 

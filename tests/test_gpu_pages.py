@@ -467,6 +467,21 @@ def test_compaction(gpu, workspace, in_place, pages, rows, page, share, layout):
     assert all(torch.equal(t, w) for t, w in zip(tensors, data))
 
 
+@pytest.mark.parametrize("pages", [50, 5000])
+def test_compaction_of_more_caches_than_a_launch_takes(gpu, workspace, pages):
+    table = np.array([[pages - 1, 3, pages // 2]])
+    lengths, count = np.array([20]), np.zeros(pages, np.int64)
+    count[table[0]] = 1
+    tensors = made_caches(9, 70, pages, 8, 1, 64, "bf16")
+    live, want_table, want_count, moves = compacted(count, lengths, table, 8)
+    data = moved(tensors, moves)
+    d_table, d_count, d_live = ints(table), ints(count), ints([0])
+    hip.paged_compact(gpu, pool_of(gpu, tensors, d_count), ints(lengths), d_table, d_live, workspace)
+    assert int(d_live) == live == 3
+    assert np.array_equal(words(d_table), want_table) and np.array_equal(words(d_count), want_count)
+    assert all(torch.equal(t, w) for t, w in zip(tensors, data))
+
+
 def test_compaction_of_wrong_numbers_and_no_rows(gpu, workspace):
     """A table that names pages counted as free, and numbers that are no pages."""
     tensors = made_caches(1, 1, 40, 8, 1, 64, "f16")
