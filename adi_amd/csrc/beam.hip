@@ -271,7 +271,9 @@ __device__ __forceinline__ uint64_t read_lane(uint64_t v, uint32_t lane) {
 // Joins a request's parts: the beams' logarithms, 64 / `group` beams a wave, then the
 // candidates. The heads of the parts' lists (all candidates, where the lists are few)
 // bound what is taken from below, and of each list what reaches that bound goes to
-// a list in LDS, whose entries find their places by counting.
+// a list in LDS, whose entries find their places by counting. Bound by its chain of
+// loads, sums and barriers: 4 beams' 488 parts about 6 us, 64 requests of 8 beams with 16
+// choices 9.4.
 __device__ __forceinline__ void join_request(const BeamArgs &args, uint32_t request, JoinShared &lds) {
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t / kWave;
     const uint32_t k = args.beams, choices = args.choices, parts = args.parts;
@@ -610,7 +612,9 @@ __device__ __forceinline__ uint32_t trim(uint64_t *list, uint32_t &entries, uint
 // its way. A lane adds up its own exponentials, in powers of two below its own
 // largest logit so far. The best: in a first tile, the `choices` best of the lanes'
 // own two largest (of their pieces' halves) bound what is taken from below, later the
-// last of those taken so far, by any wave of the block. A part of ONE tile is the same
+// last of those taken so far, by any wave of the block. Bound by its instructions, 23
+// for 64 logits, 15 of them the exponential (64 x 8 rows of 248,320 bf16 logits: 107
+// us with the join, 2.4 TB/s); few tiles a wave by its start and end. A part of ONE tile is the same
 // without the next tile and the bounds for it (16 x 4 rows of 248,320 f32 logits 22.9
 // us in place of 24.2, 32 x 4 39.4 and 41.8).
 template <typename T, uint32_t N, bool ONE>

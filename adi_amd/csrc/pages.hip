@@ -20,8 +20,11 @@ constexpr uint32_t kMaxPages = 1u << 22;
 // pages of a segment: what a block counts
 constexpr uint32_t kSegment = 2048, kSegments = kMaxPages / kSegment;
 constexpr uint32_t kOwn = kSegment / kThreads;  // pages of a thread
-// pools of which one block finds the free pages (fork), or every block counts all
-// live ones (compaction)
+// Pools of which one block finds the free pages (fork), or every block counts all
+// live ones (compaction): a compaction saves a launch (100 pages 7.8 us on the device
+// and 11.1, 4,096 9.4 and 13.2), a fork its second kernel's search for a segment (4
+// rows 7.8 and 8.4, 128 rows over two segments 13.4 either way). At 8,192 the registers
+// for a thread's pages cost smaller pools a microsecond.
 constexpr uint32_t kSmallPages = 4096;
 
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
@@ -186,7 +189,9 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t entries, uint32_t shift) {
     return (entries >> shift) + ((entries & ((1u << shift) - 1u)) != 0u ? 1u : 0u);
 }
 
-// The rows' plans by the first block. Of a small pool (kSmallPages) it counts the
+// The rows' plans by the first block (bound by its chain of loads: a row's
+// parent, its length, its last page, the page's count: 4 rows 3.7 us, 128 5.2; one
+// block, so that a row's place among those that take pages is a sum within it). Of a small pool (kSmallPages) it counts the
 // free pages too, a run of them a thread, and lists the first of them, as many as
 // rows take; of others every block but the first lists a segment's. The others
 // copy the counts, where the new ones are apart from the old.
@@ -363,7 +368,9 @@ struct ForkCopyArgs {
 
 // The tables, a column of a request's rows a thread (each entry is read before any
 // is written, so that the old table may be the new one), and the copies: what a
-// block copies is on its way before it knows where it goes.
+// block copies is on its way before it knows where it goes. (Bound by a chain of
+// four loads, 4.2 us for 4 rows in ten caches; 128 rows, half of which copy parts of
+// pages, 22 MB in all, 8.4 us.)
 template <uint32_t K>
 __global__ __launch_bounds__(kThreads) void k_fork_apply(ForkArgs args, ForkCopyArgs copy) {
     __shared__ RowPlan plans[K];
@@ -510,7 +517,9 @@ __device__ __forceinline__ void segments_before(const uint32_t *count, uint32_t 
 }
 
 // The n-th live page behind the first `live` moves to the n-th free one below it.
-// (Of a small pool every block reads all counts, so that no launch before it has to.)
+// (Of a small pool every block reads all counts, so that no launch before it has to.
+// Bound by its loads and block-wide sums, one after another: 100 pages 4.3 us, 4,096
+// 6.)
 __global__ __launch_bounds__(kThreads) void k_compact_plan(CompactArgs args) {
     constexpr uint32_t kSmall = kSmallPages / kSegment;
     __shared__ uint32_t before[kSegments + 1u];
@@ -617,6 +626,9 @@ struct CompactCopyArgs {
     uint32_t pieces, table_blocks;
 };
 
+// The moves and the tables: blocks in turn over what the plan counted, as the host does
+// not know how much it is (908 of 4,096 pages of 16 KB in ten caches' keys and values,
+// 595 MB read and written: 121.6 us, 4.9 TB/s, HBM's rate for a copy).
 __global__ __launch_bounds__(kThreads) void k_compact_apply(CompactArgs args, CompactCopyArgs copy) {
     const uint32_t moves = *args.moves, live = *args.live;
     if (blockIdx.x >= copy.table_blocks) {
