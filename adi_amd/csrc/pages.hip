@@ -26,6 +26,12 @@ constexpr uint32_t kOwn = kSegment / kThreads;  // pages of a thread
 // rows 7.8 and 8.4, 128 rows over two segments 13.4 either way). At 8,192 the registers
 // for a thread's pages cost smaller pools a microsecond.
 constexpr uint32_t kSmallPages = 4096;
+// Pools that a compaction takes in one launch, and its blocks a CU that copy: those
+// whose old counts stay (1 cache of 100 pages of 32 KB 9.9 us in two launches and 7.0, of
+// 1,000 12.2 and 8.8, 10 caches 67.5 and 67.1, 30 184 and 190; of 4,096 34 and 39, as
+// every block reads all counts), and in place where no more than a block a CU copies
+// (9.7 and 6.7; a thousand blocks wait at their ticket for 10 us).
+constexpr uint32_t kTinyPages = 1024, kTinyCopiers = 4;
 
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 
@@ -479,6 +485,7 @@ struct CompactArgs {
     uint32_t *count;                     // live pages of each segment
     uint32_t *sources, *targets, *rank;  // [pages / 2] twice, [pages]
     uint32_t *moves;
+    uint32_t *ticket;  // of a tiny pool, zero between calls
 };
 
 // The free and live pages of long pools, a segment a block.
@@ -624,6 +631,7 @@ __global__ __launch_bounds__(kThreads) void k_compact_plan(CompactArgs args) {
 struct CompactCopyArgs {
     CachesView caches;
     uint32_t pieces, table_blocks;
+    uint32_t counts;  // 1: the counts are written too
 };
 
 // The moves and the tables: blocks in turn over what the plan counted, as the host does
@@ -660,6 +668,118 @@ __global__ __launch_bounds__(kThreads) void k_compact_apply(CompactArgs args, Co
             const uint32_t rank = page >= live && page < args.pages ? args.rank[page] : kNone;
             args.table[at] = rank != kNone ? args.targets[rank] : page;
         }
+    }
+}
+
+// A tiny pool in one launch: every block reads all counts and finds all moves, and
+// takes its share of them and of the tables. The counts are written by one block: the
+// first, or where they are the old ones too, the last through the ticket, when all
+// have read them.
+__global__ __launch_bounds__(kThreads) void k_compact_tiny(CompactArgs args, CompactCopyArgs copy) {
+    constexpr uint32_t kRun = kTinyPages / kThreads;
+    __shared__ uint32_t sums[kWaves];
+    __shared__ uint16_t sources[kTinyPages / 2u], targets[kTinyPages / 2u], name[kTinyPages];
+    __shared__ uint32_t kept_below, arrived;
+    const uint32_t t = threadIdx.x, run = (args.pages + kThreads - 1u) / kThreads, first = t * run;
+    const bool in_place = args.references == args.old_references;
+    uint32_t count[kRun], held = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        count[i] = i < run ? args.old_references[min(first + i, args.pages - 1u)] : 0u;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        count[i] = i < run && first + i < args.pages ? count[i] : 0u;
+        held |= count[i] != 0u ? 1u << i : 0u;
+    }
+    uint32_t live = 0u;
+    const uint32_t before = block_before(static_cast<uint32_t>(__popc(held)), sums, live);
+    if (live - first < run) {
+        kept_below = before + static_cast<uint32_t>(__popc(held & ((1u << (live - first)) - 1u)));
+    } else if (t == 0u && live == kThreads * run) {
+        kept_below = live;
+    }
+    if (t == 0u && in_place && copy.counts != 0u) {
+        arrived = coherent_add(args.ticket, 1u);
+    }
+    __syncthreads();
+    const uint32_t kept = kept_below, moves = live - kept;
+    uint32_t at = before;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        const bool lives = (held >> i & 1u) != 0u;
+        const uint32_t page = first + i;
+        if (i < run && page < args.pages) {
+            if (lives && page >= live) {
+                sources[at - kept] = static_cast<uint16_t>(page);
+            } else if (!lives && page < live) {
+                targets[page - at] = static_cast<uint16_t>(page);
+            }
+        }
+        at += lives ? 1u : 0u;
+    }
+    __syncthreads();
+    if (blockIdx.x >= copy.table_blocks) {
+        // (pieces of 16 KB of memory that exists: their number fits)
+        const uint32_t work = moves * copy.caches.arrays * copy.pieces;
+        for (uint32_t w = blockIdx.x - copy.table_blocks; w < work; w += gridDim.x - copy.table_blocks) {
+            const uint32_t piece = w % copy.pieces, rest = w / copy.pieces;
+            const uint32_t n = rest % copy.caches.arrays, i = rest / copy.caches.arrays;
+            PieceOfPage<kAhead> x;
+            x.load(copy.caches, n, sources[i], 1u << args.page_shift, piece);
+            x.store(copy.caches, copy.caches, n, targets[i], 1u << args.page_shift, piece);
+        }
+    } else {
+        at = before;
+#pragma unroll
+        for (uint32_t i = 0; i < kRun; ++i) {
+            const bool lives = (held >> i & 1u) != 0u;
+            const uint32_t page = first + i;
+            if (i < run && page < args.pages) {
+                name[page] = lives && page >= live ? targets[at - kept] : static_cast<uint16_t>(page);
+            }
+            at += lives ? 1u : 0u;
+        }
+        __syncthreads();
+        const uint32_t step = copy.table_blocks * kThreads;
+        for (uint64_t i = blockIdx.x * kThreads + t; i < static_cast<uint64_t>(args.rows) * args.columns; i += step) {
+            const uint32_t row = static_cast<uint32_t>(i / args.columns), c = static_cast<uint32_t>(i % args.columns);
+            if (c < pages_of(args.lengths[row], args.page_shift)) {
+                const uint64_t place = static_cast<uint64_t>(row) * args.stride + c;
+                const uint32_t page = args.old_table[place];
+                args.table[place] = page < args.pages ? name[page] : page;
+            }
+        }
+    }
+    if (blockIdx.x == 0u && t == 0u) {
+        *args.live = live;
+    }
+    if (copy.counts == 0u || (in_place ? arrived != gridDim.x - 1u : blockIdx.x != 0u)) {
+        return;
+    }
+    at = before;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        const bool lives = (held >> i & 1u) != 0u;
+        const uint32_t page = first + i;
+        if (i < run && page < args.pages) {
+            if (page >= live) {
+                count[i] = 0u;
+            } else if (!lives) {
+                count[i] = args.old_references[sources[page - at]];
+            }
+        }
+        at += lives ? 1u : 0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        if (i < run && first + i < args.pages) {
+            args.references[first + i] = count[i];
+        }
+    }
+    if (t == 0u && in_place) {
+        coherent_store(args.ticket, 0u);
     }
 }
 
@@ -867,24 +987,46 @@ void paged_compact(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const a
     args.pages = c.pages;
     args.segments = ceil_div(c.pages, kSegment);
     args.live = a->live;
-    args.count = scratch.take<uint32_t>(args.segments);
-    args.sources = scratch.take<uint32_t>(c.pages / 2u + 1u);
-    args.targets = scratch.take<uint32_t>(c.pages / 2u + 1u);
-    args.rank = scratch.take<uint32_t>(c.pages);
-    args.moves = scratch.take<uint32_t>(1);
     CompactCopyArgs copy{};
     copy.pieces = pieces_of(c, c.page_size, kAhead);
-    const uint64_t words = std::max<uint64_t>(uint64_t(a->rows) * args.columns, c.pages / 2u + 1u);
-    copy.table_blocks = static_cast<uint32_t>(std::min<uint64_t>((words + kThreads - 1) / kThreads, ctx->cu_count));
+    const uint64_t work = uint64_t(c.pages / 2u) * 2u * std::min(pool->caches, kCaches) * copy.pieces;
+    const bool tiny = c.pages <= kTinyPages && (work <= ctx->cu_count || args.references != args.old_references);
+    const uint64_t words = std::max<uint64_t>(uint64_t(a->rows) * args.columns, tiny ? 1u : c.pages / 2u + 1u);
+    const uint32_t table_blocks =
+        static_cast<uint32_t>(std::min<uint64_t>((words + kThreads - 1) / kThreads, ctx->cu_count));
+    const auto copiers = [&](uint32_t a_cu) {
+        return static_cast<uint32_t>(std::min<uint64_t>(uint64_t(c.pages / 2u) * copy.caches.arrays * copy.pieces,
+                                                        a_cu * ctx->cu_count));
+    };
+    if (tiny) {
+        args.ticket = static_cast<uint32_t *>(workspace->base);
+        for (uint32_t first = 0; first < pool->caches; first += kCaches) {
+            // the tables and counts are the last launch's, as they may be the old ones
+            const bool last = pool->caches - first <= kCaches;
+            copy.caches = caches_view(*pool, first);
+            copy.table_blocks = last ? table_blocks : 0u;
+            copy.counts = last ? 1u : 0u;
+            const uint32_t blocks = copy.table_blocks + copiers(kTinyCopiers);
+            if (blocks != 0) {
+                launch(ctx, "compact_tiny", k_compact_tiny, dim3(blocks), dim3(kThreads), 0, args, copy);
+            }
+        }
+        return;
+    }
+    args.count = scratch.take<uint32_t>(args.segments);
+    args.sources = scratch.take<uint32_t>(c.pages / 2u);
+    args.targets = scratch.take<uint32_t>(c.pages / 2u);
+    args.rank = scratch.take<uint32_t>(c.pages);
+    args.moves = scratch.take<uint32_t>(1);
     if (c.pages > kSmallPages) {
         launch(ctx, "compact_count", k_compact_count, dim3(args.segments), dim3(kThreads), 0, args);
     }
     launch(ctx, "compact_plan", k_compact_plan, dim3(args.segments), dim3(kThreads), 0, args);
+    copy.table_blocks = table_blocks;
     for (uint32_t first = 0; first < pool->caches; first += kCaches) {
         copy.caches = caches_view(*pool, first);
-        const uint64_t work = uint64_t(c.pages / 2u) * copy.caches.arrays * copy.pieces;
-        const uint32_t copiers = static_cast<uint32_t>(std::min<uint64_t>(work, 16u * ctx->cu_count));
-        launch(ctx, "compact_apply", k_compact_apply, dim3(copy.table_blocks + copiers), dim3(kThreads), 0, args, copy);
+        launch(ctx, "compact_apply", k_compact_apply, dim3(copy.table_blocks + copiers(16u)), dim3(kThreads), 0, args,
+               copy);
         copy.table_blocks = 0;
     }
 }

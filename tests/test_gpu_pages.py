@@ -467,6 +467,36 @@ def test_compaction(gpu, workspace, in_place, pages, rows, page, share, layout):
     assert all(torch.equal(t, w) for t, w in zip(tensors, data))
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("pages,rows,share", [(2, 1, 0.5), (3, 2, 0.7), (16, 3, 0.5), (255, 9, 0.4), (256, 9, 1.0), (256, 9, 0.5),
+                                              (257, 9, 0.6), (700, 40, 0.05), (1023, 33, 0.5), (1024, 33, 0.97),
+                                              (1024, 33, 1.0), (1025, 33, 0.5)])
+def test_compaction_of_tiny_pools(gpu, workspace, in_place, pages, rows, share):
+    test_compaction(gpu, workspace, in_place, pages, rows, 8, share, {})
+
+
+def test_compaction_in_place_again_and_again(gpu):
+    # one workspace, calls behind one another with nothing between them
+    space = hip.PagedWorkspace(gpu, 1 << 20)
+    g = np.random.default_rng(3)
+    cases = []
+    for pages in (40, 64, 7, 40, 900):
+        table = g.permutation(pages)[:pages // 2][None, :]
+        count = np.zeros(pages, np.int64)
+        count[table[0]] = 1
+        tensors = made_caches(pages, 1, pages, 8, 1, 64, "bf16")
+        lengths = np.array([8 * table.shape[1]])
+        live, new, after, moves = compacted(count, lengths, table, 8)
+        cases.append((pool_of(gpu, tensors, ints(count)), ints(lengths), ints(table), ints([0]), tensors,
+                      moved(tensors, moves), live, new, after))
+    for pool, lengths, table, live, *_ in cases:
+        hip.paged_compact(gpu, pool, lengths, table, live, space)
+    for pool, _, table, live, tensors, data, want_live, want_table, want_count in cases:
+        assert int(live) == want_live
+        assert np.array_equal(words(table), want_table) and np.array_equal(words(pool.references), want_count)
+        assert all(torch.equal(t, w) for t, w in zip(tensors, data))
+
+
 @pytest.mark.parametrize("pages", [50, 5000])
 def test_compaction_of_more_caches_than_a_launch_takes(gpu, workspace, pages):
     table = np.array([[pages - 1, 3, pages // 2]])
@@ -476,9 +506,12 @@ def test_compaction_of_more_caches_than_a_launch_takes(gpu, workspace, pages):
     live, want_table, want_count, moves = compacted(count, lengths, table, 8)
     data = moved(tensors, moves)
     d_table, d_count, d_live = ints(table), ints(count), ints([0])
-    hip.paged_compact(gpu, pool_of(gpu, tensors, d_count), ints(lengths), d_table, d_live, workspace)
+    # (the table in place, the counts not; then all of it again, in place and with none to move)
+    after = torch.full_like(d_count, 9)
+    hip.paged_compact(gpu, pool_of(gpu, tensors, after), ints(lengths), d_table, d_live, workspace, references=d_count)
+    hip.paged_compact(gpu, pool_of(gpu, tensors, after), ints(lengths), d_table, d_live, workspace)
     assert int(d_live) == live == 3
-    assert np.array_equal(words(d_table), want_table) and np.array_equal(words(d_count), want_count)
+    assert np.array_equal(words(d_table), want_table) and np.array_equal(words(after), want_count)
     assert all(torch.equal(t, w) for t, w in zip(tensors, data))
 
 
