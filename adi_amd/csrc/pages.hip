@@ -21,10 +21,10 @@ constexpr uint32_t kMaxPages = 1u << 22;
 constexpr uint32_t kSegment = 2048, kSegments = kMaxPages / kSegment;
 constexpr uint32_t kOwn = kSegment / kThreads;  // pages of a thread
 // Pools of which one block finds the free pages (fork), or every block counts all
-// live ones (compaction): a compaction saves a launch (100 pages 7.8 us on the device
-// and 11.1, 4,096 9.4 and 13.2), a fork its second kernel's search for a segment (4
-// rows 7.8 and 8.4, 128 rows over two segments 13.4 either way). At 8,192 the registers
-// for a thread's pages cost smaller pools a microsecond.
+// live ones (compaction): a compaction saves a launch (4,096 pages 9.4 us on the device
+// and 13.2), a fork its second kernel's search for a segment (4 rows 7.8 and 8.4, 128
+// rows over two segments 13.4 either way). At 8,192 the registers for a thread's pages
+// cost smaller pools a microsecond.
 constexpr uint32_t kSmallPages = 4096;
 // Pools that a compaction takes in one launch, and its blocks a CU that copy: those
 // whose old counts stay (1 cache of 100 pages of 32 KB 9.9 us in two launches and 7.0, of
@@ -32,6 +32,11 @@ constexpr uint32_t kSmallPages = 4096;
 // every block reads all counts), and in place where no more than a block a CU copies
 // (9.7 and 6.7; a thousand blocks wait at their ticket for 10 us).
 constexpr uint32_t kTinyPages = 1024, kTinyCopiers = 4;
+// A fork does so with up to 256 rows, by the same number of blocks that copy, where the
+// one that writes the tables has so many runs of 256 columns to go through, or one
+// request's (4 beams of 2,005 entries 9.8 us in two launches and 6.9, 8 of 1,000 10.7 and
+// 8.1, 16 of 300 14.8 and 11.9; 4 requests of 4 beams, 16 runs, 9.5 and 11.4).
+constexpr uint32_t kTinyTables = 12;
 
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 
@@ -189,10 +194,55 @@ struct ForkArgs {
     uint32_t *free_count, *free_page;  // [segments], [segments][kSegment]; in a small pool [1], [pages]
     uint32_t *demand;                  // of all rows
     uint32_t small;
+    uint32_t *ticket;  // of a tiny pool, zero between calls
 };
 
 __device__ __forceinline__ uint32_t pages_of(uint32_t entries, uint32_t shift) {
     return (entries >> shift) + ((entries & ((1u << shift) - 1u)) != 0u ? 1u : 0u);
+}
+
+// A row's plan, but for the pages that rows before it take (no row: one that takes none).
+__device__ __forceinline__ RowPlan plan_of(const ForkArgs &args, uint32_t row) {
+    RowPlan plan{0u, 0u, 0u, kNone, kNone, 0u, 0u, 0u};
+    if (row >= args.rows) {
+        return plan;
+    }
+    const uint32_t page_mask = (1u << args.page_shift) - 1u;
+    const uint32_t group = row / args.beams * args.beams, parent = args.parents[row];
+    const uint32_t a = min(args.offsets[row], args.tokens), b = min(args.offsets[row + 1u], args.tokens);
+    plan.held = args.old_lengths[row];
+    plan.added = b > a ? b - a : 0u;
+    if (parent < args.beams) {
+        plan.parent = group + parent;
+        plan.parents = args.old_lengths[plan.parent];
+    }
+    const uint64_t next = static_cast<uint64_t>(plan.parents) + plan.added;
+    plan.over = plan.added > args.max_tokens || next > args.max_length ? 1u : 0u;
+    if (plan.over == 0u) {
+        plan.demand = pages_of(plan.parents + plan.added, args.page_shift) -
+                      pages_of(plan.parents, args.page_shift);
+        const uint32_t last = plan.parents >> args.page_shift;
+        if ((plan.parents & page_mask) != 0u && plan.added != 0u && last < args.old_stride) {
+            const uint32_t page = args.old_table[static_cast<uint64_t>(plan.parent) * args.old_stride + last];
+            bool eldest = true;
+            for (uint32_t others = group; others < row; others += 8u) {
+                uint32_t of_others[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    of_others[i] = args.parents[min(others + i, row)];
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    eldest = eldest && (others + i >= row || of_others[i] != parent);
+                }
+            }
+            if (page < args.pages && !(eldest && args.old_references[page] == 1u)) {
+                plan.source = page;
+                plan.demand += 1u;
+            }
+        }
+    }
+    return plan;
 }
 
 // The rows' plans by the first block (bound by its chain of loads: a row's
@@ -248,39 +298,10 @@ __global__ __launch_bounds__(kThreads) void k_fork_plan(ForkArgs args) {
             }
         }
     }
-    const uint32_t page_mask = (1u << args.page_shift) - 1u;
     uint32_t taken = 0u;
     for (uint32_t base = 0; base < args.rows; base += kThreads) {
         const uint32_t row = base + t;
-        RowPlan plan{0u, 0u, 0u, kNone, kNone, 0u, 0u, 0u};
-        if (row < args.rows) {
-            const uint32_t group = row / args.beams * args.beams, parent = args.parents[row];
-            const uint32_t a = min(args.offsets[row], args.tokens), b = min(args.offsets[row + 1u], args.tokens);
-            plan.held = args.old_lengths[row];
-            plan.added = b > a ? b - a : 0u;
-            if (parent < args.beams) {
-                plan.parent = group + parent;
-                plan.parents = args.old_lengths[plan.parent];
-            }
-            const uint64_t next = static_cast<uint64_t>(plan.parents) + plan.added;
-            plan.over = plan.added > args.max_tokens || next > args.max_length ? 1u : 0u;
-            if (plan.over == 0u) {
-                plan.demand = pages_of(plan.parents + plan.added, args.page_shift) -
-                              pages_of(plan.parents, args.page_shift);
-                const uint32_t last = plan.parents >> args.page_shift;
-                if ((plan.parents & page_mask) != 0u && plan.added != 0u && last < args.old_stride) {
-                    const uint32_t page = args.old_table[static_cast<uint64_t>(plan.parent) * args.old_stride + last];
-                    bool eldest = true;
-                    for (uint32_t other = group; other < row; ++other) {
-                        eldest = eldest && args.parents[other] != parent;
-                    }
-                    if (page < args.pages && !(eldest && args.old_references[page] == 1u)) {
-                        plan.source = page;
-                        plan.demand += 1u;
-                    }
-                }
-            }
-        }
+        RowPlan plan = plan_of(args, row);
         uint32_t all = 0u;
         plan.before = taken + block_before(plan.demand, sums, all);
         taken += all;
@@ -370,12 +391,93 @@ struct ForkCopyArgs {
     CachesView caches;
     uint32_t pieces, table_blocks, column_blocks;
     uint64_t work;  // pieces of all rows and arrays
+    uint32_t in_place;
 };
 
-// The tables, a column of a request's rows a thread (each entry is read before any
-// is written, so that the old table may be the new one), and the copies: what a
-// block copies is on its way before it knows where it goes. (Bound by a chain of
-// four loads, 4.2 us for 4 rows in ten caches; 128 rows, half of which copy parts of
+// Column c of a request's rows (its first is `group`), parent by parent: each entry is
+// read before any is written, so that the old table may be the new one. Counts change by take(page), a
+// page's first holder, and add(page, change); nth(n) is the n-th free page. Every
+// thread of the block is here.
+template <uint32_t K, typename Nth, typename Take, typename Add>
+__device__ __forceinline__ void fork_column(const ForkArgs &args, const RowPlan *plans, uint32_t group, uint32_t c,
+                                            Nth &&nth, Take &&take, Add &&add) {
+    uint32_t x[K], kept[K];
+#pragma unroll
+    for (uint32_t q = 0; q < K; ++q) {
+        x[q] = kNone;
+        kept[q] = 0u;
+        if (q < args.beams && c < min(pages_of(plans[q].held, args.page_shift), args.old_stride)) {
+            x[q] = args.old_table[static_cast<uint64_t>(group + q) * args.old_stride + c];
+        }
+    }
+    // a lane's row, read from there by its number
+    const uint32_t lane = threadIdx.x & 63u;
+    const RowPlan own = plans[min(lane, args.beams - 1u)];
+    const auto of_row = [](uint32_t v, uint32_t row) {
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), static_cast<int>(row)));
+    };
+    const auto child = [&](uint32_t s, uint32_t parents_page, uint32_t &keeps) {
+        const uint32_t parents = of_row(own.parents, s), added = of_row(own.added, s);
+        const bool has_source = of_row(own.source, s) != kNone;
+        const uint32_t held = pages_of(parents, args.page_shift);
+        const uint32_t end = static_cast<uint32_t>(
+            min((static_cast<uint64_t>(parents) + added + (1u << args.page_shift) - 1u) >> args.page_shift,
+                static_cast<uint64_t>(args.stride)));
+        const bool copies = c < end && has_source && c == parents >> args.page_shift;
+        const bool takes = copies || (c < end && c >= held && of_row(own.over, s) == 0u);
+        uint32_t page = !takes && c < held ? parents_page : kNone;
+        keeps += c < end && !takes && c < held ? 1u : 0u;
+        if (__ballot(takes) != 0u) {
+            const uint32_t n = of_row(own.before, s) + (copies ? 0u : c - held + (has_source ? 1u : 0u));
+            const uint32_t taken = nth(takes ? n : kNone);
+            if (takes && taken != kNone) {
+                page = taken;
+                take(page);
+            }
+        }
+        if (c < end) {
+            args.table[static_cast<uint64_t>(group + s) * args.stride + c] = page;
+        }
+        if (c == 0u) {
+            args.lengths[group + s] =
+                static_cast<uint32_t>(min(static_cast<uint64_t>(parents) + added, uint64_t(kNone)));
+        }
+    };
+    const uint32_t parent = lane < args.beams ? own.parent - group : K;
+#pragma unroll
+    for (uint32_t q = 0; q < K; ++q) {
+        for (uint64_t left = __ballot(parent == q); left != 0u; left &= left - 1u) {
+            child(static_cast<uint32_t>(__builtin_ctzll(left)), x[q], kept[q]);
+        }
+    }
+    uint32_t none = 0u;
+    for (uint64_t left = __ballot(lane < args.beams && own.parent == kNone); left != 0u; left &= left - 1u) {
+        child(static_cast<uint32_t>(__builtin_ctzll(left)), kNone, none);
+    }
+    // a page's holders of the request, counted once where they follow each other
+    uint32_t page = kNone, change = 0u;
+#pragma unroll
+    for (uint32_t q = 0; q < K; ++q) {
+        if (x[q] < args.pages) {
+            if (x[q] != page) {
+                if (change != 0u) {
+                    add(page, change);
+                }
+                page = x[q];
+                change = 0u;
+            }
+            change += kept[q] - 1u;
+        }
+    }
+    if (change != 0u) {
+        add(page, change);
+    }
+}
+
+// The tables, a column of a request's rows a thread, and the copies: what a block
+// copies is on its way before it knows where it goes. (Bound by a chain of
+// four loads, 4.2 us for 4 rows in ten caches, and a request's rows one after another
+// where they take pages, half a microsecond each: 64 beams 37 us in all; 128 rows of 4, half of which copy parts of
 // pages, 22 MB in all, 8.4 us.)
 template <uint32_t K>
 __global__ __launch_bounds__(kThreads) void k_fork_apply(ForkArgs args, ForkCopyArgs copy) {
@@ -409,68 +511,98 @@ __global__ __launch_bounds__(kThreads) void k_fork_apply(ForkArgs args, ForkCopy
         plans[t] = args.plan[group + t];
     }
     __syncthreads();
-    uint32_t x[K], kept[K];
+    fork_column<K>(
+        args, plans, group, c, [&](uint32_t n) { return free.nth(args, n); },
+        [&](uint32_t page) { args.references[page] = 1u; },
+        [&](uint32_t page, uint32_t change) { atomicAdd(&args.references[page], change); });
+}
+
+// Tiny pools and few rows in one launch: every block plans all rows and finds the free
+// pages, and takes its share of the copies. One block writes the tables, lengths and
+// counts (counted in LDS): the first, which copies nothing, or where any of them are the
+// old ones too the last through the ticket, when all have read them. (Bound by its
+// chain: the plan's four loads, the sums' barriers, the tables: 5.6 us for 4 rows, where
+// two launches take 8.)
+template <uint32_t K>
+__global__ __launch_bounds__(kThreads) void k_fork_tiny(ForkArgs args, ForkCopyArgs copy) {
+    constexpr uint32_t kRun = kTinyPages / kThreads;
+    __shared__ RowPlan plans[kThreads];
+    __shared__ uint32_t counts[kTinyPages];
+    __shared__ uint16_t free[kTinyPages];
+    __shared__ uint32_t sums[kWaves];
+    __shared__ uint32_t arrived;
+    const uint32_t t = threadIdx.x, run = (args.pages + kThreads - 1u) / kThreads, first = t * run;
+    uint32_t count[kRun], own = 0u;
 #pragma unroll
-    for (uint32_t q = 0; q < K; ++q) {
-        x[q] = kNone;
-        kept[q] = 0u;
-        if (q < args.beams && c < min(pages_of(plans[q].held, args.page_shift), args.old_stride)) {
-            x[q] = args.old_table[static_cast<uint64_t>(group + q) * args.old_stride + c];
+    for (uint32_t i = 0; i < kRun; ++i) {
+        count[i] = i < run ? args.old_references[min(first + i, args.pages - 1u)] : 1u;
+    }
+    RowPlan plan = plan_of(args, t);
+    uint32_t demand = 0u, all = 0u;
+    plan.before = block_before(plan.demand, sums, demand);
+    plans[t] = plan;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        count[i] = i < run && first + i < args.pages ? count[i] : 1u;
+        own += count[i] == 0u ? 1u : 0u;
+    }
+    uint32_t at = block_before(own, sums, all);
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        if (count[i] == 0u) {
+            free[at++] = static_cast<uint16_t>(first + i);
         }
     }
-    for (uint32_t s = 0; s < args.beams; ++s) {
-        const RowPlan plan = plans[s];
-        const uint32_t held = pages_of(plan.parents, args.page_shift);
-        const uint32_t end = static_cast<uint32_t>(
-            min((static_cast<uint64_t>(plan.parents) + plan.added + (1u << args.page_shift) - 1u) >> args.page_shift,
-                static_cast<uint64_t>(args.stride)));
-        const bool copies = c < end && plan.source != kNone && c == plan.parents >> args.page_shift;
-        const bool takes = copies || (c < end && c >= held && plan.over == 0u);
-        uint32_t taken = kNone;
-        if (__ballot(takes) != 0u) {
-            const uint32_t n = plan.before + (copies ? 0u : c - held + (plan.source != kNone ? 1u : 0u));
-            taken = free.nth(args, takes ? n : kNone);
-        }
-        if (c < end) {
-            uint32_t page = kNone;
-            if (takes) {
-                page = taken;
-                if (page != kNone) {
-                    args.references[page] = 1u;
-                }
-            } else if (c < held) {
-#pragma unroll
-                for (uint32_t q = 0; q < K; ++q) {
-                    if (group + q == plan.parent) {
-                        page = x[q];
-                        kept[q] += 1u;
-                    }
-                }
+    if (t == 0u && copy.in_place != 0u) {
+        arrived = coherent_add(args.ticket, 1u);
+    }
+    __syncthreads();
+    const uint32_t copiers = copy.in_place != 0u ? gridDim.x : gridDim.x - 1u;
+    if (copy.in_place != 0u || blockIdx.x != 0u) {
+        for (uint32_t w = blockIdx.x - (gridDim.x - copiers); w < copy.work; w += copiers) {
+            const uint32_t piece = w % copy.pieces, rest = w / copy.pieces;
+            const uint32_t n = rest % copy.caches.arrays;
+            const RowPlan row = plans[rest / copy.caches.arrays];
+            if (row.source != kNone && row.before < all) {
+                const uint32_t entries = row.parents & ((1u << args.page_shift) - 1u);
+                PieceOfPage<kAhead> x;
+                x.load(copy.caches, n, row.source, entries, piece);
+                x.store(copy.caches, copy.caches, n, free[row.before], entries, piece);
             }
-            args.table[static_cast<uint64_t>(group + s) * args.stride + c] = page;
-        }
-        if (blockIdx.x % copy.column_blocks == 0u && t == 0u) {
-            args.lengths[group + s] =
-                static_cast<uint32_t>(min(static_cast<uint64_t>(plan.parents) + plan.added, uint64_t(kNone)));
         }
     }
-    // a page's holders of the request, counted once where they follow each other
-    uint32_t page = kNone, change = 0u;
+    if (copy.in_place != 0u ? arrived != gridDim.x - 1u : blockIdx.x != 0u) {
+        return;
+    }
 #pragma unroll
-    for (uint32_t q = 0; q < K; ++q) {
-        if (x[q] < args.pages) {
-            if (x[q] != page) {
-                if (change != 0u) {
-                    atomicAdd(&args.references[page], change);
-                }
-                page = x[q];
-                change = 0u;
-            }
-            change += kept[q] - 1u;
+    for (uint32_t i = 0; i < kRun; ++i) {
+        if (i < run && first + i < args.pages) {
+            counts[first + i] = count[i];
         }
     }
-    if (change != 0u) {
-        atomicAdd(&args.references[page], change);
+    __syncthreads();
+    for (uint32_t b = 0; b < copy.table_blocks; ++b) {
+        const uint32_t group = b / copy.column_blocks * args.beams;
+        fork_column<K>(
+            args, plans + group, group, b % copy.column_blocks * kThreads + t,
+            [&](uint32_t n) { return n < all ? static_cast<uint32_t>(free[n]) : kNone; },
+            [&](uint32_t page) { counts[page] = 1u; },
+            [&](uint32_t page, uint32_t change) { atomicAdd(&counts[page], change); });
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) {
+        if (i < run && first + i < args.pages) {
+            args.references[first + i] = counts[first + i];
+        }
+    }
+    if (t == 0u) {
+        if (args.lacking != nullptr) {
+            *args.lacking = demand > all ? demand - all : 0u;
+        }
+        if (copy.in_place != 0u) {
+            coherent_store(args.ticket, 0u);
+        }
     }
 }
 
@@ -674,7 +806,7 @@ __global__ __launch_bounds__(kThreads) void k_compact_apply(CompactArgs args, Co
 // A tiny pool in one launch: every block reads all counts and finds all moves, and
 // takes its share of them and of the tables. The counts are written by one block: the
 // first, or where they are the old ones too, the last through the ticket, when all
-// have read them.
+// have read them. (100 pages: 4.9 us, two launches 7.8.)
 __global__ __launch_bounds__(kThreads) void k_compact_tiny(CompactArgs args, CompactCopyArgs copy) {
     constexpr uint32_t kRun = kTinyPages / kThreads;
     __shared__ uint32_t sums[kWaves];
@@ -891,14 +1023,36 @@ void paged_fork(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const adi_
     args.tokens = batch->tokens;
     args.max_tokens = batch->max_tokens;
     args.lacking = pool->lacking;
-    args.plan = scratch.take<RowPlan>(args.rows);
-    args.free_count = scratch.take<uint32_t>(args.segments);
-    args.free_page = scratch.take<uint32_t>(uint64_t(args.segments) * kSegment);
-    args.demand = scratch.take<uint32_t>(1);
     ForkCopyArgs copy{};
     copy.pieces = pieces_of(c, c.page_size - 1u, kAhead);
     copy.column_blocks = ceil_div(std::max(args.old_stride, args.stride), kThreads);
     copy.table_blocks = args.rows / args.beams * copy.column_blocks;
+    copy.work = uint64_t(args.rows) * 2u * std::min(pool->caches, kCaches) * copy.pieces;
+    copy.in_place = args.lengths == args.old_lengths || args.table == args.old_table ||
+                    args.references == args.old_references;
+    const auto of_beams = [&](auto &&go) {
+        if (args.beams <= 4) {
+            go(std::integral_constant<uint32_t, 4>());
+        } else if (args.beams <= 16) {
+            go(std::integral_constant<uint32_t, 16>());
+        } else {
+            go(std::integral_constant<uint32_t, 64>());
+        }
+    };
+    if (c.pages <= kTinyPages && args.rows <= kThreads && pool->caches <= kCaches && (copy.table_blocks == 1u || copy.table_blocks * args.beams <= kTinyTables) &&
+        copy.work <= (copy.in_place != 0u ? 1u : kTinyCopiers) * ctx->cu_count) {
+        args.ticket = static_cast<uint32_t *>(workspace->base);
+        copy.caches = caches_view(*pool, 0);
+        const dim3 grid(static_cast<uint32_t>(copy.work) + (copy.in_place != 0u ? 0u : 1u)), block(kThreads);
+        of_beams([&](auto k) {
+            launch(ctx, "fork_tiny", k_fork_tiny<decltype(k)::value>, grid, block, 0, args, copy);
+        });
+        return;
+    }
+    args.plan = scratch.take<RowPlan>(args.rows);
+    args.free_count = scratch.take<uint32_t>(args.segments);
+    args.free_page = scratch.take<uint32_t>(uint64_t(args.segments) * kSegment);
+    args.demand = scratch.take<uint32_t>(1);
     args.small = c.pages <= kSmallPages ? 1u : 0u;
     const uint32_t others = args.small != 0u && args.references == args.old_references ? 0u : args.segments;
     launch(ctx, "fork_plan", k_fork_plan, dim3(1u + others), dim3(kThreads), 0, args);
@@ -907,13 +1061,9 @@ void paged_fork(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const adi_
         copy.work = uint64_t(args.rows) * copy.caches.arrays * copy.pieces;
         const uint32_t copiers = static_cast<uint32_t>(std::min<uint64_t>(copy.work, 16u * ctx->cu_count));
         const dim3 grid(copy.table_blocks + copiers), block(kThreads);
-        if (args.beams <= 4) {
-            launch(ctx, "fork_apply", k_fork_apply<4>, grid, block, 0, args, copy);
-        } else if (args.beams <= 16) {
-            launch(ctx, "fork_apply", k_fork_apply<16>, grid, block, 0, args, copy);
-        } else {
-            launch(ctx, "fork_apply", k_fork_apply<64>, grid, block, 0, args, copy);
-        }
+        of_beams([&](auto k) {
+            launch(ctx, "fork_apply", k_fork_apply<decltype(k)::value>, grid, block, 0, args, copy);
+        });
         copy.table_blocks = 0;
     }
 }
