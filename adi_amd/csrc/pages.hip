@@ -476,9 +476,9 @@ __device__ __forceinline__ void fork_column(const ForkArgs &args, const RowPlan 
 
 // The tables, a column of a request's rows a thread, and the copies: what a block
 // copies is on its way before it knows where it goes. (Bound by a chain of
-// four loads, 4.2 us for 4 rows in ten caches, and a request's rows one after another
-// where they take pages, half a microsecond each: 64 beams 37 us in all; 128 rows of 4, half of which copy parts of
-// pages, 22 MB in all, 8.4 us.)
+// four loads, 4.2 us for 4 rows in ten caches, and by a request's rows one after another
+// where they take pages, half a microsecond each; 32 requests of 4, half of whose rows
+// copy parts of pages, 22 MB in all, 8.0 us.)
 template <uint32_t K>
 __global__ __launch_bounds__(kThreads) void k_fork_apply(ForkArgs args, ForkCopyArgs copy) {
     __shared__ RowPlan plans[K];

@@ -291,6 +291,71 @@ def test_more_caches_than_a_launch_takes(gpu, workspace):
     assert all(torch.equal(a, w) for a, w in zip(b.tensors, want))
 
 
+@pytest.mark.parametrize("pages", [1023, 1024, 1025])
+@pytest.mark.parametrize("beams,requests,columns", [(4, 1, 700), (4, 3, 200), (1, 12, 40), (1, 13, 40), (16, 1, 60), (64, 1, 256),
+                                                    (64, 1, 257)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_forks_in_one_launch_and_two(gpu, workspace, pages, beams, requests, columns, in_place):
+    """At the borders between them, the first columns and the last, to the last page."""
+    rows = beams * requests
+    b = Books(gpu, workspace, rows, beams, columns, pages, 8, caches=1, heads=1)
+    g = np.random.default_rng(pages + rows + columns)
+    first = np.zeros((requests, beams), int)
+    first[:, 0] = min(columns - 3, (pages - 30) // requests) * 8 - 5
+    b.step(np.full(rows, -1), first)
+    b.step(np.zeros(rows, int), np.ones(rows, int), in_place=in_place)
+    for i in range(3):
+        b.step(g.integers(0, beams, rows), g.integers(0, 8, rows), in_place=in_place)
+    # more than there are pages
+    b.step(g.integers(0, beams, rows), np.where(np.arange(rows) % 2 == 0, 16, 1), in_place=in_place, max_length=columns * 8)
+
+
+@pytest.mark.parametrize("own", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)])
+def test_fork_of_arrays_partly_in_place(gpu, workspace, own):
+    b = Books(gpu, workspace, 8, 4, 12, 100, 8)
+    b.step(np.full(8, -1), [21, 0, 0, 0, 9, 0, 0, 0])
+    b.step([0] * 8, [1] * 8)
+    parents, added = np.array([3, 1, 1, 0, 2, 2, 7, 0]), np.array([1, 1, 2, 0, 1, 9, 3, 1])
+    want = forked(parents, 4, added, b.lengths, b.table, b.count, 8, 100, 12, 96, 9)
+    data = moved(b.tensors, want[4])
+    old = [b.d_lengths, b.d_table, b.d_count]
+    new = [t if o else t.clone() for t, o in zip(old, own)]
+    pool = pool_of(gpu, b.tensors, new[2], b.d_lacking)
+    batch = hip.PagedBatch(gpu, ints(np.concatenate([[0], np.cumsum(added)])), new[0], new[1], int(added.sum()), 9, 96)
+    hip.paged_fork(gpu, pool, batch, ints(parents).view(2, 4), workspace, lengths=old[0], table=old[1], references=old[2])
+    for (s, c), p in want[1].items():
+        b.table[s, c] = p
+    assert np.array_equal(words(new[0]), want[0]) and np.array_equal(words(new[1]), b.table)
+    assert np.array_equal(words(new[2]), want[2]) and int(b.d_lacking) == want[3]
+    assert all(torch.equal(t, w) for t, w in zip(b.tensors, data))
+
+
+def test_one_workspace_for_calls_of_all_kinds(gpu):
+    """Selection, forks and compactions behind one another, of sizes that join through
+    the workspace's tickets and of others."""
+    space = hip.PagedWorkspace(gpu)
+    b = Books(gpu, space, 4, 4, 12, 60, 8, caches=1, heads=1)
+    b.step(np.full(4, -1), [21, 0, 0, 0])
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for i, v in enumerate((500, 9000, 33, 100000, 500)):
+        logits = torch.randn((1, 4, v), generator=g, device="cuda")
+        scores = torch.randn((1, 4), generator=g, device="cuda")
+        out = torch.empty((1, 4), device="cuda")
+        parents, tokens = ints(np.zeros((1, 4))), ints(np.zeros((1, 4)))
+        hip.beam_select(gpu, logits, scores, out, parents, tokens, space)
+        rank = (scores.double()[..., None] + torch.log_softmax(logits.double(), -1)).view(-1)
+        best = torch.argsort(rank, descending=True, stable=True)[:4]
+        assert torch.equal(parents[0].long(), best // v) and torch.equal(tokens[0].long(), best % v)
+        b.step(words(parents), [1] * 4, in_place=i % 2 == 0)
+        live, table, count, moves = compacted(b.count, b.lengths, b.table, 8)
+        data, d_live = moved(b.tensors, moves), ints([0])
+        hip.paged_compact(gpu, b.pool, b.d_lengths, b.d_table, d_live, space)
+        b.table, b.count = table, count
+        assert int(d_live) == live and np.array_equal(words(b.d_table), table)
+        assert np.array_equal(words(b.d_count), count)
+        assert all(torch.equal(t, w) for t, w in zip(b.tensors, data))
+
+
 def test_fork_captured(gpu, workspace):
     """A step recorded once, replayed with new parents over what it wrote itself."""
     b = Books(gpu, workspace, 8, 4, 12, 150, 8, caches=2)
