@@ -245,12 +245,12 @@ __device__ __forceinline__ RowPlan plan_of(const ForkArgs &args, uint32_t row) {
     return plan;
 }
 
-// The rows' plans by the first block (bound by its chain of loads: a row's
-// parent, its length, its last page, the page's count: 4 rows 3.7 us, 128 5.2; one
-// block, so that a row's place among those that take pages is a sum within it). Of a small pool (kSmallPages) it counts the
-// free pages too, a run of them a thread, and lists the first of them, as many as
-// rows take; of others every block but the first lists a segment's. The others
-// copy the counts, where the new ones are apart from the old.
+// The rows' plans by the first block (bound by its chain of loads: a row's parent, its
+// length, its last page, the page's count: 4 rows 3.7 us, 128 5.2; one block, so that a
+// row's place among those that take pages is a sum within it). Of a small pool
+// (kSmallPages) it counts the free pages too, a run of them a thread, and lists the first
+// of them, as many as rows take; of others every block but the first lists a segment's.
+// The others copy the counts, where the new ones are apart from the old.
 __global__ __launch_bounds__(kThreads) void k_fork_plan(ForkArgs args) {
     __shared__ uint32_t sums[kWaves];
     const uint32_t t = threadIdx.x;
