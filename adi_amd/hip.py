@@ -7,10 +7,12 @@ loudly when the library is not built: there is no fallback path.
 """
 from __future__ import annotations
 
+import collections
 import ctypes as C
 import os
 import struct
 from dataclasses import dataclass
+from functools import partial
 from typing import Optional
 
 import numpy as np
@@ -352,13 +354,74 @@ def _addr(t) -> Optional[int]:
     return t.data_ptr()
 
 
-class Context:
+# What objects dropped without close() held: (object, its calls).
+_dropped = collections.deque()
+
+
+def release_dropped() -> None:
+    """Frees the library's objects whose owners were dropped without close().
+    Freeing one waits for the device, which ends a capture on any stream, and
+    finalizers run wherever the collector does, so they only leave their handles
+    here; what creates or closes such an object, and Context.synchronize, call
+    this first, as they touch the device themselves. A context waits for its
+    graphs and batchers. Nothing while the current stream captures."""
+    if not _dropped:
+        return
+    import torch
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        return
+    waiting = []
+    while _dropped:
+        try:
+            owner, calls = _dropped.popleft()
+        except IndexError:  # (another thread's)
+            break
+        if owner._users:
+            waiting.append((owner, calls))
+            continue
+        for call in calls:
+            call()
+        owner = calls = None  # (which may drop what it held)
+        _dropped.extend(waiting)
+        waiting.clear()
+    _dropped.extend(waiting)
+
+
+class _Owner:
+    """An object that owns handles of the library: close() frees them at once;
+    dropped without it, they wait for release_dropped(), and so does all that the
+    object holds."""
+
+    _users = ()  # of a context: the handles that must be freed before it
+
+    def _take(self) -> list:
+        """The calls that free what is held; it is held no more."""
+        raise NotImplementedError
+
+    def close(self) -> None:
+        calls = self._take()
+        if calls:
+            release_dropped()
+        for call in calls:
+            call()
+
+    def __del__(self):
+        try:
+            calls = self._take()
+            if calls:
+                _dropped.append((self, calls))
+        except Exception:
+            pass
+
+
+class Context(_Owner):
     """One adi_hip_context bound to torch's current stream on `device`."""
 
     def __init__(self, device: int = 0, isa_lanes: int = 16):
         import torch
         self.torch = torch
         self.lib = load()
+        release_dropped()
         handle = vp()
         status = self.lib.adi_hip_context_create(device, C.byref(handle))
         if status != OK:
@@ -366,6 +429,7 @@ class Context:
         self.handle = handle
         self.device = device
         self._books = []
+        self._users = set()
         self.check(self.lib.adi_hip_set_stream(self.handle, vp(torch.cuda.current_stream(device).cuda_stream)))
         self.set_isa(isa_lanes)
 
@@ -384,6 +448,7 @@ class Context:
 
     def synchronize(self) -> None:
         self.check(self.lib.adi_hip_synchronize(self.handle))
+        release_dropped()
 
     def set_fused_decode(self, enabled) -> None:
         """One persistent launch for a MoE block of 1-12 rows and for NE
@@ -398,23 +463,18 @@ class Context:
         would grow one beyond it fails with OUT_OF_MEMORY."""
         self.check(self.lib.adi_hip_set_workspace_limit(self.handle, (1 << 64) - 1 if limit is None else limit))
 
-    def close(self) -> None:
-        if getattr(self, "handle", None):
-            for book in self._books:
-                self.lib.adi_hip_codebook_destroy(book)
-            self._books = []
-            self.lib.adi_hip_context_destroy(self.handle)
-            self.handle = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+    def _take(self) -> list:
+        if not getattr(self, "handle", None):
+            return []
+        calls = [partial(self.lib.adi_hip_codebook_destroy, book) for book in self._books]
+        calls.append(partial(self.lib.adi_hip_context_destroy, self.handle))
+        self._books, self.handle = [], None
+        return calls
 
     # -- codebooks --
     def expert_codebook(self, tlut: np.ndarray) -> int:
         tlut = np.ascontiguousarray(tlut, np.float32)
+        release_dropped()
         out = vp()
         self.check(self.lib.adi_hip_codebook_create_expert(self.handle, tlut.ctypes.data, C.byref(out)))
         self._books.append(out)
@@ -422,6 +482,7 @@ class Context:
 
     def ne_codebook(self, tlut: np.ndarray) -> int:
         tlut = np.ascontiguousarray(tlut, np.float32)
+        release_dropped()
         out = vp()
         self.check(self.lib.adi_hip_codebook_create_ne(self.handle, tlut.ctypes.data, C.byref(out)))
         self._books.append(out)
@@ -683,8 +744,14 @@ class Gguf:
             self._fail(status)
 
 
+class _GgufWeights(_Owner):
+    def _take(self) -> list:
+        weights, self.weights = getattr(self, "weights", 0), 0
+        return [partial(self.lib.adi_hip_weights_destroy, vp(weights))] if weights else []
+
+
 @dataclass
-class GgufMoeLayer:
+class GgufMoeLayer(_GgufWeights):
     """A layer uploaded from a checkpoint; owns its adi_hip_weights."""
     struct: MoeLayer
     weights: int
@@ -692,19 +759,9 @@ class GgufMoeLayer:
     hidden: int
     lib: object = None
 
-    def close(self) -> None:
-        if self.weights:
-            self.lib.adi_hip_weights_destroy(vp(self.weights))
-            self.weights = 0
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
-
 
 def upload_codebooks_gguf(ctx: Context, file: Gguf):
+    release_dropped()
     expert, ne = vp(), vp()
     ctx.check(ctx.lib.adi_hip_gguf_upload_codebooks(ctx.handle, file.handle, C.byref(expert), C.byref(ne)))
     ctx._books.extend([expert, ne])
@@ -713,6 +770,7 @@ def upload_codebooks_gguf(ctx: Context, file: Gguf):
 
 def upload_moe_layer_gguf(ctx: Context, file: Gguf, layer: int, expert_book: int,
                           ne_book: int) -> GgufMoeLayer:
+    release_dropped()
     weights = vp()
     s = MoeLayer()
     ctx.check(ctx.lib.adi_hip_gguf_upload_moe_layer(ctx.handle, file.handle, layer, vp(expert_book),
@@ -721,46 +779,25 @@ def upload_moe_layer_gguf(ctx: Context, file: Gguf, layer: int, expert_book: int
 
 
 @dataclass
-class GgufEmbedding:
+class GgufEmbedding(_GgufWeights):
     """An embedding table uploaded from a checkpoint; owns its adi_hip_weights."""
     struct: Embedding
     weights: int
     lib: object = None
 
-    def close(self) -> None:
-        if self.weights:
-            self.lib.adi_hip_weights_destroy(vp(self.weights))
-            self.weights = 0
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
-
 
 @dataclass
-class GgufDecoderLayer:
+class GgufDecoderLayer(_GgufWeights):
     """A whole decoder layer uploaded from a checkpoint (norms, attention,
     MoE block); owns its adi_hip_weights."""
     struct: DecoderLayerStruct
     weights: int
     lib: object = None
 
-    def close(self) -> None:
-        if self.weights:
-            self.lib.adi_hip_weights_destroy(vp(self.weights))
-            self.weights = 0
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
-
 
 def upload_decoder_layer_gguf(ctx: Context, file: Gguf, layer: int, expert_book: int,
                               ne_book: int) -> GgufDecoderLayer:
+    release_dropped()
     weights = vp()
     s = DecoderLayerStruct()
     ctx.check(ctx.lib.adi_hip_gguf_upload_decoder_layer(ctx.handle, file.handle, layer, vp(expert_book),
@@ -769,7 +806,7 @@ def upload_decoder_layer_gguf(ctx: Context, file: Gguf, layer: int, expert_book:
 
 
 @dataclass
-class GgufHead:
+class GgufHead(_GgufWeights):
     """The output head (eight chunks end to end) and the final norm uploaded
     from a checkpoint; owns its adi_hip_weights."""
     struct: HeadChunk
@@ -777,19 +814,9 @@ class GgufHead:
     weights: int
     lib: object = None
 
-    def close(self) -> None:
-        if self.weights:
-            self.lib.adi_hip_weights_destroy(vp(self.weights))
-            self.weights = 0
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
-
 
 def upload_head_gguf(ctx: Context, file: Gguf) -> GgufHead:
+    release_dropped()
     weights, norm = vp(), vp()
     s = HeadChunk()
     ctx.check(ctx.lib.adi_hip_gguf_upload_head(ctx.handle, file.handle, C.byref(weights), C.byref(s),
@@ -798,6 +825,7 @@ def upload_head_gguf(ctx: Context, file: Gguf) -> GgufHead:
 
 
 def upload_embedding_gguf(ctx: Context, file: Gguf) -> GgufEmbedding:
+    release_dropped()
     weights = vp()
     s = Embedding()
     ctx.check(ctx.lib.adi_hip_gguf_upload_embedding(ctx.handle, file.handle, C.byref(weights),
@@ -1120,7 +1148,7 @@ def decode_batch(ctx: Context, model: Model, tokens, sequences, logits=None) -> 
     ctx.check(status)
 
 
-class DecodeGraph:
+class DecodeGraph(_Owner):
     """adi_hip_decode_graph: one decode step of `sequences` captured as a HIP
     graph. Each launch() replays it: the step's tokens are read from
     `tokens` (device int32/uint32 [len(sequences)]), logits go to `logits`
@@ -1128,8 +1156,10 @@ class DecodeGraph:
     position advances by one."""
 
     def __init__(self, ctx: Context, model: Model, sequences, tokens, logits=None):
+        self.handle = None
         self.ctx, self.model, self.sequences = ctx, model, list(sequences)
         self._keep = (tokens, logits)
+        release_dropped()
         n = len(self.sequences)
         self._states = (DecoderStateStruct * max(n, 1))(*(s.struct for s in self.sequences))
         handle = vp()
@@ -1137,6 +1167,7 @@ class DecodeGraph:
                                                       self._states, _addr(tokens), _addr(logits),
                                                       C.byref(handle)))
         self.handle = handle
+        ctx._users.add(handle.value)
 
     def launch(self) -> None:
         for st, s in zip(self._states, self.sequences):
@@ -1150,16 +1181,12 @@ class DecodeGraph:
     def captures(self) -> int:
         return int(self.ctx.lib.adi_hip_decode_graph_captures(self.handle))
 
-    def close(self) -> None:
-        if self.handle:
-            self.ctx.lib.adi_hip_decode_graph_destroy(self.handle)
-            self.handle = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+    def _take(self) -> list:
+        handle, self.handle = self.handle, None
+        if not handle:
+            return []
+        return [partial(self.ctx.lib.adi_hip_decode_graph_destroy, handle),
+                partial(self.ctx._users.discard, handle.value)]
 
 
 def prefill(ctx: Context, model: Model, tokens, sequence: Sequence, logits=None,
@@ -1279,7 +1306,7 @@ def rope_frequencies(rotary: int, layout: str = "halves", theta: float = 1e4, sc
     return out, m.value
 
 
-class Rope:
+class Rope(_Owner):
     """A rotation's frequencies on the device (adi_hip_rope): `rotary`
     dimensions of a head, in "halves" or "pairs", scaled for a context `factor`
     times the `original` one by "linear", "ntk", "yarn" or "bands"."""
@@ -1289,20 +1316,14 @@ class Rope:
                  slow: float = 0.0, magnitude: float = 0.0):
         self.handle = None
         o = _rope_options(rotary, layout, theta, scaling, factor, original, fast, slow, magnitude)
+        release_dropped()
         handle = vp()
         ctx.check(ctx.lib.adi_hip_rope_create(ctx.handle, C.byref(o), C.byref(handle)))
         self.lib, self.handle, self.rotary = ctx.lib, handle, rotary
 
-    def close(self) -> None:
-        if self.handle:
-            self.lib.adi_hip_rope_destroy(self.handle)
-            self.handle = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+    def _take(self) -> list:
+        handle, self.handle = self.handle, None
+        return [partial(self.lib.adi_hip_rope_destroy, handle)] if handle else []
 
 
 def rope_rows(ctx: Context, rope: Rope, x, positions, out) -> None:
@@ -1374,7 +1395,7 @@ def paged_check(cache: PagedCacheStruct, offsets, lengths, table, tokens: int, m
         raise HipError(status, lib.adi_hip_last_error(None).decode())
 
 
-class PagedWorkspace:
+class PagedWorkspace(_Owner):
     """Device memory in which attention calls join the parts of long
     histories, and beam selection and the calls on a pool's pages keep what
     they join and plan (adi_hip_paged_workspace); one for calls that may run
@@ -1382,20 +1403,14 @@ class PagedWorkspace:
 
     def __init__(self, ctx: Context, size: int = 0):
         self.handle = None
+        release_dropped()
         handle = vp()
         ctx.check(ctx.lib.adi_hip_paged_workspace_create(ctx.handle, size, C.byref(handle)))
         self.lib, self.handle = ctx.lib, handle
 
-    def close(self) -> None:
-        if self.handle:
-            self.lib.adi_hip_paged_workspace_destroy(self.handle)
-            self.handle = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+    def _take(self) -> list:
+        handle, self.handle = self.handle, None
+        return [partial(self.lib.adi_hip_paged_workspace_destroy, handle)] if handle else []
 
 
 def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, keys, values, rope: Optional[Rope] = None,

@@ -19,6 +19,7 @@ import ctypes as C
 import threading
 import time
 from dataclasses import dataclass
+from functools import partial
 from typing import Callable, Optional, Sequence
 
 from . import hip
@@ -42,12 +43,14 @@ class GenerationError(RuntimeError):
     pass
 
 
-class ContinuousBatcher:
+class ContinuousBatcher(hip._Owner):
     def __init__(self, ctx: hip.Context, model: hip.Model, max_batch: int = 16,
                  capacity: int = 4096, prefill_ubatch: int = 128,
                  stop_tokens: Sequence[int] = (), masked_tokens: Sequence[int] = (),
                  start: bool = True, replay_steps: bool = True):
+        self.handle, self._thread = None, None
         self.ctx, self.model = ctx, model
+        hip.release_dropped()
         stop = (hip.u32 * max(len(stop_tokens), 1))(*stop_tokens)
         masked = (hip.u32 * max(len(masked_tokens), 1))(*masked_tokens)
         options = hip.BatcherOptions(max_batch, capacity, prefill_ubatch, stop, len(stop_tokens),
@@ -56,13 +59,13 @@ class ContinuousBatcher:
         ctx.check(ctx.lib.adi_hip_batcher_create(ctx.handle, C.byref(model.struct),
                                                  C.byref(options), C.byref(handle)))
         self.handle = handle
+        ctx._users.add(handle.value)
         self._cond = threading.Condition()
         self._stop = False
         self._work = 0          # requests pending or active, as of the last step
         self._submitted = 0     # submissions so far
         self._steps = 0
         self._failure: Optional[hip.HipError] = None
-        self._thread = None
         if start:
             self._thread = threading.Thread(target=self._run, name="adi-batcher", daemon=True)
             self._thread.start()
@@ -179,15 +182,13 @@ class ContinuousBatcher:
                 self._cond.notify_all()
             self._thread.join()
             self._thread = None
-        if self.handle:
-            self.ctx.lib.adi_hip_batcher_destroy(self.handle)
-            self.handle = None
+        super().close()
 
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+    def _take(self) -> list:
+        handle, self.handle = self.handle, None
+        if not handle:
+            return []
+        return [partial(self.ctx.lib.adi_hip_batcher_destroy, handle), partial(self.ctx._users.discard, handle.value)]
 
 
 @dataclass
@@ -302,9 +303,3 @@ class BeamSearch:
         if getattr(self, "_workspace", None) is not None:
             self._workspace.close()
             self._workspace = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass

@@ -44,7 +44,9 @@ typedef struct adi_hip_codebook adi_hip_codebook;
 /* ---- context ------------------------------------------------------------ */
 
 /* Creates a context on `device` (HIP ordinal). Replaces cpu_backend()
- * (src/backend.cpp:11-26): one context is one backend instance. */
+ * (src/backend.cpp:11-26): one context is one backend instance. Creating and
+ * destroying an object of the library allocates, frees and waits for the device,
+ * which a capture on any stream of the process may not survive: none meanwhile. */
 int adi_hip_context_create(int device, adi_hip_context **out);
 void adi_hip_context_destroy(adi_hip_context *ctx);
 
