@@ -388,7 +388,8 @@ def release_dropped() -> None:
 
 
 class _Owner:
-    """An object that owns handles of the library: close() frees them at once;
+    """An object that owns handles of the library: close() frees them at once (a
+    context's, when its graphs and batchers are closed: they use it until then);
     dropped without it, they wait for release_dropped(), and so does all that the
     object holds."""
 
@@ -402,6 +403,9 @@ class _Owner:
         calls = self._take()
         if calls:
             release_dropped()
+        if calls and self._users:
+            _dropped.append((self, calls))
+            return
         for call in calls:
             call()
 

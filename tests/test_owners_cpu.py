@@ -211,3 +211,21 @@ def test_a_dropped_search_does_not_touch_the_device(lib):
     gc.collect()
     hip.release_dropped()
     assert sorted(handle for _, handle in lib.calls) == [1, 3, 5]
+
+
+@pytest.mark.parametrize("kind", [hip.DecodeGraph, serving.ContinuousBatcher])
+@pytest.mark.parametrize("how", ["close", "drop"])
+def test_a_closed_context_outlives_what_uses_it(lib, kind, how):
+    """Freeing a graph or a batcher waits for the context's stream, so the context
+    goes after it."""
+    ctx = context(lib, 1, books=[7])
+    o = used(ctx, kind, 5)
+    ctx.close()
+    assert lib.calls == []
+    if how == "close":
+        o.close()
+    del o
+    hip.release_dropped()
+    assert [handle for _, handle in lib.calls] == [5, 7, 1]
+    ctx.close()
+    assert len(lib.calls) == 3
