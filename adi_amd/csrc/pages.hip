@@ -606,6 +606,18 @@ __global__ __launch_bounds__(kThreads) void k_fork_tiny(ForkArgs args, ForkCopyA
     }
 }
 
+// A batch of no rows: the counts as they were, and no page lacks.
+__global__ __launch_bounds__(kThreads) void k_fork_none(const uint32_t *old_references, uint32_t *references,
+                                                        uint32_t pages, uint32_t *lacking) {
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+    if (i < pages) {
+        references[i] = old_references[i];
+    }
+    if (i == 0u && lacking != nullptr) {
+        *lacking = 0u;
+    }
+}
+
 // ---- compaction -----------------------------------------------------------------
 
 struct CompactArgs {
@@ -957,6 +969,7 @@ void require_fork(const adi_hip_paged_pool *pool, const adi_hip_paged_batch *bat
     require(a->beams >= 1 && a->beams <= kMaxBeams && batch->sequences % a->beams == 0,
             "paged fork: beams must be 1 to 64, and sequences a multiple of them");
     if (batch->sequences == 0) {
+        require(aligned_to(a->references, 4), "paged fork: unaligned argument");
         return;
     }
     require(a->parents != nullptr && a->lengths != nullptr && a->table != nullptr && a->references != nullptr &&
@@ -999,10 +1012,15 @@ void paged_fork(adi_hip_context *ctx, const adi_hip_paged_pool *pool, const adi_
                 const adi_hip_paged_fork_arguments *a, const adi_hip_paged_workspace *workspace) {
     require_fork(pool, batch, a);
     Scratch scratch = scratch_of(ctx, workspace);
+    const adi_hip_paged_cache &c = pool->cache[0];
     if (batch->sequences == 0) {
+        const uint32_t copied = a->references != nullptr && a->references != pool->references ? c.pages : 0u;
+        if (copied != 0u || pool->lacking != nullptr) {
+            launch(ctx, "fork_none", k_fork_none, dim3(std::max(ceil_div(copied, kThreads), 1u)), dim3(kThreads), 0,
+                   a->references, pool->references, copied, pool->lacking);
+        }
         return;
     }
-    const adi_hip_paged_cache &c = pool->cache[0];
     ForkArgs args{};
     args.old_lengths = a->lengths;
     args.old_table = a->table;

@@ -991,7 +991,8 @@ typedef struct {
  * and the last rows' table entries for them are 0xFFFFFFFF: nothing is appended
  * there, and rows that see them are NaN. A row over the batch's bounds
  * (max_tokens, max_length) takes no pages; its length says so, its entries for
- * them are 0xFFFFFFFF. Page numbers that are not the pool's are not counted.
+ * them are 0xFFFFFFFF. Page numbers that are not the pool's are not counted. A
+ * batch of no sequences is a call too: counts as they were, none lacking.
  *
  * The old lengths, table and references may be the batch's and the pool's own
  * (in place, one stride), or others, which stay valid until the next call: a step
