@@ -419,7 +419,7 @@ class _Owner:
 
 
 class Context(_Owner):
-    """One adi_hip_context bound to torch's current stream on `device`."""
+    """One adi_hip_context bound to torch's current stream on `device` (`stream`)."""
 
     def __init__(self, device: int = 0, isa_lanes: int = 16):
         import torch
@@ -434,12 +434,13 @@ class Context(_Owner):
         self.device = device
         self._books = []
         self._users = set()
-        self.check(self.lib.adi_hip_set_stream(self.handle, vp(torch.cuda.current_stream(device).cuda_stream)))
+        self.use_stream(torch.cuda.current_stream(device))
         self.set_isa(isa_lanes)
 
     def use_stream(self, stream) -> None:
         """Launch on `stream` (a torch stream) from now on."""
         self.check(self.lib.adi_hip_set_stream(self.handle, vp(stream.cuda_stream)))
+        self.stream = stream
 
     # -- plumbing --
     def check(self, status: int) -> None:

@@ -15,6 +15,7 @@ when `cancelled()` turns true, as generate_from_prompt does. The worker owns
 the context while the batcher runs: other work must not use it meanwhile."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 import time
@@ -209,8 +210,10 @@ class BeamSearch:
     states follow their parents in place (hip.BeamStates), and the beams decode
     as a batch, recorded once as a HIP graph and replayed (replay_steps=False
     launches every step directly; both give the same bits). Beams that have ended stay as
-    one candidate each; candidates are compared by sum / length^length_penalty. One
-    search at a time; the context must not be used otherwise meanwhile."""
+    one candidate each; candidates are compared by sum / length^length_penalty. All
+    work runs on the context's stream, whichever torch's current one is, behind what
+    the caller's holds. One search at a time; the context must not be used otherwise
+    meanwhile."""
 
     def __init__(self, ctx: hip.Context, model: hip.Model, beams: int = 4, capacity: int = 4096,
                  length_penalty: float = 0.0, stop_tokens: Sequence[int] = (), masked_tokens: Sequence[int] = (),
@@ -224,18 +227,31 @@ class BeamSearch:
         torch = ctx.torch
         self.ctx, self.model, self.beams, self.capacity = ctx, model, beams, capacity
         self.length_penalty, self.ubatch, self.replay_steps = float(length_penalty), prefill_ubatch, replay_steps
-        device = f"cuda:{ctx.device}"
-        self._stop = torch.tensor(list(stop_tokens), dtype=torch.int32, device=device)
-        self._ended_token = int(stop_tokens[0]) if len(stop_tokens) else 0
-        self._masked = torch.tensor(list(masked_tokens), dtype=torch.int64, device=device)
-        self._logits = torch.empty((1, beams, model.vocabulary), dtype=torch.float32, device=device)
-        self._history = torch.zeros((1, beams, capacity), dtype=torch.int32, device=device)
-        self._tokens = torch.zeros((1, beams), dtype=torch.int32, device=device)
-        self._parents = torch.zeros((1, beams), dtype=torch.int32, device=device)
-        self._scores = [torch.zeros((1, beams), dtype=torch.float32, device=device) for _ in range(2)]
-        self._workspace = hip.PagedWorkspace(ctx)
-        self._states = hip.BeamStates(ctx, model, beams, capacity, more=[self._history])
         self._graph: Optional[hip.DecodeGraph] = None
+        self._made: Optional[object] = None  # the stream of the last work on what follows
+        with self._on_stream():
+            device = f"cuda:{ctx.device}"
+            self._stop = torch.tensor(list(stop_tokens), dtype=torch.int32, device=device)
+            self._ended_token = int(stop_tokens[0]) if len(stop_tokens) else 0
+            self._masked = torch.tensor(list(masked_tokens), dtype=torch.int64, device=device)
+            self._logits = torch.empty((1, beams, model.vocabulary), dtype=torch.float32, device=device)
+            self._history = torch.zeros((1, beams, capacity), dtype=torch.int32, device=device)
+            self._tokens = torch.zeros((1, beams), dtype=torch.int32, device=device)
+            self._parents = torch.zeros((1, beams), dtype=torch.int32, device=device)
+            self._scores = [torch.zeros((1, beams), dtype=torch.float32, device=device) for _ in range(2)]
+            self._workspace = hip.PagedWorkspace(ctx)
+            self._states = hip.BeamStates(ctx, model, beams, capacity, more=[self._history])
+
+    @contextlib.contextmanager
+    def _on_stream(self):
+        """torch's current stream is the context's."""
+        cuda, stream = self.ctx.torch.cuda, self.ctx.stream
+        for before in (cuda.current_stream(self.ctx.device), self._made):
+            if before is not None and before != stream:
+                stream.wait_stream(before)
+        self._made = stream
+        with cuda.stream(stream):
+            yield
 
     def _decode(self) -> None:
         if not self.replay_steps:
@@ -251,6 +267,10 @@ class BeamSearch:
             raise GenerationError("max_output_tokens must be positive")
         if len(prompt) < 1 or len(prompt) + max_output_tokens > self.capacity:
             raise GenerationError("the prompt and its output exceed the capacity")
+        with self._on_stream():
+            return self._search(prompt, max_output_tokens)
+
+    def _search(self, prompt: Sequence[int], max_output_tokens: int) -> list:
         torch, states = self.ctx.torch, self._states
         scores, other = self._scores
         states.start()
