@@ -262,7 +262,8 @@ class BeamSearch:
         self._graph.launch()
 
     def search(self, prompt: Sequence[int], max_output_tokens: int) -> list:
-        """The beams' hypotheses, best first."""
+        """The beams' hypotheses, best first: fewer than the beams where the tokens that are
+        not masked make no more."""
         if max_output_tokens < 1:
             raise GenerationError("max_output_tokens must be positive")
         if len(prompt) < 1 or len(prompt) + max_output_tokens > self.capacity:
@@ -283,7 +284,7 @@ class BeamSearch:
         position = len(prompt)
         for n in range(1, max_output_tokens + 1):
             if self._masked.numel():
-                self._logits.index_fill_(2, self._masked, torch.finfo(torch.float32).min)
+                self._logits.index_fill_(2, self._masked, -torch.inf)
             # (a live beam's candidates have n tokens)
             lengths = torch.where(ended != 0, lengths, float(n))
             hip.beam_select(self.ctx, self._logits, scores, other, self._parents, self._tokens, self._workspace,

@@ -151,3 +151,14 @@ def test_one_stream_waits_for_nothing(monkeypatch):
     search.search([1], 2)
     assert s.torch.default.waits == []
     assert {stream for _, stream in s.torch.uses} == {"default"}
+
+
+@pytest.mark.parametrize("allowed,steps", [([5], 3), ([5, 9], 1), ([1, 2], 2), ([], 2)])
+def test_masked_tokens_are_never_chosen(monkeypatch, allowed, steps):
+    """Also where fewer are left than there are beams: as many hypotheses as the tokens
+    make."""
+    s = Search(monkeypatch)
+    found = s.make(masked_tokens=[t for t in range(VOCAB) if t not in allowed]).search([1], steps)
+    assert len(found) == min(BEAMS, len(allowed) ** steps)
+    assert all(len(h.tokens) == steps and set(h.tokens) <= set(allowed) for h in found)
+    assert len({tuple(h.tokens) for h in found}) == len(found)

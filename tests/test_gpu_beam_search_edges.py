@@ -1,5 +1,6 @@
 """serving.BeamSearch where a call can go wrong beside its own sizes: streams other than
-the current one, threads."""
+the current one, threads, more beams than tokens."""
+import math
 import threading
 
 import pytest
@@ -59,3 +60,27 @@ def test_search_after_the_context_changed_its_stream(gpu, parts, replay):
     assert search.search([3, 9], 6) == want
     search.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("replay", [False, True])
+@pytest.mark.parametrize("beams,allowed,steps", [(4, [9], 5), (4, [9, 200], 1), (4, [9, 200], 5), (7, [1, 2, 300], 2),
+                                                 (64, [1, 2, 300], 3)])
+def test_more_beams_than_allowed_tokens(gpu, parts, replay, beams, allowed, steps):
+    """Masked tokens are never chosen: as many hypotheses as the others make, all
+    different, and where those are all there are, their probabilities sum to 1."""
+    masked = [t for t in range(VOCAB) if t not in allowed]
+    search = serving.BeamSearch(gpu, parts["two"], beams, 24, masked_tokens=masked, replay_steps=replay)
+    found = search.search([3, 9, 40], steps)
+    search.close()
+    assert len(found) == min(beams, len(allowed) ** steps)
+    assert all(len(h.tokens) == steps and set(h.tokens) <= set(allowed) for h in found)
+    assert len({tuple(h.tokens) for h in found}) == len(found)
+    if len(allowed) == 1:
+        # one token has all of the probability: a sum of logarithms good to 2^-32
+        assert abs(found[0].log_probability) <= steps * 2.0 ** -32
+    elif beams >= len(allowed) ** steps:
+        # all sequences there are: their probabilities sum to 1, each score a sum of
+        # floats rounded once a step (2^-24 of it) behind logarithms good to 2^-32
+        total = sum(math.exp(h.log_probability) for h in found)
+        worst = max(abs(h.log_probability) for h in found)
+        assert abs(total - 1.0) <= 2.0 * steps * (2.0 ** -24 * worst + 2.0 ** -32)
