@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import math
 import threading
 import time
 from dataclasses import dataclass
@@ -224,6 +225,8 @@ class BeamSearch:
             raise GenerationError("capacity exceeds model context")
         if any(not 0 <= t < model.vocabulary for t in (*stop_tokens, *masked_tokens)):
             raise GenerationError("a stop or masked token is outside the vocabulary")
+        if not math.isfinite(length_penalty):
+            raise GenerationError("length_penalty must be finite")
         torch = ctx.torch
         self.ctx, self.model, self.beams, self.capacity = ctx, model, beams, capacity
         self.length_penalty, self.ubatch, self.replay_steps = float(length_penalty), prefill_ubatch, replay_steps
@@ -268,6 +271,9 @@ class BeamSearch:
             raise GenerationError("max_output_tokens must be positive")
         if len(prompt) < 1 or len(prompt) + max_output_tokens > self.capacity:
             raise GenerationError("the prompt and its output exceed the capacity")
+        # (length^-length_penalty is held in a float)
+        if abs(self.length_penalty) * math.log2(max_output_tokens) > 126:
+            raise GenerationError("length_penalty is too large for so many tokens")
         with self._on_stream():
             return self._search(prompt, max_output_tokens)
 

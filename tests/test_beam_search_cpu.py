@@ -162,3 +162,23 @@ def test_masked_tokens_are_never_chosen(monkeypatch, allowed, steps):
     assert len(found) == min(BEAMS, len(allowed) ** steps)
     assert all(len(h.tokens) == steps and set(h.tokens) <= set(allowed) for h in found)
     assert len({tuple(h.tokens) for h in found}) == len(found)
+
+
+@pytest.mark.parametrize("penalty", [float("nan"), float("inf"), -float("inf")])
+def test_penalties_that_are_not_finite_are_refused(monkeypatch, penalty):
+    with pytest.raises(serving.GenerationError, match="finite"):
+        Search(monkeypatch).make(length_penalty=penalty)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_penalties_that_no_float_holds_are_refused(monkeypatch, sign):
+    """Before the prompt is run, and only for as many tokens as make them so: 8^42 is
+    2^126, of which a float and its inverse are normal numbers."""
+    s = Search(monkeypatch)
+    search = s.make(length_penalty=42.0 * sign)
+    with pytest.raises(serving.GenerationError, match="length_penalty"):
+        search.search([1], 9)
+    assert s.prefills == 0
+    assert len(search.search([1], 8)) == BEAMS
+    assert s.prefills == 1 and bool(torch.isfinite(s.weights).all()) and bool((s.weights >= 2.0 ** -126).all())
+    assert len(s.make(length_penalty=1e30 * sign).search([1], 1)) == BEAMS

@@ -84,3 +84,17 @@ def test_more_beams_than_allowed_tokens(gpu, parts, replay, beams, allowed, step
         total = sum(math.exp(h.log_probability) for h in found)
         worst = max(abs(h.log_probability) for h in found)
         assert abs(total - 1.0) <= 2.0 * steps * (2.0 ** -24 * worst + 2.0 ** -32)
+
+
+@pytest.mark.parametrize("penalty", [42.0, -42.0])
+def test_penalties_at_a_floats_edge(gpu, parts, penalty):
+    """8^42 is 2^126; one token more is refused before the prompt is run."""
+    search = serving.BeamSearch(gpu, parts["one"], 4, 24, penalty, stop_tokens=list(range(0, VOCAB, 5)))
+    found = search.search([3, 9], 8)
+    assert len(found) == 4
+    for h in found:
+        length = len(h.tokens) + (h.finish_reason == "stop_token")
+        assert h.score == h.log_probability / float(length) ** penalty
+    with pytest.raises(serving.GenerationError, match="length_penalty"):
+        search.search([3, 9], 9)
+    search.close()
