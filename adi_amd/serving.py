@@ -267,6 +267,8 @@ class BeamSearch:
     def search(self, prompt: Sequence[int], max_output_tokens: int) -> list:
         """The beams' hypotheses, best first: fewer than the beams where the tokens that are
         not masked make no more."""
+        if self._workspace is None:
+            raise GenerationError("the search is closed")
         if max_output_tokens < 1:
             raise GenerationError("max_output_tokens must be positive")
         if len(prompt) < 1 or len(prompt) + max_output_tokens > self.capacity:

@@ -182,3 +182,13 @@ def test_penalties_that_no_float_holds_are_refused(monkeypatch, sign):
     assert len(search.search([1], 8)) == BEAMS
     assert s.prefills == 1 and bool(torch.isfinite(s.weights).all()) and bool((s.weights >= 2.0 ** -126).all())
     assert len(s.make(length_penalty=1e30 * sign).search([1], 1)) == BEAMS
+
+
+def test_a_closed_search_is_refused(monkeypatch):
+    s = Search(monkeypatch)
+    search = s.make()
+    search.close()
+    with pytest.raises(serving.GenerationError, match="closed"):
+        search.search([1], 2)
+    assert s.prefills == 0
+    search.close()
