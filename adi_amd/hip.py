@@ -1545,7 +1545,7 @@ class StateRows:
                 _refuse(f"state rows on {t.device}, the context is on cuda:{ctx.device}")
             shape, strides, each = t.shape, t.stride(), 1
             for n, step in zip(reversed(shape[2:]), reversed(strides[2:])):
-                if n > 1 and step != each:
+                if n > 1 and step != each and t.numel():
                     _refuse("state rows: a row must be contiguous")
                 each *= n
             size = t.element_size()

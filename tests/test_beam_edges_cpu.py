@@ -1,5 +1,9 @@
 """Refusals of the beam and page-pool entry points at their edges, without a GPU."""
 import ctypes as C
+import types
+
+import pytest
+import torch
 
 from adi_amd import hip
 from test_beam_cpu import batch, fork, pool, refused
@@ -11,3 +15,17 @@ def test_a_fork_of_no_rows_checks_what_it_reads():
         C.byref(pool()), C.byref(batch(sequences=0)), C.byref(fork(parents=None, lengths=None, table=None, **change)))
     assert check() == hip.OK and check(references=None) == hip.OK
     refused(check(references=2), "unaligned")
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0), (2, 3, 4, 0), (2, 3, 0, 4), (2, 0, 5), (0, 3, 2, 4)])
+def test_state_rows_of_nothing(shape):
+    """Tensors without elements are rows of no bytes, or no rows."""
+    ctx = types.SimpleNamespace(device=-1)
+    rows = hip.StateRows(ctx, [torch.empty(shape)])
+    assert (rows.requests, rows.beams) == shape[:2]
+    size = 4
+    for n in shape[2:]:
+        size *= n
+    assert rows.struct[0].row_bytes == size
+    with pytest.raises(hip.HipError, match="contiguous"):
+        hip.StateRows(ctx, [torch.empty(2, 3, 4, 4).transpose(2, 3)])
