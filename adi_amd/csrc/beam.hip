@@ -1054,7 +1054,9 @@ void require_reorder(const adi_hip_row_array *arrays, uint32_t count, uint32_t r
                 "reorder rows: rows must be below 2^36 bytes, strides below 2^46");
         require((beams == 1 || a.row_stride >= a.row_bytes) &&
                     (requests == 1 || a.request_stride >= (beams - 1) * a.row_stride + a.row_bytes ||
-                     (a.request_stride >= a.row_bytes && a.row_stride >= (requests - 1) * a.request_stride + a.row_bytes)),
+                     // (a product may pass 64 bits here)
+                     (a.request_stride >= a.row_bytes && a.row_stride >= a.row_bytes &&
+                      (a.row_stride - a.row_bytes) / (requests - 1) >= a.request_stride)),
                 "reorder rows: an array's rows overlap");
         require(reorder_blocks(a.row_bytes, beams) * requests < kReorderBlocks,
                 "reorder rows: too many rows of such a size");

@@ -29,3 +29,22 @@ def test_state_rows_of_nothing(shape):
     assert rows.struct[0].row_bytes == size
     with pytest.raises(hip.HipError, match="contiguous"):
         hip.StateRows(ctx, [torch.empty(2, 3, 4, 4).transpose(2, 3)])
+
+
+@pytest.mark.parametrize("array,requests,ok", [
+    ((1 << 20, 1 << 45, (1 << 45) + 100, 100), (1 << 19) + 1, False),  # 2^19 strides of 2^45 are 2^64
+    ((1 << 20, 1 << 45, (1 << 46) - 1, 100), (1 << 19) + 2, False),
+    ((1 << 20, 1 << 45, 1 << 20, 100), (1 << 19) + 1, True),           # requests outermost
+    ((1 << 20, 100, 100 << 10, 100), 1 << 10, True),
+    ((1 << 20, 100, (100 << 10) - 1, 100), 1 << 10, False),
+    ((1 << 20, 101, 101 * 1023 + 100, 100), 1 << 10, True),
+    ((1 << 20, 101, 101 * 1023 + 99, 100), 1 << 10, False),
+    ((1 << 20, 100, 99, 100), 2, False)])
+def test_rows_of_requests_that_overlap(array, requests, ok):
+    """Beams outermost: all requests' rows between two of a request's."""
+    rows = (hip.RowArray * 1)(hip.RowArray(*array))
+    status = hip.load().adi_hip_reorder_check(rows, 1, requests, 2, 1 << 30)
+    if ok:
+        assert status == hip.OK
+    else:
+        refused(status, "overlap")
