@@ -1519,10 +1519,14 @@ def beam_select(ctx: Context, logits, scores, out_scores, parents, tokens, works
     _device_floats(ctx, out_scores, "out_scores", n, choices)
     _device_words(ctx, parents, "parents", n, choices)
     _device_words(ctx, tokens, "tokens", n, choices)
-    a = _pack_beam(_type_of(logits), logits.data_ptr(), request_stride, beam_stride, n, k, v, choices,
-                   scores.data_ptr(), 0 if weights is None else _device_floats(ctx, weights, "weights", n, k).data_ptr(),
-                   0 if ended is None else _device_words(ctx, ended, "ended", n, k).data_ptr(), ended_token,
-                   1 if settle else 0, out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr())
+    try:
+        a = _pack_beam(_type_of(logits), logits.data_ptr(), request_stride, beam_stride, n, k, v, choices,
+                       scores.data_ptr(),
+                       0 if weights is None else _device_floats(ctx, weights, "weights", n, k).data_ptr(),
+                       0 if ended is None else _device_words(ctx, ended, "ended", n, k).data_ptr(), ended_token,
+                       1 if settle else 0, out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr())
+    except struct.error:
+        _refuse("beam select: a size is out of range")
     status = ctx.lib.adi_hip_beam_select(ctx.handle, a, workspace.handle)
     if status:
         ctx.check(status)
@@ -1537,6 +1541,7 @@ class StateRows:
         if any(t.dim() < 2 for t in self.arrays):
             _refuse("state rows: arrays must be of shape [requests, beams, ...], one for all")
         self.requests, self.beams = (int(x) for x in self.arrays[0].shape[:2]) if self.arrays else (0, 1)
+        _words("state rows: requests or beams are out of range", self.requests, self.beams)
         rows = (RowArray * max(len(self.arrays), 1))()
         for i, t in enumerate(self.arrays):
             if tuple(t.shape[:2]) != (self.requests, self.beams):
@@ -1656,7 +1661,11 @@ def paged_fork(ctx: Context, pool: PagedPool, batch: PagedBatch, parents, worksp
     _device_words(ctx, lengths, "lengths", n * k)
     _device_words(ctx, table, "table", n * k, int(table.shape[-1]))
     _device_words(ctx, references, "references", pool.pages)
-    a = _pack_fork(k, parents.data_ptr(), lengths.data_ptr(), table.data_ptr(), table.shape[1], references.data_ptr())
+    try:
+        a = _pack_fork(k, parents.data_ptr(), lengths.data_ptr(), table.data_ptr(), table.shape[1],
+                       references.data_ptr())
+    except struct.error:
+        _refuse("paged fork: a size is out of range")
     status = ctx.lib.adi_hip_paged_fork(ctx.handle, pool.struct, batch.struct, a, workspace.handle)
     if status:
         ctx.check(status)
@@ -1666,6 +1675,8 @@ def paged_copy(ctx: Context, source: PagedPool, target: PagedPool, sources, targ
     """Pages sources[i] of a pool to pages targets[i] of another or the same (int32
     [count]), in every cache, the first entries[i] of their entries where given."""
     n = int(sources.shape[0])
+    if n >> 32:
+        _refuse("paged copy: more than 2^22 pages")
     _device_words(ctx, sources, "sources", n)
     _device_words(ctx, targets, "targets", n)
     if entries is not None:
@@ -1691,8 +1702,11 @@ def paged_compact(ctx: Context, pool: PagedPool, lengths, next_table, live, work
     _device_words(ctx, next_table, "next_table", *table.shape)
     _device_words(ctx, references, "references", pool.pages)
     _device_words(ctx, live, "live", 1)
-    a = _pack_compact(references.data_ptr(), n, lengths.data_ptr(), table.data_ptr(), next_table.data_ptr(),
-                      table.shape[1], live.data_ptr())
+    try:
+        a = _pack_compact(references.data_ptr(), n, lengths.data_ptr(), table.data_ptr(), next_table.data_ptr(),
+                          table.shape[1], live.data_ptr())
+    except struct.error:
+        _refuse("paged compact: a size is out of range")
     status = ctx.lib.adi_hip_paged_compact(ctx.handle, pool.struct, a, workspace.handle)
     if status:
         ctx.check(status)

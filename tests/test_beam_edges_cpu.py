@@ -48,3 +48,42 @@ def test_rows_of_requests_that_overlap(array, requests, ok):
         assert status == hip.OK
     else:
         refused(status, "overlap")
+
+
+class Untouched:
+    """A library of which nothing may be called."""
+
+    def __getattr__(self, name):
+        raise AssertionError(f"{name} was called")
+
+
+def meta(*shape, dtype=torch.int32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+HUGE = (1 << 32) + 1  # 1 in 32 bits
+
+
+def test_sizes_past_32_bits_are_refused():
+    """None is cut to 32 bits on its way into the library, and none ends in another
+    error than a refusal's."""
+    ctx = types.SimpleNamespace(device=-1, lib=Untouched(), handle=None)
+    space = types.SimpleNamespace(handle=None)
+    held = types.SimpleNamespace(pages=4, references=meta(4), struct=None)
+    calls = [
+        lambda: hip.StateRows(ctx, [meta(HUGE, 2, 3)]),
+        lambda: hip.StateRows(ctx, [meta(1, HUGE, 3)]),
+        lambda: hip.paged_copy(ctx, held, held, meta(HUGE), meta(HUGE)),
+        lambda: hip.beam_select(ctx, meta(1, 1, HUGE, dtype=torch.float16), meta(1, 1, dtype=torch.float32),
+                                meta(1, 1, dtype=torch.float32), meta(1, 1), meta(1, 1), space),
+        lambda: hip.beam_select(ctx, meta(HUGE, 1, 5, dtype=torch.float16), meta(HUGE, 1, dtype=torch.float32),
+                                meta(HUGE, 1, dtype=torch.float32), meta(HUGE, 1), meta(HUGE, 1), space),
+        lambda: hip.paged_fork(ctx, held, types.SimpleNamespace(lengths=meta(1), table=meta(1, HUGE), struct=None),
+                               meta(1, 1), space),
+        lambda: hip.paged_fork(ctx, held, types.SimpleNamespace(lengths=meta(HUGE), table=meta(HUGE, 1), struct=None),
+                               meta(1, HUGE), space),
+        lambda: hip.paged_compact(ctx, held, meta(HUGE), meta(HUGE, 1), meta(1), space),
+        lambda: hip.paged_compact(ctx, held, meta(1), meta(1, HUGE), meta(1), space)]
+    for call in calls:
+        with pytest.raises(hip.HipError):
+            call()
