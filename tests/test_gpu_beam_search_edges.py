@@ -1,5 +1,6 @@
 """serving.BeamSearch where a call can go wrong beside its own sizes: streams other than
-the current one, threads, more beams than tokens."""
+the current one, threads, more beams than tokens, many beams, and positions past those
+that a recorded step covers (512)."""
 import math
 import threading
 
@@ -8,6 +9,7 @@ import torch
 
 import small_model
 from adi_amd import hip, serving
+from test_gpu_beam_search import plain_search
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +100,22 @@ def test_penalties_at_a_floats_edge(gpu, parts, penalty):
     with pytest.raises(serving.GenerationError, match="length_penalty"):
         search.search([3, 9], 9)
     search.close()
+
+
+@pytest.mark.parametrize("replay", [False, True])
+@pytest.mark.parametrize("beams,prompt,steps,penalty,stop", [(4, 507, 12, 0.0, []), (3, 1021, 8, 1.0, [3, 77, 200]),
+                                                             (64, 5, 6, 0.5, list(range(0, VOCAB, 9)))])
+def test_long_prompts_and_many_beams(gpu, parts, replay, beams, prompt, steps, penalty, stop):
+    """The same as the search on the host; scores as there."""
+    tokens = [(7 * i * i + 3 * i) % VOCAB for i in range(prompt)]
+    capacity = prompt + steps
+    search = serving.BeamSearch(gpu, parts["one"], beams, capacity, penalty, stop, replay_steps=replay)
+    got = search.search(tokens, steps)
+    search.close()
+    want = plain_search(gpu, parts["one"], tokens, steps, beams, penalty, stop, [], capacity)
+    assert [h.tokens for h in got] == [w[0] for w in want]
+    assert [h.finish_reason == "stop_token" for h in got] == [w[3] for w in want]
+    for h, w in zip(got, want):
+        bound = steps * (2.0 ** -23 * abs(w[1]) + 2.0 ** -32)
+        assert abs(h.log_probability - w[1]) <= bound
+        assert abs(h.score - w[2]) <= bound + 2.0 ** -23 * abs(w[2])
