@@ -613,8 +613,9 @@ __device__ __forceinline__ uint32_t trim(uint64_t *list, uint32_t &entries, uint
 // largest logit so far. The best: in a first tile, the `choices` best of the lanes'
 // own two largest (of their pieces' halves) bound what is taken from below, later the
 // last of those taken so far, by any wave of the block. Bound by its instructions, 23
-// for 64 logits, 15 of them the exponential (64 x 8 rows of 248,320 bf16 logits: 107
-// us with the join, 2.4 TB/s); few tiles a wave by its start and end. A part of ONE tile is the same
+// for 64 logits, 15 of them the exponential (64 x 8 rows of 248,320 bf16 logits: 108 to
+// 119 us with the join on four cards, 2.4 to 2.1 TB/s; f16 113 where bf16 takes 108); few
+// tiles a wave by its start and end. A part of ONE tile is the same
 // without the next tile and the bounds for it (16 x 4 rows of 248,320 f32 logits 22.9
 // us in place of 24.2, 32 x 4 39.4 and 41.8).
 template <typename T, uint32_t N, bool ONE>
@@ -995,6 +996,8 @@ __device__ __forceinline__ void reorder_units(char *base, uint64_t row_stride, c
 // registers hold, as rows lie far apart and one unit of each leaves most of the memory's
 // channels idle (4 rows of 4 requests' 30 states, 1.05 GB: 254 us with one unit, 191
 // with four, 5.5 TB/s; 8 rows 415 with one, 198 with two and with four; 16 213 and 205).
+// More than 16 rows leave room for one (a request's 30 states, half of the rows moved:
+// 16 rows 203 us, 17 463, 32 581, 64 939).
 template <uint32_t K>
 constexpr uint32_t kUnits = K <= 4u ? 4u : K <= 16u ? 2u : 1u;
 

@@ -35,7 +35,10 @@ constexpr uint32_t kTinyPages = 1024, kTinyCopiers = 4;
 // A fork does so with up to 256 rows, by the same number of blocks that copy, where the
 // one that writes the tables has so many runs of 256 columns to go through, or one
 // request's (4 beams of 2,005 entries 9.8 us in two launches and 6.9, 8 of 1,000 10.7 and
-// 8.1, 16 of 300 14.8 and 11.9; 4 requests of 4 beams, 16 runs, 9.5 and 11.4).
+// 8.1, 16 of 300 14.8 and 11.9; 4 requests of 4 beams, 16 runs, 9.5 and 11.4; 8 rows without
+// beams 9.8 and 8.8). In place the tables wait for the last block's arrival: 1 row without
+// beams 9.9 and 6.9, 4 rows 9.6 and 8.8, 4 beams of 2,005 entries 11.2 and 9.2, but 8 rows
+// without beams 9.6 and 12.8, 10 of them 9.6 and 14.8, for which the bound is too high.
 constexpr uint32_t kTinyTables = 12;
 
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
