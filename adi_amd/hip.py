@@ -362,9 +362,9 @@ def release_dropped() -> None:
     """Frees the library's objects whose owners were dropped without close().
     Freeing one waits for the device, which ends a capture on any stream, and
     finalizers run wherever the collector does, so they only leave their handles
-    here; what creates or closes such an object, and Context.synchronize, call
-    this first, as they touch the device themselves. A context waits for its
-    graphs and batchers. Nothing while the current stream captures."""
+    here; what creates or closes such an object calls this first, as it allocates
+    or frees itself. A context waits for its graphs and batchers. Nothing while the
+    current stream captures; others' captures are the caller's to know."""
     if not _dropped:
         return
     import torch
@@ -453,7 +453,6 @@ class Context(_Owner):
 
     def synchronize(self) -> None:
         self.check(self.lib.adi_hip_synchronize(self.handle))
-        release_dropped()
 
     def set_fused_decode(self, enabled) -> None:
         """One persistent launch for a MoE block of 1-12 rows and for NE

@@ -24,7 +24,7 @@ def dropped(gpu):
 
 def test_objects_collected_during_a_capture(gpu):
     gc.collect()
-    gpu.synchronize()
+    hip.release_dropped()
     rope, positions = hip.Rope(gpu, 128, "pairs", 1e4), ints([3, 70, 5000])
     x = torch.randn(3, 4, 128, device="cuda")
     out, eager = torch.empty_like(x), torch.empty_like(x)
@@ -45,7 +45,7 @@ def test_objects_collected_during_a_capture(gpu):
         gc.enable()
         gpu.use_stream(torch.cuda.default_stream())
     assert waiting == 3
-    gpu.synchronize()
+    hip.release_dropped()
     assert not hip._dropped
     for i in range(3):
         x.normal_()

@@ -188,7 +188,7 @@ def test_calls_that_touch_the_device_free_what_was_dropped(lib):
     ctx, file = context(lib), type("File", (), {"handle": None})()
     book = hip.np.zeros(4, hip.np.float32)
     calls = [
-        lambda: hip.Rope(ctx, 64), lambda: hip.PagedWorkspace(ctx), ctx.synchronize, workspace(lib).close,
+        lambda: hip.Rope(ctx, 64), lambda: hip.PagedWorkspace(ctx), workspace(lib).close,
         lambda: ctx.expert_codebook(book), lambda: ctx.ne_codebook(book),
         lambda: hip.upload_codebooks_gguf(ctx, file), lambda: hip.upload_moe_layer_gguf(ctx, file, 0, 0, 0),
         lambda: hip.upload_decoder_layer_gguf(ctx, file, 0, 0, 0), lambda: hip.upload_head_gguf(ctx, file),
@@ -199,6 +199,13 @@ def test_calls_that_touch_the_device_free_what_was_dropped(lib):
         held = call()
         assert ("adi_hip_rope_destroy", 99) in lib.calls
         del held
+
+
+def test_synchronize_frees_nothing(lib):
+    """It waits for one stream, which another thread's capture survives."""
+    drop(lib)
+    context(lib).synchronize()
+    assert [name for name, _ in lib.calls] == ["adi_hip_synchronize"]
 
 
 def test_a_dropped_search_does_not_touch_the_device(lib):
